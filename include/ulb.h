@@ -48,6 +48,7 @@ extern "C" {
 #define ULB_TYPE_Q4_K 12
 #define ULB_TYPE_Q8_0 8  /* token_embd and output.weight only (as llama.cpp's Q4_0 files store them) */
 #define ULB_TYPE_Q6_K 14 /* token_embd and output.weight only */
+#define ULB_TYPE_BF16 30 /* rotary, tree attention, cache page and logits operators only */
 
 typedef struct ulb_ctx ulb_ctx;
 typedef struct ulb_tensor ulb_tensor;
@@ -69,6 +70,17 @@ ULB_API int ulb_destroy(ulb_ctx* ctx);
 ULB_API void* ulb_stream(ulb_ctx* ctx);
 /* Replaces ComputeDispatcher::wait_for_completion (src/vulkan_backend/compute.cpp:82-121). */
 ULB_API int ulb_stream_sync(ulb_ctx* ctx);
+/*
+ * Enqueue the context's later work on `stream` (a cudaStream_t of the context's device), so that
+ * a caller with a stream of its own (a framework's current stream) needs no synchronisation
+ * around the calls.  NULL goes back to the stream ulb_init made; the legacy default stream is
+ * named by its handle cudaStreamLegacy.  Work already enqueued by the context runs before work
+ * enqueued after the switch (an event orders the two streams).  The stream must outlive its use
+ * here; switching is refused during a capture (ulb_capture_begin), and the legacy stream
+ * cannot be captured (speculative loops with use_graphs need another one).  ulb_stream returns
+ * the stream in use.
+ */
+ULB_API int ulb_use_stream(ulb_ctx* ctx, void* stream);
 /*
  * Bounded device-side wait: enqueue on the context stream a wait until the int32 at dev_flag
  * (device memory, or memory the device can reach: another stream's or process's flag) is
@@ -273,6 +285,206 @@ ULB_API int ulb_spec_accept(ulb_ctx* ctx, const float* dev_p_logits, const float
                     const int32_t* dev_draft_tokens, int B, int k, int V, const ulb_warp* warp,
                     uint64_t seed, uint32_t round, int32_t* dev_out_tokens,
                     int32_t* dev_out_n_accepted);
+
+/* ------------------------------------------------------------------ paged cache operators */
+/*
+ * Operators for callers that run their own speculative step over a paged cache of their own
+ * shape: rotate and append rows, attend drafted trees over the pages, change the logits before
+ * sampling, and move what a step leaves in the cache.  None of them has a counterpart in the
+ * reference, whose cache is one flat host array (src/inference/model.h:49-77).  All enqueue on
+ * the context's stream and return without synchronising; all can be captured
+ * (ulb_capture_begin) after a first call outside a capture.  Contents of device arrays (page
+ * ids, positions, slots, row ranges, token ids, indexes) cannot be checked by the call: the kernels
+ * check them against the sizes given here and skip what lies outside, so a wrong entry costs
+ * results, never an access out of bounds.  Offsets into arrays whose size no argument gives
+ * (history_start, bias_start) are taken as they are.
+ *
+ * A cache as the operators see it: one pool for K, one of the same layout for V.  Element d of
+ * position t of page p for kv head h of layer l is at
+ *   l * layer_stride + p * page_stride + h * head_stride + t * pos_stride + d     (elements)
+ * A stride of 0 means dense: pos_stride = head_dim, head_stride = page * pos_stride,
+ * page_stride = n_head_kv * head_stride, layer_stride = n_pages * page_stride (the layout of
+ * ulb_kv_alloc_paged).  [page][position][head] pools give pos_stride = n_head_kv * head_dim and
+ * head_stride = head_dim.  Strides are multiples of 8 elements, pools 16-byte aligned, head_dim a
+ * multiple of 8 up to 256.  The block table int32 [n_seq][max_pages] maps positions
+ * [j * page, (j + 1) * page) of sequence s to page [s * max_pages + j]; an entry outside
+ * [0, n_pages) is unmapped: nothing is read or written there.
+ */
+typedef struct ulb_cache_desc {
+  int dtype;      /* ULB_TYPE_F16 or ULB_TYPE_BF16                                  */
+  int n_layer;    /* layers in the pools (page moves); per-layer operators ignore it */
+  int n_head_kv, head_dim;
+  int page;       /* positions per page: 16, 32, 64, 128 or 256                      */
+  int n_pages;    /* pages of one layer's pool                                       */
+  int n_seq, max_pages; /* block table rows and columns                              */
+  int64_t layer_stride, page_stride, head_stride, pos_stride;
+} ulb_cache_desc;
+
+/*
+ * Rotary positions.  The first rot_dim elements of a head (even, <= head_dim) form rot_dim / 2
+ * pairs; pair i of a row at position pos is turned by the angle pos * f_i and multiplied by m:
+ *   (a, b) -> m (a cos - b sin, a sin + b cos)
+ * The other elements pass through.  Pairs are elements (2i, 2i + 1) (ULB_ROPE_INTERLEAVED, the
+ * GGUF LLaMA layout) or (i, i + rot_dim / 2) (ULB_ROPE_HALF).  f_i = base^(-2i / rot_dim), then
+ * divided by freq_factors[i] when given (host float [rot_dim / 2], GGUF's rope_freqs.weight),
+ * then scaled:
+ *   ULB_ROPE_NONE        f_i
+ *   ULB_ROPE_LINEAR      f_i / factor
+ *   ULB_ROPE_NTK         base * factor^(rot_dim / (rot_dim - 2)) in place of base
+ *   ULB_ROPE_YARN        f_i (1 - r_i) + f_i / factor r_i, r_i = clamp((i - lo) / max(hi - lo, 0.001), 0, 1),
+ *                        lo = max(floor(e(beta_fast)), 0), hi = min(ceil(e(beta_slow)), rot_dim - 1),
+ *                        e(n) = rot_dim ln(orig_len / (2 pi n)) / (2 ln base); m = 0.1 ln(factor) + 1
+ *   ULB_ROPE_WAVELENGTH  with w = 2 pi / f_i: f_i where w < orig_len / high_freq, f_i / factor where
+ *                        w > orig_len / low_freq, else (1 - x) f_i / factor + x f_i with
+ *                        x = (orig_len / w - low_freq) / (high_freq - low_freq)
+ * m = 1 except as stated, or attn_scale when that is > 0.  Angles are exact for every int32
+ * position (negative ones too): they are kept modulo one turn in 64-bit fixed point, so long
+ * contexts lose no accuracy and there is no table of positions.
+ */
+#define ULB_ROPE_INTERLEAVED 0
+#define ULB_ROPE_HALF 1
+#define ULB_ROPE_NONE 0
+#define ULB_ROPE_LINEAR 1
+#define ULB_ROPE_NTK 2
+#define ULB_ROPE_YARN 3
+#define ULB_ROPE_WAVELENGTH 4
+typedef struct ulb_rope_desc {
+  int head_dim, rot_dim, layout, scaling;
+  double base, factor, orig_len, beta_fast, beta_slow, low_freq, high_freq, attn_scale;
+} ulb_rope_desc;
+typedef struct ulb_rope ulb_rope;
+ULB_API int ulb_rope_create(ulb_ctx* ctx, const ulb_rope_desc* desc, const float* host_freq_factors, ulb_rope** out);
+ULB_API int ulb_rope_free(ulb_rope* r);
+/*
+ * out = rows of x turned to their positions; M rows of n_head heads, element d of head h of row m
+ * at m * row_stride + h * head_stride + d (0: dense).  inverse != 0 turns by the negative angle
+ * (m still multiplies): the gradient of the forward call with respect to x, given the gradient
+ * of its output.  dtype F32, F16 or BF16 for both; computed in fp32.  out may be x (same
+ * strides).
+ */
+ULB_API int ulb_rope_apply(ulb_ctx* ctx, const ulb_rope* r, int dtype, const void* dev_x, int64_t x_row, int64_t x_head,
+                   const int32_t* dev_pos, int M, int n_head, int inverse, void* dev_out, int64_t out_row,
+                   int64_t out_head);
+/*
+ * The same for the q, k and v rows a projection leaves (in_dtype F32, F16 or BF16, heads dense
+ * inside rows of stride q_row / k_row / v_row, 0: dense): q is turned into dev_q_out (dense
+ * [M][n_head][head_dim] of the cache's type), k turned and v copied into the cache at
+ * slot dev_slot[m] of sequence dev_row_seq[m] (a tree node's slot is not its rotary position
+ * dev_pos[m]).  The pools are those of one layer.  Rows whose slot is unmapped, negative or past
+ * the table write q only.  Two rows must not share a slot.
+ */
+ULB_API int ulb_rope_append(ulb_ctx* ctx, const ulb_rope* r, const ulb_cache_desc* cache, int in_dtype, const void* dev_q,
+                    int64_t q_row, const void* dev_k, int64_t k_row, const void* dev_v, int64_t v_row, int n_head,
+                    const int32_t* dev_pos, const int32_t* dev_row_seq, const int32_t* dev_slot,
+                    const int32_t* dev_block_table, int M, void* dev_q_out, void* dev_k_pool, void* dev_v_pool);
+
+/*
+ * Attention of drafted trees over a paged cache.  Rows [row_start[s], row_start[s + 1]) of
+ * dev_q (cache type, [rows][n_head][head_dim]) belong to sequence s, whose cache holds len[s]
+ * positions: prefix[s] committed ones, then the slots of its tree (slot j at position
+ * prefix[s] + j).  Row r sees every prefix position and slot j for each set bit j of its mask
+ * row (bit j % 32 of dev_mask[r * mask_words + j / 32]; slots >= 32 * mask_words are not seen):
+ * its ancestors and itself, or anything else.  With mask_words = 0 (dev_mask NULL) rows are causal: the
+ * i-th of a sequence's n rows sees positions <= len[s] - n + i (a chain of drafts, a prompt
+ * chunk).  Unmapped pages hold no keys.
+ *   out[r][h] = sum_t p_t v_t,  p = softmax(scale q . k_t) over the visible t   (cache type)
+ *   lse[r][h] = ln sum_t exp(scale q . k_t)                                    (fp32, may be NULL)
+ * GQA: head h reads kv head h / (n_head / n_head_kv).  A row that sees nothing gives out = 0 and
+ * lse = -inf; what it does not see (stale slots, positions past len[s], infinities and NaN there)
+ * never touches its result.  head_dim 64, 80, 96, 128 or 256; n_head / n_head_kv <= 64.
+ * max_rows >= every sequence's rows, max_len >= every len[s] (clamped otherwise).  Scores, statistics and sums are fp32; the probabilities of the
+ * second product are rounded to the cache type.
+ */
+typedef struct ulb_tree_desc {
+  int n_head, rows, max_rows, max_len, mask_words;
+  float scale;
+} ulb_tree_desc;
+ULB_API int ulb_tree_attention(ulb_ctx* ctx, const ulb_cache_desc* cache, const ulb_tree_desc* desc, const void* dev_q,
+                       const void* dev_k_pool, const void* dev_v_pool, const int32_t* dev_block_table,
+                       const int32_t* dev_row_start, const int32_t* dev_prefix, const int32_t* dev_len,
+                       const uint32_t* dev_mask, void* dev_out, float* dev_lse);
+
+/*
+ * Page moves, in every layer of both pools.
+ * ulb_pages_copy: move i of dev_moves int32 [n][3] = (source page, destination page, positions)
+ * copies the first `positions` positions of a page (clamped to the page).  Destinations are
+ * distinct and no page is both a source and a destination of the call.  Moves naming a page
+ * outside [0, n_pages) are skipped.
+ * ulb_pages_compact: for every sequence s, position base[s] + i takes the K / V of position
+ * base[s] + src[s * max_src + i], i < count[s] <= max_src, in place; src strictly increasing
+ * (the nodes of an accepted path, in order).  Positions on unmapped pages are skipped.
+ */
+ULB_API int ulb_pages_copy(ulb_ctx* ctx, const ulb_cache_desc* cache, void* dev_k_pool, void* dev_v_pool,
+                   const int32_t* dev_moves, int n);
+ULB_API int ulb_pages_compact(ulb_ctx* ctx, const ulb_cache_desc* cache, void* dev_k_pool, void* dev_v_pool,
+                      const int32_t* dev_block_table, const int32_t* dev_base, const int32_t* dev_count,
+                      const int32_t* dev_src, int max_src);
+/*
+ * Book of a cache's pages: which page holds which positions of which sequence, and how many
+ * sequences share it; keeps the device block table the operators read.  All of it is host work
+ * but the copies, which go through ulb_pages_copy.  Pages are handed out lowest id first.
+ *   reserve   map positions [0, to) of a sequence and make the pages of [from, to) its own: a
+ *             shared page among them is replaced by a copy of its positions before `from`
+ *             (copy on write).  Call it before writing positions [from, to).  ULB_ENOMEM, with
+ *             nothing changed, when the pool has too few free pages.
+ *   fork      dst (which must hold no pages) shares src's pages of positions [0, n)
+ *   truncate  give back the pages past position n (roll-back; n = 0 frees the sequence)
+ *   defrag    move every page to the lowest ids: afterwards ids >= *out_used are free in both
+ *             pools (copies are enqueued; a caller may shrink or hand out the tail)
+ * The block table changes on the context's stream, in call order with the operators.
+ */
+typedef struct ulb_pages ulb_pages;
+ULB_API int ulb_pages_create(ulb_ctx* ctx, const ulb_cache_desc* cache, void* dev_k_pool, void* dev_v_pool,
+                     ulb_pages** out);
+ULB_API int ulb_pages_free(ulb_pages* p);
+ULB_API int ulb_pages_reserve(ulb_pages* p, int seq, int from, int to);
+ULB_API int ulb_pages_fork(ulb_pages* p, int src_seq, int dst_seq, int n);
+ULB_API int ulb_pages_truncate(ulb_pages* p, int seq, int n);
+ULB_API int ulb_pages_defrag(ulb_pages* p, int* out_used);
+/* the device block table; pages free; pages mapped by a sequence (seq < 0: out_mapped unused) */
+ULB_API int ulb_pages_info(const ulb_pages* p, const int32_t** out_dev_table, int* out_free, int seq, int* out_mapped);
+
+/*
+ * Logits before sampling.  Rows [row_start[s], row_start[s + 1]) belong to sequence s.  For
+ * token t of a row, with x its logit, n(t) its count among the generated tokens and S the set of
+ * prompt and generated tokens:
+ *   1. t in S:     x = x > 0 ? x / repetition : x * repetition
+ *   2. n(t) > 0:   x = x - frequency n(t) - presence
+ *   3. biases:     x = x + the sum of the sequence's biases for t
+ *   4. grammar:    x = -inf unless bit t % 32 of allow[a][t / 32] is set, a = row_allow[r]
+ * params fp32 [n_seq][3] = repetition (> 0), presence, frequency (NULL: 1, 0, 0).
+ * history int32 tokens, sequence s's at [history_start[s], history_start[s + 1]), the first
+ * prompt[s] of them the prompt, the rest generated (NULL: none).  node_tokens int32 [rows]
+ * with the rows' masks (mask_words as in ulb_tree_desc, bit j = row j of the sequence) adds the
+ * tokens of a tree node's path, its own among them, to the generated ones (NULL: none).
+ * Biases: sequence s's entries [bias_start[s], bias_start[s + 1]) of (bias_tokens,
+ * bias_values), token ids in non-decreasing order; repeated ids add up in that order (NULL:
+ * none).  allow uint32 [n_allow][ceil(V / 32)], row_allow int32 [rows] (NULL: row r takes
+ * allow[r]; an index outside [0, n_allow) leaves the row free).  Token ids outside [0, V) are
+ * ignored.  A row whose grammar allows nothing is -inf throughout.
+ * dev_in [rows][ld_in] of dtype F32, F16 or BF16, dev_out fp32 [rows][ld_out]; dev_out may be
+ * dev_in for F32 and ld_out = ld_in.
+ */
+typedef struct ulb_logits_args {
+  int dtype, V, n_seq, rows, max_rows; /* max_rows >= every sequence's rows */
+  int ld_in, ld_out;
+  int mask_words, n_allow;
+  const void* in;
+  float* out;
+  const int32_t* row_start;
+  const float* params;
+  const int32_t* history;
+  const int32_t* history_start;
+  const int32_t* prompt;
+  const int32_t* node_tokens;
+  const uint32_t* mask;
+  const int32_t* bias_start;
+  const int32_t* bias_tokens;
+  const float* bias_values;
+  const uint32_t* allow;
+  const int32_t* row_allow;
+} ulb_logits_args;
+ULB_API int ulb_logits_process(ulb_ctx* ctx, const ulb_logits_args* args);
 
 /* ------------------------------------------------------------------ models */
 /*

@@ -169,7 +169,9 @@ int ulb_init(int device, ulb_ctx** out) {
   std::unique_ptr<ulb_ctx> c(new ulb_ctx());
   c->c.device = device;
   c->c.n_sm = prop.multiProcessorCount;
-  ULB_CUDA(cudaStreamCreateWithFlags(&c->c.stream, cudaStreamNonBlocking));
+  ULB_CUDA(cudaStreamCreateWithFlags(&c->c.own_stream, cudaStreamNonBlocking));
+  c->c.stream = c->c.own_stream;
+  ULB_CUDA(cudaEventCreateWithFlags(&c->c.switch_ev, cudaEventDisableTiming));
   ULB_CUDA(cudaMalloc((void**)&c->c.dev_err, sizeof(int)));
   ULB_CUDA(cudaMemset(c->c.dev_err, 0, sizeof(int)));
   ULB_CUDA(cudaMalloc(&c->c.zero_row, kZeroRowHalves * sizeof(__half)));
@@ -237,9 +239,25 @@ int ulb_destroy(ulb_ctx* ctx) {
   cudaFree(ctx->c.zero_row);
   cudaFree(ctx->c.tc_ws);
   cudaFree(ctx->c.tc_cnt);
-
-  cudaStreamDestroy(ctx->c.stream);
+  cudaFree(ctx->c.tree_ws);
+  cudaEventDestroy(ctx->c.switch_ev);
+  cudaStreamDestroy(ctx->c.own_stream);
   delete ctx;
+  return ULB_OK;
+}
+
+int ulb_use_stream(ulb_ctx* ctx, void* stream) {
+  ULB_CHECK(ctx, ULB_EINVAL, "ulb_use_stream: NULL context");
+  Ctx* c = &ctx->c;
+  const cudaStream_t to = stream ? (cudaStream_t)stream : c->own_stream;
+  if (to == c->stream) return ULB_OK;
+  ULB_CUDA(cudaSetDevice(c->device));
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  ULB_CUDA(cudaStreamIsCapturing(c->stream, &st));
+  ULB_CHECK(st == cudaStreamCaptureStatusNone, ULB_EINVAL, "ulb_use_stream: the context's stream is being captured");
+  ULB_CUDA(cudaEventRecord(c->switch_ev, c->stream));
+  ULB_CUDA(cudaStreamWaitEvent(to, c->switch_ev, 0));
+  c->stream = to;
   return ULB_OK;
 }
 

@@ -73,7 +73,9 @@ struct Tensor {
 struct Ctx {
   int device = 0;
   int n_sm = 0;
-  cudaStream_t stream = nullptr;
+  cudaStream_t stream = nullptr;     /* the stream of every call: own_stream or ulb_use_stream's */
+  cudaStream_t own_stream = nullptr; /* made by ulb_init */
+  cudaEvent_t switch_ev = nullptr;   /* orders the old stream before the new one in ulb_use_stream */
   size_t bytes_live = 0;
   bool pdl = true; /* programmatic dependent launch between consecutive kernels */
   std::map<void*, size_t> user_allocs; /* buffers handed out by ulb_malloc */
@@ -86,6 +88,7 @@ struct Ctx {
   int* tc_cnt = nullptr;               /* kTcCounters arrival counters, zero between launches */
   int tp_rank = 0, tp_world = 1;
   int attn_form = 0; /* ULB_ATTN_AUTO / SPLIT / STREAM */
+  float* tree_ws = nullptr; /* split partials of ulb_tree_attention, made by its first split call */
   /* timing of the tensor-parallel all-reduces (on while a round is profiled): a CUDA event
      pair is recorded around each ncclAllReduce, events[2i] before and events[2i+1] after */
   /* host-side bound on waits for a stream holding tensor-parallel collectives (ms, 0 = none):

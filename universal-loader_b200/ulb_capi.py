@@ -15,7 +15,7 @@ LIB_PATH = os.path.join(HERE, "libulb_cuda.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "ulb.h")
 
 OK, EINVAL, ENOMEM, ECUDA, ENCCL, ETIMEOUT, EFORMAT, EUNSUPPORTED = 0, -1, -2, -3, -4, -5, -6, -7
-T_F32, T_F16, T_Q4_0, T_Q4_K = 0, 1, 2, 12
+T_F32, T_F16, T_Q4_0, T_Q4_K, T_BF16 = 0, 1, 2, 12, 30
 RNG_DRAFT, RNG_ACCEPT, RNG_RESID, RNG_FIRST = 1, 2, 3, 4
 
 P = C.c_void_p
@@ -43,6 +43,43 @@ class SpecDesc(C.Structure):
                 ("use_graphs", C.c_int), ("kv_pages", C.c_int), ("tree_width", C.c_int)]
 
 
+class CacheDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("n_layer", C.c_int), ("n_head_kv", C.c_int), ("head_dim", C.c_int),
+                ("page", C.c_int), ("n_pages", C.c_int), ("n_seq", C.c_int), ("max_pages", C.c_int),
+                ("layer_stride", C.c_int64), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("pos_stride", C.c_int64)]
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [("head_dim", C.c_int), ("rot_dim", C.c_int), ("layout", C.c_int), ("scaling", C.c_int),
+                ("base", C.c_double), ("factor", C.c_double), ("orig_len", C.c_double), ("beta_fast", C.c_double),
+                ("beta_slow", C.c_double), ("low_freq", C.c_double), ("high_freq", C.c_double),
+                ("attn_scale", C.c_double)]
+
+
+class TreeDesc(C.Structure):
+    _fields_ = [("n_head", C.c_int), ("rows", C.c_int), ("max_rows", C.c_int), ("max_len", C.c_int),
+                ("mask_words", C.c_int), ("scale", C.c_float)]
+
+
+class LogitsArgs(C.Structure):
+    _fields_ = ([(n, C.c_int) for n in ("dtype", "V", "n_seq", "rows", "max_rows", "ld_in", "ld_out", "mask_words",
+                                        "n_allow")] +
+                [(n, P) for n in ("in_", "out", "row_start", "params", "history", "history_start", "prompt",
+                                  "node_tokens", "mask", "bias_start", "bias_tokens", "bias_values", "allow",
+                                  "row_allow")])
+
+
+ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "wavelength": 4}
+_DTYPE_IDS = {"f32": T_F32, "f16": T_F16, "bf16": T_BF16}
+
+
+def dtype_id(name):
+    """The type id of "f32", "f16" or "bf16"."""
+    return _DTYPE_IDS[name]
+
+
 _SIGS = {
     "ulb_last_error": (C.c_char_p, []),
     "ulb_version": (C.c_char_p, []),
@@ -50,6 +87,24 @@ _SIGS = {
     "ulb_destroy": (C.c_int, [P]),
     "ulb_stream": (P, [P]),
     "ulb_stream_sync": (C.c_int, [P]),
+    "ulb_use_stream": (C.c_int, [P, P]),
+    "ulb_rope_create": (C.c_int, [P, C.POINTER(RopeDesc), P, C.POINTER(P)]),
+    "ulb_rope_free": (C.c_int, [P]),
+    "ulb_rope_apply": (C.c_int, [P, P, C.c_int, P, C.c_int64, C.c_int64, P, C.c_int, C.c_int, C.c_int, P,
+                                 C.c_int64, C.c_int64]),
+    "ulb_rope_append": (C.c_int, [P, P, P, C.c_int, P, C.c_int64, P, C.c_int64, P, C.c_int64, C.c_int, P, P, P, P,
+                                  C.c_int, P, P, P]),
+    "ulb_tree_attention": (C.c_int, [P, P, P, P, P, P, P, P, P, P, P, P, P]),
+    "ulb_pages_copy": (C.c_int, [P, P, P, P, P, C.c_int]),
+    "ulb_pages_compact": (C.c_int, [P, P, P, P, P, P, P, P, C.c_int]),
+    "ulb_pages_create": (C.c_int, [P, P, P, P, C.POINTER(P)]),
+    "ulb_pages_free": (C.c_int, [P]),
+    "ulb_pages_reserve": (C.c_int, [P, C.c_int, C.c_int, C.c_int]),
+    "ulb_pages_fork": (C.c_int, [P, C.c_int, C.c_int, C.c_int]),
+    "ulb_pages_truncate": (C.c_int, [P, C.c_int, C.c_int]),
+    "ulb_pages_defrag": (C.c_int, [P, C.POINTER(C.c_int)]),
+    "ulb_pages_info": (C.c_int, [P, C.POINTER(P), C.POINTER(C.c_int), C.c_int, C.POINTER(C.c_int)]),
+    "ulb_logits_process": (C.c_int, [P, P]),
     "ulb_mem_used": (C.c_int, [P, C.POINTER(C.c_size_t)]),
     "ulb_malloc": (C.c_int, [P, C.c_size_t, C.POINTER(P)]),
     "ulb_free": (C.c_int, [P, P]),
@@ -180,6 +235,7 @@ class Context:
         h = P()
         check(lib().ulb_init(device, C.byref(h)))
         self.h = h
+        self._stream = None
 
     def close(self):
         if self.h:
@@ -194,6 +250,36 @@ class Context:
 
     def sync(self):
         check(lib().ulb_stream_sync(self.h))
+
+    def use_stream(self, handle):
+        """Enqueue later calls on another stream: a cudaStream_t as an integer, 0 the legacy default
+        stream (as torch's current_stream().cuda_stream names it), None the context's own."""
+        if handle != self._stream:
+            check(lib().ulb_use_stream(self.h, None if handle is None else handle or 1))
+            self._stream = handle
+
+    # Paged cache operators (include/ulb.h).  Arrays are device addresses (integers, c_void_p, or
+    # None where the header allows NULL); everything is enqueued, nothing is waited for.
+    def tree_attention(self, cache, n_head, rows, max_rows, max_len, scale, q, k_pool, v_pool, block_table, row_start,
+                       prefix, length, mask, mask_words, out, lse=None):
+        d = TreeDesc(n_head, rows, max_rows, max_len, mask_words, scale)
+        check(lib().ulb_tree_attention(self.h, C.byref(cache), C.byref(d), q, k_pool, v_pool, block_table, row_start, prefix,
+                                       length, mask, out, lse))
+
+    def pages_copy(self, cache, k_pool, v_pool, moves, n):
+        check(lib().ulb_pages_copy(self.h, C.byref(cache), k_pool, v_pool, moves, n))
+
+    def pages_compact(self, cache, k_pool, v_pool, block_table, base, count, src, max_src):
+        check(lib().ulb_pages_compact(self.h, C.byref(cache), k_pool, v_pool, block_table, base, count, src, max_src))
+
+    def logits_process(self, dtype, logits, out, V, n_seq, rows, row_start, max_rows=None, ld_in=None, ld_out=None,
+                       params=None, history=None, history_start=None, prompt=None, node_tokens=None, words=None,
+                       n_words=0, bias_start=None, bias_tokens=None, bias_values=None, allow=None, row_allow=None,
+                       n_allow=0):
+        a = LogitsArgs(dtype, V, n_seq, rows, rows if max_rows is None else max_rows, V if ld_in is None else ld_in,
+                       V if ld_out is None else ld_out, n_words, n_allow, logits, out, row_start, params, history,
+                       history_start, prompt, node_tokens, words, bias_start, bias_tokens, bias_values, allow, row_allow)
+        check(lib().ulb_logits_process(self.h, C.byref(a)))
 
     def buffer(self, arr=None, nbytes=None):
         if arr is not None:
@@ -266,3 +352,83 @@ class Context:
         ms = C.c_float()
         check(lib().ulb_event_elapsed_ms(a, b, C.byref(ms)))
         return ms.value
+
+
+class Rope:
+    """Rotary positions of one model (ulb_rope): the handle a program keeps beside its weights."""
+
+    def __init__(self, ctx, head_dim, rot_dim=None, layout="interleaved", base=10000.0, scaling="none", factor=1.0,
+                 orig_len=0, beta_fast=32.0, beta_slow=1.0, low_freq=1.0, high_freq=4.0, attn_scale=0.0,
+                 freq_factors=None):
+        self.ctx = ctx
+        rot = head_dim if rot_dim is None else rot_dim
+        d = RopeDesc(head_dim, rot, ROPE_LAYOUTS[layout], ROPE_SCALINGS[scaling], base, factor, orig_len, beta_fast,
+                     beta_slow, low_freq, high_freq, attn_scale)
+        if freq_factors is not None:
+            freq_factors = np.ascontiguousarray(freq_factors, np.float32)
+            if freq_factors.shape != (rot // 2,):
+                raise ValueError("freq_factors holds one value a pair (%d)" % (rot // 2))
+        h = P()
+        check(lib().ulb_rope_create(ctx.h, C.byref(d), None if freq_factors is None else _ptr(freq_factors), C.byref(h)))
+        self.h = h
+
+    def apply(self, dtype, x, M, n_head, pos, out, x_row=0, x_head=0, out_row=0, out_head=0, inverse=False):
+        check(lib().ulb_rope_apply(self.ctx.h, self.h, dtype, x, x_row, x_head, pos, M, n_head, int(inverse), out, out_row,
+                                   out_head))
+
+    def append(self, cache, in_dtype, q, k, v, n_head, pos, row_seq, slot, block_table, M, q_out, k_pool, v_pool, q_row=0,
+               k_row=0, v_row=0):
+        check(lib().ulb_rope_append(self.ctx.h, self.h, C.byref(cache), in_dtype, q, q_row, k, k_row, v, v_row, n_head, pos,
+                                    row_seq, slot, block_table, M, q_out, k_pool, v_pool))
+
+    def close(self):
+        if self.h:
+            lib().ulb_rope_free(self.h)
+            self.h = None
+
+
+class Pages:
+    """The book of a cache's pages (ulb_pages): who holds which page, shared pages, the block table."""
+
+    def __init__(self, ctx, cache, k_pool, v_pool):
+        self.ctx = ctx
+        h = P()
+        check(lib().ulb_pages_create(ctx.h, C.byref(cache), k_pool, v_pool, C.byref(h)))
+        self.h = h
+
+    def reserve(self, seq, start, to):
+        check(lib().ulb_pages_reserve(self.h, seq, start, to))
+
+    def fork(self, src, dst, n):
+        check(lib().ulb_pages_fork(self.h, src, dst, n))
+
+    def truncate(self, seq, n):
+        check(lib().ulb_pages_truncate(self.h, seq, n))
+
+    def defrag(self):
+        n = C.c_int()
+        check(lib().ulb_pages_defrag(self.h, C.byref(n)))
+        return n.value
+
+    @property
+    def table(self):
+        """Device address of the block table."""
+        t = P()
+        check(lib().ulb_pages_info(self.h, C.byref(t), None, -1, None))
+        return t.value
+
+    @property
+    def free(self):
+        n = C.c_int()
+        check(lib().ulb_pages_info(self.h, None, C.byref(n), -1, None))
+        return n.value
+
+    def mapped(self, seq):
+        n = C.c_int()
+        check(lib().ulb_pages_info(self.h, None, None, seq, C.byref(n)))
+        return n.value
+
+    def close(self):
+        if self.h:
+            lib().ulb_pages_free(self.h)
+            self.h = None
