@@ -6,15 +6,19 @@
  * reads.
  *
  * One pass over the logits: each is read once and written once as fp32, HBM bounds large
- * calls.  A block owns a slice of the vocabulary of one sequence and first counts the
- * sequence's history over that slice in shared memory (integer atomics: any order gives the
- * same counts), one word a token:
- *   bit 0 seen (prompt or generated), bits 1-30 times generated, bit 31 has a bias
- * so the counts never travel through global memory and the rows of a tree, which share them,
- * count once.  Then each warp takes (row, chunk of the slice) units.  Four tokens whose words are
- * all zero and whose grammar bits are set are copied; only the others take the arithmetic.  The
- * tokens of a node's path come from the row's ancestor bits: a warp collects those that fall in
- * its chunk (mostly none) in a list of its own and adds them to the counts as it goes.
+ * calls.  A block owns a slice of the vocabulary of one sequence.  It first counts the sequence's
+ * history over that slice in shared memory (integer atomics: any order gives the same counts;
+ * bit 0 seen, bits 1-31 times generated), then turns each count into what steps 1 and 2 need,
+ * the amount to subtract (frequency n + presence), -0 for a token that was only seen and +0 for
+ * one that was not.  So the counts never travel through global memory, the rows of a tree, which
+ * share them, count once, and a logit costs one compare, one select and one FMA.  Biases get a
+ * second slice of shared memory, summed in list order, in the blocks that have any.
+ *
+ * Then each warp takes (row, chunk of the slice) units, all of a chunk's loads in flight at once,
+ * the first unit's issued before the counting.  What a node's path adds is settled apart, so that
+ * the loop over the logits stays short: the nodes whose token lies in the slice (few) are listed
+ * once a block; a unit asks its row's ancestor bits for those, computes their logits from the
+ * input, and stores them over the others' after its loop.
  */
 #include <algorithm>
 
@@ -25,11 +29,14 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kMaxNodes = 1024; /* 32 mask words */
+constexpr int kMaxSlice = 4096; /* 32 KB of counts and biases: several blocks an SM */
 
 struct LogitsGeom {
   int slice, chunk, n_slice; /* tokens a block, tokens a warp unit */
   int nodes;                 /* 32 * mask_words: nodes a row's bits can name */
 };
+/* loads of a unit in flight a lane, each of V tokens */
+constexpr int unit_loads(int V) { return V == 4 ? 4 : 8; }
 
 template <typename T, int V>
 __device__ __forceinline__ void load_logits(const T* p, float (&x)[V]) {
@@ -45,166 +52,261 @@ __device__ __forceinline__ void load_logits(const T* p, float (&x)[V]) {
   }
 }
 
-/* one token's logit: word = its count word, more = its count on the row's path */
-__device__ __forceinline__ float change(float x, uint32_t word, int more, float rep, float pres, float freq,
-                                        const ulb_logits_args& a, int b0, int b1, int tok) {
-  const int made = (int)((word & 0x7fffffffu) >> 1) + more;
-  if ((word & 1u) || made > 0) x = x > 0.f ? __fdiv_rn(x, rep) : x * rep;
-  if (made > 0) x = x - freq * (float)made - pres;
-  if (word >> 31) {
-    int lo = b0, hi = b1;
-    while (lo < hi) {
-      const int mid = lo + ((hi - lo) >> 1);
-      if (a.bias_tokens[mid] < tok) lo = mid + 1;
-      else hi = mid;
-    }
-    float b = 0.f;
-    for (; lo < b1 && a.bias_tokens[lo] == tok; ++lo) b += a.bias_values[lo];
-    x += b;
-  }
-  return x;
+/* steps 1 and 2 given what to subtract (`less`, +0: token not seen); x * (1 / rep) is within 1.5
+   ulp of x / rep, and the FMA rounds product and difference once */
+__device__ __forceinline__ float penal(float x, uint32_t less, float rep, float inv_rep) {
+  const float y = __fmaf_rn(x, x > 0.f ? inv_rep : rep, -__uint_as_float(less));
+  return less ? y : x;
+}
+/* what to subtract from a token seen before and generated `made` times */
+__device__ __forceinline__ uint32_t less_of(int made, float pres, float freq) {
+  const float f = made > 0 ? __fmaf_rn(freq, (float)made, pres) : 0.f;
+  return f == 0.f ? 0x80000000u : __float_as_uint(f);
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kWarps * 32) logits_kernel(const __grid_constant__ ulb_logits_args a, LogitsGeom g) {
+__global__ void __launch_bounds__(kWarps * 32, 3) logits_kernel(const __grid_constant__ ulb_logits_args a, LogitsGeom g) {
   pdl_wait();
   pdl_trigger();
-  extern __shared__ uint32_t sm[];
-  uint32_t* const cnt = sm;                                  /* [slice] */
-  int* const node_tok = reinterpret_cast<int*>(sm + g.slice); /* [nodes] */
+  constexpr int U = unit_loads(V);
+  extern __shared__ __align__(16) uint32_t sm[];
+  uint32_t* const less = sm;                                       /* [slice] counts, then what to subtract */
+  float* const bias = reinterpret_cast<float*>(sm + g.slice);      /* [slice], where the sequence has biases */
+  int* const node_at = reinterpret_cast<int*>(sm + 2 * g.slice);   /* [nodes] places of the nodes of this slice */
+  int* const node_id = node_at + g.nodes;                          /* [nodes] which nodes */
+  uint32_t* const node_cnt = reinterpret_cast<uint32_t*>(node_id + g.nodes); /* [nodes] their tokens' counts */
+  __shared__ int n_here;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  int* const list = node_tok + g.nodes + warp * g.nodes; /* this warp's path tokens in its chunk */
+  /* this warp's path tokens in its chunk: which listed node, its new logit */
+  int* const list = node_id + (2 + 2 * warp) * g.nodes;
+  float* const list_x = reinterpret_cast<float*>(list + g.nodes);
   const int s = blockIdx.x / g.n_slice, t0 = (blockIdx.x % g.n_slice) * g.slice;
   const int n_tok = min(g.slice, a.V - t0);
   const int r0 = max(0, a.row_start[s]), r1 = min(a.rows, a.row_start[s + 1]);
   if (r0 >= r1) return;
+  const int n_chunk = (n_tok + g.chunk - 1) / g.chunk, n_unit = n_chunk * (r1 - r0);
+  const int words = (a.V + 31) >> 5;
 
-  for (int i = tid; i < g.slice; i += kWarps * 32) cnt[i] = 0;
-  const int n_node = min(g.nodes, r1 - r0);
-  for (int i = tid; i < n_node; i += kWarps * 32) node_tok[i] = a.node_tokens[r0 + i];
+  auto allow_of = [&](int r) -> const uint32_t* {
+    if (!a.allow) return nullptr;
+    const int ai = a.row_allow ? a.row_allow[r] : r;
+    return ai >= 0 && ai < a.n_allow ? a.allow + (long long)ai * words : nullptr;
+  };
+  struct Unit {
+    int r, c0, c1; /* row, tokens [c0, c1) of the slice */
+    float x[U][V];
+    uint32_t ok[U];
+  };
+  auto load_unit = [&](int unit, Unit& n) {
+    n.r = r0 + unit / n_chunk;
+    n.c0 = (unit % n_chunk) * g.chunk;
+    n.c1 = min(n.c0 + g.chunk, n_tok);
+    const int i0 = n.c0 + lane * V;
+    const T* in = reinterpret_cast<const T*>(a.in) + (long long)n.r * a.ld_in + t0 + i0;
+    if (n.c1 - n.c0 == 32 * V * U) { /* a whole unit: no bounds */
+#pragma unroll
+      for (int u = 0; u < U; ++u) load_logits<T, V>(in + u * 32 * V, n.x[u]);
+      const uint32_t* allow = allow_of(n.r);
+      if (allow) {
+        allow += (t0 + i0) >> 5;
+#pragma unroll
+        for (int u = 0; u < U; ++u) n.ok[u] = allow[u * V] >> ((t0 + i0) & 31);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) n.ok[u] = 0xffffffffu;
+      }
+      return;
+    }
+    const uint32_t* allow = allow_of(n.r);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * 32 * V;
+      if (V == 1 || i + V <= n.c1) {
+        if (i < n.c1) load_logits<T, V>(in + u * 32 * V, n.x[u]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) n.x[u][e] = i + e < n.c1 ? to_f<T>(in[u * 32 * V + e]) : 0.f;
+      }
+      n.ok[u] = allow && i < n.c1 ? allow[(t0 + i) >> 5] >> ((t0 + i) & 31) : 0xffffffffu;
+    }
+  };
+  Unit cur;
+  int unit = warp;
+  if (unit < n_unit) load_unit(unit, cur);
+
+  /* the first tokens of the history and biases travel with them */
   const int b0 = a.bias_start ? a.bias_start[s] : 0, b1 = a.bias_start ? a.bias_start[s + 1] : 0;
+  const int h0 = a.history ? a.history_start[s] : 0, nh = a.history ? a.history_start[s + 1] - h0 : 0;
+  const int np = a.history && a.prompt ? a.prompt[s] : 0;
+  constexpr int HB = 8, HS = kWarps * 32;
+  int t[HB];
+  auto load_history = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < HB; ++u) t[u] = i0 + u * HS < nh ? a.history[(long long)h0 + i0 + u * HS] : -1;
+  };
+  load_history(tid);
+  int bt = -1, bp = -1;
+  float bv = 0.f;
+  auto load_bias = [&](int i) {
+    bt = a.bias_tokens[i];
+    bp = i > b0 ? a.bias_tokens[i - 1] : -1;
+    bv = a.bias_values[i];
+  };
+  if (b0 + tid < b1) load_bias(b0 + tid);
+  for (int i = tid * 4; i < g.slice; i += kWarps * 32 * 4) {
+    *reinterpret_cast<uint4*>(less + i) = make_uint4(0, 0, 0, 0);
+    if (b1 > b0) *reinterpret_cast<uint4*>(bias + i) = make_uint4(0, 0, 0, 0);
+  }
+  if (tid == 0) n_here = 0;
   float rep = 1.f, pres = 0.f, freq = 0.f;
   if (a.params) {
     rep = a.params[3 * s];
     pres = a.params[3 * s + 1];
     freq = a.params[3 * s + 2];
   }
+  const float inv_rep = __fdiv_rn(1.f, rep);
   __syncthreads();
-  if (a.history) {
-    const int h0 = a.history_start[s], n = a.history_start[s + 1] - h0, np = a.prompt ? a.prompt[s] : 0;
-    for (int i0 = tid; i0 < n; i0 += kWarps * 32 * 8) {
-      int t[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int i = i0 + u * kWarps * 32;
-        t[u] = i < n ? a.history[(long long)h0 + i] : -1;
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const unsigned at = (unsigned)t[u] - (unsigned)t0;
-        if (t[u] < 0 || at >= (unsigned)n_tok) continue;
-        if (i0 + u * kWarps * 32 < np) atomicOr(&cnt[at], 1u);
-        else atomicAdd(&cnt[at], 2u);
-      }
+  const int n_node = min(g.nodes, r1 - r0);
+  for (int i = tid; i < n_node; i += HS) {
+    const unsigned at = (unsigned)a.node_tokens[r0 + i] - (unsigned)t0;
+    if (at < (unsigned)n_tok) {
+      const int l = atomicAdd(&n_here, 1);
+      node_at[l] = (int)at;
+      node_id[l] = i;
     }
   }
-  for (int i = b0 + tid; i < b1; i += kWarps * 32) {
-    const unsigned at = (unsigned)a.bias_tokens[i] - (unsigned)t0;
-    if (at < (unsigned)n_tok) atomicOr(&cnt[at], 0x80000000u);
+  for (int i0 = tid; i0 < nh; i0 += HS * HB) {
+    if (i0 != tid) load_history(i0);
+#pragma unroll
+    for (int u = 0; u < HB; ++u) {
+      const unsigned at = (unsigned)t[u] - (unsigned)t0;
+      if (t[u] < 0 || at >= (unsigned)n_tok) continue;
+      if (i0 + u * HS < np) atomicOr(&less[at], 1u);
+      else atomicAdd(&less[at], 2u);
+    }
   }
+  bool biased = false;
+  for (int i = b0 + tid; i < b1; i += HS) {
+    if (i != b0 + tid) load_bias(i);
+    const unsigned at = (unsigned)bt - (unsigned)t0;
+    if (at >= (unsigned)n_tok || bp == bt) continue; /* the first of equal ids adds them */
+    for (int j = i + 1; j < b1 && a.bias_tokens[j] == bt; ++j) bv += a.bias_values[j];
+    bias[at] = bv;
+    biased = true;
+  }
+  biased = __syncthreads_or(biased);
+  const int n_at = n_here;
+  for (int l = tid; l < n_at; l += kWarps * 32) node_cnt[l] = less[node_at[l]];
+  if (n_at) __syncthreads();
+  for (int i = tid; i < n_tok; i += kWarps * 32)
+    if (const uint32_t w = less[i]) less[i] = less_of((int)(w >> 1), pres, freq);
   __syncthreads();
 
-  const int n_chunk = (n_tok + g.chunk - 1) / g.chunk;
-  const int words = (a.V + 31) >> 5;
-  for (int unit = warp; unit < n_chunk * (r1 - r0); unit += kWarps) {
-    const int r = r0 + unit / n_chunk, c0 = (unit % n_chunk) * g.chunk, c1 = min(c0 + g.chunk, n_tok);
+  while (unit < n_unit) {
+    Unit next; /* in flight while this one is worked on */
+    if (unit + kWarps < n_unit) load_unit(unit + kWarps, next);
+    const int r = cur.r, c0 = cur.c0, c1 = cur.c1;
     int n_list = 0;
-    for (int w = 0; w * 32 < n_node; ++w) {
-      const uint32_t bits = a.mask[(long long)r * a.mask_words + w];
-      const int j = w * 32 + lane;
-      const int at = j < n_node ? node_tok[j] - t0 : -1;
-      const bool hit = ((bits >> lane) & 1u) && at >= c0 && at < c1;
-      const uint32_t hits = __ballot_sync(0xffffffffu, hit);
-      if (hit) list[n_list + __popc(hits & ((1u << lane) - 1u))] = at;
-      n_list += __popc(hits);
+    if (n_at) {
+      for (int l0 = 0; l0 < n_at; l0 += 32) {
+        const int l = l0 + lane;
+        bool hit = false;
+        if (l < n_at) {
+          const int at = node_at[l], j = node_id[l];
+          hit = at >= c0 && at < c1 && ((a.mask[(long long)r * a.mask_words + (j >> 5)] >> (j & 31)) & 1u);
+        }
+        const uint32_t hits = __ballot_sync(0xffffffffu, hit);
+        if (hit) list[n_list + __popc(hits & ((1u << lane) - 1u))] = l;
+        n_list += __popc(hits);
+      }
+      __syncwarp();
+      const uint32_t* const allow = n_list ? allow_of(r) : nullptr;
+      for (int l = lane; l < n_list; l += 32) {
+        const int at = node_at[list[l]], tok = t0 + at;
+        const uint32_t w = node_cnt[list[l]];
+        int made = (int)(w >> 1);
+        for (int m = 0; m < n_list; ++m) made += node_at[list[m]] == at;
+        float y = penal(to_f<T>(reinterpret_cast<const T*>(a.in)[(long long)r * a.ld_in + tok]), less_of(made, pres, freq), rep, inv_rep);
+        if (biased) y += bias[at];
+        if (allow && !((allow[tok >> 5] >> (tok & 31)) & 1u)) y = -INFINITY;
+        list_x[l] = y;
+      }
+      __syncwarp();
     }
-    __syncwarp();
-    const uint32_t* allow = nullptr;
-    if (a.allow) {
-      const int ai = a.row_allow ? a.row_allow[r] : r;
-      if (ai >= 0 && ai < a.n_allow) allow = a.allow + (long long)ai * words;
-    }
-    const T* in = reinterpret_cast<const T*>(a.in) + (long long)r * a.ld_in + t0;
-    float* out = a.out + (long long)r * a.ld_out + t0;
-    constexpr int U = V == 1 ? 8 : 4; /* loads in flight */
-    for (int i0 = c0 + lane * V; i0 < c1; i0 += 32 * V * U) {
-      float x[U][V];
-      uint32_t ok[U];
+    float* const out = a.out + (long long)r * a.ld_out + t0;
+    const bool whole = c1 - c0 == 32 * V * U;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * 32 * V;
-        if (i < c1) {
-          if (V == 1 || i + V <= c1) {
-            load_logits<T, V>(in + i, x[u]);
-          } else {
+    for (int u = 0; u < U; ++u) {
+      const int i = c0 + (u * 32 + lane) * V;
+      if (!whole && i >= c1) continue;
+      float(&x)[V] = cur.x[u];
+      uint32_t w[V];
+      if constexpr (V == 4) {
+        const uint4 q = *reinterpret_cast<const uint4*>(less + i); /* past n_tok: zero */
+        w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+      } else {
+        w[0] = less[i];
+      }
+      uint32_t any = 0;
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[u][e] = i + e < c1 ? to_f<T>(in[i + e]) : 0.f;
-          }
-          ok[u] = allow ? allow[(t0 + i) >> 5] >> ((t0 + i) & 31) : 0xffffffffu;
+      for (int e = 0; e < V; ++e) any |= w[e];
+      if (any) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] = penal(x[e], w[e], rep, inv_rep);
+      }
+      if (biased) {
+        if constexpr (V == 4) {
+          const float4 f = *reinterpret_cast<const float4*>(bias + i);
+          x[0] += f.x; x[1] += f.y; x[2] += f.z; x[3] += f.w;
+        } else {
+          x[0] += bias[i];
         }
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * 32 * V;
-        if (i >= c1) continue;
-        uint32_t any = 0;
-#pragma unroll
-        for (int e = 0; e < V; ++e) any |= i + e < c1 ? cnt[i + e] : 0u;
-        if (any || n_list) {
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            if (i + e >= c1) continue;
-            int more = 0;
-            for (int l = 0; l < n_list; ++l) more += list[l] == i + e;
-            x[u][e] = change(x[u][e], cnt[i + e], more, rep, pres, freq, a, b0, b1, t0 + i + e);
-          }
-        }
+      for (int e = 0; e < V; ++e)
+        if (!((cur.ok[u] >> e) & 1u)) x[e] = -INFINITY;
+      if (V == 1) {
+        out[i] = x[0];
+      } else if (whole || i + V <= c1) {
+        *reinterpret_cast<float4*>(out + i) = make_float4(x[0], x[1 % V], x[2 % V], x[3 % V]);
+      } else {
 #pragma unroll
         for (int e = 0; e < V; ++e)
-          if (!((ok[u] >> e) & 1u)) x[u][e] = -INFINITY;
-        if (V == 1) {
-          out[i] = x[u][0];
-        } else if (i + V <= c1) {
-          *reinterpret_cast<float4*>(out + i) = make_float4(x[u][0], x[u][1 % V], x[u][2 % V], x[u][3 % V]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (i + e < c1) out[i + e] = x[u][e];
-        }
+          if (i + e < c1) out[i + e] = x[e];
       }
     }
-    __syncwarp(); /* the list is this unit's */
+    if (n_list) {
+      __syncwarp();
+      for (int l = lane; l < n_list; l += 32) out[node_at[list[l]]] = list_x[l];
+      __syncwarp();
+    }
+    unit += kWarps;
+    cur = next;
   }
 }
 
 template <typename T, int V>
 int launch_logits(Ctx* c, const ulb_logits_args& a) {
-  /* slices: about four blocks an SM over the whole call, at least 128 tokens a warp, at most 64 KB of counts */
-  const long long want = (long long)c->n_sm * 4;
+  /* slices: trees (eight rows or more) about six waves of three blocks an SM, so that the last
+     one wastes little; fewer rows, which do not pay for many countings, larger ones: a unit a warp */
+  const long long want = (long long)c->n_sm * 18;
   long long slice = ((long long)a.V * a.n_seq + want - 1) / want;
-  slice = std::min<long long>(std::max<long long>((slice + 1023) / 1024 * 1024, 1024), 16384);
+  const long long least = a.max_rows >= kWarps ? 512 : 1024;
+  slice = std::min<long long>(std::max<long long>((slice + 511) / 512 * 512, least), kMaxSlice);
   LogitsGeom g;
   g.slice = (int)std::min<long long>(slice, (a.V + 127) / 128 * 128);
   g.n_slice = (a.V + g.slice - 1) / g.slice;
-  g.chunk = a.max_rows >= kWarps ? 1024 : std::min(1024, std::max(128, (g.slice * a.max_rows / kWarps + 127) / 128 * 128));
+  /* a unit: what a lane's loads cover, less when a sequence has too few rows for every warp */
+  const int full = 32 * V * unit_loads(V);
+  g.chunk = a.max_rows >= kWarps ? full : std::min(full, std::max(128, (g.slice * a.max_rows / kWarps + 127) / 128 * 128));
   g.nodes = a.node_tokens ? 32 * a.mask_words : 0;
-  const size_t smem = (size_t)(g.slice + g.nodes * (1 + kWarps)) * 4;
+  const size_t smem = (size_t)(2 * g.slice + g.nodes * (3 + 2 * kWarps)) * 4;
   const long long blocks = (long long)g.n_slice * a.n_seq;
   ULB_CHECK(blocks < (1ll << 31), ULB_EUNSUPPORTED, "ulb_logits_process: %d sequences of %d tokens", a.n_seq, a.V);
   static bool attr = false;
   if (!attr) {
     ULB_CUDA(cudaFuncSetAttribute(logits_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  (16384 + kMaxNodes * (1 + kWarps)) * 4));
+                                  (2 * kMaxSlice + kMaxNodes * (3 + 2 * kWarps)) * 4));
     attr = true;
   }
   ULB_LAUNCH("logits launch", launch_k(c, logits_kernel<T, V>, dim3((unsigned)blocks), dim3(kWarps * 32), smem, a, g));
