@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) logits_kernel(const __grid_con
 #pragma unroll
     for (int u = 0; u < HB; ++u) {
       const unsigned at = (unsigned)t[u] - (unsigned)t0;
-      if (t[u] < 0 || at >= (unsigned)n_tok) continue;
+      if (at >= (unsigned)n_tok) continue; /* -1 too: t0 and n_tok are small */
       if (i0 + u * HS < np) atomicOr(&less[at], 1u);
       else atomicAdd(&less[at], 2u);
     }
@@ -198,8 +198,15 @@ __global__ void __launch_bounds__(kWarps * 32, 3) logits_kernel(const __grid_con
   const int n_at = n_here;
   for (int l = tid; l < n_at; l += kWarps * 32) node_cnt[l] = less[node_at[l]];
   if (n_at) __syncthreads();
-  for (int i = tid; i < n_tok; i += kWarps * 32)
-    if (const uint32_t w = less[i]) less[i] = less_of((int)(w >> 1), pres, freq);
+  for (int i = tid * 4; i < n_tok; i += HS * 4) {
+    uint4 w = *reinterpret_cast<const uint4*>(less + i);
+    if (!(w.x | w.y | w.z | w.w)) continue;
+    if (w.x) w.x = less_of((int)(w.x >> 1), pres, freq);
+    if (w.y) w.y = less_of((int)(w.y >> 1), pres, freq);
+    if (w.z) w.z = less_of((int)(w.z >> 1), pres, freq);
+    if (w.w) w.w = less_of((int)(w.w >> 1), pres, freq);
+    *reinterpret_cast<uint4*>(less + i) = w;
+  }
   __syncthreads();
 
   while (unit < n_unit) {
@@ -291,8 +298,9 @@ int launch_logits(Ctx* c, const ulb_logits_args& a) {
      one wastes little; fewer rows, which do not pay for many countings, larger ones: a unit a warp */
   const long long want = (long long)c->n_sm * 18;
   long long slice = ((long long)a.V * a.n_seq + want - 1) / want;
-  const long long least = a.max_rows >= kWarps ? 512 : 1024;
-  slice = std::min<long long>(std::max<long long>((slice + 511) / 512 * 512, least), kMaxSlice);
+  if (a.max_rows >= kWarps) slice = (slice + 511) / 512 * 512;
+  else slice = slice <= 1024 ? 1024 : kMaxSlice;
+  slice = std::min<long long>(slice, kMaxSlice);
   LogitsGeom g;
   g.slice = (int)std::min<long long>(slice, (a.V + 127) / 128 * 128);
   g.n_slice = (a.V + g.slice - 1) / g.slice;
