@@ -21,7 +21,7 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 CUDA_HOME = os.path.dirname(os.path.dirname(NVCC))
 
 CU_SOURCES = ["runtime.cu", "qgemv.cu", "qgemm_tc.cu", "attention.cu", "sampling.cu", "model.cu", "spec.cu",
-              "rope.cu", "tree_attention.cu", "pages.cu", "logits.cu"]
+              "rope.cu", "tree_attention.cu", "tree_attention_tc.cu", "pages.cu", "logits.cu"]
 CUDA_LIB = os.path.join(PKG, "libulb_cuda.so")
 BUILD_TRACE = os.path.join(PKG, "_build_trace")
 CUDA_LIB_TRACE = os.path.join(PKG, "libulb_cuda_trace.so")

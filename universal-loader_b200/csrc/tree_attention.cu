@@ -536,6 +536,8 @@ extern "C" int ulb_tree_attention(ulb_ctx* ctx, const ulb_cache_desc* cache, con
   a.rows = d->rows;
   a.max_rows = std::min(d->max_rows, d->rows);
   a.max_len = std::min(d->max_len, a.g.max_pages * a.g.page);
+  ULB_CHECK((long long)a.max_rows * a.G < (1ll << 31) && (long long)d->rows * d->n_head < (1ll << 31), ULB_EUNSUPPORTED,
+            "ulb_tree_attention: %d rows of %d heads", d->rows, d->n_head);
   ULB_CHECK(a.max_len <= 0x7fff0000, ULB_EUNSUPPORTED, "ulb_tree_attention: %d positions", a.max_len);
   a.words = d->mask_words;
   a.scale2 = d->scale * kLog2e;
@@ -552,6 +554,7 @@ extern "C" int ulb_tree_attention(ulb_ctx* ctx, const ulb_cache_desc* cache, con
   a.err = ctx->c.dev_err;
   Ctx* c = &ctx->c;
   ULB_CUDA(cudaSetDevice(c->device));
+  if (a.g.hd == 64 || a.g.hd == 128) return launch_tree_tc(c, a, cache->dtype == ULB_TYPE_F16);
   return cache->dtype == ULB_TYPE_F16 ? pick_dim<__half>(c, a) : pick_dim<__nv_bfloat16>(c, a);
 }
 

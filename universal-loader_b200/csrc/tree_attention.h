@@ -60,6 +60,9 @@ __device__ __forceinline__ float ex2(float x) {
 }
 #endif
 
+/* the tensor-core form (tree_attention_tc.cu): head dims 64 and 128 */
+int launch_tree_tc(Ctx* c, TreeArgs& a, bool f16);
+
 /* floats of split partials a context holds for this operator (128 MiB) */
 constexpr size_t kTreeWsFloats = (size_t)32 << 20;
 

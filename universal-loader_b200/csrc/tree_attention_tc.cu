@@ -1,0 +1,824 @@
+/*
+ * tree_attention_tc.cu — ulb_tree_attention on the 5th-generation tensor cores, for head
+ * dims 64 and 128.  Same mathematics and masking as tree_attention.cu.
+ *
+ * A CTA works on 128-key tiles with M = 128 query rows a stream, two streams at a time, each
+ * with its own running (m, l, o) and its own softmax warpgroup (one thread a row):
+ *   PAIR = false  (at most 128 queries a kv head): both streams hold the same rows and take the
+ *                 even and the odd tiles; they join in shared memory at the end
+ *   PAIR = true   (more): the streams hold neighbouring tiles of 128 rows and share every K / V
+ *                 tile, which halves what shared memory and L2 have to deliver
+ * so that one stream's products run while the other stream's weights are computed.  Per tile:
+ * S = Q K^T (tcgen05.mma, both operands in shared memory, fp32 in TMEM); the row's thread reads
+ * S, updates m and l, writes P (rounded to the cache's type) over S in TMEM; O += P V with P read
+ * from TMEM and V as the tile TMA wrote it (keys x hd, the MN-major operand).  O stays in TMEM; it
+ * is rescaled only when a row's maximum has grown by more than 2^8 since the last time (weights
+ * stay below 2^8, sums are fp32, so the result is the same ratio).
+ *
+ * Warps: 0 TMA (pages -> 128-byte-swizzled tiles, one box a page, pages that are unmapped or past
+ * the end read as zero through an out-of-range coordinate), 1 issues every MMA and the commits
+ * that free tiles, 2 - 3 take V elements that are not finite out of masked tiles, 4 - 7 and 8 - 11
+ * softmax.  Four barriers carry it: K / V tiles full and free, S full, P full; S full of a tile
+ * implies that the stream's previous O += P V is complete, because one thread issues in order.
+ *
+ * Work is cut evenly: the tiles of all (sequence, kv head) pairs form one line, every CTA (group
+ * of CTAs, when more than 256 rows need several row tiles: its members walk the same keys side by
+ * side, so K / V come from HBM once) takes an equal stretch of it, whatever the lengths, and
+ * walks whole sequences and pieces of two.  A pair that falls into several stretches leaves one
+ * partial a stretch, joined by a small kernel.
+ *
+ * Every mbarrier wait has a deadline (2 s): past it a role raises bit 3 of the device error word
+ * and stops issuing work; the CTA still waits (bounded) for its MMAs before freeing TMEM.
+ */
+#include "tree_attention.h"
+
+#include <cuda.h>
+
+#include <algorithm>
+#include <mutex>
+
+namespace ulb {
+namespace {
+
+constexpr int TK = 128;        /* keys a tile */
+constexpr int kThreads = 384;  /* 4 role warps, 2 x 4 softmax warps */
+constexpr int kMinTiles = 4;     /* tiles a group takes at least */
+constexpr int kJoinRows = 8;   /* rows a block of the join kernel: a warp each */
+
+__device__ __forceinline__ uint32_t sa(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint64_t gtime() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ void mb_init(uint64_t* b, uint32_t n) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sa(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void mb_expect(uint64_t* b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(sa(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mb_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sa(b)) : "memory");
+}
+__device__ __forceinline__ bool mb_try(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(ok) : "r"(sa(b)), "r"(parity) : "memory");
+  return ok != 0;
+}
+/* wait for the phase with this parity; false once 2 s have passed */
+__device__ __forceinline__ bool mb_wait(uint64_t* b, uint32_t parity) {
+  if (mb_try(b, parity)) return true;
+  const uint64_t end = gtime() + 2000000000ull;
+  while (!mb_try(b, parity))
+    if (gtime() > end) return false;
+  return true;
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint64_t* b) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sa(b)) : "memory");
+}
+__device__ __forceinline__ void tma4(void* dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+               ::"r"(sa(dst)), "l"(m), "r"(x), "r"(y), "r"(z), "r"(w), "r"(sa(bar)) : "memory");
+}
+/* D (TMEM) (+)= A (shared) B (shared) and D (+)= A (TMEM) B (shared), K = 16 */
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u) : "memory");
+}
+/* 32 consecutive columns of the thread's TMEM lane */
+__device__ __forceinline__ void tm_ld(uint32_t t, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+                 "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+                 "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+               : "r"(t));
+}
+__device__ __forceinline__ void tm_st(uint32_t t, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+               ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+               "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+               "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+               "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(t) : "memory");
+}
+__device__ __forceinline__ void tm_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+/* the 256 softmax threads */
+__device__ __forceinline__ void sync_softmax() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+/* shared-memory descriptors of 128-byte-swizzled tiles (rows of 64 elements, 8-row groups 1024 bytes
+   apart): K-major (Q, K: a row is an index of M or N, its 64 elements 64 of hd), and MN-major
+   (V: a row is a key = K index, its 64 elements 64 of N; the next 64 of N one half tile on) */
+__device__ __forceinline__ uint64_t desc_k(uint32_t s) {
+  return (uint64_t)((s >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t s) {
+  return (uint64_t)((s >> 4) & 0x3FFFu) | ((uint64_t)((TK * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+         ((uint64_t)2 << 61);
+}
+/* byte of 16-byte chunk c (of 8) of row r in a half tile */
+__device__ __forceinline__ uint32_t sw128(int r, int c) { return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4)); }
+
+template <int HD, bool PAIR>
+struct TcCfg {
+  static constexpr int TILE = TK * HD * 2;            /* K, V or Q tile bytes */
+  static constexpr int NQ = PAIR ? 2 : 1;
+  static constexpr int NK = HD == 64 ? 6 : 3;         /* K tiles in the ring */
+  static constexpr int NV = HD == 64 ? 5 : PAIR ? 2 : 3;
+  static constexpr int SMEM = (NQ + NK + NV) * TILE + 1024; /* + alignment slack */
+  static constexpr int RT = PAIR ? 256 : 128;         /* queries a CTA */
+  static constexpr int JP = HD + 4;                   /* floats a row when the streams join */
+  static_assert(SMEM <= 227 * 1024 - 1024 && 128 * JP * 4 <= (NK + NV) * TILE, "shared memory");
+};
+
+/* what the launch adds to TreeArgs */
+struct TcPlan {
+  int members, groups_max; /* CTAs that walk the same keys side by side, such groups in the grid */
+  int min_tiles;           /* tiles a group takes at least */
+  struct TcTail* tail;     /* [groups][members] */
+};
+/* the head of a pair that goes on in the next groups: what the join kernel needs */
+struct TcTail {
+  int pieces, slot, r0, nq, q0, kvh, pad0, pad1; /* pieces 0: none */
+};
+
+/* the line of tiles */
+struct Line {
+  long long total;
+  int groups;
+  __device__ __forceinline__ long long begin(int c) const { return total * c / groups; }
+};
+__device__ __forceinline__ long long seq_tiles(const TreeArgs& a, const TcPlan& p, const TreeSeq& q, int RT, int* n_tile, int* n_pass) {
+  *n_tile = max(1, (q.len + TK - 1) / TK);
+  *n_pass = (int)(((long long)q.n * a.G + (long long)RT * p.members - 1) / ((long long)RT * p.members));
+  return (long long)*n_tile * *n_pass * a.g.n_head_kv;
+}
+
+struct Piece {
+  TreeSeq q;
+  int s, kvh, q0, nq; /* sequence, kv head, first query (row x group + head) of the tile, queries in it */
+  int t0, n, n_tile;  /* tiles [t0, t0 + n) of n_tile */
+  long long first;    /* place of the pair's first tile on the line */
+  bool head;          /* the stretch's first piece */
+};
+
+/* walks the pieces of one CTA; every role runs the same walk */
+template <int RT>
+struct Walk {
+  long long at, end, base;
+  int s, n_tile, n_pass, member;
+  long long cnt, start;
+  TreeSeq q;
+  __device__ __forceinline__ void load(const TreeArgs& a, const TcPlan& p) {
+    q = tree_seq(a, s);
+    cnt = seq_tiles(a, p, q, RT, &n_tile, &n_pass);
+  }
+  __device__ __forceinline__ bool next(const TreeArgs& a, const TcPlan& p, Piece* o) {
+    while (at < end) {
+      while (at >= base + cnt) { /* ends: at < end <= total */
+        base += cnt;
+        ++s;
+        load(a, p);
+      }
+      const long long u = (at - base) / n_tile;
+      o->t0 = (int)((at - base) - u * n_tile);
+      o->n = (int)min((long long)(n_tile - o->t0), end - at);
+      o->head = at == start;
+      o->first = base + u * n_tile;
+      at += o->n;
+      o->kvh = (int)(u / n_pass);
+      o->q0 = ((int)(u % n_pass) * p.members + member) * RT;
+      o->nq = min(RT, q.n * a.G - o->q0);
+      if (o->nq <= 0) continue; /* this member has no rows of the sequence */
+      o->q = q;
+      o->s = s;
+      o->n_tile = n_tile;
+      return true;
+    }
+    return false;
+  }
+};
+
+/* which of positions [pos, pos + 32) row i sees; pages says which 16-position blocks of the tile are
+   mapped, rel = pos within the tile */
+__device__ __forceinline__ uint32_t sees32(const TreeArgs& a, const TreeSeq& q, int i, int pos, uint32_t blocks, int rel) {
+  uint32_t v = 0xffffffffu;
+  if (a.words == 0) {
+    const int n = q.len - q.n + i - pos + 1;
+    v = n <= 0 ? 0u : n >= 32 ? v : (1u << n) - 1u;
+  } else {
+    const int j = pos - q.prefix;
+    if (j > -32) {
+      const uint32_t* m = a.mask + (long long)(q.r0 + i) * a.words;
+      const int w = j >> 5;
+      const uint32_t lo = w < 0 ? 0xffffffffu : w < a.words ? m[w] : 0u;
+      const uint32_t hi = w + 1 < a.words ? m[w + 1] : 0u;
+      v = __funnelshift_r(lo, hi, j & 31);
+    }
+  }
+  const int left = q.len - pos;
+  if (left < 32) v &= left <= 0 ? 0u : (1u << left) - 1u;
+  const uint32_t b = blocks >> (rel >> 4);
+  if (!(b & 1u)) v &= 0xffff0000u;
+  if (!(b & 2u)) v &= 0x0000ffffu;
+  return v;
+}
+
+template <typename T, int HD, bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1)
+    tree_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ TreeArgs a,
+                   const __grid_constant__ TcPlan p) {
+  using C = TcCfg<HD, PAIR>;
+  constexpr bool F16 = std::is_same<T, __half>::value;
+  constexpr uint32_t FMT = F16 ? 0u : (1u << 7) | (1u << 10);
+  constexpr uint32_t ID_S = (1u << 4) | FMT | ((TK >> 3) << 17) | ((128 >> 4) << 24);
+  constexpr uint32_t ID_O = (1u << 4) | FMT | (1u << 16) | ((HD >> 3) << 17) | ((128 >> 4) << 24);
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t k_full[C::NK], k_free[C::NK], v_full[C::NV], v_free[C::NV], v_clean[C::NV], s_full[2], p_full[2], o_full[2], q_full, mma_done;
+  __shared__ uint32_t tmem_sh;
+  __shared__ int odd_v, sh_s;
+  __shared__ long long sh_base, sh_sum[kThreads / 32 + 1];
+  __shared__ float sh_ml[2][128];
+  uint8_t* const sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* const q_sm = sm;
+  uint8_t* const k_sm = sm + C::NQ * C::TILE;
+  uint8_t* const v_sm = k_sm + C::NK * C::TILE;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  pdl_wait();
+  pdl_trigger();
+  /* the line's length, then this group's place on it */
+  auto tiles_of = [&](int s) {
+    int nt, np;
+    return seq_tiles(a, p, tree_seq(a, s), C::RT, &nt, &np);
+  };
+  long long mine = 0;
+  for (int s = tid; s < a.g.n_seq; s += kThreads) mine += tiles_of(s);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) sh_sum[warp] = mine;
+  __syncthreads();
+  Line line;
+  line.total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) line.total += sh_sum[w];
+  line.groups = (int)min((long long)p.groups_max, max(1ll, (line.total + p.min_tiles - 1) / p.min_tiles));
+  const int grp = blockIdx.x / p.members, member = blockIdx.x % p.members;
+  if (grp >= line.groups || line.total == 0) {
+    if (tid == 0) p.tail[blockIdx.x].pieces = 0;
+    return;
+  }
+  const long long begin = line.begin(grp), end = line.begin(grp + 1);
+  {
+    long long base = 0;
+    for (int s0 = 0; s0 < a.g.n_seq; s0 += kThreads) { /* the sequence that holds `begin` */
+      const int s = s0 + tid;
+      const long long c = s < a.g.n_seq ? tiles_of(s) : 0;
+      long long x = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      __syncthreads();
+      if (lane == 31) sh_sum[warp] = x;
+      __syncthreads();
+      long long all = 0;
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) x += sh_sum[w];
+        all += sh_sum[w];
+      }
+      const long long b = base + x - c;
+      if (c > 0 && b <= begin && begin < b + c) {
+        sh_s = s;
+        sh_base = b;
+      }
+      base += all;
+      if (base > begin) break; /* the same for every thread */
+    }
+  }
+  if (tid == 0) {
+    for (int i = 0; i < C::NK; ++i) { mb_init(&k_full[i], 1); mb_init(&k_free[i], 1); }
+    for (int i = 0; i < C::NV; ++i) { mb_init(&v_full[i], 1); mb_init(&v_free[i], 3); mb_init(&v_clean[i], 2); }
+    for (int i = 0; i < 2; ++i) { mb_init(&s_full[i], 1); mb_init(&p_full[i], 4); mb_init(&o_full[i], 1); }
+    mb_init(&q_full, 8);
+    mb_init(&mma_done, 1);
+    odd_v = 0;
+    p.tail[blockIdx.x].pieces = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sa(&tmem_sh)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = tmem_sh;
+  Walk<C::RT> walk;
+  walk.at = walk.start = begin;
+  walk.end = end;
+  walk.s = sh_s;
+  walk.base = sh_base;
+  walk.member = member;
+  walk.load(a, p);
+  Piece pc = {};
+  bool ok = true;
+  /* stream X's tiles of a piece of n: PAIR all of them (none without rows), else every second */
+  auto n_of = [&](int X) { return PAIR ? (X == 0 || pc.nq > 128 ? pc.n : 0) : (pc.n + 1 - X) >> 1; };
+
+  if (warp == 0) {
+    /* ------------------------------------------------ TMA: K and V tiles in the order of their use */
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    uint32_t ck = 0, cv = 0; /* tiles issued */
+    const int rows = min(a.g.page, TK), boxes = TK / rows;
+    while (ok && walk.next(a, p, &pc)) {
+      auto load = [&](const CUtensorMap* m, uint8_t* ring, uint64_t* full, uint64_t* free, uint32_t& c, int nring, int t) {
+        const int slot = c % nring;
+        if (c >= (uint32_t)nring && !mb_wait(&free[slot], ((c / nring) - 1) & 1)) { ok = false; return; }
+        const int pos = (pc.t0 + t) * TK;
+        int page = a.g.n_pages; /* out of range: zeros */
+        if (lane < boxes && pos + lane * rows < pc.q.len) {
+          const int j = (pos + lane * rows) >> a.g.page_shift;
+          const int x = j < a.g.max_pages ? a.table[(long long)pc.s * a.g.max_pages + j] : -1;
+          if (x >= 0 && x < a.g.n_pages) page = x;
+        }
+        if (lane == 0) mb_expect(&full[slot], (uint32_t)C::TILE);
+        __syncwarp();
+        if (lane < boxes) {
+          uint8_t* d = ring + slot * C::TILE + lane * rows * 128;
+#pragma unroll
+          for (int h = 0; h < HD / 64; ++h) tma4(d + h * TK * 128, m, h * 64, pos & (a.g.page - 1), pc.kvh, page, &full[slot]);
+        }
+        ++c;
+      };
+      auto K = [&](int t) { if (ok) load(&mk, k_sm, k_full, k_free, ck, C::NK, t); };
+      auto V = [&](int t) { if (ok) load(&mv, v_sm, v_full, v_free, cv, C::NV, t); };
+      if (PAIR) {
+        for (int t = 0; t < pc.n && ok; ++t) { K(t); V(t); }
+      } else {
+        K(0);
+        if (pc.n > 1) K(1);
+        for (int t = 0; t < pc.n && ok; ++t) {
+          V(t);
+          if (t + 2 < pc.n) K(t + 2);
+        }
+      }
+    }
+    /* no copy is in flight when the CTA ends, whatever happened */
+    for (uint32_t c = ck > (uint32_t)C::NK ? ck - C::NK : 0; c < ck; ++c) ok &= mb_wait(&k_full[c % C::NK], (c / C::NK) & 1);
+    for (uint32_t c = cv > (uint32_t)C::NV ? cv - C::NV : 0; c < cv; ++c) ok &= mb_wait(&v_full[c % C::NV], (c / C::NV) & 1);
+    __syncwarp();
+  } else if (warp == 1) {
+    /* ------------------------------------------------ MMA issue (one lane) */
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (lane == 0) {
+      uint32_t ck = 0, cv = 0, nq = 0, np[2] = {0, 0};
+      while (ok && walk.next(a, p, &pc)) {
+        if (!mb_wait(&q_full, nq++ & 1)) { ok = false; break; }
+        const int nt[2] = {n_of(0), n_of(1)};
+        const int open = tree_open(a, pc.q);
+        /* K / V tiles are used in order; PAIR uses each twice, so stream 1 looks at the one stream 0 took */
+        auto qk = [&](int X, bool take) {
+          const uint32_t c = take ? ck : ck - 1;
+          const int slot = c % C::NK;
+          if (take) {
+            if (!mb_wait(&k_full[slot], (c / C::NK) & 1)) { ok = false; return; }
+            ++ck;
+          }
+          tc_after();
+          const uint32_t q0 = sa(q_sm + (PAIR ? X : 0) * C::TILE), k0 = sa(k_sm + slot * C::TILE);
+#pragma unroll
+          for (int i = 0; i < HD / 16; ++i) {
+            const uint32_t off = (i >> 2) * (TK * 128) + (i & 3) * 32;
+            mma_ss(tmem + X * 128, desc_k(q0 + off), desc_k(k0 + off), ID_S, i > 0);
+          }
+          commit(&s_full[X]);
+          if (!PAIR || X == 1 || nt[1] == 0) commit(&k_free[slot]);
+        };
+        auto pv = [&](int X, int i, bool take) {
+          const uint32_t c = take ? cv : cv - 1;
+          const int slot = c % C::NV;
+          if (take) {
+            const int t = PAIR ? i : 2 * i + X;
+            const bool masked = (pc.t0 + t + 1) * TK > min(open, pc.q.len);
+            if (!mb_wait(masked ? &v_clean[slot] : &v_full[slot], (c / C::NV) & 1)) { ok = false; return; }
+            ++cv;
+          }
+          if (!mb_wait(&p_full[X], np[X]++ & 1)) { ok = false; return; }
+          tc_after();
+          const uint32_t v0 = sa(v_sm + slot * C::TILE);
+#pragma unroll
+          for (int k = 0; k < TK / 16; ++k)
+            mma_ts(tmem + 256 + X * HD, tmem + X * 128 + k * 8, desc_mn(v0 + k * 2048), ID_O, i > 0 || k > 0);
+          if (!PAIR || X == 1 || nt[1] == 0) commit(&v_free[slot]);
+        };
+        qk(0, true);
+        if (ok && nt[1]) qk(1, !PAIR);
+        for (int i = 0; i < nt[0] && ok; ++i) {
+          pv(0, i, true);
+          if (ok && i + 1 < nt[0]) qk(0, true);
+          if (i + 1 == nt[0] && ok) commit(&o_full[0]);
+          if (ok && i < nt[1]) {
+            pv(1, i, !PAIR);
+            if (ok && i + 1 < nt[1]) qk(1, !PAIR);
+            if (i + 1 == nt[1] && ok) commit(&o_full[1]);
+          }
+        }
+      }
+      /* everything issued completes before TMEM is freed */
+      commit(&mma_done);
+      if (!mb_wait(&mma_done, 0)) ok = false;
+    }
+    __syncwarp();
+  } else if (warp < 4) {
+    /* ------------------------------------------------ V elements that are not finite, in masked tiles */
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    uint32_t cv = 0;
+    while (ok && walk.next(a, p, &pc)) {
+      const int clear = min(tree_open(a, pc.q), pc.q.len);
+      for (int t = 0; t < pc.n; ++t, ++cv) {
+        const int slot = cv % C::NV;
+        if (!mb_wait(&v_full[slot], (cv / C::NV) & 1)) { ok = false; break; }
+        if ((pc.t0 + t + 1) * TK > clear) {
+          uint4* v = reinterpret_cast<uint4*>(v_sm + slot * C::TILE);
+          constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+          bool any = false;
+          for (int i = tid - 64; i < C::TILE / 16; i += 64) {
+            uint4 x = v[i];
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            bool hit = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if ((w[e] & E) == E) { w[e] &= 0xffff0000u; hit = true; }
+              if (((w[e] >> 16) & E) == E) { w[e] &= 0x0000ffffu; hit = true; }
+            }
+            if (hit) v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            any |= hit;
+          }
+          if (any) odd_v = 1;
+          fence_async();
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mb_arrive(&v_clean[slot]);
+          mb_arrive(&v_free[slot]);
+        }
+      }
+    }
+  } else {
+    /* ------------------------------------------------ softmax: one thread a row */
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    const int X = (warp - 4) >> 2, row = tid - 128 - X * 128; /* stream, row of its tile = TMEM lane */
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + X * 128, to = tmem + lanes + 256 + X * HD;
+    constexpr int n_blk = TK / 16; /* 16-position blocks of a tile */
+    uint32_t ns = 0, no = 0;
+    while (walk.next(a, p, &pc)) {
+      /* Q of this CTA's rows, swizzled; rows past the tile's queries are zero */
+      for (int i = tid - 128; i < C::NQ * 128 * (HD / 8); i += 256) {
+        const int r = i / (HD / 8), ch = i % (HD / 8), qi = pc.q0 + r;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < pc.nq)
+          x = *reinterpret_cast<const uint4*>((const T*)a.q + ((long long)(pc.q.r0 + qi / a.G) * a.H + pc.kvh * a.G + qi % a.G) * HD + ch * 8);
+        *reinterpret_cast<uint4*>(q_sm + (r >> 7) * C::TILE + (ch >> 3) * (TK * 128) + sw128(r & 127, ch & 7)) = x;
+      }
+      fence_async();
+      __syncwarp();
+      if (lane == 0) mb_arrive(&q_full);
+
+      const int r = (PAIR ? X * 128 : 0) + row, qi = pc.q0 + r;
+      const bool live = r < pc.nq, warp_live = r - lane < pc.nq;
+      const int ri = live ? qi / a.G : 0;
+      const int n = n_of(X), open = tree_open(a, pc.q);
+      float m = -INFINITY, l = 0.f; /* m: the maximum that weights are taken against */
+      for (int i = 0; i < n && ok; ++i) {
+        const int t = pc.t0 + (PAIR ? i : 2 * i + X), pos = t * TK;
+        /* which 16-position blocks of the tile are mapped */
+        bool here = true;
+        if (lane < n_blk && pos + lane * 16 < pc.q.len) {
+          const int j = (pos >> a.g.page_shift) + (((pos & (a.g.page - 1)) + lane * 16) >> a.g.page_shift);
+          const int x = j < a.g.max_pages ? a.table[(long long)pc.s * a.g.max_pages + j] : -1;
+          here = x >= 0 && x < a.g.n_pages;
+        }
+        const uint32_t blocks = __ballot_sync(0xffffffffu, here);
+        if (!mb_wait(&s_full[X], ns++ & 1)) { ok = false; break; }
+        tc_after();
+        if (warp_live) {
+          uint32_t sr[TK];
+#pragma unroll
+          for (int c = 0; c < TK; c += 32) tm_ld(ts + c, sr + c);
+          tm_ld_wait();
+          if ((t + 1) * TK > open || pos + TK > pc.q.len || blocks != 0xffffffffu) {
+#pragma unroll
+            for (int c = 0; c < TK; c += 32) {
+              const uint32_t see = sees32(a, pc.q, ri, pos + c, blocks, c);
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!((see >> e) & 1u)) sr[c + e] = 0xff800000u; /* -inf */
+            }
+          }
+          float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < TK; c += 4) {
+            x0 = fmaxf(x0, __uint_as_float(sr[c]));
+            x1 = fmaxf(x1, __uint_as_float(sr[c + 1]));
+            x2 = fmaxf(x2, __uint_as_float(sr[c + 2]));
+            x3 = fmaxf(x3, __uint_as_float(sr[c + 3]));
+          }
+          const float top = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * a.scale2;
+          const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float f = grow ? (m == -INFINITY ? 0.f : ex2(m - top)) : 1.f;
+            if (grow) m = top;
+            l *= f;
+            if (i > 0) { /* the first product overwrites O */
+              uint32_t or_[32];
+#pragma unroll
+              for (int c = 0; c < HD; c += 32) {
+                tm_ld(to + c, or_);
+                tm_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) or_[e] = __float_as_uint(__uint_as_float(or_[e]) * f);
+                tm_st(to + c, or_);
+              }
+            }
+          }
+          const float u = m == -INFINITY ? 0.f : m;
+          float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
+#pragma unroll
+          for (int c = 0; c < TK; c += 4) {
+            const float p0 = ex2(__fmaf_rn(__uint_as_float(sr[c]), a.scale2, -u));
+            const float p1 = ex2(__fmaf_rn(__uint_as_float(sr[c + 1]), a.scale2, -u));
+            const float p2 = ex2(__fmaf_rn(__uint_as_float(sr[c + 2]), a.scale2, -u));
+            const float p3 = ex2(__fmaf_rn(__uint_as_float(sr[c + 3]), a.scale2, -u));
+            l0 += p0;
+            l1 += p1;
+            l2 += p2;
+            l3 += p3;
+            sr[c / 2] = pack2<T>(p0, p1);
+            sr[c / 2 + 1] = pack2<T>(p2, p3);
+          }
+          l += (l0 + l1) + (l2 + l3);
+          tm_st(ts, sr);
+          tm_st(ts + 32, sr + 32);
+          tm_st_wait();
+        }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mb_arrive(&p_full[X]);
+      }
+      /* ---- the piece's end */
+      if (n > 0 && ok && !mb_wait(&o_full[X], no++ & 1)) ok = false;
+      tc_after();
+      const bool whole = pc.n == pc.n_tile;
+      const int slot = pc.head ? 0 : 1;
+      if (!whole && pc.t0 == 0 && tid == 128) { /* the head of a pair that goes on in the next groups */
+        TcTail& tl = p.tail[blockIdx.x];
+        const int last = (int)(((pc.first + pc.n_tile) * line.groups - 1) / line.total);
+        tl.slot = slot;
+        tl.r0 = pc.q.r0;
+        tl.nq = pc.nq;
+        tl.q0 = pc.q0;
+        tl.kvh = pc.kvh;
+        tl.pieces = last - grp + 1;
+      }
+      float o[HD];
+      if (n > 0 && warp_live && ok) {
+#pragma unroll
+        for (int c = 0; c < HD; c += 32) tm_ld(to + c, reinterpret_cast<uint32_t*>(o) + c);
+        tm_ld_wait();
+      } else {
+#pragma unroll
+        for (int c = 0; c < HD; ++c) o[c] = 0.f;
+      }
+      tc_before();
+      /* values taken out of masked tiles go to the rows that see them */
+      if (odd_v && live && ok) {
+        const T* qr = (const T*)a.q + ((long long)(pc.q.r0 + ri) * a.H + pc.kvh * a.G + qi % a.G) * HD;
+        const int from = max(pc.t0 * TK, min(open, pc.q.len) / TK * TK), upto = min(pc.q.len, (pc.t0 + pc.n) * TK);
+        for (int pos = from; pos < upto; ++pos) {
+          if (!PAIR && ((pos / TK - pc.t0) & 1) != X) continue;
+          const int j = pos >> a.g.page_shift;
+          const int pg = j < a.g.max_pages ? a.table[(long long)pc.s * a.g.max_pages + j] : -1;
+          if (pg < 0 || pg >= a.g.n_pages || !tree_sees(a, pc.q, ri, pos)) continue;
+          const long long off = pg * a.g.pstride + (pos & (a.g.page - 1)) * a.g.pos + pc.kvh * a.g.head;
+          const T *kr = (const T*)a.k + off, *vr = (const T*)a.v + off;
+          float s = 0.f;
+          bool hit = false;
+#pragma unroll 1
+          for (int e = 0; e < HD; ++e) {
+            s = __fmaf_rn(to_f<T>(qr[e]), to_f<T>(kr[e]), s);
+            hit |= !isfinite(to_f<T>(vr[e]));
+          }
+          if (!hit) continue;
+          const float w = ex2(__fmaf_rn(s, a.scale2, -(m == -INFINITY ? 0.f : m)));
+#pragma unroll
+          for (int d = 0; d < HD; ++d) {
+            const float x = to_f<T>(vr[d]);
+            if (!isfinite(x)) o[d] += w * x;
+          }
+        }
+      }
+      if (!PAIR) {
+        /* stream 1 hands its rows to stream 0, half of hd at a time, in the Q tile (every product that
+           read it is complete); float4 c of all rows side by side: no bank conflicts */
+        float4* const hand = reinterpret_cast<float4*>(q_sm);
+        sync_softmax();
+        if (X == 1) {
+          sh_ml[0][row] = m;
+          sh_ml[1][row] = l;
+        }
+        float f0 = 1.f, f1 = 0.f;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (X == 1) {
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+              const int d = half * (HD / 2) + c * 4;
+              hand[c * 128 + row] = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+            }
+          }
+          sync_softmax();
+          if (X == 0) {
+            if (half == 0) {
+              const float m1 = sh_ml[0][row], top = fmaxf(m, m1), u = top == -INFINITY ? 0.f : top;
+              f0 = ex2(m - u);
+              f1 = ex2(m1 - u);
+              l = l * f0 + sh_ml[1][row] * f1;
+              m = top;
+            }
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+              const int d = half * (HD / 2) + c * 4;
+              const float4 y = hand[c * 128 + row];
+              o[d] = o[d] * f0 + y.x * f1;
+              o[d + 1] = o[d + 1] * f0 + y.y * f1;
+              o[d + 2] = o[d + 2] * f0 + y.z * f1;
+              o[d + 3] = o[d + 3] * f0 + y.w * f1;
+            }
+          }
+          sync_softmax();
+        }
+      }
+      if (PAIR) sync_softmax(); /* both streams are through: Q may be replaced */
+      if (live && ok && (PAIR || X == 0)) {
+        const long long at = (long long)(pc.q.r0 + ri) * a.H + pc.kvh * a.G + qi % a.G;
+        if (whole) {
+          const float inv = l == 0.f ? 0.f : __fdividef(1.f, l); /* 0: the row sees nothing */
+#pragma unroll
+          for (int c = 0; c < HD; c += 8)
+            *reinterpret_cast<uint4*>((T*)a.out + at * HD + c) =
+                make_uint4(pack2<T>(o[c] * inv, o[c + 1] * inv), pack2<T>(o[c + 2] * inv, o[c + 3] * inv),
+                           pack2<T>(o[c + 4] * inv, o[c + 5] * inv), pack2<T>(o[c + 6] * inv, o[c + 7] * inv));
+          if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+        } else {
+          const long long ps = ((long long)blockIdx.x * 2 + slot) * C::RT + r;
+#pragma unroll
+          for (int c = 0; c < HD; c += 4) __stcg(reinterpret_cast<float4*>(a.po + ps * HD + c), make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]));
+          __stcg(reinterpret_cast<float2*>(a.pml + ps * 2), make_float2(m, l));
+        }
+      }
+    }
+  }
+  tc_before();
+  __syncthreads();
+  if (!ok && lane == 0) atomicOr(a.err, 8);
+  if (warp == 1) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+/* join the pieces of a pair that several groups worked on: a warp a row, pieces in order */
+template <typename T, int HD>
+__global__ void __launch_bounds__(kJoinRows * 32) tree_tc_join_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ TcPlan p, int RT) {
+  pdl_wait();
+  pdl_trigger();
+  const TcTail t = p.tail[blockIdx.x];
+  const int r = blockIdx.y * kJoinRows + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (t.pieces == 0 || r >= t.nq) return;
+  auto place = [&](int i) { return ((long long)(blockIdx.x + i * p.members) * 2 + (i == 0 ? t.slot : 0)) * RT + r; };
+  float M = -INFINITY;
+  for (int i = lane; i < t.pieces; i += 32) M = fmaxf(M, __ldcg(a.pml + place(i) * 2));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const float U = M == -INFINITY ? 0.f : M;
+  constexpr int E = HD / 32;
+  float x[E] = {}, L = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < t.pieces; ++i) {
+    const long long at = place(i);
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.pml + at * 2));
+    float y[E];
+    if constexpr (E == 4) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.po + at * HD + lane * 4));
+      y[0] = v.x; y[1] = v.y; y[2] = v.z; y[3] = v.w;
+    } else {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(a.po + at * HD + lane * 2));
+      y[0] = v.x; y[1] = v.y;
+    }
+    const float f = ex2(ml.x - U);
+    L += ml.y * f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] += y[e] * f;
+  }
+  const float inv = L == 0.f ? 0.f : __fdividef(1.f, L);
+  const int qi = t.q0 + r;
+  const long long at = (long long)(t.r0 + qi / a.G) * a.H + t.kvh * a.G + qi % a.G;
+  T* out = (T*)a.out + at * HD + lane * E;
+  if constexpr (E == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv));
+  else *reinterpret_cast<uint32_t*>(out) = pack2<T>(x[0] * inv, x[1] * inv);
+  if (lane == 0 && a.lse) a.lse[at] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled() {
+  static std::once_flag once;
+  static EncodeTiledFn fn = nullptr;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      fn = (EncodeTiledFn)f;
+  });
+  return fn;
+}
+
+/* K or V pool as [page][head][position][hd], a box = 64 of hd x the positions of a page in a tile */
+int pool_map(const TreeArgs& a, bool f16, const void* pool, CUtensorMap* m) {
+  EncodeTiledFn enc = encode_tiled();
+  ULB_CHECK(enc, ULB_ECUDA, "ulb_tree_attention: no cuTensorMapEncodeTiled entry point");
+  const CacheGeom& g = a.g;
+  const cuuint64_t dim[4] = {(cuuint64_t)g.hd, (cuuint64_t)g.page, (cuuint64_t)g.n_head_kv, (cuuint64_t)g.n_pages};
+  const cuuint64_t str[3] = {(cuuint64_t)g.pos * 2, (cuuint64_t)g.head * 2, (cuuint64_t)g.pstride * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)std::min(g.page, TK), 1, 1}, es[4] = {1, 1, 1, 1};
+  const CUresult r = enc(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(pool), dim, str,
+                         box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  ULB_CHECK(r == CUDA_SUCCESS, ULB_EINVAL, "ulb_tree_attention: the cache's layout has no tensor map (CUresult %d)", (int)r);
+  return ULB_OK;
+}
+
+template <typename T, int HD, bool PAIR>
+int launch_tc(Ctx* c, TreeArgs& a) {
+  using C = TcCfg<HD, PAIR>;
+  static bool attr = false;
+  if (!attr) {
+    ULB_CUDA(cudaFuncSetAttribute(tree_tc_kernel<T, HD, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    attr = true;
+  }
+  CUtensorMap mk, mv;
+  constexpr bool f16 = std::is_same<T, __half>::value;
+  ULB_TRY(pool_map(a, f16, a.k, &mk));
+  ULB_TRY(pool_map(a, f16, a.v, &mv));
+  TcPlan p;
+  const long long tiles = ((long long)a.max_rows * a.G + C::RT - 1) / C::RT;
+  p.members = (int)std::min<long long>(tiles, c->n_sm);
+  p.groups_max = c->n_sm / p.members;
+  p.min_tiles = kMinTiles;
+  const int grid = p.groups_max * p.members;
+  if (!c->tree_ws) ULB_CUDA(cudaMalloc((void**)&c->tree_ws, kTreeWsFloats * sizeof(float)));
+  const size_t rows = (size_t)grid * 2 * C::RT;
+  ULB_CHECK(rows * (HD + 2) + (size_t)grid * 8 <= kTreeWsFloats, ULB_EUNSUPPORTED, "ulb_tree_attention: workspace for %d SMs", c->n_sm);
+  a.po = c->tree_ws;
+  a.pml = a.po + rows * HD;
+  p.tail = reinterpret_cast<TcTail*>(a.pml + rows * 2);
+  ULB_LAUNCH("tree attention launch", launch_k(c, tree_tc_kernel<T, HD, PAIR>, dim3(grid), dim3(kThreads), C::SMEM, mk, mv, a, p));
+  /* a launch that one group covers leaves nothing to join */
+  const long long most = (long long)a.g.n_seq * a.g.n_head_kv * std::max(1, (a.max_len + TK - 1) / TK) *
+                         ((tiles + p.members - 1) / p.members);
+  if (most > p.min_tiles && p.groups_max > 1)
+    ULB_LAUNCH("tree join launch", launch_k(c, tree_tc_join_kernel<T, HD>, dim3(grid, C::RT / kJoinRows), dim3(kJoinRows * 32), 0, a, p, C::RT));
+  return ULB_OK;
+}
+
+template <typename T>
+int pick_tc(Ctx* c, TreeArgs& a) {
+  const bool pair = (long long)a.max_rows * a.G > 128;
+  if (a.g.hd == 64) return pair ? launch_tc<T, 64, true>(c, a) : launch_tc<T, 64, false>(c, a);
+  return pair ? launch_tc<T, 128, true>(c, a) : launch_tc<T, 128, false>(c, a);
+}
+
+}  // namespace
+
+int launch_tree_tc(Ctx* c, TreeArgs& a, bool f16) { return f16 ? pick_tc<__half>(c, a) : pick_tc<__nv_bfloat16>(c, a); }
+
+}  // namespace ulb
+
+ULB_TRACE_UNIT(tree_attention_tc)
