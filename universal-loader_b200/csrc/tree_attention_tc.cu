@@ -2,13 +2,16 @@
  * tree_attention_tc.cu — ulb_tree_attention on the 5th-generation tensor cores, for head
  * dims 64 and 128.  Same mathematics and masking as tree_attention.cu.
  *
- * A CTA works on 128-key tiles with M = 128 query rows a stream, two streams at a time, each
+ * A CTA works on 64-key tiles with M = 128 query rows a stream, two streams at a time, each
  * with its own running (m, l, o) and its own softmax warpgroup (one thread a row):
  *   PAIR = false  (at most 128 queries a kv head): both streams hold the same rows and take the
  *                 even and the odd tiles; they join in shared memory at the end
  *   PAIR = true   (more): the streams hold neighbouring tiles of 128 rows and share every K / V
  *                 tile, which halves what shared memory and L2 have to deliver
- * so that one stream's products run while the other stream's weights are computed.  Per tile:
+ * so that one stream's products run while the other stream's weights are computed.  Each stream has
+ * two score buffers, so the next tile's scores are there when a tile's weights are done: the
+ * exponentials, not the round trip between tensor cores and softmax, set the pace (with 128-key
+ * tiles and one buffer a stream the largest case took 323 us).  Per tile:
  * S = Q K^T (tcgen05.mma, both operands in shared memory, fp32 in TMEM); the row's thread reads
  * S, updates m and l, writes P (rounded to the cache's type) over S in TMEM; O += P V with P read
  * from TMEM and V as the tile TMA wrote it (keys x hd, the MN-major operand).  O stays in TMEM; it
@@ -18,8 +21,9 @@
  * Warps: 0 TMA (pages -> 128-byte-swizzled tiles, one box a page, pages that are unmapped or past
  * the end read as zero through an out-of-range coordinate), 1 issues every MMA and the commits
  * that free tiles, 2 - 3 take V elements that are not finite out of masked tiles, 4 - 7 and 8 - 11
- * softmax.  Four barriers carry it: K / V tiles full and free, S full, P full; S full of a tile
- * implies that the stream's previous O += P V is complete, because one thread issues in order.
+ * softmax.  Barriers carry it: K / V tiles full and free, S full, P full, O += P V done (waited for
+ * only to rescale O and at the end); MMAs issued by one thread complete in order, so a score buffer
+ * is free for the next scores once the product that reads its weights has been issued.
  *
  * Work is cut evenly: the tiles of all (sequence, kv head) pairs form one line, every CTA (group
  * of CTAs, when more than 256 rows need several row tiles: its members walk the same keys side by
@@ -40,9 +44,10 @@
 namespace ulb {
 namespace {
 
-constexpr int TK = 128;        /* keys a tile */
+constexpr int TK = 64;         /* keys a tile */
+constexpr int TQ = 128;        /* query rows a stream: M */
 constexpr int kThreads = 384;  /* 4 role warps, 2 x 4 softmax warps */
-constexpr int kMinTiles = 4;     /* tiles a group takes at least */
+constexpr int kMinTiles = 8;     /* tiles a group takes at least */
 constexpr int kJoinRows = 8;   /* rows a block of the join kernel: a warp each */
 
 __device__ __forceinline__ uint32_t sa(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -74,6 +79,8 @@ __device__ __forceinline__ bool mb_wait(uint64_t* b, uint32_t parity) {
     if (gtime() > end) return false;
   return true;
 }
+/* the same for a converged warp, one answer for all lanes */
+__device__ __forceinline__ bool mb_wait_warp(uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, mb_wait(b, parity)); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -83,6 +90,14 @@ __device__ __forceinline__ void commit(uint64_t* b) {
 __device__ __forceinline__ void tma4(void* dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                ::"r"(sa(dst)), "l"(m), "r"(x), "r"(y), "r"(z), "r"(w), "r"(sa(bar)) : "memory");
+}
+/* one lane of a converged warp: the compiler knows that what the branch holds runs once, and keeps
+   the operands of tcgen05 instructions in uniform registers (under `lane == 0` each MMA took about
+   70 cycles to issue) */
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
 }
 /* D (TMEM) (+)= A (shared) B (shared) and D (+)= A (TMEM) B (shared), K = 16 */
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -133,14 +148,14 @@ __device__ __forceinline__ uint32_t sw128(int r, int c) { return (uint32_t)((r >
 
 template <int HD, bool PAIR>
 struct TcCfg {
-  static constexpr int TILE = TK * HD * 2;            /* K, V or Q tile bytes */
+  static constexpr int TILE = TK * HD * 2;            /* bytes of a K or V tile */
+  static constexpr int QTILE = TQ * HD * 2;
   static constexpr int NQ = PAIR ? 2 : 1;
-  static constexpr int NK = HD == 64 ? 6 : 3;         /* K tiles in the ring */
-  static constexpr int NV = HD == 64 ? 5 : PAIR ? 2 : 3;
-  static constexpr int SMEM = (NQ + NK + NV) * TILE + 1024; /* + alignment slack */
+  static constexpr int NK = HD == 64 ? 8 : PAIR ? 5 : 6; /* K tiles in the ring: five are in use or next in turn */
+  static constexpr int NV = HD == 64 ? 8 : PAIR ? 5 : 6;
+  static constexpr int SMEM = NQ * QTILE + (NK + NV) * TILE + 1024; /* + alignment slack */
   static constexpr int RT = PAIR ? 256 : 128;         /* queries a CTA */
-  static constexpr int JP = HD + 4;                   /* floats a row when the streams join */
-  static_assert(SMEM <= 227 * 1024 - 1024 && 128 * JP * 4 <= (NK + NV) * TILE, "shared memory");
+  static_assert(SMEM <= 226 * 1024, "shared memory");
 };
 
 /* what the launch adds to TreeArgs */
@@ -246,14 +261,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr uint32_t ID_S = (1u << 4) | FMT | ((TK >> 3) << 17) | ((128 >> 4) << 24);
   constexpr uint32_t ID_O = (1u << 4) | FMT | (1u << 16) | ((HD >> 3) << 17) | ((128 >> 4) << 24);
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t k_full[C::NK], k_free[C::NK], v_full[C::NV], v_free[C::NV], v_clean[C::NV], s_full[2], p_full[2], o_full[2], q_full, mma_done;
+  __shared__ uint64_t k_full[C::NK], k_free[C::NK], v_full[C::NV], v_free[C::NV], v_clean[C::NV], s_full[2][2], p_full[2][2], o_done[2][2], q_full, mma_done;
   __shared__ uint32_t tmem_sh;
   __shared__ int odd_v, sh_s;
   __shared__ long long sh_base, sh_sum[kThreads / 32 + 1];
   __shared__ float sh_ml[2][128];
   uint8_t* const sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* const q_sm = sm;
-  uint8_t* const k_sm = sm + C::NQ * C::TILE;
+  uint8_t* const k_sm = sm + C::NQ * C::QTILE;
   uint8_t* const v_sm = k_sm + C::NK * C::TILE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -313,7 +328,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < C::NK; ++i) { mb_init(&k_full[i], 1); mb_init(&k_free[i], 1); }
     for (int i = 0; i < C::NV; ++i) { mb_init(&v_full[i], 1); mb_init(&v_free[i], 3); mb_init(&v_clean[i], 2); }
-    for (int i = 0; i < 2; ++i) { mb_init(&s_full[i], 1); mb_init(&p_full[i], 4); mb_init(&o_full[i], 1); }
+    for (int i = 0; i < 2; ++i) {
+      for (int b = 0; b < 2; ++b) { mb_init(&s_full[i][b], 1); mb_init(&p_full[i][b], 4); mb_init(&o_done[i][b], 1); }
+    }
     mb_init(&q_full, 8);
     mb_init(&mma_done, 1);
     odd_v = 0;
@@ -342,7 +359,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     /* ------------------------------------------------ TMA: K and V tiles in the order of their use */
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     uint32_t ck = 0, cv = 0; /* tiles issued */
     const int rows = min(a.g.page, TK), boxes = TK / rows;
     while (ok && walk.next(a, p, &pc)) {
@@ -367,15 +383,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto K = [&](int t) { if (ok) load(&mk, k_sm, k_full, k_free, ck, C::NK, t); };
       auto V = [&](int t) { if (ok) load(&mv, v_sm, v_full, v_free, cv, C::NV, t); };
-      if (PAIR) {
-        for (int t = 0; t < pc.n && ok; ++t) { K(t); V(t); }
-      } else {
-        K(0);
-        if (pc.n > 1) K(1);
-        for (int t = 0; t < pc.n && ok; ++t) {
-          V(t);
-          if (t + 2 < pc.n) K(t + 2);
-        }
+      constexpr int AHEAD = PAIR ? 2 : 4; /* K tiles whose scores are asked for before the first V tile */
+      for (int t = 0; t < min(AHEAD, pc.n); ++t) K(t);
+      for (int t = 0; t < pc.n && ok; ++t) {
+        V(t);
+        if (t + AHEAD < pc.n) K(t + AHEAD);
       }
     }
     /* no copy is in flight when the CTA ends, whatever happened */
@@ -383,70 +395,82 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (uint32_t c = cv > (uint32_t)C::NV ? cv - C::NV : 0; c < cv; ++c) ok &= mb_wait(&v_full[c % C::NV], (c / C::NV) & 1);
     __syncwarp();
   } else if (warp == 1) {
-    /* ------------------------------------------------ MMA issue (one lane) */
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    if (lane == 0) {
-      uint32_t ck = 0, cv = 0, nq = 0, np[2] = {0, 0};
-      while (ok && walk.next(a, p, &pc)) {
-        if (!mb_wait(&q_full, nq++ & 1)) { ok = false; break; }
-        const int nt[2] = {n_of(0), n_of(1)};
-        const int open = tree_open(a, pc.q);
-        /* K / V tiles are used in order; PAIR uses each twice, so stream 1 looks at the one stream 0 took */
-        auto qk = [&](int X, bool take) {
-          const uint32_t c = take ? ck : ck - 1;
-          const int slot = c % C::NK;
-          if (take) {
-            if (!mb_wait(&k_full[slot], (c / C::NK) & 1)) { ok = false; return; }
-            ++ck;
-          }
-          tc_after();
-          const uint32_t q0 = sa(q_sm + (PAIR ? X : 0) * C::TILE), k0 = sa(k_sm + slot * C::TILE);
-#pragma unroll
-          for (int i = 0; i < HD / 16; ++i) {
-            const uint32_t off = (i >> 2) * (TK * 128) + (i & 3) * 32;
-            mma_ss(tmem + X * 128, desc_k(q0 + off), desc_k(k0 + off), ID_S, i > 0);
-          }
-          commit(&s_full[X]);
-          if (!PAIR || X == 1 || nt[1] == 0) commit(&k_free[slot]);
-        };
-        auto pv = [&](int X, int i, bool take) {
-          const uint32_t c = take ? cv : cv - 1;
-          const int slot = c % C::NV;
-          if (take) {
-            const int t = PAIR ? i : 2 * i + X;
-            const bool masked = (pc.t0 + t + 1) * TK > min(open, pc.q.len);
-            if (!mb_wait(masked ? &v_clean[slot] : &v_full[slot], (c / C::NV) & 1)) { ok = false; return; }
-            ++cv;
-          }
-          if (!mb_wait(&p_full[X], np[X]++ & 1)) { ok = false; return; }
-          tc_after();
-          const uint32_t v0 = sa(v_sm + slot * C::TILE);
-#pragma unroll
-          for (int k = 0; k < TK / 16; ++k)
-            mma_ts(tmem + 256 + X * HD, tmem + X * 128 + k * 8, desc_mn(v0 + k * 2048), ID_O, i > 0 || k > 0);
-          if (!PAIR || X == 1 || nt[1] == 0) commit(&v_free[slot]);
-        };
-        qk(0, true);
-        if (ok && nt[1]) qk(1, !PAIR);
-        for (int i = 0; i < nt[0] && ok; ++i) {
-          pv(0, i, true);
-          if (ok && i + 1 < nt[0]) qk(0, true);
-          if (i + 1 == nt[0] && ok) commit(&o_full[0]);
-          if (ok && i < nt[1]) {
-            pv(1, i, !PAIR);
-            if (ok && i + 1 < nt[1]) qk(1, !PAIR);
-            if (i + 1 == nt[1] && ok) commit(&o_full[1]);
-          }
+    /* ------------------------------------------------ MMA issue (the warp walks, one elected lane issues) */
+    /* one thread feeds the tensor cores, so its loop is kept short: descriptors are a base plus
+       a constant, ring places and phases are counted, not divided */
+    uint32_t ks = 0, kp = 0, vs = 0, vp = 0; /* next K / V tile of the ring and its phase */
+    uint32_t kcur = 0, vcur = 0;             /* the tile stream 0 took last */
+    uint32_t qp = 0, pp = 0;                 /* phases of q_full, and of p_full[X][b] in bit 2 X + b */
+    const uint64_t dq = desc_k(sa(q_sm)), dk = desc_k(sa(k_sm)), dv = desc_mn(sa(v_sm));
+    while (ok && walk.next(a, p, &pc)) {
+      if (!mb_wait_warp(&q_full, qp)) { ok = false; break; }
+      qp ^= 1;
+      const int n0 = n_of(0), n1 = n_of(1);
+      /* first tile that some row does not see whole */
+      const int clear = min(tree_open(a, pc.q), pc.q.len) / TK - pc.t0;
+      /* K / V tiles are used in order; PAIR uses each twice, stream 1 the one that stream 0 took last */
+      auto qk = [&](auto x, int b) {
+        constexpr int X = decltype(x)::value;
+        if (!PAIR || X == 0) {
+          if (!mb_wait_warp(&k_full[ks], kp)) { ok = false; return; }
+          kcur = ks;
+          if (++ks == C::NK) { ks = 0; kp ^= 1; }
         }
+        tc_after();
+        if (elect()) {
+          const uint64_t q0 = dq + (PAIR ? X * (C::QTILE >> 4) : 0), k0 = dk + kcur * (C::TILE >> 4);
+#pragma unroll
+          for (int j = 0; j < HD / 16; ++j)
+            mma_ss(tmem + X * 128 + b * TK, q0 + (((j >> 2) * (TQ * 128) + (j & 3) * 32) >> 4),
+                   k0 + (((j >> 2) * (TK * 128) + (j & 3) * 32) >> 4), ID_S, j > 0);
+          commit(&s_full[X][b]);
+          if (!PAIR || X == 1 || n1 == 0) commit(&k_free[kcur]);
+        }
+        __syncwarp();
+      };
+      auto pv = [&](auto x, int i) {
+        constexpr int X = decltype(x)::value;
+        const int b = i & 1;
+        if (!PAIR || X == 0) {
+          /* v_full first: it says that the slot's earlier phases, v_clean's too, are over */
+          if (!mb_wait_warp(&v_full[vs], vp)) { ok = false; return; }
+          if ((PAIR ? i : 2 * i + X) >= clear && !mb_wait_warp(&v_clean[vs], vp)) { ok = false; return; }
+          vcur = vs;
+          if (++vs == C::NV) { vs = 0; vp ^= 1; }
+        }
+        if (!mb_wait_warp(&p_full[X][b], (pp >> (2 * X + b)) & 1)) { ok = false; return; }
+        pp ^= 1u << (2 * X + b);
+        tc_after();
+        if (elect()) {
+          const uint64_t v0 = dv + vcur * (C::TILE >> 4);
+          const uint32_t d = tmem + 256 + X * HD, pa = tmem + X * 128 + b * TK;
+          mma_ts(d, pa, v0, ID_O, i > 0);
+#pragma unroll
+          for (int j = 1; j < TK / 16; ++j) mma_ts(d, pa + j * 8, v0 + ((j * 2048) >> 4), ID_O, 1);
+          commit(&o_done[X][b]);
+          if (!PAIR || X == 1 || n1 == 0) commit(&v_free[vcur]);
+        }
+        __syncwarp();
+      };
+      constexpr std::integral_constant<int, 0> S0{};
+      constexpr std::integral_constant<int, 1> S1{};
+      qk(S0, 0); /* a piece has a tile, and stream 0 the first */
+      if (ok && n1 > 0) qk(S1, 0);
+      if (ok && n0 > 1) qk(S0, 1);
+      if (ok && n1 > 1) qk(S1, 1);
+      for (int i = 0; i < n0 && ok; ++i) {
+        pv(S0, i);
+        if (ok && i + 2 < n0) qk(S0, i & 1);
+        if (ok && i < n1) pv(S1, i);
+        if (ok && i + 2 < n1) qk(S1, i & 1);
       }
-      /* everything issued completes before TMEM is freed */
-      commit(&mma_done);
-      if (!mb_wait(&mma_done, 0)) ok = false;
     }
+    /* everything issued completes before TMEM is freed */
+    if (elect()) commit(&mma_done);
     __syncwarp();
+    if (!mb_wait_warp(&mma_done, 0)) ok = false;
   } else if (warp < 4) {
     /* ------------------------------------------------ V elements that are not finite, in masked tiles */
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     uint32_t cv = 0;
     while (ok && walk.next(a, p, &pc)) {
       const int clear = min(tree_open(a, pc.q), pc.q.len);
@@ -481,20 +505,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     /* ------------------------------------------------ softmax: one thread a row */
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int X = (warp - 4) >> 2, row = tid - 128 - X * 128; /* stream, row of its tile = TMEM lane */
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + X * 128, to = tmem + lanes + 256 + X * HD;
+    const uint32_t to = tmem + lanes + 256 + X * HD;
     constexpr int n_blk = TK / 16; /* 16-position blocks of a tile */
-    uint32_t ns = 0, no = 0;
+    uint32_t ns[2] = {0, 0}; /* tiles seen a buffer: phases of its s_full, p_full and o_done */
     while (walk.next(a, p, &pc)) {
       /* Q of this CTA's rows, swizzled; rows past the tile's queries are zero */
-      for (int i = tid - 128; i < C::NQ * 128 * (HD / 8); i += 256) {
+      for (int i = tid - 128; i < C::NQ * TQ * (HD / 8); i += 256) {
         const int r = i / (HD / 8), ch = i % (HD / 8), qi = pc.q0 + r;
         uint4 x = make_uint4(0, 0, 0, 0);
         if (r < pc.nq)
           x = *reinterpret_cast<const uint4*>((const T*)a.q + ((long long)(pc.q.r0 + qi / a.G) * a.H + pc.kvh * a.G + qi % a.G) * HD + ch * 8);
-        *reinterpret_cast<uint4*>(q_sm + (r >> 7) * C::TILE + (ch >> 3) * (TK * 128) + sw128(r & 127, ch & 7)) = x;
+        *reinterpret_cast<uint4*>(q_sm + (r >> 7) * C::QTILE + (ch >> 3) * (TQ * 128) + sw128(r & 127, ch & 7)) = x;
       }
       fence_async();
       __syncwarp();
@@ -504,18 +527,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool live = r < pc.nq, warp_live = r - lane < pc.nq;
       const int ri = live ? qi / a.G : 0;
       const int n = n_of(X), open = tree_open(a, pc.q);
+      /* the page of a position: -1 past the end, -2 unmapped */
+      auto page_at = [&](int pos) {
+        if (pos >= pc.q.len) return -1;
+        const int j = pos >> a.g.page_shift;
+        const int x = j < a.g.max_pages ? a.table[(long long)pc.s * a.g.max_pages + j] : -1;
+        return x >= 0 && x < a.g.n_pages ? x : -2;
+      };
+      bool holes = false; /* some page of the piece is unmapped */
+      for (long long q = (long long)pc.t0 * TK + lane * a.g.page; q < (long long)(pc.t0 + pc.n) * TK + a.g.page; q += 32 * a.g.page)
+        holes |= q < pc.q.len && page_at((int)q) == -2;
+      holes = __any_sync(0xffffffffu, holes);
       float m = -INFINITY, l = 0.f; /* m: the maximum that weights are taken against */
       for (int i = 0; i < n && ok; ++i) {
         const int t = pc.t0 + (PAIR ? i : 2 * i + X), pos = t * TK;
-        /* which 16-position blocks of the tile are mapped */
-        bool here = true;
-        if (lane < n_blk && pos + lane * 16 < pc.q.len) {
-          const int j = (pos >> a.g.page_shift) + (((pos & (a.g.page - 1)) + lane * 16) >> a.g.page_shift);
-          const int x = j < a.g.max_pages ? a.table[(long long)pc.s * a.g.max_pages + j] : -1;
-          here = x >= 0 && x < a.g.n_pages;
-        }
-        const uint32_t blocks = __ballot_sync(0xffffffffu, here);
-        if (!mb_wait(&s_full[X], ns++ & 1)) { ok = false; break; }
+        uint32_t blocks = 0xffffffffu; /* which 16-position blocks of the tile are mapped */
+        if (holes) blocks = __ballot_sync(0xffffffffu, lane >= n_blk || page_at(pos + lane * 16) != -2);
+        const int b = i & 1;
+        const uint32_t ts = tmem + lanes + X * 128 + b * TK;
+        if (!mb_wait(&s_full[X][b], (b ? ns[1]++ : ns[0]++) & 1)) { ok = false; break; }
         tc_after();
         if (warp_live) {
           uint32_t sr[TK];
@@ -546,6 +576,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (grow) m = top;
             l *= f;
             if (i > 0) { /* the first product overwrites O */
+              if (!mb_wait(&o_done[X][b ^ 1], ((b ? ns[0] : ns[1]) - 1) & 1)) ok = false;
+              tc_after();
               uint32_t or_[32];
 #pragma unroll
               for (int c = 0; c < HD; c += 32) {
@@ -574,15 +606,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           l += (l0 + l1) + (l2 + l3);
           tm_st(ts, sr);
-          tm_st(ts + 32, sr + 32);
           tm_st_wait();
         }
         tc_before();
         __syncwarp();
-        if (lane == 0) mb_arrive(&p_full[X]);
+        if (lane == 0) mb_arrive(&p_full[X][b]);
       }
       /* ---- the piece's end */
-      if (n > 0 && ok && !mb_wait(&o_full[X], no++ & 1)) ok = false;
+      /* the last two products may be under way, one a buffer (scores n - 1 came after product n - 3) */
+      if (n > 0 && ok) ok = mb_wait(&o_done[X][0], (ns[0] - 1) & 1);
+      if (n > 1 && ok) ok = mb_wait(&o_done[X][1], (ns[1] - 1) & 1);
       tc_after();
       const bool whole = pc.n == pc.n_tile;
       const int slot = pc.head ? 0 : 1;
