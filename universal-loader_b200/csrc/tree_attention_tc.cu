@@ -79,8 +79,6 @@ __device__ __forceinline__ bool mb_wait(uint64_t* b, uint32_t parity) {
     if (gtime() > end) return false;
   return true;
 }
-/* the same for a converged warp, one answer for all lanes */
-__device__ __forceinline__ bool mb_wait_warp(uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, mb_wait(b, parity)); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -326,13 +324,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   if (tid == 0) {
-    for (int i = 0; i < C::NK; ++i) { mb_init(&k_full[i], 1); mb_init(&k_free[i], 1); }
-    for (int i = 0; i < C::NV; ++i) { mb_init(&v_full[i], 1); mb_init(&v_free[i], 3); mb_init(&v_clean[i], 2); }
+    for (int i = 0; i < C::NK; ++i) { mb_init(&k_full[i], 1); mb_init(&k_free[i], PAIR ? 2 : 1); }
+    for (int i = 0; i < C::NV; ++i) { mb_init(&v_full[i], 1); mb_init(&v_free[i], PAIR ? 3 : 2); mb_init(&v_clean[i], 1); }
     for (int i = 0; i < 2; ++i) {
       for (int b = 0; b < 2; ++b) { mb_init(&s_full[i][b], 1); mb_init(&p_full[i][b], 4); mb_init(&o_done[i][b], 1); }
     }
     mb_init(&q_full, 8);
-    mb_init(&mma_done, 1);
+    mb_init(&mma_done, 2);
     odd_v = 0;
     p.tail[blockIdx.x].pieces = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -394,81 +392,83 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (uint32_t c = ck > (uint32_t)C::NK ? ck - C::NK : 0; c < ck; ++c) ok &= mb_wait(&k_full[c % C::NK], (c / C::NK) & 1);
     for (uint32_t c = cv > (uint32_t)C::NV ? cv - C::NV : 0; c < cv; ++c) ok &= mb_wait(&v_full[c % C::NV], (c / C::NV) & 1);
     __syncwarp();
-  } else if (warp == 1) {
-    /* ------------------------------------------------ MMA issue (the warp walks, one elected lane issues) */
-    /* one thread feeds the tensor cores, so its loop is kept short: descriptors are a base plus
-       a constant, ring places and phases are counted, not divided */
-    uint32_t ks = 0, kp = 0, vs = 0, vp = 0; /* next K / V tile of the ring and its phase */
-    uint32_t kcur = 0, vcur = 0;             /* the tile stream 0 took last */
-    uint32_t qp = 0, pp = 0;                 /* phases of q_full, and of p_full[X][b] in bit 2 X + b */
-    const uint64_t dq = desc_k(sa(q_sm)), dk = desc_k(sa(k_sm)), dv = desc_mn(sa(v_sm));
-    while (ok && walk.next(a, p, &pc)) {
-      if (!mb_wait_warp(&q_full, qp)) { ok = false; break; }
+  } else if (warp < 3) {
+    /* ------------------------------------------------ MMA issue: a warp a stream walks, one elected lane
+       issues.  Issuing is what limits a stream (waits, MMAs and commits of a tile take one thread some
+       800 cycles), so the loop is kept short: descriptors are a base plus a constant, ring places
+       are counted, and a wait that failed only makes the later ones pass (nothing leaves the loop) */
+    const int X = warp - 1;
+    constexpr int STEP = PAIR ? 1 : 2; /* tiles of the ring from one of this stream's to the next */
+    uint32_t used = 0, qp = 0, pp = 0; /* tiles of earlier pieces, phases of q_full and of p_full[X][b] in bit b */
+    const uint64_t dq = desc_k(sa(q_sm)) + (PAIR ? X * (C::QTILE >> 4) : 0), dk = desc_k(sa(k_sm)), dv = desc_mn(sa(v_sm));
+    const uint32_t ds = tmem + X * 128, dov = tmem + 256 + X * HD;
+    auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && mb_wait(bar, parity); };
+    while (walk.next(a, p, &pc)) {
+      wait(&q_full, qp);
       qp ^= 1;
-      const int n0 = n_of(0), n1 = n_of(1);
-      /* first tile that some row does not see whole */
-      const int clear = min(tree_open(a, pc.q), pc.q.len) / TK - pc.t0;
-      /* K / V tiles are used in order; PAIR uses each twice, stream 1 the one that stream 0 took last */
-      auto qk = [&](auto x, int b) {
-        constexpr int X = decltype(x)::value;
-        if (!PAIR || X == 0) {
-          if (!mb_wait_warp(&k_full[ks], kp)) { ok = false; return; }
-          kcur = ks;
+      const int n = n_of(X);
+      const uint32_t first = used + (PAIR ? 0 : X);
+      int ks = first % C::NK, vs = first % C::NV;
+      uint32_t kp = first / C::NK & 1, vp = first / C::NV & 1;
+      used += pc.n;
+      if (PAIR && n == 0) { /* no rows: the tiles pass by */
+        for (int i = 0; i < pc.n; ++i) {
+          wait(&k_full[ks], kp);
+          wait(&v_full[vs], vp);
+          __syncwarp();
+          if (lane == 0) { mb_arrive(&k_free[ks]); mb_arrive(&v_free[vs]); }
           if (++ks == C::NK) { ks = 0; kp ^= 1; }
-        }
-        tc_after();
-        if (elect()) {
-          const uint64_t q0 = dq + (PAIR ? X * (C::QTILE >> 4) : 0), k0 = dk + kcur * (C::TILE >> 4);
-#pragma unroll
-          for (int j = 0; j < HD / 16; ++j)
-            mma_ss(tmem + X * 128 + b * TK, q0 + (((j >> 2) * (TQ * 128) + (j & 3) * 32) >> 4),
-                   k0 + (((j >> 2) * (TK * 128) + (j & 3) * 32) >> 4), ID_S, j > 0);
-          commit(&s_full[X][b]);
-          if (!PAIR || X == 1 || n1 == 0) commit(&k_free[kcur]);
-        }
-        __syncwarp();
-      };
-      auto pv = [&](auto x, int i) {
-        constexpr int X = decltype(x)::value;
-        const int b = i & 1;
-        if (!PAIR || X == 0) {
-          /* v_full first: it says that the slot's earlier phases, v_clean's too, are over */
-          if (!mb_wait_warp(&v_full[vs], vp)) { ok = false; return; }
-          if ((PAIR ? i : 2 * i + X) >= clear && !mb_wait_warp(&v_clean[vs], vp)) { ok = false; return; }
-          vcur = vs;
           if (++vs == C::NV) { vs = 0; vp ^= 1; }
         }
-        if (!mb_wait_warp(&p_full[X][b], (pp >> (2 * X + b)) & 1)) { ok = false; return; }
-        pp ^= 1u << (2 * X + b);
+        continue;
+      }
+      /* this stream's first tile that some row does not see whole */
+      const int clear = max(0, (min(tree_open(a, pc.q), pc.q.len) / TK - pc.t0 - (PAIR ? 0 : X) + STEP - 1) / STEP);
+      auto qk = [&](int b) {
+        wait(&k_full[ks], kp);
         tc_after();
         if (elect()) {
-          const uint64_t v0 = dv + vcur * (C::TILE >> 4);
-          const uint32_t d = tmem + 256 + X * HD, pa = tmem + X * 128 + b * TK;
-          mma_ts(d, pa, v0, ID_O, i > 0);
+          const uint64_t k0 = dk + ks * (C::TILE >> 4);
 #pragma unroll
-          for (int j = 1; j < TK / 16; ++j) mma_ts(d, pa + j * 8, v0 + ((j * 2048) >> 4), ID_O, 1);
-          commit(&o_done[X][b]);
-          if (!PAIR || X == 1 || n1 == 0) commit(&v_free[vcur]);
+          for (int j = 0; j < HD / 16; ++j)
+            mma_ss(ds + b * TK, dq + (((j >> 2) * (TQ * 128) + (j & 3) * 32) >> 4), k0 + (((j >> 2) * (TK * 128) + (j & 3) * 32) >> 4),
+                   ID_S, j > 0);
+          commit(&s_full[X][b]);
+          commit(&k_free[ks]);
         }
         __syncwarp();
+        ks += STEP;
+        if (ks >= C::NK) { ks -= C::NK; kp ^= 1; }
       };
-      constexpr std::integral_constant<int, 0> S0{};
-      constexpr std::integral_constant<int, 1> S1{};
-      qk(S0, 0); /* a piece has a tile, and stream 0 the first */
-      if (ok && n1 > 0) qk(S1, 0);
-      if (ok && n0 > 1) qk(S0, 1);
-      if (ok && n1 > 1) qk(S1, 1);
-      for (int i = 0; i < n0 && ok; ++i) {
-        pv(S0, i);
-        if (ok && i + 2 < n0) qk(S0, i & 1);
-        if (ok && i < n1) pv(S1, i);
-        if (ok && i + 2 < n1) qk(S1, i & 1);
+      if (n > 0) qk(0);
+      if (n > 1) qk(1);
+      for (int i = 0; i < n; ++i) {
+        const int b = i & 1;
+        /* v_full first: it says that the slot's earlier phases, v_clean's too, are over */
+        wait(&v_full[vs], vp);
+        if (i >= clear) wait(&v_clean[vs], vp);
+        wait(&p_full[X][b], (pp >> b) & 1);
+        pp ^= 1u << b;
+        tc_after();
+        if (elect()) {
+          const uint64_t v0 = dv + vs * (C::TILE >> 4);
+          const uint32_t pa = ds + b * TK;
+          mma_ts(dov, pa, v0, ID_O, i > 0);
+#pragma unroll
+          for (int j = 1; j < TK / 16; ++j) mma_ts(dov, pa + j * 8, v0 + ((j * 2048) >> 4), ID_O, 1);
+          commit(&o_done[X][b]);
+          commit(&v_free[vs]);
+        }
+        __syncwarp();
+        vs += STEP;
+        if (vs >= C::NV) { vs -= C::NV; vp ^= 1; }
+        if (i + 2 < n) qk(b);
       }
     }
     /* everything issued completes before TMEM is freed */
     if (elect()) commit(&mma_done);
     __syncwarp();
-    if (!mb_wait_warp(&mma_done, 0)) ok = false;
+    wait(&mma_done, 0);
   } else if (warp < 4) {
     /* ------------------------------------------------ V elements that are not finite, in masked tiles */
     uint32_t cv = 0;
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint4* v = reinterpret_cast<uint4*>(v_sm + slot * C::TILE);
           constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
           bool any = false;
-          for (int i = tid - 64; i < C::TILE / 16; i += 64) {
+          for (int i = lane; i < C::TILE / 16; i += 32) {
             uint4 x = v[i];
             uint32_t w[4] = {x.x, x.y, x.z, x.w};
             bool hit = false;
