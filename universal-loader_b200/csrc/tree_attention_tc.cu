@@ -128,6 +128,32 @@ __device__ __forceinline__ void tm_st(uint32_t t, const uint32_t* r) {
 }
 __device__ __forceinline__ void tm_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+/* two fp32 operations in one instruction */
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 both(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 /* the 256 softmax threads */
 __device__ __forceinline__ void sync_softmax() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
@@ -512,12 +538,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t ns[2] = {0, 0}; /* tiles seen a buffer: phases of its s_full, p_full and o_done */
     while (walk.next(a, p, &pc)) {
       /* Q of this CTA's rows, swizzled; rows past the tile's queries are zero */
-      for (int i = tid - 128; i < C::NQ * TQ * (HD / 8); i += 256) {
-        const int r = i / (HD / 8), ch = i % (HD / 8), qi = pc.q0 + r;
-        uint4 x = make_uint4(0, 0, 0, 0);
+      constexpr int QW = C::NQ * TQ * (HD / 8) / 256; /* 16-byte words a thread: all loads first */
+      uint4 qx[QW];
+#pragma unroll
+      for (int j = 0; j < QW; ++j) {
+        const int i = tid - 128 + j * 256, r = i / (HD / 8), ch = i % (HD / 8), qi = pc.q0 + r;
+        qx[j] = make_uint4(0, 0, 0, 0);
         if (r < pc.nq)
-          x = *reinterpret_cast<const uint4*>((const T*)a.q + ((long long)(pc.q.r0 + qi / a.G) * a.H + pc.kvh * a.G + qi % a.G) * HD + ch * 8);
-        *reinterpret_cast<uint4*>(q_sm + (r >> 7) * C::QTILE + (ch >> 3) * (TQ * 128) + sw128(r & 127, ch & 7)) = x;
+          qx[j] = *reinterpret_cast<const uint4*>((const T*)a.q + ((long long)(pc.q.r0 + qi / a.G) * a.H + pc.kvh * a.G + qi % a.G) * HD + ch * 8);
+      }
+#pragma unroll
+      for (int j = 0; j < QW; ++j) {
+        const int i = tid - 128 + j * 256, r = i / (HD / 8), ch = i % (HD / 8);
+        *reinterpret_cast<uint4*>(q_sm + (r >> 7) * C::QTILE + (ch >> 3) * (TQ * 128) + sw128(r & 127, ch & 7)) = qx[j];
       }
       fence_async();
       __syncwarp();
@@ -561,15 +594,34 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!((see >> e) & 1u)) sr[c + e] = 0xff800000u; /* -inf */
             }
           }
-          float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
+          /* weights against the maximum so far, the tile's own maximum beside them: only when a row's
+             has grown by more than 2^8 (its first tile, seldom later) are they taken again */
+          uint32_t pk[TK / 2];
+          float sum = 0.f;
+          auto weights = [&](float u) {
+            const uint64_t sc2 = two(a.scale2, a.scale2), mu = two(-u, -u);
+            uint64_t l0 = two(0.f, 0.f), l1 = l0;
 #pragma unroll
-          for (int c = 0; c < TK; c += 4) {
-            x0 = fmaxf(x0, __uint_as_float(sr[c]));
-            x1 = fmaxf(x1, __uint_as_float(sr[c + 1]));
-            x2 = fmaxf(x2, __uint_as_float(sr[c + 2]));
-            x3 = fmaxf(x3, __uint_as_float(sr[c + 3]));
+            for (int c = 0; c < TK; c += 4) {
+              const float2 e0 = both(fma2(two(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), sc2, mu));
+              const float2 e1 = both(fma2(two(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), sc2, mu));
+              const float p0 = ex2(e0.x), p1 = ex2(e0.y), p2 = ex2(e1.x), p3 = ex2(e1.y);
+              l0 = add2(l0, two(p0, p1));
+              l1 = add2(l1, two(p2, p3));
+              pk[c / 2] = pack2<T>(p0, p1);
+              pk[c / 2 + 1] = pack2<T>(p2, p3);
+            }
+            const float2 y = both(add2(l0, l1));
+            sum = y.x + y.y;
+          };
+          weights(m == -INFINITY ? 0.f : m);
+          float x0 = __uint_as_float(sr[0]), x1 = __uint_as_float(sr[1]);
+#pragma unroll
+          for (int c = 2; c + 3 < TK; c += 4) {
+            x0 = max3(x0, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+            x1 = max3(x1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
           }
-          const float top = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * a.scale2;
+          const float top = fmaxf(max3(x0, __uint_as_float(sr[TK - 2]), __uint_as_float(sr[TK - 1])), x1) * a.scale2;
           const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
           if (__any_sync(0xffffffffu, grow)) {
             const float f = grow ? (m == -INFINITY ? 0.f : ex2(m - top)) : 1.f;
@@ -588,24 +640,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tm_st(to + c, or_);
               }
             }
+            weights(m == -INFINITY ? 0.f : m);
           }
-          const float u = m == -INFINITY ? 0.f : m;
-          float l0 = 0.f, l1 = 0.f, l2 = 0.f, l3 = 0.f;
-#pragma unroll
-          for (int c = 0; c < TK; c += 4) {
-            const float p0 = ex2(__fmaf_rn(__uint_as_float(sr[c]), a.scale2, -u));
-            const float p1 = ex2(__fmaf_rn(__uint_as_float(sr[c + 1]), a.scale2, -u));
-            const float p2 = ex2(__fmaf_rn(__uint_as_float(sr[c + 2]), a.scale2, -u));
-            const float p3 = ex2(__fmaf_rn(__uint_as_float(sr[c + 3]), a.scale2, -u));
-            l0 += p0;
-            l1 += p1;
-            l2 += p2;
-            l3 += p3;
-            sr[c / 2] = pack2<T>(p0, p1);
-            sr[c / 2 + 1] = pack2<T>(p2, p3);
-          }
-          l += (l0 + l1) + (l2 + l3);
-          tm_st(ts, sr);
+          l += sum;
+          tm_st(ts, pk);
           tm_st_wait();
         }
         tc_before();
