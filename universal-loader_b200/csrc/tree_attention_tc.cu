@@ -79,6 +79,15 @@ __device__ __forceinline__ bool mb_wait(uint64_t* b, uint32_t parity) {
     if (gtime() > end) return false;
   return true;
 }
+/* the same for a converged warp, one answer for all lanes (a vote: a shuffle would queue behind the
+   softmax warps' exponentials, as every shared-memory operation does, for some 300 cycles) */
+__device__ __forceinline__ bool mb_wait_warp(uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, mb_wait(b, parity)); }
+__device__ __forceinline__ bool mb_test(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(ok) : "r"(sa(b)), "r"(parity) : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -388,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (ok && walk.next(a, p, &pc)) {
       auto load = [&](const CUtensorMap* m, uint8_t* ring, uint64_t* full, uint64_t* free, uint32_t& c, int nring, int t) {
         const int slot = c % nring;
-        if (c >= (uint32_t)nring && !mb_wait(&free[slot], ((c / nring) - 1) & 1)) { ok = false; return; }
+        if (c >= (uint32_t)nring && !mb_wait_warp(&free[slot], ((c / nring) - 1) & 1)) { ok = false; return; }
         const int pos = (pc.t0 + t) * TK;
         int page = a.g.n_pages; /* out of range: zeros */
         if (lane < boxes && pos + lane * rows < pc.q.len) {
@@ -451,7 +460,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       /* this stream's first tile that some row does not see whole */
       const int clear = max(0, (min(tree_open(a, pc.q), pc.q.len) / TK - pc.t0 - (PAIR ? 0 : X) + STEP - 1) / STEP);
       auto qk = [&](int b) {
-        wait(&k_full[ks], kp);
         tc_after();
         if (elect()) {
           const uint64_t k0 = dk + ks * (C::TILE >> 4);
@@ -466,15 +474,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         ks += STEP;
         if (ks >= C::NK) { ks -= C::NK; kp ^= 1; }
       };
-      if (n > 0) qk(0);
-      if (n > 1) qk(1);
+      for (int i = 0; i < min(n, 2); ++i) {
+        wait(&k_full[ks], kp);
+        qk(i);
+      }
       for (int i = 0; i < n; ++i) {
         const int b = i & 1;
-        /* v_full first: it says that the slot's earlier phases, v_clean's too, are over */
-        wait(&v_full[vs], vp);
+        const bool more = i + 2 < n;
+        /* V and weights for this tile's product, K for the scores after the next: asked for together,
+           since an answer takes long; waited for one by one if they are not there */
+        const bool hv = mb_test(&v_full[vs], vp), hk = !more || mb_test(&k_full[ks], kp);
+        const bool hp = mb_test(&p_full[X][b], (pp >> b) & 1);
+        if (!hv) wait(&v_full[vs], vp);
+        /* after v_full, which says that the slot's earlier phases, v_clean's too, are over */
         if (i >= clear) wait(&v_clean[vs], vp);
-        wait(&p_full[X][b], (pp >> b) & 1);
+        if (!hp) wait(&p_full[X][b], (pp >> b) & 1);
         pp ^= 1u << b;
+        if (!hk) wait(&k_full[ks], kp);
+        __syncwarp();
         tc_after();
         if (elect()) {
           const uint64_t v0 = dv + vs * (C::TILE >> 4);
@@ -488,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         vs += STEP;
         if (vs >= C::NV) { vs -= C::NV; vp ^= 1; }
-        if (i + 2 < n) qk(b);
+        if (more) qk(b);
       }
     }
     /* everything issued completes before TMEM is freed */
@@ -502,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int clear = min(tree_open(a, pc.q), pc.q.len);
       for (int t = 0; t < pc.n; ++t, ++cv) {
         const int slot = cv % C::NV;
-        if (!mb_wait(&v_full[slot], (cv / C::NV) & 1)) { ok = false; break; }
+        if (!mb_wait_warp(&v_full[slot], (cv / C::NV) & 1)) { ok = false; break; }
         if ((pc.t0 + t + 1) * TK > clear) {
           uint4* v = reinterpret_cast<uint4*>(v_sm + slot * C::TILE);
           constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
@@ -578,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (holes) blocks = __ballot_sync(0xffffffffu, lane >= n_blk || page_at(pos + lane * 16) != -2);
         const int b = i & 1;
         const uint32_t ts = tmem + lanes + X * 128 + b * TK;
-        if (!mb_wait(&s_full[X][b], (b ? ns[1]++ : ns[0]++) & 1)) { ok = false; break; }
+        if (!mb_wait_warp(&s_full[X][b], (b ? ns[1]++ : ns[0]++) & 1)) { ok = false; break; }
         tc_after();
         if (warp_live) {
           uint32_t sr[TK];
@@ -628,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (grow) m = top;
             l *= f;
             if (i > 0) { /* the first product overwrites O */
-              if (!mb_wait(&o_done[X][b ^ 1], ((b ? ns[0] : ns[1]) - 1) & 1)) ok = false;
+              if (!mb_wait_warp(&o_done[X][b ^ 1], ((b ? ns[0] : ns[1]) - 1) & 1)) ok = false;
               tc_after();
               uint32_t or_[32];
 #pragma unroll
@@ -652,8 +669,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       /* ---- the piece's end */
       /* the last two products may be under way, one a buffer (scores n - 1 came after product n - 3) */
-      if (n > 0 && ok) ok = mb_wait(&o_done[X][0], (ns[0] - 1) & 1);
-      if (n > 1 && ok) ok = mb_wait(&o_done[X][1], (ns[1] - 1) & 1);
+      if (n > 0 && ok) ok = mb_wait_warp(&o_done[X][0], (ns[0] - 1) & 1);
+      if (n > 1 && ok) ok = mb_wait_warp(&o_done[X][1], (ns[1] - 1) & 1);
       tc_after();
       const bool whole = pc.n == pc.n_tile;
       const int slot = pc.head ? 0 : 1;
