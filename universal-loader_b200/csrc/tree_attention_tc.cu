@@ -391,36 +391,64 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto n_of = [&](int X) { return PAIR ? (X == 0 || pc.nq > 128 ? pc.n : 0) : (pc.n + 1 - X) >> 1; };
 
   if (warp == 0) {
-    /* ------------------------------------------------ TMA: K and V tiles in the order of their use */
+    /* ------------------------------------------------ TMA: K and V tiles in the order of their use.  A
+       tile's page ids are read one tile ahead and the free barriers of a step's V and K tiles asked for
+       together: the two latencies one after the other took as long as a tile's products. */
     uint32_t ck = 0, cv = 0; /* tiles issued */
     const int rows = min(a.g.page, TK), boxes = TK / rows;
+    constexpr int MB = TK / 16;
     while (ok && walk.next(a, p, &pc)) {
-      auto load = [&](const CUtensorMap* m, uint8_t* ring, uint64_t* full, uint64_t* free, uint32_t& c, int nring, int t) {
-        const int slot = c % nring;
-        if (c >= (uint32_t)nring && !mb_wait_warp(&free[slot], ((c / nring) - 1) & 1)) { ok = false; return; }
-        const int pos = (pc.t0 + t) * TK;
-        int page = a.g.n_pages; /* out of range: zeros */
-        if (lane < boxes && pos + lane * rows < pc.q.len) {
-          const int j = (pos + lane * rows) >> a.g.page_shift;
-          const int x = j < a.g.max_pages ? a.table[(long long)pc.s * a.g.max_pages + j] : -1;
-          if (x >= 0 && x < a.g.n_pages) page = x;
-        }
-        if (lane == 0) mb_expect(&full[slot], (uint32_t)C::TILE);
-        __syncwarp();
-        if (lane < boxes) {
-          uint8_t* d = ring + slot * C::TILE + lane * rows * 128;
+      const int* const tb = a.table + (long long)pc.s * a.g.max_pages;
+      int kpg[MB], vpg[MB]; /* pages of the next K and V tile; n_pages, out of range, reads zeros */
+      auto ids = [&](int t, int (&pg)[MB]) {
 #pragma unroll
-          for (int h = 0; h < HD / 64; ++h) tma4(d + h * TK * 128, m, h * 64, pos & (a.g.page - 1), pc.kvh, page, &full[slot]);
+        for (int i = 0; i < MB; ++i) {
+          pg[i] = a.g.n_pages;
+          if (i >= boxes || t >= pc.n) continue;
+          const long long pos = (long long)(pc.t0 + t) * TK + i * rows;
+          const int j = (int)(pos >> a.g.page_shift);
+          if (pos < pc.q.len && j < a.g.max_pages) pg[i] = tb[j];
         }
-        ++c;
       };
-      auto K = [&](int t) { if (ok) load(&mk, k_sm, k_full, k_free, ck, C::NK, t); };
-      auto V = [&](int t) { if (ok) load(&mv, v_sm, v_full, v_free, cv, C::NV, t); };
+      auto load = [&](const CUtensorMap* m, uint8_t* ring, uint64_t* full, int slot, int t, const int (&pg)[MB]) {
+        if (elect()) {
+          const int pos = ((pc.t0 + t) * TK) & (a.g.page - 1);
+          uint8_t* const d = ring + slot * C::TILE;
+          mb_expect(&full[slot], (uint32_t)C::TILE);
+#pragma unroll
+          for (int i = 0; i < MB; ++i) {
+            if (i >= boxes) break;
+            const int page = pg[i] >= 0 && pg[i] < a.g.n_pages ? pg[i] : a.g.n_pages;
+#pragma unroll
+            for (int h = 0; h < HD / 64; ++h) tma4(d + i * rows * 128 + h * TK * 128, m, h * 64, pos, pc.kvh, page, &full[slot]);
+          }
+        }
+        __syncwarp();
+      };
+      auto free_k = [&]() { return ck < (uint32_t)C::NK || mb_test(&k_free[ck % C::NK], (ck / C::NK - 1) & 1); };
+      auto free_v = [&]() { return cv < (uint32_t)C::NV || mb_test(&v_free[cv % C::NV], (cv / C::NV - 1) & 1); };
+      auto K = [&](int t, bool ready) {
+        if (!__all_sync(0xffffffffu, ready)) ok = ok && mb_wait_warp(&k_free[ck % C::NK], (ck / C::NK - 1) & 1);
+        if (!ok) return;
+        load(&mk, k_sm, k_full, ck % C::NK, t, kpg);
+        ids(t + 1, kpg);
+        ++ck;
+      };
+      auto V = [&](int t, bool ready) {
+        if (!__all_sync(0xffffffffu, ready)) ok = ok && mb_wait_warp(&v_free[cv % C::NV], (cv / C::NV - 1) & 1);
+        if (!ok) return;
+        load(&mv, v_sm, v_full, cv % C::NV, t, vpg);
+        ids(t + 1, vpg);
+        ++cv;
+      };
       constexpr int AHEAD = PAIR ? 2 : 4; /* K tiles whose scores are asked for before the first V tile */
-      for (int t = 0; t < min(AHEAD, pc.n); ++t) K(t);
+      ids(0, kpg);
+      ids(0, vpg);
+      for (int t = 0; t < min(AHEAD, pc.n); ++t) K(t, free_k());
       for (int t = 0; t < pc.n && ok; ++t) {
-        V(t);
-        if (t + AHEAD < pc.n) K(t + AHEAD);
+        const bool more = t + AHEAD < pc.n, rv = free_v(), rk = !more || free_k();
+        V(t, rv);
+        if (more) K(t + AHEAD, rk);
       }
     }
     /* no copy is in flight when the CTA ends, whatever happened */
