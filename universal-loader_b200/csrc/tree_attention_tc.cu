@@ -31,7 +31,7 @@
  * walks whole sequences and pieces of two.  A pair that falls into several stretches leaves one
  * partial a stretch, joined by a small kernel.
  *
- * Every mbarrier wait has a deadline (2 s): past it a role raises bit 3 of the device error word
+ * Every mbarrier wait has a limit: past it a role raises bit 3 of the device error word
  * and stops issuing work; the CTA still waits (bounded) for its MMAs before freeing TMEM.
  */
 #include "tree_attention.h"
@@ -51,11 +51,6 @@ constexpr int kMinTiles = 8;     /* tiles a group takes at least */
 constexpr int kJoinRows = 8;   /* rows a block of the join kernel: a warp each */
 
 __device__ __forceinline__ uint32_t sa(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ uint64_t gtime() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
 __device__ __forceinline__ void mb_init(uint64_t* b, uint32_t n) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sa(b)), "r"(n) : "memory");
 }
@@ -71,13 +66,13 @@ __device__ __forceinline__ bool mb_try(uint64_t* b, uint32_t parity) {
                : "=r"(ok) : "r"(sa(b)), "r"(parity) : "memory");
   return ok != 0;
 }
-/* wait for the phase with this parity; false once 2 s have passed */
+/* wait for the phase with this parity; false after kTries looks, each of which the hardware may stretch
+   (seconds in all; reading a clock between looks costs more than the looks) */
+constexpr int kTries = 1 << 23;
 __device__ __forceinline__ bool mb_wait(uint64_t* b, uint32_t parity) {
-  if (mb_try(b, parity)) return true;
-  const uint64_t end = gtime() + 2000000000ull;
-  while (!mb_try(b, parity))
-    if (gtime() > end) return false;
-  return true;
+  for (int i = 0; i < kTries; ++i)
+    if (mb_try(b, parity)) return true;
+  return false;
 }
 /* the same for a converged warp, one answer for all lanes (a vote: a shuffle would queue behind the
    softmax warps' exponentials, as every shared-memory operation does, for some 300 cycles) */
@@ -294,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr uint32_t ID_S = (1u << 4) | FMT | ((TK >> 3) << 17) | ((128 >> 4) << 24);
   constexpr uint32_t ID_O = (1u << 4) | FMT | (1u << 16) | ((HD >> 3) << 17) | ((128 >> 4) << 24);
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t k_full[C::NK], k_free[C::NK], v_full[C::NV], v_free[C::NV], v_clean[C::NV], s_full[2][2], p_full[2][2], o_done[2][2], q_full, mma_done;
+  __shared__ uint64_t k_full[C::NK], k_free[C::NK], v_full[C::NV], v_free[C::NV], s_full[2][2], p_full[2][2], o_done[2][2], q_full, mma_done;
   __shared__ uint32_t tmem_sh;
   __shared__ int odd_v, sh_s;
   __shared__ long long sh_base, sh_sum[kThreads / 32 + 1];
@@ -360,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (tid == 0) {
     for (int i = 0; i < C::NK; ++i) { mb_init(&k_full[i], 1); mb_init(&k_free[i], PAIR ? 2 : 1); }
-    for (int i = 0; i < C::NV; ++i) { mb_init(&v_full[i], 1); mb_init(&v_free[i], PAIR ? 3 : 2); mb_init(&v_clean[i], 1); }
+    for (int i = 0; i < C::NV; ++i) { mb_init(&v_full[i], 1); mb_init(&v_free[i], PAIR ? 2 : 1); }
     for (int i = 0; i < 2; ++i) {
       for (int b = 0; b < 2; ++b) { mb_init(&s_full[i][b], 1); mb_init(&p_full[i][b], 4); mb_init(&o_done[i][b], 1); }
     }
@@ -390,27 +385,33 @@ __global__ void __launch_bounds__(kThreads, 1)
   /* stream X's tiles of a piece of n: PAIR all of them (none without rows), else every second */
   auto n_of = [&](int X) { return PAIR ? (X == 0 || pc.nq > 128 ? pc.n : 0) : (pc.n + 1 - X) >> 1; };
 
-  if (warp == 0) {
-    /* ------------------------------------------------ TMA: K and V tiles in the order of their use.  A
-       tile's page ids are read one tile ahead and the free barriers of a step's V and K tiles asked for
-       together: the two latencies one after the other took as long as a tile's products. */
-    uint32_t ck = 0, cv = 0; /* tiles issued */
+  if (warp == 0 || warp == 3) {
+    /* ------------------------------------------------ TMA: warp 0 the K tiles, warp 3 the V tiles, in order.
+       Asking for a free slot, issuing and looking up pages take some 750 cycles a tile, so each
+       has a warp and the page ids are read a tile ahead. */
+    const CUtensorMap* const map = warp == 0 ? &mk : &mv;
+    uint8_t* const ring = warp == 0 ? k_sm : v_sm;
+    uint64_t* const full = warp == 0 ? k_full : v_full;
+    uint64_t* const free = warp == 0 ? k_free : v_free;
+    const int nring = warp == 0 ? C::NK : C::NV;
+    int slot = 0, issued = 0;
+    uint32_t phase = 1; /* of the free barrier: the first round passes */
     const int rows = min(a.g.page, TK), boxes = TK / rows;
     constexpr int MB = TK / 16;
     while (ok && walk.next(a, p, &pc)) {
       const int* const tb = a.table + (long long)pc.s * a.g.max_pages;
-      int kpg[MB], vpg[MB]; /* pages of the next K and V tile; n_pages, out of range, reads zeros */
-      auto ids = [&](int t, int (&pg)[MB]) {
+      int pg[MB]; /* pages of the next tile; n_pages, out of range, reads zeros */
+      auto ids = [&](int t) {
+        const int pos = (pc.t0 + t) * TK; /* at most len + 63 */
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
-          pg[i] = a.g.n_pages;
-          if (i >= boxes || t >= pc.n) continue;
-          const long long pos = (long long)(pc.t0 + t) * TK + i * rows;
-          const int j = (int)(pos >> a.g.page_shift);
-          if (pos < pc.q.len && j < a.g.max_pages) pg[i] = tb[j];
+          const int at = pos + i * rows, j = at >> a.g.page_shift;
+          pg[i] = i < boxes && t < pc.n && at < pc.q.len && j < a.g.max_pages ? tb[j] : -1;
         }
       };
-      auto load = [&](const CUtensorMap* m, uint8_t* ring, uint64_t* full, int slot, int t, const int (&pg)[MB]) {
+      ids(0);
+      for (int t = 0; t < pc.n && ok; ++t) {
+        ok = mb_wait_warp(&free[slot], phase);
         if (elect()) {
           const int pos = ((pc.t0 + t) * TK) & (a.g.page - 1);
           uint8_t* const d = ring + slot * C::TILE;
@@ -420,41 +421,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (i >= boxes) break;
             const int page = pg[i] >= 0 && pg[i] < a.g.n_pages ? pg[i] : a.g.n_pages;
 #pragma unroll
-            for (int h = 0; h < HD / 64; ++h) tma4(d + i * rows * 128 + h * TK * 128, m, h * 64, pos, pc.kvh, page, &full[slot]);
+            for (int h = 0; h < HD / 64; ++h) tma4(d + i * rows * 128 + h * TK * 128, map, h * 64, pos, pc.kvh, page, &full[slot]);
           }
         }
         __syncwarp();
-      };
-      auto free_k = [&]() { return ck < (uint32_t)C::NK || mb_test(&k_free[ck % C::NK], (ck / C::NK - 1) & 1); };
-      auto free_v = [&]() { return cv < (uint32_t)C::NV || mb_test(&v_free[cv % C::NV], (cv / C::NV - 1) & 1); };
-      auto K = [&](int t, bool ready) {
-        if (!__all_sync(0xffffffffu, ready)) ok = ok && mb_wait_warp(&k_free[ck % C::NK], (ck / C::NK - 1) & 1);
-        if (!ok) return;
-        load(&mk, k_sm, k_full, ck % C::NK, t, kpg);
-        ids(t + 1, kpg);
-        ++ck;
-      };
-      auto V = [&](int t, bool ready) {
-        if (!__all_sync(0xffffffffu, ready)) ok = ok && mb_wait_warp(&v_free[cv % C::NV], (cv / C::NV - 1) & 1);
-        if (!ok) return;
-        load(&mv, v_sm, v_full, cv % C::NV, t, vpg);
-        ids(t + 1, vpg);
-        ++cv;
-      };
-      constexpr int AHEAD = PAIR ? 2 : 4; /* K tiles whose scores are asked for before the first V tile */
-      ids(0, kpg);
-      ids(0, vpg);
-      for (int t = 0; t < min(AHEAD, pc.n); ++t) K(t, free_k());
-      for (int t = 0; t < pc.n && ok; ++t) {
-        const bool more = t + AHEAD < pc.n, rv = free_v(), rk = !more || free_k();
-        V(t, rv);
-        if (more) K(t + AHEAD, rk);
+        ids(t + 1);
+        ++issued;
+        if (++slot == nring) { slot = 0; phase ^= 1; }
       }
     }
-    /* no copy is in flight when the CTA ends, whatever happened */
-    for (uint32_t c = ck > (uint32_t)C::NK ? ck - C::NK : 0; c < ck; ++c) ok &= mb_wait(&k_full[c % C::NK], (c / C::NK) & 1);
-    for (uint32_t c = cv > (uint32_t)C::NV ? cv - C::NV : 0; c < cv; ++c) ok &= mb_wait(&v_full[c % C::NV], (c / C::NV) & 1);
-    __syncwarp();
+    /* no copy is in flight when the CTA ends, whatever happened: the last round's tiles, in turn */
+    for (int c = max(0, issued - nring); c < issued; ++c) ok &= mb_wait_warp(&full[c % nring], (c / nring) & 1);
   } else if (warp < 3) {
     /* ------------------------------------------------ MMA issue: a warp a stream walks, one elected lane
        issues.  Issuing is what limits a stream (waits, MMAs and commits of a tile take one thread some
@@ -485,8 +462,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         continue;
       }
-      /* this stream's first tile that some row does not see whole */
-      const int clear = max(0, (min(tree_open(a, pc.q), pc.q.len) / TK - pc.t0 - (PAIR ? 0 : X) + STEP - 1) / STEP);
       auto qk = [&](int b) {
         tc_after();
         if (elect()) {
@@ -514,8 +489,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool hv = mb_test(&v_full[vs], vp), hk = !more || mb_test(&k_full[ks], kp);
         const bool hp = mb_test(&p_full[X][b], (pp >> b) & 1);
         if (!hv) wait(&v_full[vs], vp);
-        /* after v_full, which says that the slot's earlier phases, v_clean's too, are over */
-        if (i >= clear) wait(&v_clean[vs], vp);
         if (!hp) wait(&p_full[X][b], (pp >> b) & 1);
         pp ^= 1u << b;
         if (!hk) wait(&k_full[ks], kp);
@@ -540,46 +513,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (elect()) commit(&mma_done);
     __syncwarp();
     wait(&mma_done, 0);
-  } else if (warp < 4) {
-    /* ------------------------------------------------ V elements that are not finite, in masked tiles */
-    uint32_t cv = 0;
-    while (ok && walk.next(a, p, &pc)) {
-      const int clear = min(tree_open(a, pc.q), pc.q.len);
-      for (int t = 0; t < pc.n; ++t, ++cv) {
-        const int slot = cv % C::NV;
-        if (!mb_wait_warp(&v_full[slot], (cv / C::NV) & 1)) { ok = false; break; }
-        if ((pc.t0 + t + 1) * TK > clear) {
-          uint4* v = reinterpret_cast<uint4*>(v_sm + slot * C::TILE);
-          constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
-          bool any = false;
-          for (int i = lane; i < C::TILE / 16; i += 32) {
-            uint4 x = v[i];
-            uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            bool hit = false;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if ((w[e] & E) == E) { w[e] &= 0xffff0000u; hit = true; }
-              if (((w[e] >> 16) & E) == E) { w[e] &= 0x0000ffffu; hit = true; }
-            }
-            if (hit) v[i] = make_uint4(w[0], w[1], w[2], w[3]);
-            any |= hit;
-          }
-          if (any) odd_v = 1;
-          fence_async();
-        }
-        __syncwarp();
-        if (lane == 0) {
-          mb_arrive(&v_clean[slot]);
-          mb_arrive(&v_free[slot]);
-        }
-      }
-    }
   } else {
     /* ------------------------------------------------ softmax: one thread a row */
     const int X = (warp - 4) >> 2, row = tid - 128 - X * 128; /* stream, row of its tile = TMEM lane */
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t to = tmem + lanes + 256 + X * HD;
     constexpr int n_blk = TK / 16; /* 16-position blocks of a tile */
+    uint32_t used = 0;       /* V tiles of earlier pieces */
     uint32_t ns[2] = {0, 0}; /* tiles seen a buffer: phases of its s_full, p_full and o_done */
     while (walk.next(a, p, &pc)) {
       /* Q of this CTA's rows, swizzled; rows past the tile's queries are zero */
@@ -689,8 +629,32 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           l += sum;
           tm_st(ts, pk);
-          tm_st_wait();
         }
+        if ((t + 1) * TK > open || pos + TK > pc.q.len) {
+          /* masked tile: its V elements that are not finite leave it before the product reads it.  With
+             PAIR both streams look; what one has cleared the other finds clear, and no product of a
+             stream starts before that stream has looked at the whole tile. */
+          const uint32_t cvt = used + (uint32_t)(t - pc.t0);
+          ok = ok && mb_wait_warp(&v_full[cvt % C::NV], (cvt / C::NV) & 1);
+          uint4* const v = reinterpret_cast<uint4*>(v_sm + cvt % C::NV * C::TILE);
+          constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+          for (int j = row; j < C::TILE / 16; j += 128) {
+            const uint4 x = v[j];
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            bool hit = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if ((w[e] & E) == E) { w[e] &= 0xffff0000u; hit = true; }
+              if (((w[e] >> 16) & E) == E) { w[e] &= 0x0000ffffu; hit = true; }
+            }
+            if (hit) {
+              odd_v = 1;
+              v[j] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+          fence_async();
+        }
+        if (warp_live) tm_st_wait();
         tc_before();
         __syncwarp();
         if (lane == 0) mb_arrive(&p_full[X][b]);
@@ -699,6 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       /* the last two products may be under way, one a buffer (scores n - 1 came after product n - 3) */
       if (n > 0 && ok) ok = mb_wait_warp(&o_done[X][0], (ns[0] - 1) & 1);
       if (n > 1 && ok) ok = mb_wait_warp(&o_done[X][1], (ns[1] - 1) & 1);
+      used += pc.n;
       tc_after();
       const bool whole = pc.n == pc.n_tile;
       const int slot = pc.head ? 0 : 1;
@@ -723,6 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_before();
       /* values taken out of masked tiles go to the rows that see them */
+      if (PAIR) sync_softmax(); /* either stream may have found them */
       if (odd_v && live && ok) {
         const T* qr = (const T*)a.q + ((long long)(pc.q.r0 + ri) * a.H + pc.kvh * a.G + qi % a.G) * HD;
         const int from = max(pc.t0 * TK, min(open, pc.q.len) / TK * TK), upto = min(pc.q.len, (pc.t0 + pc.n) * TK);
