@@ -2,16 +2,13 @@
  * tree_attention_tc.cu — ulb_tree_attention on the 5th-generation tensor cores, for head
  * dims 64 and 128.  Same mathematics and masking as tree_attention.cu.
  *
- * A CTA works on 64-key tiles with M = 128 query rows a stream, two streams at a time, each
+ * A CTA works on 128-key tiles with M = 128 query rows a stream, two streams at a time, each
  * with its own running (m, l, o) and its own softmax warpgroup (one thread a row):
  *   PAIR = false  (at most 128 queries a kv head): both streams hold the same rows and take the
  *                 even and the odd tiles; they join in shared memory at the end
  *   PAIR = true   (more): the streams hold neighbouring tiles of 128 rows and share every K / V
  *                 tile, which halves what shared memory and L2 have to deliver
- * so that one stream's products run while the other stream's weights are computed.  Each stream has
- * two score buffers, so the next tile's scores are there when a tile's weights are done: the
- * exponentials, not the round trip between tensor cores and softmax, set the pace (with 128-key
- * tiles and one buffer a stream the largest case took 323 us).  Per tile:
+ * so that one stream's products run while the other stream's weights are computed.  Per tile:
  * S = Q K^T (tcgen05.mma, both operands in shared memory, fp32 in TMEM); the row's thread reads
  * S, updates m and l, writes P (rounded to the cache's type) over S in TMEM; O += P V with P read
  * from TMEM and V as the tile TMA wrote it (keys x hd, the MN-major operand).  O stays in TMEM; it
@@ -21,9 +18,11 @@
  * Warps: 0 TMA (pages -> 128-byte-swizzled tiles, one box a page, pages that are unmapped or past
  * the end read as zero through an out-of-range coordinate), 1 issues every MMA and the commits
  * that free tiles, 2 - 3 take V elements that are not finite out of masked tiles, 4 - 7 and 8 - 11
- * softmax.  Barriers carry it: K / V tiles full and free, S full, P full, O += P V done (waited for
- * only to rescale O and at the end); MMAs issued by one thread complete in order, so a score buffer
- * is free for the next scores once the product that reads its weights has been issued.
+ * softmax.  Barriers carry it: K / V tiles full and free, S full, P full (a half tile each, so that the
+ * first half's product runs beside the second half's exponentials).  One thread issues a stream's
+ * MMAs and they complete in order: S full of a tile means that O holds every earlier tile.
+ * (64-key tiles with two score buffers a stream took 297 us where this takes HERE: what a tile costs
+ * besides its arithmetic, waits, commits and the narrower product, then counts twice.)
  *
  * Work is cut evenly: the tiles of all (sequence, kv head) pairs form one line, every CTA (group
  * of CTAs, when more than 256 rows need several row tiles: its members walk the same keys side by
@@ -31,8 +30,9 @@
  * walks whole sequences and pieces of two.  A pair that falls into several stretches leaves one
  * partial a stretch, joined by a small kernel.
  *
- * Every mbarrier wait has a limit: past it a role raises bit 3 of the device error word
- * and stops issuing work; the CTA still waits (bounded) for its MMAs before freeing TMEM.
+ * Every mbarrier wait has a limit: past it a role raises bit 3 of the device error word,
+ * arrives nowhere and issues nothing any more, so that the others run into theirs; the CTA still
+ * waits (bounded) for its MMAs before it frees TMEM.
  */
 #include "tree_attention.h"
 
@@ -44,10 +44,11 @@
 namespace ulb {
 namespace {
 
-constexpr int TK = 64;         /* keys a tile */
+constexpr int TK = 128;        /* keys a tile */
+constexpr int TH = 64;         /* keys of half a tile: the step of softmax and of O += P V */
 constexpr int TQ = 128;        /* query rows a stream: M */
 constexpr int kThreads = 384;  /* 4 role warps, 2 x 4 softmax warps */
-constexpr int kMinTiles = 8;     /* tiles a group takes at least */
+constexpr int kMinTiles = 4;   /* tiles a group takes at least */
 constexpr int kJoinRows = 8;   /* rows a block of the join kernel: a warp each */
 
 __device__ __forceinline__ uint32_t sa(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -68,7 +69,7 @@ __device__ __forceinline__ bool mb_try(uint64_t* b, uint32_t parity) {
 }
 /* wait for the phase with this parity; false after kTries looks, each of which the hardware may stretch
    (seconds in all; reading a clock between looks costs more than the looks) */
-constexpr int kTries = 1 << 23;
+constexpr int kTries = 1 << 21;
 __device__ __forceinline__ bool mb_wait(uint64_t* b, uint32_t parity) {
   for (int i = 0; i < kTries; ++i)
     if (mb_try(b, parity)) return true;
@@ -179,8 +180,8 @@ struct TcCfg {
   static constexpr int TILE = TK * HD * 2;            /* bytes of a K or V tile */
   static constexpr int QTILE = TQ * HD * 2;
   static constexpr int NQ = PAIR ? 2 : 1;
-  static constexpr int NK = HD == 64 ? 8 : PAIR ? 5 : 6; /* K tiles in the ring: five are in use or next in turn */
-  static constexpr int NV = HD == 64 ? 8 : PAIR ? 5 : 6;
+  static constexpr int NK = HD == 64 ? 5 : 3;         /* K tiles in the ring */
+  static constexpr int NV = HD == 64 ? 5 : PAIR ? 2 : 3;
   static constexpr int SMEM = NQ * QTILE + (NK + NV) * TILE + 1024; /* + alignment slack */
   static constexpr int RT = PAIR ? 256 : 128;         /* queries a CTA */
   static_assert(SMEM <= 226 * 1024, "shared memory");
@@ -289,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr uint32_t ID_S = (1u << 4) | FMT | ((TK >> 3) << 17) | ((128 >> 4) << 24);
   constexpr uint32_t ID_O = (1u << 4) | FMT | (1u << 16) | ((HD >> 3) << 17) | ((128 >> 4) << 24);
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t k_full[C::NK], k_free[C::NK], v_full[C::NV], v_free[C::NV], s_full[2][2], p_full[2][2], o_done[2][2], q_full, mma_done;
+  __shared__ uint64_t k_full[C::NK], k_free[C::NK], v_full[C::NV], v_free[C::NV], s_full[2], p_full[2][2], h_done[2], o_done[2], v_seen[2], q_full, mma_done;
   __shared__ uint32_t tmem_sh;
   __shared__ int odd_v, sh_s;
   __shared__ long long sh_base, sh_sum[kThreads / 32 + 1];
@@ -354,10 +355,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   if (tid == 0) {
-    for (int i = 0; i < C::NK; ++i) { mb_init(&k_full[i], 1); mb_init(&k_free[i], PAIR ? 2 : 1); }
-    for (int i = 0; i < C::NV; ++i) { mb_init(&v_full[i], 1); mb_init(&v_free[i], PAIR ? 2 : 1); }
+    for (int i = 0; i < C::NK; ++i) { mb_init(&k_full[i], 1); mb_init(&k_free[i], 2); }
+    for (int i = 0; i < C::NV; ++i) { mb_init(&v_full[i], 1); mb_init(&v_free[i], 2); }
     for (int i = 0; i < 2; ++i) {
-      for (int b = 0; b < 2; ++b) { mb_init(&s_full[i][b], 1); mb_init(&p_full[i][b], 4); mb_init(&o_done[i][b], 1); }
+      mb_init(&s_full[i], 1);
+      mb_init(&h_done[i], 1);
+      mb_init(&o_done[i], 1);
+      mb_init(&v_seen[i], 1);
+      for (int h = 0; h < 2; ++h) mb_init(&p_full[i][h], 4);
     }
     mb_init(&q_full, 8);
     mb_init(&mma_done, 2);
@@ -434,93 +439,105 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int c = max(0, issued - nring); c < issued; ++c) ok &= mb_wait_warp(&full[c % nring], (c / nring) & 1);
   } else if (warp < 3) {
     /* ------------------------------------------------ MMA issue: a warp a stream walks, one elected lane
-       issues.  Issuing is what limits a stream (waits, MMAs and commits of a tile take one thread some
-       800 cycles), so the loop is kept short: descriptors are a base plus a constant, ring places
-       are counted, and a wait that failed only makes the later ones pass (nothing leaves the loop) */
+       issues.  What one thread does for a tile (waits, MMAs, commits) takes about as long as its
+       arithmetic, so descriptors are a base plus a constant and ring places are counted.
+       A parity wait can tell a phase from the one before and after only, so nobody may skip one: both
+       warps look at every K and V tile, and a tile is free when both have (the stream that does not
+       use it at once).  On a wait that fails the warp stops; nothing is issued after that. */
     const int X = warp - 1;
-    constexpr int STEP = PAIR ? 1 : 2; /* tiles of the ring from one of this stream's to the next */
-    uint32_t used = 0, qp = 0, pp = 0; /* tiles of earlier pieces, phases of q_full and of p_full[X][b] in bit b */
+    uint32_t qp = 0, pp = 0; /* phases of q_full and of p_full[X] */
+    int ks = 0, vs = 0;      /* next tile of the rings, and its phase */
+    uint32_t kp = 0, vp = 0;
     const uint64_t dq = desc_k(sa(q_sm)) + (PAIR ? X * (C::QTILE >> 4) : 0), dk = desc_k(sa(k_sm)), dv = desc_mn(sa(v_sm));
     const uint32_t ds = tmem + X * 128, dov = tmem + 256 + X * HD;
-    auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && mb_wait(bar, parity); };
-    while (walk.next(a, p, &pc)) {
-      wait(&q_full, qp);
+    while (ok && walk.next(a, p, &pc)) {
+      ok = mb_wait_warp(&q_full, qp);
       qp ^= 1;
-      const int n = n_of(X);
-      const uint32_t first = used + (PAIR ? 0 : X);
-      int ks = first % C::NK, vs = first % C::NV;
-      uint32_t kp = first / C::NK & 1, vp = first / C::NV & 1;
-      used += pc.n;
-      if (PAIR && n == 0) { /* no rows: the tiles pass by */
-        for (int i = 0; i < pc.n; ++i) {
-          wait(&k_full[ks], kp);
-          wait(&v_full[vs], vp);
-          __syncwarp();
-          if (lane == 0) { mb_arrive(&k_free[ks]); mb_arrive(&v_free[vs]); }
+      const int n = n_of(X), clear = min(tree_open(a, pc.q), pc.q.len);
+      int kt = 0, vt = 0; /* tiles of the piece seen so far */
+      auto mine = [&](int t) { return PAIR ? n > 0 : (t & 1) == X; };
+      /* pass the other stream's tiles up to this stream's next, or to the end */
+      auto next_k = [&]() {
+        while (ok && kt < pc.n && !mine(kt)) {
+          ok = mb_wait_warp(&k_full[ks], kp);
+          if (ok && lane == 0) mb_arrive(&k_free[ks]);
           if (++ks == C::NK) { ks = 0; kp ^= 1; }
-          if (++vs == C::NV) { vs = 0; vp ^= 1; }
+          ++kt;
         }
-        continue;
-      }
-      auto qk = [&](int b) {
+        return ok && kt < pc.n;
+      };
+      auto next_v = [&]() {
+        while (ok && vt < pc.n && !mine(vt)) {
+          ok = mb_wait_warp(&v_full[vs], vp);
+          if (ok && lane == 0) mb_arrive(&v_free[vs]);
+          if (++vs == C::NV) { vs = 0; vp ^= 1; }
+          ++vt;
+        }
+        return ok && vt < pc.n;
+      };
+      auto qk = [&]() {
+        if (!next_k()) return;
+        ok = mb_wait_warp(&k_full[ks], kp);
+        if (!ok) return;
         tc_after();
         if (elect()) {
           const uint64_t k0 = dk + ks * (C::TILE >> 4);
 #pragma unroll
           for (int j = 0; j < HD / 16; ++j)
-            mma_ss(ds + b * TK, dq + (((j >> 2) * (TQ * 128) + (j & 3) * 32) >> 4), k0 + (((j >> 2) * (TK * 128) + (j & 3) * 32) >> 4),
-                   ID_S, j > 0);
-          commit(&s_full[X][b]);
+            mma_ss(ds, dq + (((j >> 2) * (TQ * 128) + (j & 3) * 32) >> 4), k0 + (((j >> 2) * (TK * 128) + (j & 3) * 32) >> 4), ID_S, j > 0);
+          commit(&s_full[X]);
           commit(&k_free[ks]);
         }
         __syncwarp();
-        ks += STEP;
-        if (ks >= C::NK) { ks -= C::NK; kp ^= 1; }
+        if (++ks == C::NK) { ks = 0; kp ^= 1; }
+        ++kt;
       };
-      for (int i = 0; i < min(n, 2); ++i) {
-        wait(&k_full[ks], kp);
-        qk(i);
-      }
-      for (int i = 0; i < n; ++i) {
-        const int b = i & 1;
-        const bool more = i + 2 < n;
-        /* V and weights for this tile's product, K for the scores after the next: asked for together,
-           since an answer takes long; waited for one by one if they are not there */
-        const bool hv = mb_test(&v_full[vs], vp), hk = !more || mb_test(&k_full[ks], kp);
-        const bool hp = mb_test(&p_full[X][b], (pp >> b) & 1);
-        if (!hv) wait(&v_full[vs], vp);
-        if (!hp) wait(&p_full[X][b], (pp >> b) & 1);
-        pp ^= 1u << b;
-        if (!hk) wait(&k_full[ks], kp);
-        __syncwarp();
-        tc_after();
-        if (elect()) {
-          const uint64_t v0 = dv + vs * (C::TILE >> 4);
-          const uint32_t pa = ds + b * TK;
-          mma_ts(dov, pa, v0, ID_O, i > 0);
+      if (ok) qk();
+      for (int i = 0; i < n && ok; ++i) {
+        if (!next_v()) break;
+        ok = mb_wait_warp(&v_full[vs], vp);
+        if (!ok) break;
+        if ((pc.t0 + vt + 1) * TK > clear && lane == 0) mb_arrive(&v_seen[X]); /* masked: the softmax warps look it over */
+        const uint64_t v0 = dv + vs * (C::TILE >> 4);
 #pragma unroll
-          for (int j = 1; j < TK / 16; ++j) mma_ts(dov, pa + j * 8, v0 + ((j * 2048) >> 4), ID_O, 1);
-          commit(&o_done[X][b]);
-          commit(&v_free[vs]);
+        for (int h = 0; h < 2; ++h) {
+          ok = ok && mb_wait_warp(&p_full[X][h], pp);
+          if (!ok) break;
+          tc_after();
+          if (elect()) {
+            mma_ts(dov, ds + h * 32, v0 + ((h * TH * 128) >> 4), ID_O, i > 0 || h > 0);
+#pragma unroll
+            for (int j = 1; j < TH / 16; ++j) mma_ts(dov, ds + h * 32 + j * 8, v0 + ((h * TH * 128 + j * 2048) >> 4), ID_O, 1);
+            if (h == 0) commit(&h_done[X]);
+            else commit(&v_free[vs]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
-        vs += STEP;
-        if (vs >= C::NV) { vs -= C::NV; vp ^= 1; }
-        if (more) qk(b);
+        if (!ok) break;
+        pp ^= 1;
+        if (++vs == C::NV) { vs = 0; vp ^= 1; }
+        ++vt;
+        qk();
       }
+      next_k();
+      next_v();
+      /* the piece is through, without tiles too: the softmax warps wait for it, so they cannot start two
+         pieces while this warp has not seen one */
+      if (ok && elect()) commit(&o_done[X]);
+      __syncwarp();
     }
     /* everything issued completes before TMEM is freed */
     if (elect()) commit(&mma_done);
     __syncwarp();
-    wait(&mma_done, 0);
+    ok = mb_wait_warp(&mma_done, 0) && ok;
   } else {
     /* ------------------------------------------------ softmax: one thread a row */
     const int X = (warp - 4) >> 2, row = tid - 128 - X * 128; /* stream, row of its tile = TMEM lane */
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t to = tmem + lanes + 256 + X * HD;
+    const uint32_t ts = tmem + lanes + X * 128, to = tmem + lanes + 256 + X * HD;
     constexpr int n_blk = TK / 16; /* 16-position blocks of a tile */
     uint32_t used = 0;       /* V tiles of earlier pieces */
-    uint32_t ns[2] = {0, 0}; /* tiles seen a buffer: phases of its s_full, p_full and o_done */
+    uint32_t sp = 0, op = 0, vsp = 0; /* phases of s_full and h_done (a tile each), o_done (a piece), v_seen (a masked tile) */
     while (walk.next(a, p, &pc)) {
       /* Q of this CTA's rows, swizzled; rows past the tile's queries are zero */
       constexpr int QW = C::NQ * TQ * (HD / 8) / 256; /* 16-byte words a thread: all loads first */
@@ -539,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       fence_async();
       __syncwarp();
-      if (lane == 0) mb_arrive(&q_full);
+      if (lane == 0 && ok) mb_arrive(&q_full);
 
       const int r = (PAIR ? X * 128 : 0) + row, qi = pc.q0 + r;
       const bool live = r < pc.nq, warp_live = r - lane < pc.nq;
@@ -561,108 +578,112 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int t = pc.t0 + (PAIR ? i : 2 * i + X), pos = t * TK;
         uint32_t blocks = 0xffffffffu; /* which 16-position blocks of the tile are mapped */
         if (holes) blocks = __ballot_sync(0xffffffffu, lane >= n_blk || page_at(pos + lane * 16) != -2);
-        const int b = i & 1;
-        const uint32_t ts = tmem + lanes + X * 128 + b * TK;
-        if (!mb_wait_warp(&s_full[X][b], (b ? ns[1]++ : ns[0]++) & 1)) { ok = false; break; }
+        if (!mb_wait_warp(&s_full[X], sp)) { ok = false; break; }
         tc_after();
-        if (warp_live) {
-          uint32_t sr[TK];
+        const bool masked = (t + 1) * TK > open || pos + TK > pc.q.len;
+#pragma unroll 1
+        for (int h = 0; h < 2 && ok; ++h) {
+          if (warp_live) {
+            uint32_t sr[TH];
 #pragma unroll
-          for (int c = 0; c < TK; c += 32) tm_ld(ts + c, sr + c);
-          tm_ld_wait();
-          if ((t + 1) * TK > open || pos + TK > pc.q.len || blocks != 0xffffffffu) {
+            for (int c = 0; c < TH; c += 32) tm_ld(ts + h * TH + c, sr + c);
+            tm_ld_wait();
+            if (masked || blocks != 0xffffffffu) {
 #pragma unroll
-            for (int c = 0; c < TK; c += 32) {
-              const uint32_t see = sees32(a, pc.q, ri, pos + c, blocks, c);
+              for (int c = 0; c < TH; c += 32) {
+                const uint32_t see = sees32(a, pc.q, ri, pos + h * TH + c, blocks, h * TH + c);
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!((see >> e) & 1u)) sr[c + e] = 0xff800000u; /* -inf */
-            }
-          }
-          /* weights against the maximum so far, the tile's own maximum beside them: only when a row's
-             has grown by more than 2^8 (its first tile, seldom later) are they taken again */
-          uint32_t pk[TK / 2];
-          float sum = 0.f;
-          auto weights = [&](float u) {
-            const uint64_t sc2 = two(a.scale2, a.scale2), mu = two(-u, -u);
-            uint64_t l0 = two(0.f, 0.f), l1 = l0;
-#pragma unroll
-            for (int c = 0; c < TK; c += 4) {
-              const float2 e0 = both(fma2(two(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), sc2, mu));
-              const float2 e1 = both(fma2(two(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), sc2, mu));
-              const float p0 = ex2(e0.x), p1 = ex2(e0.y), p2 = ex2(e1.x), p3 = ex2(e1.y);
-              l0 = add2(l0, two(p0, p1));
-              l1 = add2(l1, two(p2, p3));
-              pk[c / 2] = pack2<T>(p0, p1);
-              pk[c / 2 + 1] = pack2<T>(p2, p3);
-            }
-            const float2 y = both(add2(l0, l1));
-            sum = y.x + y.y;
-          };
-          weights(m == -INFINITY ? 0.f : m);
-          float x0 = __uint_as_float(sr[0]), x1 = __uint_as_float(sr[1]);
-#pragma unroll
-          for (int c = 2; c + 3 < TK; c += 4) {
-            x0 = max3(x0, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
-            x1 = max3(x1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
-          }
-          const float top = fmaxf(max3(x0, __uint_as_float(sr[TK - 2]), __uint_as_float(sr[TK - 1])), x1) * a.scale2;
-          const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
-          if (__any_sync(0xffffffffu, grow)) {
-            const float f = grow ? (m == -INFINITY ? 0.f : ex2(m - top)) : 1.f;
-            if (grow) m = top;
-            l *= f;
-            if (i > 0) { /* the first product overwrites O */
-              if (!mb_wait_warp(&o_done[X][b ^ 1], ((b ? ns[0] : ns[1]) - 1) & 1)) ok = false;
-              tc_after();
-              uint32_t or_[32];
-#pragma unroll
-              for (int c = 0; c < HD; c += 32) {
-                tm_ld(to + c, or_);
-                tm_ld_wait();
-#pragma unroll
-                for (int e = 0; e < 32; ++e) or_[e] = __float_as_uint(__uint_as_float(or_[e]) * f);
-                tm_st(to + c, or_);
+                for (int e = 0; e < 32; ++e)
+                  if (!((see >> e) & 1u)) sr[c + e] = 0xff800000u; /* -inf */
               }
             }
-            weights(m == -INFINITY ? 0.f : m);
-          }
-          l += sum;
-          tm_st(ts, pk);
-        }
-        if ((t + 1) * TK > open || pos + TK > pc.q.len) {
-          /* masked tile: its V elements that are not finite leave it before the product reads it.  With
-             PAIR both streams look; what one has cleared the other finds clear, and no product of a
-             stream starts before that stream has looked at the whole tile. */
-          const uint32_t cvt = used + (uint32_t)(t - pc.t0);
-          ok = ok && mb_wait_warp(&v_full[cvt % C::NV], (cvt / C::NV) & 1);
-          uint4* const v = reinterpret_cast<uint4*>(v_sm + cvt % C::NV * C::TILE);
-          constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
-          for (int j = row; j < C::TILE / 16; j += 128) {
-            const uint4 x = v[j];
-            uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            bool hit = false;
+            /* weights against the maximum so far, the half tile's own maximum beside them: only when a
+               row's has grown by more than 2^8 (its first tile, seldom later) are they taken again */
+            uint32_t pk[TH / 2];
+            float sum = 0.f;
+            auto weights = [&](float u) {
+              const uint64_t sc2 = two(a.scale2, a.scale2), mu = two(-u, -u);
+              uint64_t l0 = two(0.f, 0.f), l1 = l0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if ((w[e] & E) == E) { w[e] &= 0xffff0000u; hit = true; }
-              if (((w[e] >> 16) & E) == E) { w[e] &= 0x0000ffffu; hit = true; }
+              for (int c = 0; c < TH; c += 4) {
+                const float2 e0 = both(fma2(two(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), sc2, mu));
+                const float2 e1 = both(fma2(two(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), sc2, mu));
+                const float p0 = ex2(e0.x), p1 = ex2(e0.y), p2 = ex2(e1.x), p3 = ex2(e1.y);
+                l0 = add2(l0, two(p0, p1));
+                l1 = add2(l1, two(p2, p3));
+                pk[c / 2] = pack2<T>(p0, p1);
+                pk[c / 2 + 1] = pack2<T>(p2, p3);
+              }
+              const float2 y = both(add2(l0, l1));
+              sum = y.x + y.y;
+            };
+            weights(m == -INFINITY ? 0.f : m);
+            float x0 = __uint_as_float(sr[0]), x1 = __uint_as_float(sr[1]);
+#pragma unroll
+            for (int c = 2; c + 3 < TH; c += 4) {
+              x0 = max3(x0, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+              x1 = max3(x1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
             }
-            if (hit) {
-              odd_v = 1;
-              v[j] = make_uint4(w[0], w[1], w[2], w[3]);
+            const float top = fmaxf(max3(x0, __uint_as_float(sr[TH - 2]), __uint_as_float(sr[TH - 1])), x1) * a.scale2;
+            const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
+            if (__any_sync(0xffffffffu, grow)) {
+              const float f = grow ? (m == -INFINITY ? 0.f : ex2(m - top)) : 1.f;
+              if (grow) m = top;
+              l *= f;
+              if (i > 0 || h > 0) { /* the first product overwrites O */
+                /* products of earlier tiles are complete (they were issued before this tile's scores) */
+                if (h > 0 && !mb_wait_warp(&h_done[X], sp)) ok = false;
+                tc_after();
+                uint32_t or_[32];
+#pragma unroll
+                for (int c = 0; c < HD; c += 32) {
+                  tm_ld(to + c, or_);
+                  tm_ld_wait();
+#pragma unroll
+                  for (int e = 0; e < 32; ++e) or_[e] = __float_as_uint(__uint_as_float(or_[e]) * f);
+                  tm_st(to + c, or_);
+                }
+              }
+              weights(m == -INFINITY ? 0.f : m);
             }
+            l += sum;
+            tm_st(ts + h * 32, pk); /* over scores already read */
           }
-          fence_async();
+          if (masked && h == 0) {
+            /* V elements of a masked tile that are not finite leave it before the products read it.  With
+               PAIR both streams look; what one has cleared the other finds clear, and no product of a
+               stream starts before that stream has looked at the whole tile. */
+            const uint32_t cvt = used + (uint32_t)(t - pc.t0);
+            ok = mb_wait_warp(&v_seen[X], vsp) && ok;
+            vsp ^= 1;
+            uint4* const v = reinterpret_cast<uint4*>(v_sm + cvt % C::NV * C::TILE);
+            constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+            for (int j = row; j < C::TILE / 16; j += 128) {
+              const uint4 x = v[j];
+              uint32_t w[4] = {x.x, x.y, x.z, x.w};
+              bool hit = false;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if ((w[e] & E) == E) { w[e] &= 0xffff0000u; hit = true; }
+                if (((w[e] >> 16) & E) == E) { w[e] &= 0x0000ffffu; hit = true; }
+              }
+              if (hit) {
+                odd_v = 1;
+                v[j] = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            }
+            fence_async();
+          }
+          if (warp_live) tm_st_wait();
+          tc_before();
+          __syncwarp();
+          if (lane == 0 && ok) mb_arrive(&p_full[X][h]);
         }
-        if (warp_live) tm_st_wait();
-        tc_before();
-        __syncwarp();
-        if (lane == 0) mb_arrive(&p_full[X][b]);
+        sp ^= 1;
       }
       /* ---- the piece's end */
-      /* the last two products may be under way, one a buffer (scores n - 1 came after product n - 3) */
-      if (n > 0 && ok) ok = mb_wait_warp(&o_done[X][0], (ns[0] - 1) & 1);
-      if (n > 1 && ok) ok = mb_wait_warp(&o_done[X][1], (ns[1] - 1) & 1);
+      if (ok) ok = mb_wait_warp(&o_done[X], op);
+      op ^= 1;
       used += pc.n;
       tc_after();
       const bool whole = pc.n == pc.n_tile;
