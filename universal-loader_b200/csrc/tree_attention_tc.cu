@@ -2,7 +2,7 @@
  * tree_attention_tc.cu — ulb_tree_attention on the 5th-generation tensor cores, for head
  * dims 64 and 128.  Same mathematics and masking as tree_attention.cu.
  *
- * A CTA works on 128-key tiles with M = 128 query rows a stream, two streams at a time, each
+ * A CTA works on 64-key tiles with M = 128 query rows a stream, two streams at a time, each
  * with its own running (m, l, o) and its own softmax warpgroup (one thread a row):
  *   PAIR = false  (at most 128 queries a kv head): both streams hold the same rows and take the
  *                 even and the odd tiles; they join in shared memory at the end
@@ -18,11 +18,11 @@
  * Warps: 0 TMA (pages -> 128-byte-swizzled tiles, one box a page, pages that are unmapped or past
  * the end read as zero through an out-of-range coordinate), 1 issues every MMA and the commits
  * that free tiles, 2 - 3 take V elements that are not finite out of masked tiles, 4 - 7 and 8 - 11
- * softmax.  Barriers carry it: K / V tiles full and free, S full, P full (a half tile each, so that the
- * first half's product runs beside the second half's exponentials).  One thread issues a stream's
- * MMAs and they complete in order: S full of a tile means that O holds every earlier tile.
- * (64-key tiles with two score buffers a stream took 297 us where this takes HERE: what a tile costs
- * besides its arithmetic, waits, commits and the narrower product, then counts twice.)
+ * softmax.  Barriers carry it: K / V tiles full and free, S full, P full, O += P V done (looked at only to
+ * rescale O).  A stream has two score buffers; one thread issues its MMAs and they complete in order,
+ * so a buffer is free for the tile after the next once the product that reads its weights has been
+ * issued, and the scores of the next tile are there while weights are computed (128-key tiles with one
+ * buffer, weights handed over in halves, took 339 us where this took 297).
  *
  * Work is cut evenly: the tiles of all (sequence, kv head) pairs form one line, every CTA (group
  * of CTAs, when more than 256 rows need several row tiles: its members walk the same keys side by
@@ -44,11 +44,10 @@
 namespace ulb {
 namespace {
 
-constexpr int TK = 128;        /* keys a tile */
-constexpr int TH = 64;         /* keys of half a tile: the step of softmax and of O += P V */
+constexpr int TK = 64;         /* keys a tile */
 constexpr int TQ = 128;        /* query rows a stream: M */
 constexpr int kThreads = 384;  /* 4 role warps, 2 x 4 softmax warps */
-constexpr int kMinTiles = 4;   /* tiles a group takes at least */
+constexpr int kMinTiles = 8;   /* tiles a group takes at least */
 constexpr int kJoinRows = 8;   /* rows a block of the join kernel: a warp each */
 
 __device__ __forceinline__ uint32_t sa(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -180,8 +179,8 @@ struct TcCfg {
   static constexpr int TILE = TK * HD * 2;            /* bytes of a K or V tile */
   static constexpr int QTILE = TQ * HD * 2;
   static constexpr int NQ = PAIR ? 2 : 1;
-  static constexpr int NK = HD == 64 ? 5 : 3;         /* K tiles in the ring */
-  static constexpr int NV = HD == 64 ? 5 : PAIR ? 2 : 3;
+  static constexpr int NK = HD == 64 ? 8 : PAIR ? 5 : 6; /* K tiles in the ring */
+  static constexpr int NV = HD == 64 ? 8 : PAIR ? 5 : 6;
   static constexpr int SMEM = NQ * QTILE + (NK + NV) * TILE + 1024; /* + alignment slack */
   static constexpr int RT = PAIR ? 256 : 128;         /* queries a CTA */
   static_assert(SMEM <= 226 * 1024, "shared memory");
@@ -290,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr uint32_t ID_S = (1u << 4) | FMT | ((TK >> 3) << 17) | ((128 >> 4) << 24);
   constexpr uint32_t ID_O = (1u << 4) | FMT | (1u << 16) | ((HD >> 3) << 17) | ((128 >> 4) << 24);
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t k_full[C::NK], k_free[C::NK], v_full[C::NV], v_free[C::NV], s_full[2], p_full[2][2], h_done[2], o_done[2], v_seen[2], q_full, mma_done;
+  __shared__ uint64_t k_full[C::NK], k_free[C::NK], v_full[C::NV], v_free[C::NV], s_full[2][2], p_full[2][2], o_done[2][2], v_seen[2], piece[2], q_full, mma_done;
   __shared__ uint32_t tmem_sh;
   __shared__ int odd_v, sh_s;
   __shared__ long long sh_base, sh_sum[kThreads / 32 + 1];
@@ -358,11 +357,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < C::NK; ++i) { mb_init(&k_full[i], 1); mb_init(&k_free[i], 2); }
     for (int i = 0; i < C::NV; ++i) { mb_init(&v_full[i], 1); mb_init(&v_free[i], 2); }
     for (int i = 0; i < 2; ++i) {
-      mb_init(&s_full[i], 1);
-      mb_init(&h_done[i], 1);
-      mb_init(&o_done[i], 1);
       mb_init(&v_seen[i], 1);
-      for (int h = 0; h < 2; ++h) mb_init(&p_full[i][h], 4);
+      mb_init(&piece[i], 1);
+      for (int b = 0; b < 2; ++b) { mb_init(&s_full[i][b], 1); mb_init(&p_full[i][b], 4); mb_init(&o_done[i][b], 1); }
     }
     mb_init(&q_full, 8);
     mb_init(&mma_done, 2);
@@ -445,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1)
        warps look at every K and V tile, and a tile is free when both have (the stream that does not
        use it at once).  On a wait that fails the warp stops; nothing is issued after that. */
     const int X = warp - 1;
-    uint32_t qp = 0, pp = 0; /* phases of q_full and of p_full[X] */
+    uint32_t qp = 0, pp = 0; /* phases of q_full, and of p_full[X][b] in bit b */
     int ks = 0, vs = 0;      /* next tile of the rings, and its phase */
     uint32_t kp = 0, vp = 0;
     const uint64_t dq = desc_k(sa(q_sm)) + (PAIR ? X * (C::QTILE >> 4) : 0), dk = desc_k(sa(k_sm)), dv = desc_mn(sa(v_sm));
@@ -475,55 +472,59 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         return ok && vt < pc.n;
       };
-      auto qk = [&]() {
-        if (!next_k()) return;
-        ok = mb_wait_warp(&k_full[ks], kp);
-        if (!ok) return;
-        tc_after();
-        if (elect()) {
-          const uint64_t k0 = dk + ks * (C::TILE >> 4);
+      auto qk = [&](int b) { /* scores of K tile kt into buffer b (one lane) */
+        const uint64_t k0 = dk + ks * (C::TILE >> 4);
 #pragma unroll
-          for (int j = 0; j < HD / 16; ++j)
-            mma_ss(ds, dq + (((j >> 2) * (TQ * 128) + (j & 3) * 32) >> 4), k0 + (((j >> 2) * (TK * 128) + (j & 3) * 32) >> 4), ID_S, j > 0);
-          commit(&s_full[X]);
-          commit(&k_free[ks]);
-        }
-        __syncwarp();
+        for (int j = 0; j < HD / 16; ++j)
+          mma_ss(ds + b * TK, dq + (((j >> 2) * (TQ * 128) + (j & 3) * 32) >> 4), k0 + (((j >> 2) * (TK * 128) + (j & 3) * 32) >> 4), ID_S,
+                 j > 0);
+        commit(&s_full[X][b]);
+        commit(&k_free[ks]);
+      };
+      auto step_k = [&]() {
         if (++ks == C::NK) { ks = 0; kp ^= 1; }
         ++kt;
       };
-      if (ok) qk();
+      for (int i = 0; i < min(n, 2) && ok; ++i) {
+        ok = next_k() && mb_wait_warp(&k_full[ks], kp);
+        if (!ok) break;
+        tc_after();
+        if (elect()) qk(i);
+        __syncwarp();
+        step_k();
+      }
       for (int i = 0; i < n && ok; ++i) {
-        if (!next_v()) break;
-        ok = mb_wait_warp(&v_full[vs], vp);
+        const int b = i & 1;
+        const bool more = i + 2 < n;
+        /* the rings first, they are mostly ready; then the weights */
+        ok = next_v() && mb_wait_warp(&v_full[vs], vp);
         if (!ok) break;
         if ((pc.t0 + vt + 1) * TK > clear && lane == 0) mb_arrive(&v_seen[X]); /* masked: the softmax warps look it over */
-        const uint64_t v0 = dv + vs * (C::TILE >> 4);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          ok = ok && mb_wait_warp(&p_full[X][h], pp);
-          if (!ok) break;
-          tc_after();
-          if (elect()) {
-            mma_ts(dov, ds + h * 32, v0 + ((h * TH * 128) >> 4), ID_O, i > 0 || h > 0);
-#pragma unroll
-            for (int j = 1; j < TH / 16; ++j) mma_ts(dov, ds + h * 32 + j * 8, v0 + ((h * TH * 128 + j * 2048) >> 4), ID_O, 1);
-            if (h == 0) commit(&h_done[X]);
-            else commit(&v_free[vs]);
-          }
-          __syncwarp();
-        }
+        if (more) ok = next_k() && mb_wait_warp(&k_full[ks], kp);
+        ok = ok && mb_wait_warp(&p_full[X][b], (pp >> b) & 1);
         if (!ok) break;
-        pp ^= 1;
+        pp ^= 1u << b;
+        tc_after();
+        if (elect()) {
+          const uint64_t v0 = dv + vs * (C::TILE >> 4);
+          const uint32_t pa = ds + b * TK;
+          mma_ts(dov, pa, v0, ID_O, i > 0);
+#pragma unroll
+          for (int j = 1; j < TK / 16; ++j) mma_ts(dov, pa + j * 8, v0 + ((j * 2048) >> 4), ID_O, 1);
+          commit(&o_done[X][b]);
+          commit(&v_free[vs]);
+          if (more) qk(b);
+        }
+        __syncwarp();
         if (++vs == C::NV) { vs = 0; vp ^= 1; }
         ++vt;
-        qk();
+        if (more) step_k();
       }
       next_k();
       next_v();
       /* the piece is through, without tiles too: the softmax warps wait for it, so they cannot start two
          pieces while this warp has not seen one */
-      if (ok && elect()) commit(&o_done[X]);
+      if (ok && elect()) commit(&piece[X]);
       __syncwarp();
     }
     /* everything issued completes before TMEM is freed */
@@ -534,10 +535,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     /* ------------------------------------------------ softmax: one thread a row */
     const int X = (warp - 4) >> 2, row = tid - 128 - X * 128; /* stream, row of its tile = TMEM lane */
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + X * 128, to = tmem + lanes + 256 + X * HD;
+    const uint32_t to = tmem + lanes + 256 + X * HD;
     constexpr int n_blk = TK / 16; /* 16-position blocks of a tile */
     uint32_t used = 0;       /* V tiles of earlier pieces */
-    uint32_t sp = 0, op = 0, vsp = 0; /* phases of s_full and h_done (a tile each), o_done (a piece), v_seen (a masked tile) */
+    uint32_t sp = 0, op = 0, vsp = 0; /* phases of s_full[X][b] and o_done[X][b] in bit b, of piece and v_seen */
     while (walk.next(a, p, &pc)) {
       /* Q of this CTA's rows, swizzled; rows past the tile's queries are zero */
       constexpr int QW = C::NQ * TQ * (HD / 8) / 256; /* 16-byte words a thread: all loads first */
@@ -578,111 +579,106 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int t = pc.t0 + (PAIR ? i : 2 * i + X), pos = t * TK;
         uint32_t blocks = 0xffffffffu; /* which 16-position blocks of the tile are mapped */
         if (holes) blocks = __ballot_sync(0xffffffffu, lane >= n_blk || page_at(pos + lane * 16) != -2);
-        if (!mb_wait_warp(&s_full[X], sp)) { ok = false; break; }
+        const int b = i & 1;
+        const uint32_t ts = tmem + lanes + X * 128 + b * TK;
+        if (!mb_wait_warp(&s_full[X][b], (sp >> b) & 1)) { ok = false; break; }
         tc_after();
         const bool masked = (t + 1) * TK > open || pos + TK > pc.q.len;
-#pragma unroll 1
-        for (int h = 0; h < 2 && ok; ++h) {
-          if (warp_live) {
-            uint32_t sr[TH];
+        if (warp_live) {
+          uint32_t sr[TK];
 #pragma unroll
-            for (int c = 0; c < TH; c += 32) tm_ld(ts + h * TH + c, sr + c);
-            tm_ld_wait();
-            if (masked || blocks != 0xffffffffu) {
+          for (int c = 0; c < TK; c += 32) tm_ld(ts + c, sr + c);
+          tm_ld_wait();
+          if (masked || blocks != 0xffffffffu) {
 #pragma unroll
-              for (int c = 0; c < TH; c += 32) {
-                const uint32_t see = sees32(a, pc.q, ri, pos + h * TH + c, blocks, h * TH + c);
+            for (int c = 0; c < TK; c += 32) {
+              const uint32_t see = sees32(a, pc.q, ri, pos + c, blocks, c);
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                  if (!((see >> e) & 1u)) sr[c + e] = 0xff800000u; /* -inf */
-              }
+              for (int e = 0; e < 32; ++e)
+                if (!((see >> e) & 1u)) sr[c + e] = 0xff800000u; /* -inf */
             }
-            /* weights against the maximum so far, the half tile's own maximum beside them: only when a
-               row's has grown by more than 2^8 (its first tile, seldom later) are they taken again */
-            uint32_t pk[TH / 2];
-            float sum = 0.f;
-            auto weights = [&](float u) {
-              const uint64_t sc2 = two(a.scale2, a.scale2), mu = two(-u, -u);
-              uint64_t l0 = two(0.f, 0.f), l1 = l0;
+          }
+          /* weights against the maximum so far, the tile's own maximum beside them: only when a row's
+             has grown by more than 2^8 (its first tile, seldom later) are they taken again */
+          uint32_t pk[TK / 2];
+          float sum = 0.f, top = 0.f;
+          auto weights = [&](float u) {
+            const uint64_t sc2 = two(a.scale2, a.scale2), mu = two(-u, -u);
+            uint64_t l0 = two(0.f, 0.f), l1 = l0;
+            float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
-              for (int c = 0; c < TH; c += 4) {
-                const float2 e0 = both(fma2(two(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), sc2, mu));
-                const float2 e1 = both(fma2(two(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), sc2, mu));
-                const float p0 = ex2(e0.x), p1 = ex2(e0.y), p2 = ex2(e1.x), p3 = ex2(e1.y);
-                l0 = add2(l0, two(p0, p1));
-                l1 = add2(l1, two(p2, p3));
-                pk[c / 2] = pack2<T>(p0, p1);
-                pk[c / 2 + 1] = pack2<T>(p2, p3);
-              }
-              const float2 y = both(add2(l0, l1));
-              sum = y.x + y.y;
-            };
-            weights(m == -INFINITY ? 0.f : m);
-            float x0 = __uint_as_float(sr[0]), x1 = __uint_as_float(sr[1]);
-#pragma unroll
-            for (int c = 2; c + 3 < TH; c += 4) {
+            for (int c = 0; c < TK; c += 4) {
+              const float2 e0 = both(fma2(two(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), sc2, mu));
+              const float2 e1 = both(fma2(two(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), sc2, mu));
+              const float p0 = ex2(e0.x), p1 = ex2(e0.y), p2 = ex2(e1.x), p3 = ex2(e1.y);
               x0 = max3(x0, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
               x1 = max3(x1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
+              l0 = add2(l0, two(p0, p1));
+              l1 = add2(l1, two(p2, p3));
+              pk[c / 2] = pack2<T>(p0, p1);
+              pk[c / 2 + 1] = pack2<T>(p2, p3);
             }
-            const float top = fmaxf(max3(x0, __uint_as_float(sr[TH - 2]), __uint_as_float(sr[TH - 1])), x1) * a.scale2;
-            const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
-            if (__any_sync(0xffffffffu, grow)) {
-              const float f = grow ? (m == -INFINITY ? 0.f : ex2(m - top)) : 1.f;
-              if (grow) m = top;
-              l *= f;
-              if (i > 0 || h > 0) { /* the first product overwrites O */
-                /* products of earlier tiles are complete (they were issued before this tile's scores) */
-                if (h > 0 && !mb_wait_warp(&h_done[X], sp)) ok = false;
-                tc_after();
-                uint32_t or_[32];
+            const float2 y = both(add2(l0, l1));
+            sum = y.x + y.y;
+            top = fmaxf(x0, x1) * a.scale2;
+          };
+          weights(m == -INFINITY ? 0.f : m);
+          const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float f = grow ? (m == -INFINITY ? 0.f : ex2(m - top)) : 1.f;
+            if (grow) m = top;
+            l *= f;
+            if (i > 0) { /* the first product overwrites O; products before the last are complete */
+              if (!mb_wait_warp(&o_done[X][b ^ 1], ((sp >> (b ^ 1)) & 1) ^ 1)) ok = false;
+              tc_after();
+              uint32_t or_[32];
 #pragma unroll
-                for (int c = 0; c < HD; c += 32) {
-                  tm_ld(to + c, or_);
-                  tm_ld_wait();
+              for (int c = 0; c < HD; c += 32) {
+                tm_ld(to + c, or_);
+                tm_ld_wait();
 #pragma unroll
-                  for (int e = 0; e < 32; ++e) or_[e] = __float_as_uint(__uint_as_float(or_[e]) * f);
-                  tm_st(to + c, or_);
-                }
+                for (int e = 0; e < 32; ++e) or_[e] = __float_as_uint(__uint_as_float(or_[e]) * f);
+                tm_st(to + c, or_);
               }
-              weights(m == -INFINITY ? 0.f : m);
             }
-            l += sum;
-            tm_st(ts + h * 32, pk); /* over scores already read */
+            weights(m == -INFINITY ? 0.f : m);
           }
-          if (masked && h == 0) {
-            /* V elements of a masked tile that are not finite leave it before the products read it.  With
-               PAIR both streams look; what one has cleared the other finds clear, and no product of a
-               stream starts before that stream has looked at the whole tile. */
-            const uint32_t cvt = used + (uint32_t)(t - pc.t0);
-            ok = mb_wait_warp(&v_seen[X], vsp) && ok;
-            vsp ^= 1;
-            uint4* const v = reinterpret_cast<uint4*>(v_sm + cvt % C::NV * C::TILE);
-            constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
-            for (int j = row; j < C::TILE / 16; j += 128) {
-              const uint4 x = v[j];
-              uint32_t w[4] = {x.x, x.y, x.z, x.w};
-              bool hit = false;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if ((w[e] & E) == E) { w[e] &= 0xffff0000u; hit = true; }
-                if (((w[e] >> 16) & E) == E) { w[e] &= 0x0000ffffu; hit = true; }
-              }
-              if (hit) {
-                odd_v = 1;
-                v[j] = make_uint4(w[0], w[1], w[2], w[3]);
-              }
-            }
-            fence_async();
-          }
-          if (warp_live) tm_st_wait();
-          tc_before();
-          __syncwarp();
-          if (lane == 0 && ok) mb_arrive(&p_full[X][h]);
+          l += sum;
+          tm_st(ts, pk); /* over the scores */
         }
-        sp ^= 1;
+        if (masked) {
+          /* V elements of a masked tile that are not finite leave it before the product reads it.  With
+             PAIR both streams look; what one has cleared the other finds clear, and no product of a
+             stream starts before that stream has looked at the whole tile. */
+          const uint32_t cvt = used + (uint32_t)(t - pc.t0);
+          ok = mb_wait_warp(&v_seen[X], vsp) && ok;
+          vsp ^= 1;
+          uint4* const v = reinterpret_cast<uint4*>(v_sm + cvt % C::NV * C::TILE);
+          constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+          for (int j = row; j < C::TILE / 16; j += 128) {
+            const uint4 x = v[j];
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            bool hit = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if ((w[e] & E) == E) { w[e] &= 0xffff0000u; hit = true; }
+              if (((w[e] >> 16) & E) == E) { w[e] &= 0x0000ffffu; hit = true; }
+            }
+            if (hit) {
+              odd_v = 1;
+              v[j] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+          fence_async();
+        }
+        if (warp_live) tm_st_wait();
+        tc_before();
+        __syncwarp();
+        if (lane == 0 && ok) mb_arrive(&p_full[X][b]);
+        sp ^= 1u << b;
       }
       /* ---- the piece's end */
-      if (ok) ok = mb_wait_warp(&o_done[X], op);
+      if (ok) ok = mb_wait_warp(&piece[X], op);
       op ^= 1;
       used += pc.n;
       tc_after();
