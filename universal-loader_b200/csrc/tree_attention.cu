@@ -554,7 +554,7 @@ extern "C" int ulb_tree_attention(ulb_ctx* ctx, const ulb_cache_desc* cache, con
   a.err = ctx->c.dev_err;
   Ctx* c = &ctx->c;
   ULB_CUDA(cudaSetDevice(c->device));
-  if (a.g.hd == 64 || a.g.hd == 128) return launch_tree_tc(c, a, cache->dtype == ULB_TYPE_F16);
+  if (tree_tc_fits(c, a)) return launch_tree_tc(c, a, cache->dtype == ULB_TYPE_F16);
   return cache->dtype == ULB_TYPE_F16 ? pick_dim<__half>(c, a) : pick_dim<__nv_bfloat16>(c, a);
 }
 

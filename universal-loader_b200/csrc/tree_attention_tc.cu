@@ -47,7 +47,8 @@ namespace {
 constexpr int TK = 64;         /* keys a tile */
 constexpr int TQ = 128;        /* query rows a stream: M */
 constexpr int kThreads = 384;  /* 4 role warps, 2 x 4 softmax warps */
-constexpr int kMinTiles = 8;   /* tiles a group takes at least */
+constexpr int kPairCost = 6;   /* what a pair costs besides its tiles, in tiles */
+constexpr int kMinTiles = 12;  /* tiles of the line a group takes at least */
 constexpr int kJoinRows = 8;   /* rows a block of the join kernel: a warp each */
 
 __device__ __forceinline__ uint32_t sa(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -77,12 +78,6 @@ __device__ __forceinline__ bool mb_wait(uint64_t* b, uint32_t parity) {
 /* the same for a converged warp, one answer for all lanes (a vote: a shuffle would queue behind the
    softmax warps' exponentials, as every shared-memory operation does, for some 300 cycles) */
 __device__ __forceinline__ bool mb_wait_warp(uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, mb_wait(b, parity)); }
-__device__ __forceinline__ bool mb_test(uint64_t* b, uint32_t parity) {
-  uint32_t ok;
-  asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-               : "=r"(ok) : "r"(sa(b)), "r"(parity) : "memory");
-  return ok != 0;
-}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -189,7 +184,7 @@ struct TcCfg {
 /* what the launch adds to TreeArgs */
 struct TcPlan {
   int members, groups_max; /* CTAs that walk the same keys side by side, such groups in the grid */
-  int min_tiles;           /* tiles a group takes at least */
+  int min_tiles;           /* tiles of the line a group takes at least */
   struct TcTail* tail;     /* [groups][members] */
 };
 /* the head of a pair that goes on in the next groups: what the join kernel needs */
@@ -197,36 +192,45 @@ struct TcTail {
   int pieces, slot, r0, nq, q0, kvh, pad0, pad1; /* pieces 0: none */
 };
 
-/* the line of tiles */
+/* The line of work, in tiles.  A (sequence, kv head, pass) takes kPairCost places before its tiles, for what
+   it costs besides them: its rows are loaded, its outputs joined and written.  Group c's stretch. */
 struct Line {
-  long long total;
-  int groups;
-  __device__ __forceinline__ long long begin(int c) const { return total * c / groups; }
+  int total, groups, per, rem;
+  __device__ __forceinline__ void cut(int n) {
+    groups = n;
+    per = total / n;
+    rem = total - per * n;
+  }
+  __device__ __forceinline__ int begin(int c) const { return c * per + min(c, rem); }
+  __device__ __forceinline__ int group_of(int place) const {
+    const int big = rem * (per + 1);
+    return place < big ? place / (per + 1) : rem + (place - big) / per;
+  }
 };
-__device__ __forceinline__ long long seq_tiles(const TreeArgs& a, const TcPlan& p, const TreeSeq& q, int RT, int* n_tile, int* n_pass) {
+/* places of one sequence, its tiles a pair and passes over its rows */
+__device__ __forceinline__ int seq_places(const TreeArgs& a, const TcPlan& p, const TreeSeq& q, int RT, int* n_tile, int* n_pass) {
   *n_tile = max(1, (q.len + TK - 1) / TK);
-  *n_pass = (int)(((long long)q.n * a.G + (long long)RT * p.members - 1) / ((long long)RT * p.members));
-  return (long long)*n_tile * *n_pass * a.g.n_head_kv;
+  const int rows = RT * p.members;
+  *n_pass = q.n * a.G <= rows ? (q.n > 0 ? 1 : 0) : (q.n * a.G + rows - 1) / rows;
+  return (*n_tile + kPairCost) * *n_pass * a.g.n_head_kv;
 }
 
 struct Piece {
   TreeSeq q;
   int s, kvh, q0, nq; /* sequence, kv head, first query (row x group + head) of the tile, queries in it */
   int t0, n, n_tile;  /* tiles [t0, t0 + n) of n_tile */
-  long long first;    /* place of the pair's first tile on the line */
-  bool head;          /* the stretch's first piece */
+  int last;           /* place of the pair's last tile on the line */
+  int nth;            /* pieces of this CTA before it */
 };
 
 /* walks the pieces of one CTA; every role runs the same walk */
 template <int RT>
 struct Walk {
-  long long at, end, base;
-  int s, n_tile, n_pass, member;
-  long long cnt, start;
+  int at, end, base, cnt, s, n_tile, n_pass, member, nth;
   TreeSeq q;
   __device__ __forceinline__ void load(const TreeArgs& a, const TcPlan& p) {
     q = tree_seq(a, s);
-    cnt = seq_tiles(a, p, q, RT, &n_tile, &n_pass);
+    cnt = seq_places(a, p, q, RT, &n_tile, &n_pass);
   }
   __device__ __forceinline__ bool next(const TreeArgs& a, const TcPlan& p, Piece* o) {
     while (at < end) {
@@ -235,19 +239,20 @@ struct Walk {
         ++s;
         load(a, p);
       }
-      const long long u = (at - base) / n_tile;
-      o->t0 = (int)((at - base) - u * n_tile);
-      o->n = (int)min((long long)(n_tile - o->t0), end - at);
-      o->head = at == start;
-      o->first = base + u * n_tile;
-      at += o->n;
-      o->kvh = (int)(u / n_pass);
-      o->q0 = ((int)(u % n_pass) * p.members + member) * RT;
+      const int len = n_tile + kPairCost, u = (at - base) / len, in = at - base - u * len;
+      const int upto = min(len, in + end - at);
+      o->t0 = max(in - kPairCost, 0);
+      o->n = max(upto - kPairCost, 0) - o->t0;
+      o->last = base + u * len + len - 1;
+      at += upto - in;
+      o->kvh = n_pass == 1 ? u : u / n_pass;
+      o->q0 = ((n_pass == 1 ? 0 : u % n_pass) * p.members + member) * RT;
       o->nq = min(RT, q.n * a.G - o->q0);
-      if (o->nq <= 0) continue; /* this member has no rows of the sequence */
+      if (o->nq <= 0 || o->n <= 0) continue; /* this member has no rows of the sequence, or no tile yet */
       o->q = q;
       o->s = s;
       o->n_tile = n_tile;
+      o->nth = nth++;
       return true;
     }
     return false;
@@ -291,68 +296,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t k_full[C::NK], k_free[C::NK], v_full[C::NV], v_free[C::NV], s_full[2][2], p_full[2][2], o_done[2][2], v_seen[2], piece[2], q_full, mma_done;
   __shared__ uint32_t tmem_sh;
-  __shared__ int odd_v, sh_s;
-  __shared__ long long sh_base, sh_sum[kThreads / 32 + 1];
-  __shared__ float sh_ml[2][128];
+  __shared__ int odd_v, holes, sh_s, sh_base, sh_sum[kThreads / 32];
   uint8_t* const sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* const q_sm = sm;
   uint8_t* const k_sm = sm + C::NQ * C::QTILE;
   uint8_t* const v_sm = k_sm + C::NK * C::TILE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  pdl_wait();
-  pdl_trigger();
-  /* the line's length, then this group's place on it */
-  auto tiles_of = [&](int s) {
-    int nt, np;
-    return seq_tiles(a, p, tree_seq(a, s), C::RT, &nt, &np);
-  };
-  long long mine = 0;
-  for (int s = tid; s < a.g.n_seq; s += kThreads) mine += tiles_of(s);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) sh_sum[warp] = mine;
-  __syncthreads();
-  Line line;
-  line.total = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) line.total += sh_sum[w];
-  line.groups = (int)min((long long)p.groups_max, max(1ll, (line.total + p.min_tiles - 1) / p.min_tiles));
-  const int grp = blockIdx.x / p.members, member = blockIdx.x % p.members;
-  if (grp >= line.groups || line.total == 0) {
-    if (tid == 0) p.tail[blockIdx.x].pieces = 0;
-    return;
-  }
-  const long long begin = line.begin(grp), end = line.begin(grp + 1);
-  {
-    long long base = 0;
-    for (int s0 = 0; s0 < a.g.n_seq; s0 += kThreads) { /* the sequence that holds `begin` */
-      const int s = s0 + tid;
-      const long long c = s < a.g.n_seq ? tiles_of(s) : 0;
-      long long x = c;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      __syncthreads();
-      if (lane == 31) sh_sum[warp] = x;
-      __syncthreads();
-      long long all = 0;
-#pragma unroll
-      for (int w = 0; w < kThreads / 32; ++w) {
-        if (w < warp) x += sh_sum[w];
-        all += sh_sum[w];
-      }
-      const long long b = base + x - c;
-      if (c > 0 && b <= begin && begin < b + c) {
-        sh_s = s;
-        sh_base = b;
-      }
-      base += all;
-      if (base > begin) break; /* the same for every thread */
-    }
-  }
+  /* nothing here depends on earlier kernels */
   if (tid == 0) {
     for (int i = 0; i < C::NK; ++i) { mb_init(&k_full[i], 1); mb_init(&k_free[i], 2); }
     for (int i = 0; i < C::NV; ++i) { mb_init(&v_full[i], 1); mb_init(&v_free[i], 2); }
@@ -364,23 +315,74 @@ __global__ void __launch_bounds__(kThreads, 1)
     mb_init(&q_full, 8);
     mb_init(&mma_done, 2);
     odd_v = 0;
-    p.tail[blockIdx.x].pieces = 0;
+    holes = 0;
+    sh_s = 0;
+    sh_base = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sa(&tmem_sh)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  pdl_wait();
+  pdl_trigger();
+  if (tid == 0) p.tail[blockIdx.x].pieces = 0;
+  /* the line's length, then this group's place on it */
+  auto places_of = [&](int s) {
+    int nt, np;
+    return s < a.g.n_seq ? seq_places(a, p, tree_seq(a, s), C::RT, &nt, &np) : 0;
+  };
+  const int cnt0 = places_of(tid);
+  int mine = cnt0;
+  for (int s = tid + kThreads; s < a.g.n_seq; s += kThreads) mine += places_of(s);
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  if (lane == 0) sh_sum[warp] = mine;
   tc_before();
   __syncthreads();
   tc_after();
-  const uint32_t tmem = tmem_sh;
+  Line line;
+  line.total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) line.total += sh_sum[w];
+  line.cut(max(1, min(p.groups_max, (line.total + p.min_tiles - 1) / p.min_tiles)));
+  const int grp = blockIdx.x / p.members, member = blockIdx.x % p.members;
   Walk<C::RT> walk;
-  walk.at = walk.start = begin;
-  walk.end = end;
+  walk.at = grp < line.groups ? line.begin(grp) : line.total;
+  walk.end = grp < line.groups ? line.begin(grp + 1) : line.total;
+  {
+    int base = 0;
+    for (int s0 = 0; s0 < a.g.n_seq && walk.at < walk.end; s0 += kThreads) { /* the sequence that holds the stretch's begin */
+      const int c = s0 == 0 ? cnt0 : places_of(s0 + tid);
+      int x = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      __syncthreads();
+      if (lane == 31) sh_sum[warp] = x;
+      __syncthreads();
+      int all = 0;
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) x += sh_sum[w];
+        all += sh_sum[w];
+      }
+      const int b = base + x - c;
+      if (c > 0 && b <= walk.at && walk.at < b + c) {
+        sh_s = s0 + tid;
+        sh_base = b;
+      }
+      base += all;
+      if (base > walk.at) break; /* the same for every thread */
+    }
+    __syncthreads();
+  }
+  const uint32_t tmem = tmem_sh;
   walk.s = sh_s;
   walk.base = sh_base;
   walk.member = member;
+  walk.nth = 0;
   walk.load(a, p);
   Piece pc = {};
   bool ok = true;
@@ -417,6 +419,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (elect()) {
           const int pos = ((pc.t0 + t) * TK) & (a.g.page - 1);
           uint8_t* const d = ring + slot * C::TILE;
+#pragma unroll
+          for (int i = 0; i < MB; ++i) /* unmapped inside the sequence: the softmax warps look closer from now on */
+            if (i < boxes && (pg[i] < 0 || pg[i] >= a.g.n_pages) && (pc.t0 + t) * TK + i * rows < pc.q.len) holes = 1;
           mb_expect(&full[slot], (uint32_t)C::TILE);
 #pragma unroll
           for (int i = 0; i < MB; ++i) {
@@ -539,21 +544,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int n_blk = TK / 16; /* 16-position blocks of a tile */
     uint32_t used = 0;       /* V tiles of earlier pieces */
     uint32_t sp = 0, op = 0, vsp = 0; /* phases of s_full[X][b] and o_done[X][b] in bit b, of piece and v_seen */
-    while (walk.next(a, p, &pc)) {
-      /* Q of this CTA's rows, swizzled; rows past the tile's queries are zero */
-      constexpr int QW = C::NQ * TQ * (HD / 8) / 256; /* 16-byte words a thread: all loads first */
-      uint4 qx[QW];
+    constexpr int QW = C::NQ * TQ * (HD / 8) / 256; /* 16-byte words of Q a thread */
+    auto q_at = [&](const Piece& c, int j, int* r, int* ch) { /* word j of this thread; null past the tile's queries */
+      const int i = tid - 128 + j * 256;
+      *r = i / (HD / 8);
+      *ch = i % (HD / 8);
+      const int qi = c.q0 + *r;
+      return *r < c.nq ? (const T*)a.q + ((long long)(c.q.r0 + qi / a.G) * a.H + c.kvh * a.G + qi % a.G) * HD + *ch * 8 : nullptr;
+    };
+    bool have = walk.next(a, p, &pc);
+    while (have) {
+      {
+        uint4 qx[QW];
+        int r, ch;
 #pragma unroll
-      for (int j = 0; j < QW; ++j) {
-        const int i = tid - 128 + j * 256, r = i / (HD / 8), ch = i % (HD / 8), qi = pc.q0 + r;
-        qx[j] = make_uint4(0, 0, 0, 0);
-        if (r < pc.nq)
-          qx[j] = *reinterpret_cast<const uint4*>((const T*)a.q + ((long long)(pc.q.r0 + qi / a.G) * a.H + pc.kvh * a.G + qi % a.G) * HD + ch * 8);
-      }
+        for (int j = 0; j < QW; ++j) {
+          const T* src = q_at(pc, j, &r, &ch);
+          qx[j] = src ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
-      for (int j = 0; j < QW; ++j) {
-        const int i = tid - 128 + j * 256, r = i / (HD / 8), ch = i % (HD / 8);
-        *reinterpret_cast<uint4*>(q_sm + (r >> 7) * C::QTILE + (ch >> 3) * (TQ * 128) + sw128(r & 127, ch & 7)) = qx[j];
+        for (int j = 0; j < QW; ++j) {
+          q_at(pc, j, &r, &ch);
+          *reinterpret_cast<uint4*>(q_sm + (r >> 7) * C::QTILE + (ch >> 3) * (TQ * 128) + sw128(r & 127, ch & 7)) = qx[j];
+        }
       }
       fence_async();
       __syncwarp();
@@ -563,26 +576,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool live = r < pc.nq, warp_live = r - lane < pc.nq;
       const int ri = live ? qi / a.G : 0;
       const int n = n_of(X), open = tree_open(a, pc.q);
-      /* the page of a position: -1 past the end, -2 unmapped */
-      auto page_at = [&](int pos) {
-        if (pos >= pc.q.len) return -1;
+      auto mapped = [&](int pos) { /* or past the end */
+        if (pos >= pc.q.len) return true;
         const int j = pos >> a.g.page_shift;
         const int x = j < a.g.max_pages ? a.table[(long long)pc.s * a.g.max_pages + j] : -1;
-        return x >= 0 && x < a.g.n_pages ? x : -2;
+        return x >= 0 && x < a.g.n_pages;
       };
-      bool holes = false; /* some page of the piece is unmapped */
-      for (long long q = (long long)pc.t0 * TK + lane * a.g.page; q < (long long)(pc.t0 + pc.n) * TK + a.g.page; q += 32 * a.g.page)
-        holes |= q < pc.q.len && page_at((int)q) == -2;
-      holes = __any_sync(0xffffffffu, holes);
       float m = -INFINITY, l = 0.f; /* m: the maximum that weights are taken against */
       for (int i = 0; i < n && ok; ++i) {
         const int t = pc.t0 + (PAIR ? i : 2 * i + X), pos = t * TK;
-        uint32_t blocks = 0xffffffffu; /* which 16-position blocks of the tile are mapped */
-        if (holes) blocks = __ballot_sync(0xffffffffu, lane >= n_blk || page_at(pos + lane * 16) != -2);
         const int b = i & 1;
         const uint32_t ts = tmem + lanes + X * 128 + b * TK;
         if (!mb_wait_warp(&s_full[X][b], (sp >> b) & 1)) { ok = false; break; }
         tc_after();
+        uint32_t blocks = 0xffffffffu; /* which 16-position blocks of the tile are mapped */
+        if (*(volatile int*)&holes) blocks = __ballot_sync(0xffffffffu, lane >= n_blk || mapped(pos + lane * 16));
         const bool masked = (t + 1) * TK > open || pos + TK > pc.q.len;
         if (warp_live) {
           uint32_t sr[TK];
@@ -677,120 +685,112 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0 && ok) mb_arrive(&p_full[X][b]);
         sp ^= 1u << b;
       }
-      /* ---- the piece's end */
+      /* ---- the piece's end; the next one's rows are brought into L2 meanwhile */
+      const Piece c = pc;
+      have = walk.next(a, p, &pc);
+      if (have) {
+#pragma unroll 1
+        for (int j = 0; j < QW; ++j) {
+          int r1, ch1;
+          const T* src = q_at(pc, j, &r1, &ch1);
+          if (src && (ch1 & 7) == 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
+        }
+      }
       if (ok) ok = mb_wait_warp(&piece[X], op);
       op ^= 1;
-      used += pc.n;
+      used += c.n;
+      tc_before();
+      sync_softmax(); /* both streams are through: Q may be replaced, O of either is whole */
       tc_after();
-      const bool whole = pc.n == pc.n_tile;
-      const int slot = pc.head ? 0 : 1;
-      if (!whole && pc.t0 == 0 && tid == 128) { /* the head of a pair that goes on in the next groups */
+      const bool whole = c.n == c.n_tile;
+      const int slot = c.nth == 0 ? 0 : 1; /* only a CTA's first and last pieces can be parts */
+      if (!whole && c.t0 == 0 && tid == 128) { /* the head of a pair that goes on in the next groups */
         TcTail& tl = p.tail[blockIdx.x];
-        const int last = (int)(((pc.first + pc.n_tile) * line.groups - 1) / line.total);
         tl.slot = slot;
-        tl.r0 = pc.q.r0;
-        tl.nq = pc.nq;
-        tl.q0 = pc.q0;
-        tl.kvh = pc.kvh;
-        tl.pieces = last - grp + 1;
+        tl.r0 = c.q.r0;
+        tl.nq = c.nq;
+        tl.q0 = c.q0;
+        tl.kvh = c.kvh;
+        tl.pieces = line.group_of(c.last) - grp + 1;
       }
-      float o[HD];
-      if (n > 0 && warp_live && ok) {
+      /* PAIR false: the streams' rows are the same and their lanes of TMEM too, so each warpgroup joins
+         and writes half of hd */
+      float f = 1.f, g = 0.f;
+      if (!PAIR) {
+        float2* const ml = reinterpret_cast<float2*>(q_sm);
+        ml[X * TQ + row] = make_float2(m, l);
+        sync_softmax();
+        const float2 o1 = ml[(X ^ 1) * TQ + row];
+        const float top = fmaxf(m, o1.x), u = top == -INFINITY ? 0.f : top;
+        f = ex2(m - u);
+        g = ex2(o1.x - u);
+        l = l * f + o1.y * g;
+        m = top;
+      }
+      const bool own = n > 0, other = !PAIR && (X == 0 ? c.n > 1 : true);
+      const long long at = live ? (long long)(c.q.r0 + ri) * a.H + c.kvh * a.G + qi % a.G : 0;
+      const long long ps = ((long long)blockIdx.x * 2 + slot) * C::RT + r;
+      const float inv = l == 0.f ? 0.f : __fdividef(1.f, l); /* 0: the row sees nothing */
+      if (warp_live && ok) {
+        constexpr int COLS = PAIR ? HD : HD / 2;
+#pragma unroll 1
+        for (int d0 = PAIR ? 0 : X * COLS; d0 < (PAIR ? HD : (X + 1) * COLS); d0 += 32) {
+          uint32_t u[32];
+          float o[32];
+          tm_ld(tmem + lanes + 256 + X * HD + d0, u); /* whatever was there, where the stream had no tile */
+          tm_ld_wait();
 #pragma unroll
-        for (int c = 0; c < HD; c += 32) tm_ld(to + c, reinterpret_cast<uint32_t*>(o) + c);
-        tm_ld_wait();
-      } else {
+          for (int e = 0; e < 32; ++e) o[e] = own ? __uint_as_float(u[e]) * f : 0.f;
+          if (!PAIR) {
+            tm_ld(tmem + lanes + 256 + (X ^ 1) * HD + d0, u);
+            tm_ld_wait();
 #pragma unroll
-        for (int c = 0; c < HD; ++c) o[c] = 0.f;
+            for (int e = 0; e < 32; ++e) o[e] += other ? __uint_as_float(u[e]) * g : 0.f;
+          }
+          if (odd_v && live) { /* values taken out of masked tiles go to the rows that see them */
+            const T* qr = (const T*)a.q + at * HD;
+            const int from = max(c.t0 * TK, min(open, c.q.len) / TK * TK), upto = min(c.q.len, (c.t0 + c.n) * TK);
+            for (int pos = from; pos < upto; ++pos) {
+              const int j = pos >> a.g.page_shift;
+              const int pg = j < a.g.max_pages ? a.table[(long long)c.s * a.g.max_pages + j] : -1;
+              if (pg < 0 || pg >= a.g.n_pages || !tree_sees(a, c.q, ri, pos)) continue;
+              const long long off = pg * a.g.pstride + (pos & (a.g.page - 1)) * a.g.pos + c.kvh * a.g.head;
+              const T *kr = (const T*)a.k + off, *vr = (const T*)a.v + off + d0;
+              bool hit = false;
+#pragma unroll 1
+              for (int e = 0; e < 32; ++e) hit |= !isfinite(to_f<T>(vr[e]));
+              if (!hit) continue;
+              float s = 0.f;
+#pragma unroll 1
+              for (int e = 0; e < HD; ++e) s = __fmaf_rn(to_f<T>(qr[e]), to_f<T>(kr[e]), s);
+              const float w = ex2(__fmaf_rn(s, a.scale2, -(m == -INFINITY ? 0.f : m)));
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const float x = to_f<T>(vr[e]);
+                if (!isfinite(x)) o[e] += w * x;
+              }
+            }
+          }
+          if (live && whole) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+              *reinterpret_cast<uint4*>((T*)a.out + at * HD + d0 + e) =
+                  make_uint4(pack2<T>(o[e] * inv, o[e + 1] * inv), pack2<T>(o[e + 2] * inv, o[e + 3] * inv),
+                             pack2<T>(o[e + 4] * inv, o[e + 5] * inv), pack2<T>(o[e + 6] * inv, o[e + 7] * inv));
+          } else if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              __stcg(reinterpret_cast<float4*>(a.po + ps * HD + d0 + e), make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+          }
+          __syncwarp(); /* the next TMEM load is the whole warp's */
+        }
+        if (live && (PAIR || X == 0)) {
+          if (!whole) __stcg(reinterpret_cast<float2*>(a.pml + ps * 2), make_float2(m, l));
+          else if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+        }
       }
       tc_before();
-      /* values taken out of masked tiles go to the rows that see them */
-      if (PAIR) sync_softmax(); /* either stream may have found them */
-      if (odd_v && live && ok) {
-        const T* qr = (const T*)a.q + ((long long)(pc.q.r0 + ri) * a.H + pc.kvh * a.G + qi % a.G) * HD;
-        const int from = max(pc.t0 * TK, min(open, pc.q.len) / TK * TK), upto = min(pc.q.len, (pc.t0 + pc.n) * TK);
-        for (int pos = from; pos < upto; ++pos) {
-          if (!PAIR && ((pos / TK - pc.t0) & 1) != X) continue;
-          const int j = pos >> a.g.page_shift;
-          const int pg = j < a.g.max_pages ? a.table[(long long)pc.s * a.g.max_pages + j] : -1;
-          if (pg < 0 || pg >= a.g.n_pages || !tree_sees(a, pc.q, ri, pos)) continue;
-          const long long off = pg * a.g.pstride + (pos & (a.g.page - 1)) * a.g.pos + pc.kvh * a.g.head;
-          const T *kr = (const T*)a.k + off, *vr = (const T*)a.v + off;
-          float s = 0.f;
-          bool hit = false;
-#pragma unroll 1
-          for (int e = 0; e < HD; ++e) {
-            s = __fmaf_rn(to_f<T>(qr[e]), to_f<T>(kr[e]), s);
-            hit |= !isfinite(to_f<T>(vr[e]));
-          }
-          if (!hit) continue;
-          const float w = ex2(__fmaf_rn(s, a.scale2, -(m == -INFINITY ? 0.f : m)));
-#pragma unroll
-          for (int d = 0; d < HD; ++d) {
-            const float x = to_f<T>(vr[d]);
-            if (!isfinite(x)) o[d] += w * x;
-          }
-        }
-      }
-      if (!PAIR) {
-        /* stream 1 hands its rows to stream 0, half of hd at a time, in the Q tile (every product that
-           read it is complete); float4 c of all rows side by side: no bank conflicts */
-        float4* const hand = reinterpret_cast<float4*>(q_sm);
-        sync_softmax();
-        if (X == 1) {
-          sh_ml[0][row] = m;
-          sh_ml[1][row] = l;
-        }
-        float f0 = 1.f, f1 = 0.f;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (X == 1) {
-#pragma unroll
-            for (int c = 0; c < HD / 8; ++c) {
-              const int d = half * (HD / 2) + c * 4;
-              hand[c * 128 + row] = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
-            }
-          }
-          sync_softmax();
-          if (X == 0) {
-            if (half == 0) {
-              const float m1 = sh_ml[0][row], top = fmaxf(m, m1), u = top == -INFINITY ? 0.f : top;
-              f0 = ex2(m - u);
-              f1 = ex2(m1 - u);
-              l = l * f0 + sh_ml[1][row] * f1;
-              m = top;
-            }
-#pragma unroll
-            for (int c = 0; c < HD / 8; ++c) {
-              const int d = half * (HD / 2) + c * 4;
-              const float4 y = hand[c * 128 + row];
-              o[d] = o[d] * f0 + y.x * f1;
-              o[d + 1] = o[d + 1] * f0 + y.y * f1;
-              o[d + 2] = o[d + 2] * f0 + y.z * f1;
-              o[d + 3] = o[d + 3] * f0 + y.w * f1;
-            }
-          }
-          sync_softmax();
-        }
-      }
-      if (PAIR) sync_softmax(); /* both streams are through: Q may be replaced */
-      if (live && ok && (PAIR || X == 0)) {
-        const long long at = (long long)(pc.q.r0 + ri) * a.H + pc.kvh * a.G + qi % a.G;
-        if (whole) {
-          const float inv = l == 0.f ? 0.f : __fdividef(1.f, l); /* 0: the row sees nothing */
-#pragma unroll
-          for (int c = 0; c < HD; c += 8)
-            *reinterpret_cast<uint4*>((T*)a.out + at * HD + c) =
-                make_uint4(pack2<T>(o[c] * inv, o[c + 1] * inv), pack2<T>(o[c + 2] * inv, o[c + 3] * inv),
-                           pack2<T>(o[c + 4] * inv, o[c + 5] * inv), pack2<T>(o[c + 6] * inv, o[c + 7] * inv));
-          if (a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-        } else {
-          const long long ps = ((long long)blockIdx.x * 2 + slot) * C::RT + r;
-#pragma unroll
-          for (int c = 0; c < HD; c += 4) __stcg(reinterpret_cast<float4*>(a.po + ps * HD + c), make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]));
-          __stcg(reinterpret_cast<float2*>(a.pml + ps * 2), make_float2(m, l));
-        }
-      }
+      if (!PAIR) sync_softmax(); /* each has read the other's O */
     }
   }
   tc_before();
@@ -874,6 +874,12 @@ int pool_map(const TreeArgs& a, bool f16, const void* pool, CUtensorMap* m) {
   return ULB_OK;
 }
 
+/* the longest line a call can have */
+long long line_most(const TreeArgs& a, int RT, int n_sm) {
+  const long long tiles = ((long long)a.max_rows * a.G + RT - 1) / RT, members = std::min<long long>(tiles, n_sm);
+  return (long long)a.g.n_seq * a.g.n_head_kv * (std::max(1, (a.max_len + TK - 1) / TK) + kPairCost) * ((tiles + members - 1) / members);
+}
+
 template <typename T, int HD, bool PAIR>
 int launch_tc(Ctx* c, TreeArgs& a) {
   using C = TcCfg<HD, PAIR>;
@@ -900,8 +906,7 @@ int launch_tc(Ctx* c, TreeArgs& a) {
   p.tail = reinterpret_cast<TcTail*>(a.pml + rows * 2);
   ULB_LAUNCH("tree attention launch", launch_k(c, tree_tc_kernel<T, HD, PAIR>, dim3(grid), dim3(kThreads), C::SMEM, mk, mv, a, p));
   /* a launch that one group covers leaves nothing to join */
-  const long long most = (long long)a.g.n_seq * a.g.n_head_kv * std::max(1, (a.max_len + TK - 1) / TK) *
-                         ((tiles + p.members - 1) / p.members);
+  const long long most = line_most(a, C::RT, c->n_sm);
   if (most > p.min_tiles && p.groups_max > 1)
     ULB_LAUNCH("tree join launch", launch_k(c, tree_tc_join_kernel<T, HD>, dim3(grid, C::RT / kJoinRows), dim3(kJoinRows * 32), 0, a, p, C::RT));
   return ULB_OK;
@@ -915,6 +920,11 @@ int pick_tc(Ctx* c, TreeArgs& a) {
 }
 
 }  // namespace
+
+/* the line is counted in 32 bits */
+bool tree_tc_fits(const Ctx* c, const TreeArgs& a) {
+  return (a.g.hd == 64 || a.g.hd == 128) && line_most(a, (long long)a.max_rows * a.G > 128 ? 256 : 128, c->n_sm) < (1ll << 31) - 65536;
+}
 
 int launch_tree_tc(Ctx* c, TreeArgs& a, bool f16) { return f16 ? pick_tc<__half>(c, a) : pick_tc<__nv_bfloat16>(c, a); }
 
