@@ -176,7 +176,8 @@ struct TcCfg {
   static constexpr int NQ = PAIR ? 2 : 1;
   static constexpr int NK = HD == 64 ? 8 : PAIR ? 5 : 6; /* K tiles in the ring */
   static constexpr int NV = HD == 64 ? 8 : PAIR ? 5 : 6;
-  static constexpr int SMEM = NQ * QTILE + (NK + NV) * TILE + 1024; /* + alignment slack */
+  static constexpr int STAGE = NQ * QTILE >= 32768 ? 0 : 32768; /* outputs pass through Q's place, or their own */
+  static constexpr int SMEM = NQ * QTILE + (NK + NV) * TILE + STAGE + 1024; /* + alignment slack */
   static constexpr int RT = PAIR ? 256 : 128;         /* queries a CTA */
   static_assert(SMEM <= 226 * 1024, "shared memory");
 };
@@ -271,8 +272,8 @@ __device__ __forceinline__ uint32_t sees32(const TreeArgs& a, const TreeSeq& q, 
     if (j > -32) {
       const uint32_t* m = a.mask + (long long)(q.r0 + i) * a.words;
       const int w = j >> 5;
-      const uint32_t lo = w < 0 ? 0xffffffffu : w < a.words ? m[w] : 0u;
-      const uint32_t hi = w + 1 < a.words ? m[w + 1] : 0u;
+      auto word = [&](int k) { return k < 0 ? 0xffffffffu : k >= a.words ? 0u : m[k]; };
+      const uint32_t lo = word(w), hi = word(w + 1);
       v = __funnelshift_r(lo, hi, j & 31);
     }
   }
@@ -296,11 +297,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t k_full[C::NK], k_free[C::NK], v_full[C::NV], v_free[C::NV], s_full[2][2], p_full[2][2], o_done[2][2], v_seen[2], piece[2], q_full, mma_done;
   __shared__ uint32_t tmem_sh;
-  __shared__ int odd_v, holes, sh_s, sh_base, sh_sum[kThreads / 32];
+  __shared__ int odd_v, sh_s, sh_base, sh_sum[kThreads / 32];
   uint8_t* const sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* const q_sm = sm;
   uint8_t* const k_sm = sm + C::NQ * C::QTILE;
   uint8_t* const v_sm = k_sm + C::NK * C::TILE;
+  uint8_t* const stage_sm = C::STAGE ? v_sm + C::NV * C::TILE : q_sm;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   /* nothing here depends on earlier kernels */
@@ -315,7 +317,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     mb_init(&q_full, 8);
     mb_init(&mma_done, 2);
     odd_v = 0;
-    holes = 0;
     sh_s = 0;
     sh_base = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -389,6 +390,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   /* stream X's tiles of a piece of n: PAIR all of them (none without rows), else every second */
   auto n_of = [&](int X) { return PAIR ? (X == 0 || pc.nq > 128 ? pc.n : 0) : (pc.n + 1 - X) >> 1; };
 
+  /* registers: 128 x 104 + 256 x 200 = 384 x 168, what the block was launched with */
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
   if (warp == 0 || warp == 3) {
     /* ------------------------------------------------ TMA: warp 0 the K tiles, warp 3 the V tiles, in order.
        Asking for a free slot, issuing and looking up pages take some 750 cycles a tile, so each
@@ -419,9 +423,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (elect()) {
           const int pos = ((pc.t0 + t) * TK) & (a.g.page - 1);
           uint8_t* const d = ring + slot * C::TILE;
-#pragma unroll
-          for (int i = 0; i < MB; ++i) /* unmapped inside the sequence: the softmax warps look closer from now on */
-            if (i < boxes && (pg[i] < 0 || pg[i] >= a.g.n_pages) && (pc.t0 + t) * TK + i * rows < pc.q.len) holes = 1;
           mb_expect(&full[slot], (uint32_t)C::TILE);
 #pragma unroll
           for (int i = 0; i < MB; ++i) {
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     /* no copy is in flight when the CTA ends, whatever happened: the last round's tiles, in turn */
     for (int c = max(0, issued - nring); c < issued; ++c) ok &= mb_wait_warp(&full[c % nring], (c / nring) & 1);
-  } else if (warp < 3) {
+  } else {
     /* ------------------------------------------------ MMA issue: a warp a stream walks, one elected lane
        issues.  What one thread does for a tile (waits, MMAs, commits) takes about as long as its
        arithmetic, so descriptors are a base plus a constant and ring places are counted.
@@ -536,8 +537,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (elect()) commit(&mma_done);
     __syncwarp();
     ok = mb_wait_warp(&mma_done, 0) && ok;
+  }
   } else {
     /* ------------------------------------------------ softmax: one thread a row */
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int X = (warp - 4) >> 2, row = tid - 128 - X * 128; /* stream, row of its tile = TMEM lane */
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t to = tmem + lanes + 256 + X * HD;
@@ -554,6 +557,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     bool have = walk.next(a, p, &pc);
     while (have) {
+      auto mapped = [&](long long pos) { /* or past the end */
+        if (pos >= pc.q.len) return true;
+        const int j = (int)(pos >> a.g.page_shift);
+        const int x = j < a.g.max_pages ? a.table[(long long)pc.s * a.g.max_pages + j] : -1;
+        return x >= 0 && x < a.g.n_pages;
+      };
+      /* is some page of the piece unmapped?  A page a lane, its load under way beside those of Q */
+      const int j0 = ((pc.t0 * TK) >> a.g.page_shift) + lane, j1 = (int)min(((long long)(pc.t0 + pc.n) * TK - 1) >> a.g.page_shift, (long long)(pc.q.len - 1) >> a.g.page_shift);
+      const int page0 = j0 <= j1 && j0 < a.g.max_pages ? a.table[(long long)pc.s * a.g.max_pages + j0] : j0 <= j1 ? -1 : 0;
       {
         uint4 qx[QW];
         int r, ch;
@@ -568,6 +580,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           *reinterpret_cast<uint4*>(q_sm + (r >> 7) * C::QTILE + (ch >> 3) * (TQ * 128) + sw128(r & 127, ch & 7)) = qx[j];
         }
       }
+      bool holes = page0 < 0 || page0 >= a.g.n_pages;
+      for (int j = j0 + 32; j <= j1; j += 32) holes |= !mapped((long long)j << a.g.page_shift);
+      holes = __any_sync(0xffffffffu, holes);
       fence_async();
       __syncwarp();
       if (lane == 0 && ok) mb_arrive(&q_full);
@@ -576,12 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool live = r < pc.nq, warp_live = r - lane < pc.nq;
       const int ri = live ? qi / a.G : 0;
       const int n = n_of(X), open = tree_open(a, pc.q);
-      auto mapped = [&](int pos) { /* or past the end */
-        if (pos >= pc.q.len) return true;
-        const int j = pos >> a.g.page_shift;
-        const int x = j < a.g.max_pages ? a.table[(long long)pc.s * a.g.max_pages + j] : -1;
-        return x >= 0 && x < a.g.n_pages;
-      };
+      if (live && a.words > 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.mask + (long long)(pc.q.r0 + ri) * a.words));
       float m = -INFINITY, l = 0.f; /* m: the maximum that weights are taken against */
       for (int i = 0; i < n && ok; ++i) {
         const int t = pc.t0 + (PAIR ? i : 2 * i + X), pos = t * TK;
@@ -590,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!mb_wait_warp(&s_full[X][b], (sp >> b) & 1)) { ok = false; break; }
         tc_after();
         uint32_t blocks = 0xffffffffu; /* which 16-position blocks of the tile are mapped */
-        if (*(volatile int*)&holes) blocks = __ballot_sync(0xffffffffu, lane >= n_blk || mapped(pos + lane * 16));
+        if (holes) blocks = __ballot_sync(0xffffffffu, lane >= n_blk || mapped(pos + lane * 16));
         const bool masked = (t + 1) * TK > open || pos + TK > pc.q.len;
         if (warp_live) {
           uint32_t sr[TK];
@@ -663,7 +673,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           vsp ^= 1;
           uint4* const v = reinterpret_cast<uint4*>(v_sm + cvt % C::NV * C::TILE);
           constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
+          const int lo = max(0, min(open, pc.q.len) - pos); /* first key of the tile that some row does not see */
           for (int j = row; j < C::TILE / 16; j += 128) {
+            if (((j >> 3) & (TK - 1)) < lo) continue;
             const uint4 x = v[j];
             uint32_t w[4] = {x.x, x.y, x.z, x.w};
             bool hit = false;
@@ -721,6 +733,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ml[X * TQ + row] = make_float2(m, l);
         sync_softmax();
         const float2 o1 = ml[(X ^ 1) * TQ + row];
+        if (HD == 128) sync_softmax(); /* read, before the outputs pass through the same place */
         const float top = fmaxf(m, o1.x), u = top == -INFINITY ? 0.f : top;
         f = ex2(m - u);
         g = ex2(o1.x - u);
@@ -733,6 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float inv = l == 0.f ? 0.f : __fdividef(1.f, l); /* 0: the row sees nothing */
       if (warp_live && ok) {
         constexpr int COLS = PAIR ? HD : HD / 2;
+        uint4* const stage = reinterpret_cast<uint4*>(stage_sm) + (warp - 4) * 256;
 #pragma unroll 1
         for (int d0 = PAIR ? 0 : X * COLS; d0 < (PAIR ? HD : (X + 1) * COLS); d0 += 32) {
           uint32_t u[32];
@@ -771,18 +785,36 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
-          if (live && whole) {
+          /* 32 rows x 32 columns change sides in shared memory, so that a row leaves in one piece (a lane
+             writing its own row takes a transaction every 16 bytes): 16-byte word w of row y at w ^ y */
+          if (whole) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              *reinterpret_cast<uint4*>((T*)a.out + at * HD + d0 + e) =
-                  make_uint4(pack2<T>(o[e] * inv, o[e + 1] * inv), pack2<T>(o[e + 2] * inv, o[e + 3] * inv),
-                             pack2<T>(o[e + 4] * inv, o[e + 5] * inv), pack2<T>(o[e + 6] * inv, o[e + 7] * inv));
-          } else if (live) {
+            for (int e = 0; e < 4; ++e)
+              stage[lane * 4 + (e ^ ((lane >> 1) & 3))] =
+                  make_uint4(pack2<T>(o[8 * e] * inv, o[8 * e + 1] * inv), pack2<T>(o[8 * e + 2] * inv, o[8 * e + 3] * inv),
+                             pack2<T>(o[8 * e + 4] * inv, o[8 * e + 5] * inv), pack2<T>(o[8 * e + 6] * inv, o[8 * e + 7] * inv));
+            __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              __stcg(reinterpret_cast<float4*>(a.po + ps * HD + d0 + e), make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+            for (int k = 0; k < 4; ++k) {
+              const int y = k * 8 + (lane >> 2), w = lane & 3;
+              const long long row_at = __shfl_sync(0xffffffffu, at, y);
+              const uint4 x = stage[y * 4 + (w ^ ((y >> 1) & 3))];
+              if (r - lane + y < c.nq) *reinterpret_cast<uint4*>((T*)a.out + row_at * HD + d0 + w * 8) = x;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              stage[lane * 8 + (e ^ (lane & 7))] = make_uint4(__float_as_uint(o[4 * e]), __float_as_uint(o[4 * e + 1]),
+                                                              __float_as_uint(o[4 * e + 2]), __float_as_uint(o[4 * e + 3]));
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int y = k * 4 + (lane >> 3), w = lane & 7;
+              const uint4 x = stage[y * 8 + (w ^ (y & 7))];
+              if (r - lane + y < c.nq) __stcg(reinterpret_cast<uint4*>(a.po + (ps - lane + y) * HD + d0 + w * 4), x);
+            }
           }
-          __syncwarp(); /* the next TMEM load is the whole warp's */
+          __syncwarp(); /* the words may be replaced, the next TMEM load is the whole warp's */
         }
         if (live && (PAIR || X == 0)) {
           if (!whole) __stcg(reinterpret_cast<float2*>(a.pml + ps * 2), make_float2(m, l));
@@ -790,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       tc_before();
-      if (!PAIR) sync_softmax(); /* each has read the other's O */
+      sync_softmax(); /* each has read the other's O, and Q's place is free again */
     }
   }
   tc_before();
