@@ -597,24 +597,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int t = pc.t0 + (PAIR ? i : 2 * i + X), pos = t * TK;
         const int b = i & 1;
         const uint32_t ts = tmem + lanes + X * 128 + b * TK;
-        if (!mb_wait_warp(&s_full[X][b], (sp >> b) & 1)) { ok = false; break; }
-        tc_after();
+        const bool masked = (t + 1) * TK > open || pos + TK > pc.q.len;
         uint32_t blocks = 0xffffffffu; /* which 16-position blocks of the tile are mapped */
         if (holes) blocks = __ballot_sync(0xffffffffu, lane >= n_blk || mapped(pos + lane * 16));
-        const bool masked = (t + 1) * TK > open || pos + TK > pc.q.len;
+        const bool cut = masked || blocks != 0xffffffffu;
+        uint32_t see[TK / 32];
+        if (cut) { /* looked up while the scores are computed */
+#pragma unroll
+          for (int c = 0; c < TK; c += 32) see[c / 32] = sees32(a, pc.q, ri, pos + c, blocks, c);
+        }
+        if (!mb_wait_warp(&s_full[X][b], (sp >> b) & 1)) { ok = false; break; }
+        tc_after();
         if (warp_live) {
           uint32_t sr[TK];
 #pragma unroll
           for (int c = 0; c < TK; c += 32) tm_ld(ts + c, sr + c);
           tm_ld_wait();
-          if (masked || blocks != 0xffffffffu) {
+          if (cut) {
 #pragma unroll
-            for (int c = 0; c < TK; c += 32) {
-              const uint32_t see = sees32(a, pc.q, ri, pos + c, blocks, c);
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!((see >> e) & 1u)) sr[c + e] = 0xff800000u; /* -inf */
-            }
+            for (int c = 0; c < TK; ++c)
+              if (!((see[c / 32] >> (c & 31)) & 1u)) sr[c] = 0xff800000u; /* -inf */
           }
           /* weights against the maximum so far, the tile's own maximum beside them: only when a row's
              has grown by more than 2^8 (its first tile, seldom later) are they taken again */
@@ -674,8 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint4* const v = reinterpret_cast<uint4*>(v_sm + cvt % C::NV * C::TILE);
           constexpr uint32_t E = F16 ? 0x7c00u : 0x7f80u;
           const int lo = max(0, min(open, pc.q.len) - pos); /* first key of the tile that some row does not see */
-          for (int j = row; j < C::TILE / 16; j += 128) {
-            if (((j >> 3) & (TK - 1)) < lo) continue;
+          auto clear = [&](int j) {
             const uint4 x = v[j];
             uint32_t w[4] = {x.x, x.y, x.z, x.w};
             bool hit = false;
@@ -688,6 +689,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               odd_v = 1;
               v[j] = make_uint4(w[0], w[1], w[2], w[3]);
             }
+          };
+          for (int j = lo * 8 + row; j < TK * 8; j += 128) {
+            clear(j);
+            if (HD == 128) clear(TK * 8 + j);
           }
           fence_async();
         }
