@@ -47,7 +47,7 @@ namespace {
 constexpr int TK = 64;         /* keys a tile */
 constexpr int TQ = 128;        /* query rows a stream: M */
 constexpr int kThreads = 384;  /* 4 role warps, 2 x 4 softmax warps */
-constexpr int kPairCost = 6;   /* what a pair costs besides its tiles, in tiles */
+constexpr int kPairCost = 16;   /* what a pair costs besides its tiles, in tiles */
 constexpr int kMinTiles = 12;  /* tiles of the line a group takes at least */
 constexpr int kJoinRows = 8;   /* rows a block of the join kernel: a warp each */
 
@@ -958,9 +958,19 @@ int pick_tc(Ctx* c, TreeArgs& a) {
 
 }  // namespace
 
-/* the line is counted in 32 bits */
+/*
+ * When this form runs: from 65 queries a kv head on, or from 32 MB of K and V (by the longest sequence)
+ * in sequences of 512 positions or more.  Below, starting up (barriers, TMEM, tensor maps, two
+ * pipelines to fill) costs more than the tensor cores save.  Measured here / mma.sync form, us:
+ * 1 row x 500 keys 14.3 / 8.6, 1 x 4000 keys 17.3 / 8.4, 8 x 1 x 1000 keys (32 MB) 20.5 / 19.2,
+ * 64 x 1 x 300 keys of 32 kv heads 115 / 90; 1 x 8000 keys of 32 kv heads (131 MB) 34.1 / 38.0,
+ * 64 x 1 x 4000 keys 114 / 165.  The line is counted in 32 bits.
+ */
 bool tree_tc_fits(const Ctx* c, const TreeArgs& a) {
-  return (a.g.hd == 64 || a.g.hd == 128) && line_most(a, (long long)a.max_rows * a.G > 128 ? 256 : 128, c->n_sm) < (1ll << 31) - 65536;
+  const long long nq = (long long)a.max_rows * a.G, bytes = 4ll * a.g.n_seq * a.max_len * a.g.n_head_kv * a.g.hd;
+  if (a.g.hd != 64 && a.g.hd != 128) return false;
+  if (nq <= 64 && (bytes < (32ll << 20) || a.max_len < 512)) return false;
+  return line_most(a, nq > 128 ? 256 : 128, c->n_sm) < (1ll << 31) - 65536;
 }
 
 int launch_tree_tc(Ctx* c, TreeArgs& a, bool f16) { return f16 ? pick_tc<__half>(c, a) : pick_tc<__nv_bfloat16>(c, a); }
