@@ -65,7 +65,7 @@ __device__ __forceinline__ uint32_t less_of(int made, float pres, float freq) {
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kWarps * 32, 3) logits_kernel(const __grid_constant__ ulb_logits_args a, LogitsGeom g) {
+__global__ void __launch_bounds__(kWarps * 32, 5) logits_kernel(const __grid_constant__ ulb_logits_args a, LogitsGeom g) {
   pdl_wait();
   pdl_trigger();
   constexpr int U = unit_loads(V);
@@ -210,8 +210,6 @@ __global__ void __launch_bounds__(kWarps * 32, 3) logits_kernel(const __grid_con
   __syncthreads();
 
   while (unit < n_unit) {
-    Unit next; /* in flight while this one is worked on */
-    if (unit + kWarps < n_unit) load_unit(unit + kWarps, next);
     const int r = cur.r, c0 = cur.c0, c1 = cur.c1;
     int n_list = 0;
     if (n_at) {
@@ -288,7 +286,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) logits_kernel(const __grid_con
       __syncwarp();
     }
     unit += kWarps;
-    cur = next;
+    if (unit < n_unit) load_unit(unit, cur);
   }
 }
 
