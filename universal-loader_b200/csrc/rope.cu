@@ -226,13 +226,18 @@ int pick_rope(Ctx* c, RopeArgs& a) {
   auto fits = [&](int e) {
     return all % e == 0 && in % std::min<size_t>(16, e * sizeof(TI)) == 0 && out % std::min<size_t>(16, e * sizeof(TO)) == 0;
   };
-  if (fits(8)) {
-    /* four heads a thread once that still fills the device: one pass of sines for four heads
-       and four loads in flight; below, more threads */
-    if ((long long)a.M * heads * (a.hd / 8) >= (long long)c->n_sm * 2048 * 4) return launch_rope<TI, TO, 8, 4, APPEND>(c, a);
-    return launch_rope<TI, TO, 8, 1, APPEND>(c, a);
+  /* 16 bytes a load (32 a thread, f32 in units of eight, measured 117 us where units of four took 111:
+     16381 rows of 40 heads), and several heads a thread once that still fills the device: one pass
+     of sines for all of them and as many loads in flight.  1024 rows of 80 heads of 128: two heads a
+     thread 15.2 us, four 17.8, one 17.6. */
+  constexpr int W = sizeof(TI) == 4 ? 4 : 8;
+  if (fits(W)) {
+    const long long full = (long long)c->n_sm * 2048, units = (long long)a.M * heads * (a.hd / W);
+    if (units >= 32 * full) return launch_rope<TI, TO, W, 4, APPEND>(c, a);
+    if (units >= 4 * full) return launch_rope<TI, TO, W, 2, APPEND>(c, a);
+    return launch_rope<TI, TO, W, 1, APPEND>(c, a);
   }
-  if (fits(4)) return launch_rope<TI, TO, 4, 2, APPEND>(c, a);
+  if (W == 8 && fits(4)) return launch_rope<TI, TO, 4, 2, APPEND>(c, a);
   return launch_rope<TI, TO, 1, 1, APPEND>(c, a);
 }
 
@@ -240,6 +245,12 @@ int pick_rope(Ctx* c, RopeArgs& a) {
 }  // namespace ulb
 
 using namespace ulb;
+
+static const long double kTwoPi = 6.283185307179586476925286766559005768L;
+/* the (fractional) pair that makes t turns over L positions */
+static long double pair_with_turns(long double t, long double rot, long double L, long double base) {
+  return rot * logl(L / (kTwoPi * t)) / (2.0L * logl(base));
+}
 
 struct ulb_rope {
   ulb_ctx* owner = nullptr;
@@ -275,16 +286,14 @@ int ulb_rope_create(ulb_ctx* ctx, const ulb_rope_desc* d, const float* ff, ulb_r
   for (int i = 0; ff && i < n; ++i)
     ULB_CHECK(std::isfinite(ff[i]) && ff[i] > 0, ULB_EINVAL, "ulb_rope_create: freq_factors[%d] = %g", i, (double)ff[i]);
 
-  const long double pi2 = 6.283185307179586476925286766559005768L;
   long double base = d->base, m = 1.0L;
   const long double f = d->scaling == ULB_ROPE_NONE ? 1.0L : (long double)d->factor, rot = d->rot_dim, L = d->orig_len;
   if (d->scaling == ULB_ROPE_NTK) base *= powl(f, rot / (rot - 2.0L));
   long double lo = 0, hi = 0;
   if (d->scaling == ULB_ROPE_YARN) {
-    auto e = [&](long double t) { return rot * logl(L / (pi2 * t)) / (2.0L * logl(base)); };
-    lo = floorl(e(d->beta_fast));
+    lo = floorl(pair_with_turns(d->beta_fast, rot, L, base));
     if (lo < 0) lo = 0;
-    hi = ceill(e(d->beta_slow));
+    hi = ceill(pair_with_turns(d->beta_slow, rot, L, base));
     if (hi > rot - 1) hi = rot - 1;
     m = 0.1L * logl(f) + 1.0L;
   }
@@ -299,7 +308,7 @@ int ulb_rope_create(ulb_ctx* ctx, const ulb_rope_desc* d, const float* ff, ulb_r
       const long double r = ramp < 0 ? 0.0L : ramp > 1 ? 1.0L : ramp;
       w = w * (1.0L - r) + w / f * r;
     } else if (d->scaling == ULB_ROPE_WAVELENGTH) {
-      const long double wave = pi2 / w;
+      const long double wave = kTwoPi / w;
       if (wave > L / d->low_freq) {
         w /= f;
       } else if (wave >= L / d->high_freq) {
@@ -307,7 +316,7 @@ int ulb_rope_create(ulb_ctx* ctx, const ulb_rope_desc* d, const float* ff, ulb_r
         w = (1.0L - x) * w / f + x * w;
       }
     }
-    const long double t = w / pi2;
+    const long double t = w / kTwoPi;
     long double scaled = roundl((t - floorl(t)) * 18446744073709551616.0L);
     h_turn[i] = scaled >= 18446744073709551616.0L ? 0ull : (unsigned long long)scaled;
   }
