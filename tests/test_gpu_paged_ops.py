@@ -540,6 +540,42 @@ def test_tree_attention_follows_the_stream(tctx):
         tctx.use_stream(torch.cuda.current_stream().cuda_stream)
 
 
+@pytest.mark.parametrize("D", [64, 80, 96, 128])
+@pytest.mark.parametrize("H,Hkv,rows", [(8, 1, 9), (16, 2, 16), (6, 2, 40), (8, 1, 33)])
+def test_tree_attention_tensor_core_form(tctx, D, H, Hkv, rows):
+    """65 queries a kv head and more, which run on the tensor cores whatever the length: one tile of
+    rows and two, tile and page edges, ragged batches, empty rows, unmapped pages, other layouts."""
+    for prefix in (0, 1, 63, 64, 65, 190, 700):
+        Attention("bf16", H, Hkv, D, 16, [(prefix, rows)], seed=prefix + D).check(tctx)
+    Attention("f16", H, Hkv, D, 64, [(500, rows), (3, 1), (0, 0), (129, rows // 2), (0, rows)], seed=D, nhd=True).check(tctx)
+    Attention("f16", H, Hkv, D, 32, [(0, rows), (100, rows), (0, 1)], empty_rows=True, stale=math.nan, seed=D + 1).check(tctx)
+    Attention("bf16", H, Hkv, D, 128, [(0, rows), (300, rows)], empty_rows=True, stale=-math.inf, seed=D + 2).check(tctx)
+    Attention("f16", H, Hkv, D, 16, [(333, rows), (90, rows)], unmapped=[(0, 0, -1), (0, 5, 3), (0, 20, -9), (1, 5, -1)], seed=D + 3).check(tctx)
+    Attention("f16", H, Hkv, D, 256, [(900, rows), (0, rows)], causal=True, seed=D + 4).check(tctx)
+    Attention("bf16", H, Hkv, D, 64, [(77, rows), (5, rows)], slots=[rows + 90, rows], seed=D + 5).check(tctx)
+
+
+@pytest.mark.parametrize("D", [64, 80, 96, 128])
+@pytest.mark.parametrize("H,Hkv,rows", [(2, 2, 1), (8, 2, 3), (8, 4, 16)])
+def test_tree_attention_tensor_core_form_by_bytes(tctx, D, H, Hkv, rows):
+    """Few queries over 32 MB of K and V and more (by the longest sequence) run there too."""
+    import ulb_capi as U
+    need = (32 << 20) // (4 * Hkv * D * 3)
+    a = Attention("f16", H, Hkv, D, 64, [(700, rows), (2500, rows), (0, rows)], seed=D + rows)
+    assert max(a.len) < need
+    out, ls = a.run(tctx)
+    # the same call with a bound on the lengths that makes it large: the other form
+    c = U.CacheDesc(dtype=U.T_F16, n_head_kv=Hkv, head_dim=D, page=64, n_pages=a.n_pages, n_seq=3, max_pages=a.most + need // 64 + 1)
+    table = np.full((3, c.max_pages), -1)
+    table[:, :a.most] = a.table
+    o2, l2 = torch.empty_like(out), torch.empty_like(ls)
+    tctx.tree_attention(c, H, a.rows, rows, need + 64, 1 / math.sqrt(D), ptr(a.q), ptr(a.k), ptr(a.v), ptr(dev(table)),
+                        *[ptr(t) for t in a.keep[1:]], ptr(a.mask), a.words, ptr(o2), ptr(l2))
+    # either form is within the weights' and the output's rounding of the exact result (values within 5)
+    assert float((out.double() - o2.double()).abs().max()) <= 4 * UNIT["f16"] * 5
+    assert float((ls.double() - l2.double()).abs().max()) <= 4e-5 * (1 + float(ls.abs().max()))
+
+
 def test_tree_attention_refusals(tctx):
     import ulb_capi as U
     x = torch.zeros(1 << 16, dtype=torch.float16, device="cuda")

@@ -60,7 +60,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 #endif
 
-/* the tensor-core form (tree_attention_tc.cu): head dims 64 and 128 */
+/* the tcgen05 form (tree_attention_tc.cu): head dims up to 128 */
 bool tree_tc_fits(const Ctx* c, const TreeArgs& a);
 int launch_tree_tc(Ctx* c, TreeArgs& a, bool f16);
 

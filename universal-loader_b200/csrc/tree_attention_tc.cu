@@ -1,6 +1,7 @@
 /*
  * tree_attention_tc.cu — ulb_tree_attention on the 5th-generation tensor cores, for head
- * dims 64 and 128.  Same mathematics and masking as tree_attention.cu.
+ * dims up to 128 (80 and 96 run in tiles of 128 whose other columns the copies fill with zeros:
+ * nothing is read for them).  Same mathematics and masking as tree_attention.cu.
  *
  * A CTA works on 64-key tiles with M = 128 query rows a stream, two streams at a time, each
  * with its own running (m, l, o) and its own softmax warpgroup (one thread a row):
@@ -304,6 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* const v_sm = k_sm + C::NK * C::TILE;
   uint8_t* const stage_sm = C::STAGE ? v_sm + C::NV * C::TILE : q_sm;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int hd = HD == 64 ? 64 : a.g.hd; /* HD = 128: 80, 96 or 128, the tiles' columns past it are zeros */
 
   /* nothing here depends on earlier kernels */
   if (tid == 0) {
@@ -548,12 +550,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t used = 0;       /* V tiles of earlier pieces */
     uint32_t sp = 0, op = 0, vsp = 0; /* phases of s_full[X][b] and o_done[X][b] in bit b, of piece and v_seen */
     constexpr int QW = C::NQ * TQ * (HD / 8) / 256; /* 16-byte words of Q a thread */
-    auto q_at = [&](const Piece& c, int j, int* r, int* ch) { /* word j of this thread; null past the tile's queries */
+    auto q_at = [&](const Piece& c, int j, int* r, int* ch) { /* word j of this thread; null past the tile's queries and past hd */
       const int i = tid - 128 + j * 256;
       *r = i / (HD / 8);
       *ch = i % (HD / 8);
       const int qi = c.q0 + *r;
-      return *r < c.nq ? (const T*)a.q + ((long long)(c.q.r0 + qi / a.G) * a.H + c.kvh * a.G + qi % a.G) * HD + *ch * 8 : nullptr;
+      return *r < c.nq && *ch * 8 < hd ? (const T*)a.q + ((long long)(c.q.r0 + qi / a.G) * a.H + c.kvh * a.G + qi % a.G) * hd + *ch * 8
+                                       : nullptr;
     };
     bool have = walk.next(a, p, &pc);
     while (have) {
@@ -754,6 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint4* const stage = reinterpret_cast<uint4*>(stage_sm) + (warp - 4) * 256;
 #pragma unroll 1
         for (int d0 = PAIR ? 0 : X * COLS; d0 < (PAIR ? HD : (X + 1) * COLS); d0 += 32) {
+          if (d0 >= hd) break;
           uint32_t u[32];
           float o[32];
           tm_ld(tmem + lanes + 256 + X * HD + d0, u); /* whatever was there, where the stream had no tile */
@@ -767,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int e = 0; e < 32; ++e) o[e] += other ? __uint_as_float(u[e]) * g : 0.f;
           }
           if (odd_v && live) { /* values taken out of masked tiles go to the rows that see them */
-            const T* qr = (const T*)a.q + at * HD;
+            const T* qr = (const T*)a.q + at * hd;
             const int from = max(c.t0 * TK, min(open, c.q.len) / TK * TK), upto = min(c.q.len, (c.t0 + c.n) * TK);
             for (int pos = from; pos < upto; ++pos) {
               const int j = pos >> a.g.page_shift;
@@ -777,15 +781,15 @@ __global__ void __launch_bounds__(kThreads, 1)
               const T *kr = (const T*)a.k + off, *vr = (const T*)a.v + off + d0;
               bool hit = false;
 #pragma unroll 1
-              for (int e = 0; e < 32; ++e) hit |= !isfinite(to_f<T>(vr[e]));
+              for (int e = 0; e < min(32, hd - d0); ++e) hit |= !isfinite(to_f<T>(vr[e]));
               if (!hit) continue;
               float s = 0.f;
 #pragma unroll 1
-              for (int e = 0; e < HD; ++e) s = __fmaf_rn(to_f<T>(qr[e]), to_f<T>(kr[e]), s);
+              for (int e = 0; e < hd; ++e) s = __fmaf_rn(to_f<T>(qr[e]), to_f<T>(kr[e]), s);
               const float w = ex2(__fmaf_rn(s, a.scale2, -(m == -INFINITY ? 0.f : m)));
 #pragma unroll
               for (int e = 0; e < 32; ++e) {
-                const float x = to_f<T>(vr[e]);
+                const float x = d0 + e < hd ? to_f<T>(vr[e]) : 0.f;
                 if (!isfinite(x)) o[e] += w * x;
               }
             }
@@ -804,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int y = k * 8 + (lane >> 2), w = lane & 3;
               const long long row_at = __shfl_sync(0xffffffffu, at, y);
               const uint4 x = stage[y * 4 + (w ^ ((y >> 1) & 3))];
-              if (r - lane + y < c.nq) *reinterpret_cast<uint4*>((T*)a.out + row_at * HD + d0 + w * 8) = x;
+              if (r - lane + y < c.nq && d0 + w * 8 < hd) *reinterpret_cast<uint4*>((T*)a.out + row_at * hd + d0 + w * 8) = x;
             }
           } else {
 #pragma unroll
@@ -875,10 +879,12 @@ __global__ void __launch_bounds__(kJoinRows * 32) tree_tc_join_kernel(const __gr
   const float inv = L == 0.f ? 0.f : __fdividef(1.f, L);
   const int qi = t.q0 + r;
   const long long at = (long long)(t.r0 + qi / a.G) * a.H + t.kvh * a.G + qi % a.G;
-  T* out = (T*)a.out + at * HD + lane * E;
+  const int hd = a.g.hd;
+  if (lane == 0 && a.lse) a.lse[at] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+  if (lane * E >= hd) return;
+  T* out = (T*)a.out + at * hd + lane * E;
   if constexpr (E == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv));
   else *reinterpret_cast<uint32_t*>(out) = pack2<T>(x[0] * inv, x[1] * inv);
-  if (lane == 0 && a.lse) a.lse[at] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -968,7 +974,7 @@ int pick_tc(Ctx* c, TreeArgs& a) {
  */
 bool tree_tc_fits(const Ctx* c, const TreeArgs& a) {
   const long long nq = (long long)a.max_rows * a.G, bytes = 4ll * a.g.n_seq * a.max_len * a.g.n_head_kv * a.g.hd;
-  if (a.g.hd != 64 && a.g.hd != 128) return false;
+  if (a.g.hd > 128) return false;
   if (nq <= 64 && (bytes < (32ll << 20) || a.max_len < 512)) return false;
   return line_most(a, nq > 128 ? 256 : 128, c->n_sm) < (1ll << 31) - 65536;
 }
