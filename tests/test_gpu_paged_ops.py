@@ -418,7 +418,7 @@ def test_tree_attention_rows_that_see_nothing_and_stale_places(tctx, stale, D, H
         Attention(kind, H, 1, D, 16, [(0, rows), (40, rows), (0, 1)], empty_rows=True, stale=stale, seed=6).check(tctx)
 
 
-@pytest.mark.parametrize("D,H,rows", [(64, 2, 3), (128, 1, 40), (128, 4, 40)])
+@pytest.mark.parametrize("D,H,rows", [(64, 2, 3), (128, 1, 40), (128, 4, 40), (128, 8, 10), (64, 16, 12), (96, 4, 40)])
 @pytest.mark.parametrize("value", [math.nan, math.inf])
 def test_tree_attention_value_that_some_rows_see(tctx, D, H, rows, value):
     """An infinite or NaN V in a slot reaches the rows that see the slot and no other."""
