@@ -77,7 +77,11 @@ struct Cfg {
   static constexpr int WARPS = WM * WK, NT = WARPS * 32, RT = 16 * WM, KW = BK / WK;
   static constexpr int PITCH = (HD + 8) * 2;                 /* bytes between rows of a tile */
   static constexpr int STAGE = 2 * BK * PITCH;               /* K and V */
-  static constexpr int NST = 150000 / STAGE > 6 ? 6 : 150000 / STAGE;
+  /* stages of the ring: small blocks (one row tile of 16) several to an SM, since a short sequence is
+     mostly start and end (64 rows x 300 keys of 32 kv heads: 38 us, 90 with one block an SM) */
+  static constexpr int ROOM = WM == 1 ? 50000 : 75000;
+  static constexpr int NST = ROOM / STAGE < 2 ? 2 : ROOM / STAGE;
+  static constexpr int MIN_BLOCKS = WM > 1 && HD <= 96 ? 2 : 1; /* 64 x 16 rows x 116 keys, hd 64: 22 us, 33 with one */
   static constexpr int OP = HD + 4;                          /* floats between rows of the warps' outputs */
   static constexpr int JOIN = WK * RT * OP * 4;
   static constexpr int SMEM = NST * STAGE > JOIN ? NST * STAGE : JOIN;
@@ -85,7 +89,7 @@ struct Cfg {
 };
 
 template <typename T, int HD, int WM, int WK>
-__global__ void __launch_bounds__(WM* WK * 32, 1) tree_attn_kernel(const __grid_constant__ TreeArgs a) {
+__global__ void __launch_bounds__(WM* WK * 32, Cfg<HD, WM, WK>::MIN_BLOCKS) tree_attn_kernel(const __grid_constant__ TreeArgs a) {
   using C = Cfg<HD, WM, WK>;
   constexpr int KS = HD / 16, NB = C::KW / 8, DB = HD / 8;
   pdl_wait();

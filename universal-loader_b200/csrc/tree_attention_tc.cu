@@ -965,17 +965,20 @@ int pick_tc(Ctx* c, TreeArgs& a) {
 }  // namespace
 
 /*
- * When this form runs: from 65 queries a kv head on, or from 32 MB of K and V (by the longest sequence)
- * in sequences of 512 positions or more.  Below, starting up (barriers, TMEM, tensor maps, two
- * pipelines to fill) costs more than the tensor cores save.  Measured here / mma.sync form, us:
- * 1 row x 500 keys 14.3 / 8.6, 1 x 4000 keys 17.3 / 8.4, 8 x 1 x 1000 keys (32 MB) 20.5 / 19.2,
- * 64 x 1 x 300 keys of 32 kv heads 115 / 90; 1 x 8000 keys of 32 kv heads (131 MB) 34.1 / 38.0,
- * 64 x 1 x 4000 keys 114 / 165.  The line is counted in 32 bits.
+ * When this form runs, by queries a kv head and bytes of K and V (every sequence as long as the longest):
+ * from 65 queries on; from 17 with 16 MB or more; below with 64 MB or more in sequences of 2048
+ * positions or more.  Otherwise starting up (barriers, TMEM, tensor maps, two pipelines to fill) and
+ * what a (sequence, kv head) costs besides its tiles outweigh the tensor cores.  Measured here / mma.sync
+ * form, us (rows x keys): 1 x 500, 8 queries 14.3 / 8.6; 1 x 4000, 8 queries 17.3 / 8.4; 64 x 1 x 1000 mha
+ * 167 / 80; 16 x 1 x 2000, 4 queries 32.6 / 34.4; 64 x 1 x 4000, 4 queries 114 / 149; 1 x 8000 mha 34 / 47;
+ * 8 x 16 x 1000, 64 queries 21.7 / 33.6; 1 x 63 x 2000 mha 22.6 / 27.7; 1 x 64 x 1000, 512 queries 35.3 / 35.6.
+ * The line is counted in 32 bits.
  */
 bool tree_tc_fits(const Ctx* c, const TreeArgs& a) {
   const long long nq = (long long)a.max_rows * a.G, bytes = 4ll * a.g.n_seq * a.max_len * a.g.n_head_kv * a.g.hd;
   if (a.g.hd > 128) return false;
-  if (nq <= 64 && (bytes < (32ll << 20) || a.max_len < 512)) return false;
+  if (nq <= 16 && (bytes < (64ll << 20) || a.max_len < 2048)) return false;
+  if (nq <= 64 && bytes < (16ll << 20)) return false;
   return line_most(a, nq > 128 ? 256 : 128, c->n_sm) < (1ll << 31) - 65536;
 }
 
