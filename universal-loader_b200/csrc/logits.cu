@@ -19,6 +19,11 @@
  * the loop over the logits stays short: the nodes whose token lies in the slice (few) are listed
  * once a block; a unit asks its row's ancestor bits for those, computes their logits from the
  * input, and stores them over the others' after its loop.
+ *
+ * Measured: 504 tree rows x 128256 (fp16 in, 308 MB) 78 us, 64 rows x 128256 (fp32) 24.5 us, one row x
+ * 32000 5 us: 62 %, 42 % and a launch.  Instructions bound the first (some 70 for four tokens a lane),
+ * with occupancy: five blocks an SM and one unit in flight a warp, 96 us with two in flight and three
+ * blocks; the second is mostly the counting's latency in each of its blocks.
  */
 #include <algorithm>
 
@@ -309,11 +314,11 @@ int launch_logits(Ctx* c, const ulb_logits_args& a) {
   const size_t smem = (size_t)(2 * g.slice + g.nodes * (3 + 2 * kWarps)) * 4;
   const long long blocks = (long long)g.n_slice * a.n_seq;
   ULB_CHECK(blocks < (1ll << 31), ULB_EUNSUPPORTED, "ulb_logits_process: %d sequences of %d tokens", a.n_seq, a.V);
-  static bool attr = false;
-  if (!attr) {
+  static uint64_t attr = 0; /* devices it is set on */
+  if (!(attr >> (c->device & 63) & 1)) {
     ULB_CUDA(cudaFuncSetAttribute(logits_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   (2 * kMaxSlice + kMaxNodes * (3 + 2 * kWarps)) * 4));
-    attr = true;
+    attr |= 1ull << (c->device & 63);
   }
   ULB_LAUNCH("logits launch", launch_k(c, logits_kernel<T, V>, dim3((unsigned)blocks), dim3(kWarps * 32), smem, a, g));
   return ULB_OK;

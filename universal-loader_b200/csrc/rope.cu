@@ -17,6 +17,8 @@
  * interleaved pairs), or the two runs of E elements that form E pairs of the half layout, or E
  * elements past rot_dim that pass through.  It computes the unit's sines once and applies them to
  * HPT heads of the row, all of whose loads are in flight before the first is used.
+ * Measured: 16381 fp32 rows of 40 heads of 128 (671 MB) 111 us, 94 % of the copy rate; append of 1024
+ * fp32 rows of 80 heads of 128 into bf16 (63 MB) 15.3 us; of 8 rows 3.7 us.
  */
 #include <algorithm>
 #include <cmath>

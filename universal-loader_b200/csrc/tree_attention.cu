@@ -13,11 +13,16 @@
  *
  * Work of a CTA: RT = 16 WM rows (row = node x head of the GQA group, so a K / V tile is read
  * once for all heads that share it) against the keys of one split, in tiles of 64 keys that
- * stream through a ring of NST shared-memory stages by cp.async.  The 8 (4) warps are WM row
+ * stream through a ring of NST shared-memory stages by cp.async.  The 8 (or 4) warps are WM row
  * groups x WK key groups; a key group has its own (m, l, o), joined in shared memory at the end.
  * S = Q K^T and O = P V are mma.sync m16n8k16 with fp32 accumulators; P stays in registers,
  * rounded to the cache's type (2^-12 or 2^-9 relative a weight, averaged over the keys; the
  * output itself is rounded the same).
+ *
+ * Used for head dim 256 and for calls too small for the tcgen05 form (tree_attention_tc.cu, which has
+ * the rule).  Measured: 1 row x 500 keys, 32 heads over 4, hd 64: 8.6 us, a launch each for the splits
+ * and their join; 64 rows x 300 keys, 32 kv heads of 64: 38 us; 1 row x 30000 keys, 64 heads over 8 of
+ * 256 (246 MB): 62 us, 61 % of the copy rate, bound by the two stages that fit at hd 256.
  *
  * Rows of shared memory are hd + 8 elements apart: 16-byte row pitch odd in units of 16 bytes,
  * so the eight rows of an ldmatrix phase fall in eight different bank groups.
@@ -458,10 +463,10 @@ void plan_splits(TreeArgs* a, long long units, int slots) {
 template <typename T, int HD, int WM, int WK>
 int launch_tree(Ctx* c, TreeArgs& a) {
   using C = Cfg<HD, WM, WK>;
-  static bool attr = false;
-  if (!attr) {
+  static uint64_t attr = 0; /* devices it is set on */
+  if (!(attr >> (c->device & 63) & 1)) {
     ULB_CUDA(cudaFuncSetAttribute(tree_attn_kernel<T, HD, WM, WK>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    attr = true;
+    attr |= 1ull << (c->device & 63);
   }
   a.n_tile = (int)(((long long)a.max_rows * a.G + C::RT - 1) / C::RT);
   const long long units = (long long)a.n_tile * a.g.n_head_kv * a.g.n_seq;
@@ -471,7 +476,6 @@ int launch_tree(Ctx* c, TreeArgs& a) {
     ULB_CHECK(per * a.n_split <= (long long)kTreeWsFloats && a.n_split <= 8192, ULB_EUNSUPPORTED,
               "ulb_tree_attention: %d rows of %d heads over %d positions in pages of %d need %d splits, more than the workspace holds",
               a.rows, a.H, a.max_len, a.g.page, a.n_split);
-    if (!c->tree_ws) ULB_CUDA(cudaMalloc((void**)&c->tree_ws, kTreeWsFloats * sizeof(float)));
     a.po = c->tree_ws;
     a.pml = c->tree_ws + (long long)a.rows * a.H * a.g.hd * a.n_split;
   }
@@ -558,6 +562,8 @@ extern "C" int ulb_tree_attention(ulb_ctx* ctx, const ulb_cache_desc* cache, con
   a.err = ctx->c.dev_err;
   Ctx* c = &ctx->c;
   ULB_CUDA(cudaSetDevice(c->device));
+  /* at the first call, whatever its shape, so that any later one can be captured */
+  if (!c->tree_ws) ULB_CUDA(cudaMalloc((void**)&c->tree_ws, kTreeWsFloats * sizeof(float)));
   if (tree_tc_fits(c, a)) return launch_tree_tc(c, a, cache->dtype == ULB_TYPE_F16);
   return cache->dtype == ULB_TYPE_F16 ? pick_dim<__half>(c, a) : pick_dim<__nv_bfloat16>(c, a);
 }

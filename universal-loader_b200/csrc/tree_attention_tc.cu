@@ -23,13 +23,19 @@
  * rescale O).  A stream has two score buffers; one thread issues its MMAs and they complete in order,
  * so a buffer is free for the tile after the next once the product that reads its weights has been
  * issued, and the scores of the next tile are there while weights are computed (128-key tiles with one
- * buffer, weights handed over in halves, took 339 us where this took 297).
+ * buffer, weights handed over in halves, took 339 us where this took 300).
  *
  * Work is cut evenly: the tiles of all (sequence, kv head) pairs form one line, every CTA (group
  * of CTAs, when more than 256 rows need several row tiles: its members walk the same keys side by
  * side, so K / V come from HBM once) takes an equal stretch of it, whatever the lengths, and
  * walks whole sequences and pieces of two.  A pair that falls into several stretches leaves one
  * partial a stretch, joined by a small kernel.
+ *
+ * Measured: 64 rows x 64 heads (8 kv heads of 128) x 131072 keys 289 us, 950 TFLOP/s (57 % of the measured
+ * burst): the round trip between products and softmax, with two streams of two score buffers, which is
+ * what TMEM holds, bounds it (tensor pipe 54 %, exponentials 44 %).  64 sequences of 256 to 4096 keys with
+ * 8 to 16 rows, 32 heads over 8: 123 us, 4.8 TB/s of K and V: HBM and some 6 us a (sequence, kv head).
+ * 63 rows x 8191 keys, 32 kv heads: 39 us, of which 12 are a CTA's start and end and 5 the join.
  *
  * Every mbarrier wait has a limit: past it a role raises bit 3 of the device error word,
  * arrives nowhere and issues nothing any more, so that the others run into theirs; the CTA still
@@ -296,7 +302,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr uint32_t ID_S = (1u << 4) | FMT | ((TK >> 3) << 17) | ((128 >> 4) << 24);
   constexpr uint32_t ID_O = (1u << 4) | FMT | (1u << 16) | ((HD >> 3) << 17) | ((128 >> 4) << 24);
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t k_full[C::NK], k_free[C::NK], v_full[C::NV], v_free[C::NV], s_full[2][2], p_full[2][2], o_done[2][2], v_seen[2], piece[2], q_full, mma_done;
+  __shared__ uint64_t k_full[C::NK], k_free[C::NK], v_full[C::NV], v_free[C::NV], s_full[2][2], p_full[2][2], o_done[2][2], v_seen[2],
+      piece[2], q_full, mma_done;
   __shared__ uint32_t tmem_sh;
   __shared__ int odd_v, sh_s, sh_base, sh_sum[kThreads / 32];
   uint8_t* const sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -394,152 +401,152 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   /* registers: 128 x 104 + 256 x 200 = 384 x 168, what the block was launched with */
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-  if (warp == 0 || warp == 3) {
-    /* ------------------------------------------------ TMA: warp 0 the K tiles, warp 3 the V tiles, in order.
-       Asking for a free slot, issuing and looking up pages take some 750 cycles a tile, so each
-       has a warp and the page ids are read a tile ahead. */
-    const CUtensorMap* const map = warp == 0 ? &mk : &mv;
-    uint8_t* const ring = warp == 0 ? k_sm : v_sm;
-    uint64_t* const full = warp == 0 ? k_full : v_full;
-    uint64_t* const free = warp == 0 ? k_free : v_free;
-    const int nring = warp == 0 ? C::NK : C::NV;
-    int slot = 0, issued = 0;
-    uint32_t phase = 1; /* of the free barrier: the first round passes */
-    const int rows = min(a.g.page, TK), boxes = TK / rows;
-    constexpr int MB = TK / 16;
-    while (ok && walk.next(a, p, &pc)) {
-      const int* const tb = a.table + (long long)pc.s * a.g.max_pages;
-      int pg[MB]; /* pages of the next tile; n_pages, out of range, reads zeros */
-      auto ids = [&](int t) {
-        const int pos = (pc.t0 + t) * TK; /* at most len + 63 */
-#pragma unroll
-        for (int i = 0; i < MB; ++i) {
-          const int at = pos + i * rows, j = at >> a.g.page_shift;
-          pg[i] = i < boxes && t < pc.n && at < pc.q.len && j < a.g.max_pages ? tb[j] : -1;
-        }
-      };
-      ids(0);
-      for (int t = 0; t < pc.n && ok; ++t) {
-        ok = mb_wait_warp(&free[slot], phase);
-        if (elect()) {
-          const int pos = ((pc.t0 + t) * TK) & (a.g.page - 1);
-          uint8_t* const d = ring + slot * C::TILE;
-          mb_expect(&full[slot], (uint32_t)C::TILE);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == 0 || warp == 3) {
+      /* ------------------------------------------------ TMA: warp 0 the K tiles, warp 3 the V tiles, in order.
+         Asking for a free slot, issuing and looking up pages take some 750 cycles a tile, so each
+         has a warp and the page ids are read a tile ahead. */
+      const CUtensorMap* const map = warp == 0 ? &mk : &mv;
+      uint8_t* const ring = warp == 0 ? k_sm : v_sm;
+      uint64_t* const full = warp == 0 ? k_full : v_full;
+      uint64_t* const free = warp == 0 ? k_free : v_free;
+      const int nring = warp == 0 ? C::NK : C::NV;
+      int slot = 0, issued = 0;
+      uint32_t phase = 1; /* of the free barrier: the first round passes */
+      const int rows = min(a.g.page, TK), boxes = TK / rows;
+      constexpr int MB = TK / 16;
+      while (ok && walk.next(a, p, &pc)) {
+        const int* const tb = a.table + (long long)pc.s * a.g.max_pages;
+        int pg[MB]; /* pages of the next tile; n_pages, out of range, reads zeros */
+        auto ids = [&](int t) {
+          const int pos = (pc.t0 + t) * TK; /* at most len + 63 */
 #pragma unroll
           for (int i = 0; i < MB; ++i) {
-            if (i >= boxes) break;
-            const int page = pg[i] >= 0 && pg[i] < a.g.n_pages ? pg[i] : a.g.n_pages;
-#pragma unroll
-            for (int h = 0; h < HD / 64; ++h) tma4(d + i * rows * 128 + h * TK * 128, map, h * 64, pos, pc.kvh, page, &full[slot]);
+            const int at = pos + i * rows, j = at >> a.g.page_shift;
+            pg[i] = i < boxes && t < pc.n && at < pc.q.len && j < a.g.max_pages ? tb[j] : -1;
           }
+        };
+        ids(0);
+        for (int t = 0; t < pc.n && ok; ++t) {
+          ok = mb_wait_warp(&free[slot], phase);
+          if (elect()) {
+            const int pos = ((pc.t0 + t) * TK) & (a.g.page - 1);
+            uint8_t* const d = ring + slot * C::TILE;
+            mb_expect(&full[slot], (uint32_t)C::TILE);
+#pragma unroll
+            for (int i = 0; i < MB; ++i) {
+              if (i >= boxes) break;
+              const int page = pg[i] >= 0 && pg[i] < a.g.n_pages ? pg[i] : a.g.n_pages;
+#pragma unroll
+              for (int h = 0; h < HD / 64; ++h) tma4(d + i * rows * 128 + h * TK * 128, map, h * 64, pos, pc.kvh, page, &full[slot]);
+            }
+          }
+          __syncwarp();
+          ids(t + 1);
+          ++issued;
+          if (++slot == nring) { slot = 0; phase ^= 1; }
         }
-        __syncwarp();
-        ids(t + 1);
-        ++issued;
-        if (++slot == nring) { slot = 0; phase ^= 1; }
       }
-    }
-    /* no copy is in flight when the CTA ends, whatever happened: the last round's tiles, in turn */
-    for (int c = max(0, issued - nring); c < issued; ++c) ok &= mb_wait_warp(&full[c % nring], (c / nring) & 1);
-  } else {
-    /* ------------------------------------------------ MMA issue: a warp a stream walks, one elected lane
-       issues.  What one thread does for a tile (waits, MMAs, commits) takes about as long as its
-       arithmetic, so descriptors are a base plus a constant and ring places are counted.
-       A parity wait can tell a phase from the one before and after only, so nobody may skip one: both
-       warps look at every K and V tile, and a tile is free when both have (the stream that does not
-       use it at once).  On a wait that fails the warp stops; nothing is issued after that. */
-    const int X = warp - 1;
-    uint32_t qp = 0, pp = 0; /* phases of q_full, and of p_full[X][b] in bit b */
-    int ks = 0, vs = 0;      /* next tile of the rings, and its phase */
-    uint32_t kp = 0, vp = 0;
-    const uint64_t dq = desc_k(sa(q_sm)) + (PAIR ? X * (C::QTILE >> 4) : 0), dk = desc_k(sa(k_sm)), dv = desc_mn(sa(v_sm));
-    const uint32_t ds = tmem + X * 128, dov = tmem + 256 + X * HD;
-    while (ok && walk.next(a, p, &pc)) {
-      ok = mb_wait_warp(&q_full, qp);
-      qp ^= 1;
-      const int n = n_of(X), clear = min(tree_open(a, pc.q), pc.q.len);
-      int kt = 0, vt = 0; /* tiles of the piece seen so far */
-      auto mine = [&](int t) { return PAIR ? n > 0 : (t & 1) == X; };
-      /* pass the other stream's tiles up to this stream's next, or to the end */
-      auto next_k = [&]() {
-        while (ok && kt < pc.n && !mine(kt)) {
-          ok = mb_wait_warp(&k_full[ks], kp);
-          if (ok && lane == 0) mb_arrive(&k_free[ks]);
+      /* no copy is in flight when the CTA ends, whatever happened: the last round's tiles, in turn */
+      for (int c = max(0, issued - nring); c < issued; ++c) ok &= mb_wait_warp(&full[c % nring], (c / nring) & 1);
+    } else {
+      /* ------------------------------------------------ MMA issue: a warp a stream walks, one elected lane
+         issues.  What one thread does for a tile (waits, MMAs, commits) takes about as long as its
+         arithmetic, so descriptors are a base plus a constant and ring places are counted.
+         A parity wait can tell a phase from the one before and after only, so nobody may skip one: both
+         warps look at every K and V tile, and a tile is free when both have (the stream that does not
+         use it at once).  On a wait that fails the warp stops; nothing is issued after that. */
+      const int X = warp - 1;
+      uint32_t qp = 0, pp = 0; /* phases of q_full, and of p_full[X][b] in bit b */
+      int ks = 0, vs = 0;      /* next tile of the rings, and its phase */
+      uint32_t kp = 0, vp = 0;
+      const uint64_t dq = desc_k(sa(q_sm)) + (PAIR ? X * (C::QTILE >> 4) : 0), dk = desc_k(sa(k_sm)), dv = desc_mn(sa(v_sm));
+      const uint32_t ds = tmem + X * 128, dov = tmem + 256 + X * HD;
+      while (ok && walk.next(a, p, &pc)) {
+        ok = mb_wait_warp(&q_full, qp);
+        qp ^= 1;
+        const int n = n_of(X), clear = min(tree_open(a, pc.q), pc.q.len);
+        int kt = 0, vt = 0; /* tiles of the piece seen so far */
+        auto mine = [&](int t) { return PAIR ? n > 0 : (t & 1) == X; };
+        /* pass the other stream's tiles up to this stream's next, or to the end */
+        auto next_k = [&]() {
+          while (ok && kt < pc.n && !mine(kt)) {
+            ok = mb_wait_warp(&k_full[ks], kp);
+            if (ok && lane == 0) mb_arrive(&k_free[ks]);
+            if (++ks == C::NK) { ks = 0; kp ^= 1; }
+            ++kt;
+          }
+          return ok && kt < pc.n;
+        };
+        auto next_v = [&]() {
+          while (ok && vt < pc.n && !mine(vt)) {
+            ok = mb_wait_warp(&v_full[vs], vp);
+            if (ok && lane == 0) mb_arrive(&v_free[vs]);
+            if (++vs == C::NV) { vs = 0; vp ^= 1; }
+            ++vt;
+          }
+          return ok && vt < pc.n;
+        };
+        auto qk = [&](int b) { /* scores of K tile kt into buffer b (one lane) */
+          const uint64_t k0 = dk + ks * (C::TILE >> 4);
+#pragma unroll
+          for (int j = 0; j < HD / 16; ++j)
+            mma_ss(ds + b * TK, dq + (((j >> 2) * (TQ * 128) + (j & 3) * 32) >> 4), k0 + (((j >> 2) * (TK * 128) + (j & 3) * 32) >> 4), ID_S,
+                   j > 0);
+          commit(&s_full[X][b]);
+          commit(&k_free[ks]);
+        };
+        auto step_k = [&]() {
           if (++ks == C::NK) { ks = 0; kp ^= 1; }
           ++kt;
+        };
+        for (int i = 0; i < min(n, 2) && ok; ++i) {
+          ok = next_k() && mb_wait_warp(&k_full[ks], kp);
+          if (!ok) break;
+          tc_after();
+          if (elect()) qk(i);
+          __syncwarp();
+          step_k();
         }
-        return ok && kt < pc.n;
-      };
-      auto next_v = [&]() {
-        while (ok && vt < pc.n && !mine(vt)) {
-          ok = mb_wait_warp(&v_full[vs], vp);
-          if (ok && lane == 0) mb_arrive(&v_free[vs]);
+        for (int i = 0; i < n && ok; ++i) {
+          const int b = i & 1;
+          const bool more = i + 2 < n;
+          /* the rings first, they are mostly ready; then the weights */
+          ok = next_v() && mb_wait_warp(&v_full[vs], vp);
+          if (!ok) break;
+          if ((pc.t0 + vt + 1) * TK > clear && lane == 0) mb_arrive(&v_seen[X]); /* masked: the softmax warps look it over */
+          if (more) ok = next_k() && mb_wait_warp(&k_full[ks], kp);
+          ok = ok && mb_wait_warp(&p_full[X][b], (pp >> b) & 1);
+          if (!ok) break;
+          pp ^= 1u << b;
+          tc_after();
+          if (elect()) {
+            const uint64_t v0 = dv + vs * (C::TILE >> 4);
+            const uint32_t pa = ds + b * TK;
+            mma_ts(dov, pa, v0, ID_O, i > 0);
+#pragma unroll
+            for (int j = 1; j < TK / 16; ++j) mma_ts(dov, pa + j * 8, v0 + ((j * 2048) >> 4), ID_O, 1);
+            commit(&o_done[X][b]);
+            commit(&v_free[vs]);
+            if (more) qk(b);
+          }
+          __syncwarp();
           if (++vs == C::NV) { vs = 0; vp ^= 1; }
           ++vt;
+          if (more) step_k();
         }
-        return ok && vt < pc.n;
-      };
-      auto qk = [&](int b) { /* scores of K tile kt into buffer b (one lane) */
-        const uint64_t k0 = dk + ks * (C::TILE >> 4);
-#pragma unroll
-        for (int j = 0; j < HD / 16; ++j)
-          mma_ss(ds + b * TK, dq + (((j >> 2) * (TQ * 128) + (j & 3) * 32) >> 4), k0 + (((j >> 2) * (TK * 128) + (j & 3) * 32) >> 4), ID_S,
-                 j > 0);
-        commit(&s_full[X][b]);
-        commit(&k_free[ks]);
-      };
-      auto step_k = [&]() {
-        if (++ks == C::NK) { ks = 0; kp ^= 1; }
-        ++kt;
-      };
-      for (int i = 0; i < min(n, 2) && ok; ++i) {
-        ok = next_k() && mb_wait_warp(&k_full[ks], kp);
-        if (!ok) break;
-        tc_after();
-        if (elect()) qk(i);
+        next_k();
+        next_v();
+        /* the piece is through, without tiles too: the softmax warps wait for it, so they cannot start two
+           pieces while this warp has not seen one */
+        if (ok && elect()) commit(&piece[X]);
         __syncwarp();
-        step_k();
       }
-      for (int i = 0; i < n && ok; ++i) {
-        const int b = i & 1;
-        const bool more = i + 2 < n;
-        /* the rings first, they are mostly ready; then the weights */
-        ok = next_v() && mb_wait_warp(&v_full[vs], vp);
-        if (!ok) break;
-        if ((pc.t0 + vt + 1) * TK > clear && lane == 0) mb_arrive(&v_seen[X]); /* masked: the softmax warps look it over */
-        if (more) ok = next_k() && mb_wait_warp(&k_full[ks], kp);
-        ok = ok && mb_wait_warp(&p_full[X][b], (pp >> b) & 1);
-        if (!ok) break;
-        pp ^= 1u << b;
-        tc_after();
-        if (elect()) {
-          const uint64_t v0 = dv + vs * (C::TILE >> 4);
-          const uint32_t pa = ds + b * TK;
-          mma_ts(dov, pa, v0, ID_O, i > 0);
-#pragma unroll
-          for (int j = 1; j < TK / 16; ++j) mma_ts(dov, pa + j * 8, v0 + ((j * 2048) >> 4), ID_O, 1);
-          commit(&o_done[X][b]);
-          commit(&v_free[vs]);
-          if (more) qk(b);
-        }
-        __syncwarp();
-        if (++vs == C::NV) { vs = 0; vp ^= 1; }
-        ++vt;
-        if (more) step_k();
-      }
-      next_k();
-      next_v();
-      /* the piece is through, without tiles too: the softmax warps wait for it, so they cannot start two
-         pieces while this warp has not seen one */
-      if (ok && elect()) commit(&piece[X]);
+      /* everything issued completes before TMEM is freed */
+      if (elect()) commit(&mma_done);
       __syncwarp();
+      ok = mb_wait_warp(&mma_done, 0) && ok;
     }
-    /* everything issued completes before TMEM is freed */
-    if (elect()) commit(&mma_done);
-    __syncwarp();
-    ok = mb_wait_warp(&mma_done, 0) && ok;
-  }
   } else {
     /* ------------------------------------------------ softmax: one thread a row */
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
@@ -567,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return x >= 0 && x < a.g.n_pages;
       };
       /* is some page of the piece unmapped?  A page a lane, its load under way beside those of Q */
-      const int j0 = ((pc.t0 * TK) >> a.g.page_shift) + lane, j1 = (int)min(((long long)(pc.t0 + pc.n) * TK - 1) >> a.g.page_shift, (long long)(pc.q.len - 1) >> a.g.page_shift);
+      const int j0 = ((pc.t0 * TK) >> a.g.page_shift) + lane, j1 = (min((pc.t0 + pc.n) * TK, pc.q.len) - 1) >> a.g.page_shift;
       const int page0 = j0 <= j1 && j0 < a.g.max_pages ? a.table[(long long)pc.s * a.g.max_pages + j0] : j0 <= j1 ? -1 : 0;
       {
         uint4 qx[QW];
@@ -926,10 +933,10 @@ long long line_most(const TreeArgs& a, int RT, int n_sm) {
 template <typename T, int HD, bool PAIR>
 int launch_tc(Ctx* c, TreeArgs& a) {
   using C = TcCfg<HD, PAIR>;
-  static bool attr = false;
-  if (!attr) {
+  static uint64_t attr = 0; /* devices it is set on */
+  if (!(attr >> (c->device & 63) & 1)) {
     ULB_CUDA(cudaFuncSetAttribute(tree_tc_kernel<T, HD, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    attr = true;
+    attr |= 1ull << (c->device & 63);
   }
   CUtensorMap mk, mv;
   constexpr bool f16 = std::is_same<T, __half>::value;
@@ -941,7 +948,6 @@ int launch_tc(Ctx* c, TreeArgs& a) {
   p.groups_max = c->n_sm / p.members;
   p.min_tiles = kMinTiles;
   const int grid = p.groups_max * p.members;
-  if (!c->tree_ws) ULB_CUDA(cudaMalloc((void**)&c->tree_ws, kTreeWsFloats * sizeof(float)));
   const size_t rows = (size_t)grid * 2 * C::RT;
   ULB_CHECK(rows * (HD + 2) + (size_t)grid * 8 <= kTreeWsFloats, ULB_EUNSUPPORTED, "ulb_tree_attention: workspace for %d SMs", c->n_sm);
   a.po = c->tree_ws;
