@@ -393,7 +393,7 @@ ULB_API int ulb_rope_append(ulb_ctx* ctx, const ulb_rope* r, const ulb_cache_des
  * lse = -inf; what it does not see (stale slots, positions past len[s], infinities and NaN there)
  * never touches its result.  head_dim 64, 80, 96, 128 or 256; n_head / n_head_kv <= 64.
  * max_rows >= every sequence's rows, max_len >= every len[s] (clamped otherwise).  Scores, statistics and sums are fp32; the probabilities of the
- * second product are rounded to the cache type.  The first call on a context allocates 128 MiB of
+ * second product are rounded to the cache type (small bf16 calls keep two parts of them).  The first call on a context allocates 128 MiB of
  * device memory for partial results, kept until ulb_destroy.
  */
 typedef struct ulb_tree_desc {

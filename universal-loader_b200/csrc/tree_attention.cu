@@ -15,9 +15,9 @@
  * once for all heads that share it) against the keys of one split, in tiles of 64 keys that
  * stream through a ring of NST shared-memory stages by cp.async.  The 8 (or 4) warps are WM row
  * groups x WK key groups; a key group has its own (m, l, o), joined in shared memory at the end.
- * S = Q K^T and O = P V are mma.sync m16n8k16 with fp32 accumulators; P stays in registers,
- * rounded to the cache's type (2^-12 or 2^-9 relative a weight, averaged over the keys; the
- * output itself is rounded the same).
+ * S = Q K^T and O = P V are mma.sync m16n8k16 with fp32 accumulators; P stays in registers, rounded to
+ * fp16 (2^-12 relative a weight, averaged over the keys; the output itself is rounded the same) or
+ * kept as two bf16 parts.
  *
  * Used for head dim 256 and for calls too small for the tcgen05 form (tree_attention_tc.cu, which has
  * the rule).  Measured: 1 row x 500 keys, 32 heads over 4, hd 64: 8.6 us, a launch each for the splits
@@ -282,12 +282,28 @@ __global__ void __launch_bounds__(WM* WK * 32, Cfg<HD, WM, WK>::MIN_BLOCKS) tree
     for (int n = 0; n < NB; n += 2) {
       const uint32_t pf[4] = {pack2<T>(sc[n][0], sc[n][1]), pack2<T>(sc[n][2], sc[n][3]), pack2<T>(sc[n + 1][0], sc[n + 1][1]),
                               pack2<T>(sc[n + 1][2], sc[n + 1][3])};
+      /* what bf16 leaves of a weight is a second operand: these calls wait for memory, not for products,
+         and the output's own rounding stays the only one */
+      constexpr bool REST = std::is_same<T, __nv_bfloat16>::value;
+      [[maybe_unused]] uint32_t pr[4] = {};
+      if constexpr (REST) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 h = unpack2<T>(pf[e]);
+          const float* w = &sc[n + (e >> 1)][2 * (e & 1)];
+          pr[e] = pack2<T>(w[0] - h.x, w[1] - h.y);
+        }
+      }
 #pragma unroll
       for (int d = 0; d < DB; d += 2) {
         uint32_t b[4];
         ldsm4t(vaddr + n * 8 * C::PITCH + d * 16, b);
         mma<T>(o[d], pf, b[0], b[1]);
         mma<T>(o[d + 1], pf, b[2], b[3]);
+        if constexpr (REST) {
+          mma<T>(o[d], pr, b[0], b[1]);
+          mma<T>(o[d + 1], pr, b[2], b[3]);
+        }
       }
     }
     if (fix) { /* what left the tile, to the rows that see it */

@@ -55,7 +55,7 @@ constexpr int TK = 64;         /* keys a tile */
 constexpr int TQ = 128;        /* query rows a stream: M */
 constexpr int kThreads = 384;  /* 4 role warps, 2 x 4 softmax warps */
 constexpr int kPairCost = 16;   /* what a pair costs besides its tiles, in tiles */
-constexpr int kMinTiles = 12;  /* tiles of the line a group takes at least */
+constexpr int kMinTiles = 12;  /* places of the line a group takes at least */
 constexpr int kJoinRows = 8;   /* rows a block of the join kernel: a warp each */
 
 __device__ __forceinline__ uint32_t sa(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
