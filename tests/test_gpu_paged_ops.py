@@ -576,6 +576,17 @@ def test_tree_attention_tensor_core_form_by_bytes(tctx, D, H, Hkv, rows):
     assert float((ls.double() - l2.double()).abs().max()) <= 4e-5 * (1 + float(ls.abs().max()))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_tree_attention_row_tiles_half_empty_over_long_pieces(tctx, D):
+    """Two streams of 128 queries of which the second has none, over more K and V tiles than both rings
+    hold: a last row tile of 64 queries, and sequences on either side of 128 queries in one call."""
+    Attention("bf16", 32, 4, D, 64, [(32000, 40)], seed=D).check(tctx)
+    tctx.sync()
+    a = [(6000 + 97 * i, 17 + (5 * i) % 17) for i in range(16)]
+    Attention("f16", 8, 2, D, 128, a, seed=D + 1).check(tctx)
+    tctx.sync()
+
+
 def test_tree_attention_refusals(tctx):
     import ulb_capi as U
     x = torch.zeros(1 << 16, dtype=torch.float16, device="cuda")

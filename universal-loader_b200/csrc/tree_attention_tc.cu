@@ -42,6 +42,7 @@
  * waits (bounded) for its MMAs before it frees TMEM.
  */
 #include "tree_attention.h"
+#include "tree_plan.h"
 
 #include <cuda.h>
 
@@ -451,11 +452,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = max(0, issued - nring); c < issued; ++c) ok &= mb_wait_warp(&full[c % nring], (c / nring) & 1);
     } else {
       /* ------------------------------------------------ MMA issue: a warp a stream walks, one elected lane
-         issues.  What one thread does for a tile (waits, MMAs, commits) takes about as long as its
-         arithmetic, so descriptors are a base plus a constant and ring places are counted.
-         A parity wait can tell a phase from the one before and after only, so nobody may skip one: both
-         warps look at every K and V tile, and a tile is free when both have (the stream that does not
-         use it at once).  On a wait that fails the warp stops; nothing is issued after that. */
+         issues, in the order of ring_issue.  What one thread does for a tile (waits, MMAs, commits) takes
+         about as long as its arithmetic, so descriptors are a base plus a constant and ring places are
+         counted.  A parity wait can tell a phase from the one before and after only, so nobody may skip
+         one: both warps look at every K and V tile, and a tile is free when both have (the stream that
+         does not use it at once).  On a wait that fails the warp stops; nothing is issued after that. */
       const int X = warp - 1;
       uint32_t qp = 0, pp = 0; /* phases of q_full, and of p_full[X][b] in bit b */
       int ks = 0, vs = 0;      /* next tile of the rings, and its phase */
@@ -466,28 +467,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = mb_wait_warp(&q_full, qp);
         qp ^= 1;
         const int n = n_of(X), clear = min(tree_open(a, pc.q), pc.q.len);
-        int kt = 0, vt = 0; /* tiles of the piece seen so far */
-        auto mine = [&](int t) { return PAIR ? n > 0 : (t & 1) == X; };
-        /* pass the other stream's tiles up to this stream's next, or to the end */
-        auto next_k = [&]() {
-          while (ok && kt < pc.n && !mine(kt)) {
-            ok = mb_wait_warp(&k_full[ks], kp);
-            if (ok && lane == 0) mb_arrive(&k_free[ks]);
-            if (++ks == C::NK) { ks = 0; kp ^= 1; }
-            ++kt;
-          }
-          return ok && kt < pc.n;
+        auto step_k = [&]() { if (++ks == C::NK) { ks = 0; kp ^= 1; } };
+        auto step_v = [&]() { if (++vs == C::NV) { vs = 0; vp ^= 1; } };
+        auto wait_k = [&]() { return mb_wait_warp(&k_full[ks], kp); };
+        auto wait_v = [&]() { return mb_wait_warp(&v_full[vs], vp); };
+        auto pass_k = [&]() {
+          if (!wait_k()) return false;
+          if (lane == 0) mb_arrive(&k_free[ks]);
+          step_k();
+          return true;
         };
-        auto next_v = [&]() {
-          while (ok && vt < pc.n && !mine(vt)) {
-            ok = mb_wait_warp(&v_full[vs], vp);
-            if (ok && lane == 0) mb_arrive(&v_free[vs]);
-            if (++vs == C::NV) { vs = 0; vp ^= 1; }
-            ++vt;
-          }
-          return ok && vt < pc.n;
+        auto pass_v = [&]() {
+          if (!wait_v()) return false;
+          if (lane == 0) mb_arrive(&v_free[vs]);
+          step_v();
+          return true;
         };
-        auto qk = [&](int b) { /* scores of K tile kt into buffer b (one lane) */
+        auto qk = [&](int b) { /* scores of the next K tile into buffer b (one lane) */
           const uint64_t k0 = dk + ks * (C::TILE >> 4);
 #pragma unroll
           for (int j = 0; j < HD / 16; ++j)
@@ -496,47 +492,38 @@ __global__ void __launch_bounds__(kThreads, 1)
           commit(&s_full[X][b]);
           commit(&k_free[ks]);
         };
-        auto step_k = [&]() {
-          if (++ks == C::NK) { ks = 0; kp ^= 1; }
-          ++kt;
-        };
-        for (int i = 0; i < min(n, 2) && ok; ++i) {
-          ok = next_k() && mb_wait_warp(&k_full[ks], kp);
-          if (!ok) break;
-          tc_after();
-          if (elect()) qk(i);
-          __syncwarp();
-          step_k();
-        }
-        for (int i = 0; i < n && ok; ++i) {
-          const int b = i & 1;
-          const bool more = i + 2 < n;
-          /* the rings first, they are mostly ready; then the weights */
-          ok = next_v() && mb_wait_warp(&v_full[vs], vp);
-          if (!ok) break;
-          if ((pc.t0 + vt + 1) * TK > clear && lane == 0) mb_arrive(&v_seen[X]); /* masked: the softmax warps look it over */
-          if (more) ok = next_k() && mb_wait_warp(&k_full[ks], kp);
-          ok = ok && mb_wait_warp(&p_full[X][b], (pp >> b) & 1);
-          if (!ok) break;
-          pp ^= 1u << b;
-          tc_after();
-          if (elect()) {
-            const uint64_t v0 = dv + vs * (C::TILE >> 4);
-            const uint32_t pa = ds + b * TK;
-            mma_ts(dov, pa, v0, ID_O, i > 0);
+        ok = ok && ring_issue<PAIR>(
+            X, n, pc.n, pass_k, pass_v, wait_k, wait_v,
+            [&](int b) {
+              tc_after();
+              if (elect()) qk(b);
+              __syncwarp();
+              step_k();
+            },
+            [&](int vt) { /* masked: the softmax warps look it over */
+              if ((pc.t0 + vt + 1) * TK > clear && lane == 0) mb_arrive(&v_seen[X]);
+            },
+            [&](int b) {
+              if (!mb_wait_warp(&p_full[X][b], (pp >> b) & 1)) return false;
+              pp ^= 1u << b;
+              return true;
+            },
+            [&](int b, int i, bool more) {
+              tc_after();
+              if (elect()) {
+                const uint64_t v0 = dv + vs * (C::TILE >> 4);
+                const uint32_t pa = ds + b * TK;
+                mma_ts(dov, pa, v0, ID_O, i > 0);
 #pragma unroll
-            for (int j = 1; j < TK / 16; ++j) mma_ts(dov, pa + j * 8, v0 + ((j * 2048) >> 4), ID_O, 1);
-            commit(&o_done[X][b]);
-            commit(&v_free[vs]);
-            if (more) qk(b);
-          }
-          __syncwarp();
-          if (++vs == C::NV) { vs = 0; vp ^= 1; }
-          ++vt;
-          if (more) step_k();
-        }
-        next_k();
-        next_v();
+                for (int j = 1; j < TK / 16; ++j) mma_ts(dov, pa + j * 8, v0 + ((j * 2048) >> 4), ID_O, 1);
+                commit(&o_done[X][b]);
+                commit(&v_free[vs]);
+                if (more) qk(b);
+              }
+              __syncwarp();
+              step_v();
+              if (more) step_k();
+            });
         /* the piece is through, without tiles too: the softmax warps wait for it, so they cannot start two
            pieces while this warp has not seen one */
         if (ok && elect()) commit(&piece[X]);
