@@ -185,3 +185,28 @@ int main() {
 
 def test_a_failed_wait_ends_the_issuing_role(tmp_path):
     run(tmp_path, STOP)
+
+
+COPY = r'''
+#include <cstdio>
+#include "tree_plan.h"
+int main() {
+  for (int n = 0; n < 20; ++n)
+    for (int fail = 0; fail <= n; ++fail) {
+      int waits = 0, copies = 0, looks = 0, bad = 0;
+      const bool whole = ulb::ring_copy(
+          n, [&](int t) { bad += t != looks++; }, [&] { return waits++ != fail; },
+          [&](int t) { bad += t != copies++ || copies > fail || looks != t + 1; });
+      if (bad || copies != (fail < n ? fail : n) || whole != (fail >= n)) {
+        std::printf("%d tiles, wait %d: %d copies\n", n, fail, copies);
+        return 1;
+      }
+    }
+  std::printf("ok\n");
+}
+'''
+
+
+def test_a_failed_wait_ends_the_copies(tmp_path):
+    """A place that was not seen free is not copied into, nor any after it."""
+    run(tmp_path, COPY)

@@ -427,9 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             pg[i] = i < boxes && t < pc.n && at < pc.q.len && j < a.g.max_pages ? tb[j] : -1;
           }
         };
-        ids(0);
-        for (int t = 0; t < pc.n && ok; ++t) {
-          ok = mb_wait_warp(&free[slot], phase);
+        ok = ring_copy(pc.n, ids, [&]() { return mb_wait_warp(&free[slot], phase); }, [&](int t) {
           if (elect()) {
             const int pos = ((pc.t0 + t) * TK) & (a.g.page - 1);
             uint8_t* const d = ring + slot * C::TILE;
@@ -443,10 +441,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           __syncwarp();
-          ids(t + 1);
           ++issued;
           if (++slot == nring) { slot = 0; phase ^= 1; }
-        }
+        });
       }
       /* no copy is in flight when the CTA ends, whatever happened: the last round's tiles, in turn */
       for (int c = max(0, issued - nring); c < issued; ++c) ok &= mb_wait_warp(&full[c % nring], (c / nring) & 1);
@@ -687,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               v[j] = make_uint4(w[0], w[1], w[2], w[3]);
             }
           };
-          for (int j = lo * 8 + row; j < TK * 8; j += 128) {
+          for (int j = lo * 8 + row; j < TK * 8 && ok; j += 128) {
             clear(j);
             if (HD == 128) clear(TK * 8 + j);
           }

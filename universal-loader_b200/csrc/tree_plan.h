@@ -70,4 +70,20 @@ ULB_ROLE bool ring_issue(int X, int n, int tiles, PassK&& pass_k, PassV&& pass_v
   return next_k() && next_v();
 }
 
+/*
+ * What a copying warp does with the n tiles of a piece: a place is waited for, then filled; look(t)
+ * reads ahead what the copy of tile t needs.  After a wait that did not end, nothing is copied any more
+ * (the place may still be read) and the answer is false.
+ */
+template <typename Look, typename WaitFree, typename Copy>
+ULB_ROLE bool ring_copy(int n, Look&& look, WaitFree&& wait_free, Copy&& copy) {
+  look(0);
+  for (int t = 0; t < n; ++t) {
+    if (!wait_free()) return false;
+    copy(t);
+    look(t + 1);
+  }
+  return true;
+}
+
 }  // namespace ulb
