@@ -587,6 +587,27 @@ def test_tree_attention_row_tiles_half_empty_over_long_pieces(tctx, D):
     tctx.sync()
 
 
+@pytest.mark.parametrize("D,H,Hkv", [(64, 4, 4), (128, 8, 1), (256, 4, 1)])
+def test_tree_attention_row_ranges_out_of_order(tctx, D, H, Hkv):
+    """Row ranges that end before they begin or lie outside the call's rows touch no row of others."""
+    import ulb_capi as U
+    low, high = -2 ** 31, 2 ** 31 - 1
+    a = Attention("f16", H, Hkv, D, 64, [(200, 40)] * 4, seed=D)
+    want, _ = a.run(tctx)
+    c = U.CacheDesc(dtype=U.T_F16, n_head_kv=Hkv, head_dim=D, page=64, n_pages=a.n_pages, n_seq=4, max_pages=a.most)
+    for start, rows in (([high, high, 160, 120, 160], [(120, 160)]), ([0, 150, low, -1, -1], [(0, 40)]),
+                        ([high, low, low, low, low], []), ([500, 40, 80, low, 0], [(40, 80)])):
+        out = torch.full((a.rows + 40, H, D), 9.0, dtype=torch.float16, device="cuda")
+        q = torch.cat([a.q, a.q[:40] + 1])  # rows past the call's, which it must not read or write
+        tctx.tree_attention(c, H, a.rows, 40, max(a.len), 1 / math.sqrt(D), ptr(q), ptr(a.k), ptr(a.v), ptr(a.keep[0]), ptr(dev(start)),
+                            ptr(a.keep[2]), ptr(a.keep[3]), ptr(a.mask), a.words, ptr(out), None)
+        tctx.sync()
+        for b, e in rows:
+            assert torch.equal(out[b:e], want[b:e])
+            out[b:e] = 9.0
+        assert bool((out == 9.0).all())
+
+
 def test_tree_attention_refusals(tctx):
     import ulb_capi as U
     x = torch.zeros(1 << 16, dtype=torch.float16, device="cuda")

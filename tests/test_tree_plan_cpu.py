@@ -210,3 +210,33 @@ int main() {
 def test_a_failed_wait_ends_the_copies(tmp_path):
     """A place that was not seen free is not copied into, nor any after it."""
     run(tmp_path, COPY)
+
+
+ROWS = r'''
+#include <climits>
+#include <cstdio>
+#include "tree_plan.h"
+int main() {
+  const int at[] = {INT_MIN, INT_MIN + 1, -1000, -1, 0, 1, 5, 99, 100, 101, 4000, INT_MAX - 1, INT_MAX};
+  const int sizes[] = {0, 1, 7, 100, INT_MAX};
+  for (int rows : sizes)
+    for (int most : sizes)
+      for (int b : at)
+        for (int e : at) {
+          int r0 = -7;
+          const int n = ulb::rows_of(b, e, rows, most, &r0);
+          const long long lo = b < 0 ? 0 : b, hi = e < rows ? e : rows;  /* the rows that [b, e) and [0, rows) share */
+          const long long want = hi > lo ? (hi - lo < most ? hi - lo : most) : 0;
+          if (n != want || r0 < 0 || r0 > rows || (n > 0 && r0 != lo) || (long long)r0 + n > rows) {
+            std::printf("[%d, %d) of %d, at most %d: %d rows from %d\n", b, e, rows, most, n, r0);
+            return 1;
+          }
+        }
+  std::printf("ok\n");
+}
+'''
+
+
+def test_rows_of_a_sequence_stay_in_range(tmp_path):
+    """Whatever row_start holds, a sequence's rows are rows of the call."""
+    run(tmp_path, ROWS)

@@ -5,6 +5,7 @@
 #pragma once
 
 #include "paged_ops.h"
+#include "tree_plan.h"
 
 namespace ulb {
 
@@ -34,9 +35,7 @@ struct TreeSeq {
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int s) {
   TreeSeq q;
-  const int b = a.row_start[s], e = a.row_start[s + 1];
-  q.r0 = min(max(b, 0), a.rows);
-  q.n = min(max(min(e, a.rows) - q.r0, 0), a.max_rows);
+  q.n = rows_of(a.row_start[s], a.row_start[s + 1], a.rows, a.max_rows, &q.r0);
   q.len = min(max(a.len[s], 0), a.max_len);
   q.prefix = min(max(a.prefix[s], 0), q.len);
   return q;

@@ -42,7 +42,6 @@
  * waits (bounded) for its MMAs before it frees TMEM.
  */
 #include "tree_attention.h"
-#include "tree_plan.h"
 
 #include <cuda.h>
 

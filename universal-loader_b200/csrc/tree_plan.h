@@ -12,6 +12,14 @@
 
 namespace ulb {
 
+/* rows of a sequence from its places in row_start, whatever those hold: *r0 and the answer name rows
+   of [0, rows), at most max_rows */
+ULB_ROLE int rows_of(int begin, int end, int rows, int max_rows, int* r0) {
+  const int b = begin < 0 ? 0 : begin > rows ? rows : begin, e = end < b ? b : end > rows ? rows : end;
+  *r0 = b;
+  return e - b < max_rows ? e - b : max_rows;
+}
+
 /*
  * The order in which the issuing warp of stream X passes the K and V rings in a piece of `tiles`
  * tiles, n of them its own: all (PAIR) or every second (t % 2 == X).  A ring's place is free when
