@@ -587,6 +587,33 @@ def test_tree_attention_row_tiles_half_empty_over_long_pieces(tctx, D):
     tctx.sync()
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("bits", [17.0, 17.3, 25.5])
+@pytest.mark.parametrize("at", [0, 4000])
+@pytest.mark.parametrize("D,H,rows,seqs,n", [(256, 2, 1, 600, 8191), (64, 4, 1, 160, 30001), (128, 8, 10, 160, 30001), (64, 8, 40, 80, 30001)])
+def test_tree_attention_one_key_that_outweighs_thousands(tctx, D, H, rows, seqs, n, at, bits, kind):
+    """A key of score s whose V is zero, all others of score zero with V = 1: they answer, however
+    little each of them weighs.  Every sequence reads the same pages."""
+    import ulb_capi as U
+    page = 256
+    pages = (n + page - 1) // page
+    scale = float(np.float32(bits * math.log(2) / 16))
+    q, k, v = (torch.zeros(*sh, dtype=DT[kind], device="cuda") for sh in ((seqs * rows, H, D), (pages, 1, page, D), (pages, 1, page, D)))
+    q[:, :, 0], v[:] = 4.0, 1.0
+    k[at // page, 0, at % page, 0], v[at // page, 0, at % page] = 4.0, 0.0
+    c = U.CacheDesc(dtype=U.dtype_id(kind), n_head_kv=1, head_dim=D, page=page, n_pages=pages, n_seq=seqs, max_pages=pages)
+    out, lse = torch.zeros_like(q), torch.zeros(seqs * rows, H, device="cuda")
+    mask = torch.full((seqs * rows, 1), -1, dtype=torch.int32, device="cuda")
+    tctx.tree_attention(c, H, seqs * rows, rows, n, scale, ptr(q), ptr(k), ptr(v), ptr(dev(np.tile(np.arange(pages), (seqs, 1)))),
+                        ptr(dev(np.arange(seqs + 1) * rows)), ptr(dev([n - 32] * seqs)), ptr(dev([n] * seqs)), ptr(mask), 1, ptr(out), ptr(lse))
+    tctx.sync()
+    top = math.exp(16 * scale)
+    want, l = (n - 1) / (n - 1 + top), math.log(n - 1 + top)
+    # a weight and the output rounded once each; the score (|s| < 2^5) and its exponential in fp32
+    assert float((out.double() - want).abs().max()) <= (2 * UNIT[kind] + 2.0 ** -15) * want
+    assert float((lse.double() - l).abs().max()) <= 2e-5 * (1 + l)
+
+
 @pytest.mark.parametrize("D,H,Hkv", [(64, 4, 4), (128, 8, 1), (256, 4, 1)])
 def test_tree_attention_row_ranges_out_of_order(tctx, D, H, Hkv):
     """Row ranges that end before they begin or lie outside the call's rows touch no row of others."""

@@ -16,8 +16,7 @@
  * stream through a ring of NST shared-memory stages by cp.async.  The 8 (or 4) warps are WM row
  * groups x WK key groups; a key group has its own (m, l, o), joined in shared memory at the end.
  * S = Q K^T and O = P V are mma.sync m16n8k16 with fp32 accumulators; P stays in registers, rounded to
- * fp16 (2^-12 relative a weight, averaged over the keys; the output itself is rounded the same) or
- * kept as two bf16 parts.
+ * fp16 (2^-11 relative a weight, as the output is; see kRaise) or kept as two bf16 parts.
  *
  * Used for head dim 256 and for calls too small for the tcgen05 form (tree_attention_tc.cu, which has
  * the rule).  Measured: 1 row x 500 keys, 32 heads over 4, hd 64: 8.6 us, a launch each for the splits
@@ -76,6 +75,15 @@ template <typename T> __device__ __forceinline__ bool odd_lo(uint32_t w) {
   return (w & E) == E;
 }
 template <typename T> __device__ __forceinline__ bool odd_hi(uint32_t w) { return odd_lo<T>(w >> 16); }
+
+/*
+ * Weights are exp(s - m + raise): fp16 holds 11 bits of a weight from 2^-14 on, so with the heaviest at
+ * 2^14 (65504 is the largest) a weight keeps them down to 2^-28 of it, and what thousands of keys far
+ * below one heavy key weigh together is not lost.  The statistics m - raise and l, and so the partials,
+ * carry the factor; it drops out of o / l and of m + log l.  Scores in base 2 up to 2^25: past them a
+ * maximum rounded to fp32 could leave weights past 65504.
+ */
+template <typename T> constexpr float kRaise = std::is_same<T, __half>::value ? 14.f : 0.f;
 
 template <int HD, int WM, int WK>
 struct Cfg {
@@ -177,7 +185,7 @@ __global__ void __launch_bounds__(WM* WK * 32, Cfg<HD, WM, WK>::MIN_BLOCKS) tree
     }
   }
 
-  float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
+  float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f; /* m: the maximum less kRaise */
   float o[DB][4];
 #pragma unroll
   for (int d = 0; d < DB; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
@@ -253,7 +261,7 @@ __global__ void __launch_bounds__(WM* WK * 32, Cfg<HD, WM, WK>::MIN_BLOCKS) tree
     xB = fmaxf(xB, __shfl_xor_sync(0xffffffffu, xB, 1));
     xA = fmaxf(xA, __shfl_xor_sync(0xffffffffu, xA, 2));
     xB = fmaxf(xB, __shfl_xor_sync(0xffffffffu, xB, 2));
-    const float nA = fmaxf(mA, xA * a.scale2), nB = fmaxf(mB, xB * a.scale2);
+    const float nA = fmaxf(mA, __fmaf_rn(xA, a.scale2, -kRaise<T>)), nB = fmaxf(mB, __fmaf_rn(xB, a.scale2, -kRaise<T>));
     const float uA = nA == -INFINITY ? 0.f : nA, uB = nB == -INFINITY ? 0.f : nB;
     const float fA = ex2(mA - uA), fB = ex2(mB - uB);
     mA = nA;

@@ -13,8 +13,8 @@
  * S = Q K^T (tcgen05.mma, both operands in shared memory, fp32 in TMEM); the row's thread reads
  * S, updates m and l, writes P (rounded to the cache's type) over S in TMEM; O += P V with P read
  * from TMEM and V as the tile TMA wrote it (keys x hd, the MN-major operand).  O stays in TMEM; it
- * is rescaled only when a row's maximum has grown by more than 2^8 since the last time (weights
- * stay below 2^8, sums are fp32, so the result is the same ratio).
+ * is rescaled only when a row's maximum has grown by more than 2^GROW since the last time (weights
+ * stay below 2^(RAISE + GROW), sums are fp32, so the result is the same ratio).
  *
  * Warps: 0 TMA (pages -> 128-byte-swizzled tiles, one box a page, pages that are unmapped or past
  * the end read as zero through an out-of-range coordinate), 1 issues every MMA and the commits
@@ -298,6 +298,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                    const __grid_constant__ TcPlan p) {
   using C = TcCfg<HD, PAIR>;
   constexpr bool F16 = std::is_same<T, __half>::value;
+  /* Weights are at most 2^(RAISE + GROW): fp16, whose range ends at 2^16, holds 11 bits of one down to 2^-26
+     of the maximum (tree_attention.cu, kRaise); bf16 has the range without.  fp16, 64 rows x 64 heads x
+     131072 keys: 300 us with GROW 3 as with 8, 320 with 2; 346 against 318 where scores are four times
+     as wide. */
+  constexpr float RAISE = F16 ? 12.f : 0.f, GROW = F16 ? 3.f : 8.f;
   constexpr uint32_t FMT = F16 ? 0u : (1u << 7) | (1u << 10);
   constexpr uint32_t ID_S = (1u << 4) | FMT | ((TK >> 3) << 17) | ((128 >> 4) << 24);
   constexpr uint32_t ID_O = (1u << 4) | FMT | (1u << 16) | ((HD >> 3) << 17) | ((128 >> 4) << 24);
@@ -585,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int ri = live ? qi / a.G : 0;
       const int n = n_of(X), open = tree_open(a, pc.q);
       if (live && a.words > 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.mask + (long long)(pc.q.r0 + ri) * a.words));
-      float m = -INFINITY, l = 0.f; /* m: the maximum that weights are taken against */
+      float m = -INFINITY, l = 0.f; /* m: the maximum that weights are taken against, less RAISE */
       for (int i = 0; i < n && ok; ++i) {
         const int t = pc.t0 + (PAIR ? i : 2 * i + X), pos = t * TK;
         const int b = i & 1;
@@ -612,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!((see[c / 32] >> (c & 31)) & 1u)) sr[c] = 0xff800000u; /* -inf */
           }
           /* weights against the maximum so far, the tile's own maximum beside them: only when a row's
-             has grown by more than 2^8 (its first tile, seldom later) are they taken again */
+             has grown by more than 2^GROW (its first tile, seldom later) are they taken again */
           uint32_t pk[TK / 2];
           float sum = 0.f, top = 0.f;
           auto weights = [&](float u) {
@@ -633,13 +638,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const float2 y = both(add2(l0, l1));
             sum = y.x + y.y;
-            top = fmaxf(x0, x1) * a.scale2;
+            top = fmaxf(x0, x1);
           };
           weights(m == -INFINITY ? 0.f : m);
-          const bool grow = top > m + 8.f || (m == -INFINITY && top > m);
+          const bool grow = __fmaf_rn(top, a.scale2, -m) > RAISE + GROW; /* m -inf: a first key */
           if (__any_sync(0xffffffffu, grow)) {
-            const float f = grow ? (m == -INFINITY ? 0.f : ex2(m - top)) : 1.f;
-            if (grow) m = top;
+            const float to_m = __fmaf_rn(top, a.scale2, -RAISE), f = grow ? (m == -INFINITY ? 0.f : ex2(m - to_m)) : 1.f;
+            if (grow) m = to_m;
             l *= f;
             if (i > 0) { /* the first product overwrites O; products before the last are complete */
               if (!mb_wait_warp(&o_done[X][b ^ 1], ((sp >> (b ^ 1)) & 1) ^ 1)) ok = false;
