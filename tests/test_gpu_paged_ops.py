@@ -587,6 +587,46 @@ def test_tree_attention_row_tiles_half_empty_over_long_pieces(tctx, D):
     tctx.sync()
 
 
+@pytest.mark.parametrize("kind,causal", [("f16", True), ("bf16", False)])
+def test_tree_attention_many_rows_over_many_small_pages(tctx, kind, causal):
+    """Head dim 256, a thousand rows over 1537 pages of 16 positions, which one block walks: page ids
+    come and go under way, some of them unmapped."""
+    import ulb_capi as U
+    rng = np.random.default_rng(31)
+    H, D, page, rows, n = 32, 256, 16, 1024, 24580
+    pages = (n + page - 1) // page
+    table = rng.permutation(pages)
+    for j, value in ((3, -1), (511, -5), (512, pages), (700, -1), (1023, -1), (1400, pages + 9), (1530, -1)):
+        table[j] = value
+    g = torch.Generator(device="cuda").manual_seed(31)
+    q, k, v = (torch.randn(*sh, device="cuda", generator=g).to(DT[kind]) for sh in ((rows, H, D), (pages, 1, page, D), (pages, 1, page, D)))
+    see = np.ones((rows, n), bool)
+    see[:, n - 40:] = rng.random((rows, 40)) < 0.5
+    if causal:
+        see = np.arange(n)[None] <= np.arange(rows)[:, None] + n - rows
+    see &= ((table >= 0) & (table < pages))[np.arange(n) // page]
+    mask = None if causal else torch.as_tensor(pack_bits(see[:, n - 40:], 2)).cuda()
+    # unmapped or past the end: nothing that a row may see
+    k[:, 0].view(-1, D)[int(table[-1]) * page + n % page:(int(table[-1]) + 1) * page] = math.nan
+    v[:, 0].view(-1, D)[int(table[-1]) * page + n % page:(int(table[-1]) + 1) * page] = math.inf
+    c = U.CacheDesc(dtype=U.dtype_id(kind), n_head_kv=1, head_dim=D, page=page, n_pages=pages, n_seq=1, max_pages=pages)
+    out, lse = torch.zeros_like(q), torch.zeros(rows, H, device="cuda")
+    tctx.tree_attention(c, H, rows, rows, n, 1 / 16, ptr(q), ptr(k), ptr(v), ptr(dev(table)), ptr(dev([0, rows])), ptr(dev([n - 40])),
+                        ptr(dev([n])), ptr(mask), 0 if causal else 2, ptr(out), ptr(lse))
+    tctx.sync()
+    at = torch.as_tensor(np.clip(table, 0, pages - 1)).cuda()
+    kk, vv = (x[at, 0].reshape(-1, D)[:n].double() for x in (k, v))
+    u = UNIT[kind]
+    for r in (0, 1, 63, 500, 777, 1023):
+        s = torch.as_tensor(see[r]).cuda()
+        sc = (q[r].double() @ kk.T / 16).masked_fill(~s[None], -math.inf)
+        l = torch.logsumexp(sc, 1)
+        p, vz = torch.exp(sc - l[:, None]), torch.where(s[:, None], vv, torch.zeros_like(vv))
+        want, size = p @ vz, p @ vz.abs()
+        assert bool(((out[r].double() - want).abs() <= (u + 2.0 ** -15) * size + u * want.abs() + 1e-6).all())
+        assert bool(((lse[r].double() - l).abs() <= 2e-5 * (1 + l.abs())).all())
+
+
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 @pytest.mark.parametrize("bits", [17.0, 17.3, 25.5])
 @pytest.mark.parametrize("at", [0, 4000])

@@ -41,8 +41,7 @@ namespace ulb {
 namespace {
 
 constexpr int BK = 64;         /* keys a tile */
-constexpr int kTbl = 516;      /* pages a split may touch */
-constexpr int kTblPages = 512; /* whole pages a split may span */
+constexpr int kTbl = 512;      /* page ids a block holds: a ring, half of it replaced at a time */
 
 __device__ __forceinline__ uint32_t saddr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
@@ -99,6 +98,7 @@ struct Cfg {
   static constexpr int JOIN = WK * RT * OP * 4;
   static constexpr int SMEM = NST * STAGE > JOIN ? NST * STAGE : JOIN;
   static_assert(NST >= 2 && SMEM <= 200 * 1024, "shared memory");
+  static_assert((NST + 1) * BK / 16 + 2 <= kTbl / 2, "the tiles in flight are in the newer half of the page ids");
 };
 
 template <typename T, int HD, int WM, int WK>
@@ -132,14 +132,20 @@ __global__ void __launch_bounds__(WM* WK * 32, Cfg<HD, WM, WK>::MIN_BLOCKS) tree
   /* the split's pages */
   const int p0 = k0 >> a.g.page_shift, np = k1 > k0 ? ((k1 - 1) >> a.g.page_shift) - p0 + 1 : 0;
   if (tid == 0) odd_v = 0;
-  int bad = 0;
-  for (int i = tid; i < np; i += C::NT) {
-    const int p = p0 + i < a.g.max_pages ? a.table[(long long)s * a.g.max_pages + p0 + i] : -1;
-    const bool ok = p >= 0 && p < a.g.n_pages;
-    tbl[i] = ok ? p : -1;
-    bad |= !ok;
-  }
-  bad = __syncthreads_or(bad);
+  auto page_ids = [&](int from, int to) { /* is one of them unmapped? */
+    int bad = 0;
+    for (int i = from + tid; i < to; i += C::NT) {
+      const int p = p0 + i < a.g.max_pages ? a.table[(long long)s * a.g.max_pages + p0 + i] : -1;
+      const bool ok = p >= 0 && p < a.g.n_pages;
+      tbl[i & (kTbl - 1)] = ok ? p : -1;
+      bad |= !ok;
+    }
+    return __syncthreads_or(bad);
+  };
+  auto page_of = [&](int pos) { return tbl[((pos >> a.g.page_shift) - p0) & (kTbl - 1)]; };
+  int have = min(np, kTbl), bad = page_ids(0, have);
+  auto ids_upto = [&]() { return have < np ? (p0 + have) << a.g.page_shift : 0x7fffffff; }; /* positions whose page ids are here */
+  int upto = ids_upto();
 
   const T* const kb = (const T*)a.k + kvh * a.g.head;
   const T* const vb = (const T*)a.v + kvh * a.g.head;
@@ -148,7 +154,7 @@ __global__ void __launch_bounds__(WM* WK * 32, Cfg<HD, WM, WK>::MIN_BLOCKS) tree
     uint8_t* const ks = sm + (it % C::NST) * C::STAGE;
     for (int j = tid >> 3; j < BK; j += C::NT / 8) {
       const int pos = k0 + it * BK + j;
-      const int pg = pos < k1 ? tbl[(pos >> a.g.page_shift) - p0] : -1;
+      const int pg = pos < k1 ? page_of(pos) : -1;
       const bool ok = pg >= 0;
       const long long off = ok ? pg * a.g.pstride + (pos & (a.g.page - 1)) * a.g.pos : 0;
       const uint32_t d = saddr(ks + j * C::PITCH);
@@ -193,7 +199,14 @@ __global__ void __launch_bounds__(WM* WK * 32, Cfg<HD, WM, WK>::MIN_BLOCKS) tree
   for (int it = 0; it < n_it; ++it) {
     cp_wait<C::NST - 2>();
     __syncthreads();
-    if (it + C::NST - 1 < n_it) stage(it + C::NST - 1);
+    if (it + C::NST - 1 < n_it) {
+      if (k0 + (it + C::NST) * BK > upto) { /* every 256 pages of a longer split */
+        bad |= page_ids(have, min(np, have + kTbl / 2));
+        have = min(np, have + kTbl / 2);
+        upto = ids_upto();
+      }
+      stage(it + C::NST - 1);
+    }
     cp_commit();
     uint8_t* const ks = sm + (it % C::NST) * C::STAGE;
     const int tile0 = k0 + it * BK;
@@ -238,7 +251,7 @@ __global__ void __launch_bounds__(WM* WK * 32, Cfg<HD, WM, WK>::MIN_BLOCKS) tree
     }
     const int key0 = tile0 + wk * C::KW + 2 * t;
     auto sees = [&](int i, int pos) {
-      return pos < k1 && tbl[(pos >> a.g.page_shift) - p0] >= 0 && (pos < open || tree_sees(a, q, i, pos));
+      return pos < k1 && page_of(pos) >= 0 && (pos < open || tree_sees(a, q, i, pos));
     };
     if (masked) {
 #pragma unroll
@@ -326,7 +339,7 @@ __global__ void __launch_bounds__(WM* WK * 32, Cfg<HD, WM, WK>::MIN_BLOCKS) tree
           }
         pa = __shfl_sync(0xffffffffu, pa, from);
         pb = __shfl_sync(0xffffffffu, pb, from);
-        const int pg = pos < k1 ? tbl[(pos >> a.g.page_shift) - p0] : -1;
+        const int pg = pos < k1 ? page_of(pos) : -1;
         if (pg < 0) continue;
         const T* vr = vb + pg * a.g.pstride + (pos & (a.g.page - 1)) * a.g.pos;
         const bool sa = sees(ia, pos), sb = sees(ib, pos);
@@ -470,7 +483,7 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
  * Keys a split.  `units` CTAs (row tiles x kv heads x sequences) walk whole sequences; `slots`
  * run at once.  One sequence: as many splits as fill the slots once.  Several: about four waves,
  * because their lengths differ and short splits let the last wave even out.  Never under 128 keys,
- * never more partials than the workspace holds or pages than the split's table holds.
+ * never more partials than the workspace holds (one split needs none).
  */
 void plan_splits(TreeArgs* a, long long units, int slots) {
   long long want = (a->g.n_seq == 1 ? (long long)slots : 4ll * slots) / std::max(1ll, units);
@@ -478,8 +491,7 @@ void plan_splits(TreeArgs* a, long long units, int slots) {
   const long long per = (long long)a->rows * a->H * (a->g.hd + 2);
   want = std::min(want, std::max(1ll, (long long)kTreeWsFloats / std::max(1ll, per) - 1));
   auto round = [](long long x) { return (x + 127) / 128 * 128; };
-  long long keys = std::max(128ll, round((a->max_len + want - 1) / want));
-  keys = std::min(keys, (long long)kTblPages * a->g.page);
+  const long long keys = std::max(128ll, round((a->max_len + want - 1) / want));
   a->split_keys = (int)keys;
   a->n_split = (int)std::max(1ll, (a->max_len + keys - 1) / keys);
 }
@@ -495,11 +507,7 @@ int launch_tree(Ctx* c, TreeArgs& a) {
   a.n_tile = (int)(((long long)a.max_rows * a.G + C::RT - 1) / C::RT);
   const long long units = (long long)a.n_tile * a.g.n_head_kv * a.g.n_seq;
   plan_splits(&a, units, c->n_sm);
-  const long long per = (long long)a.rows * a.H * (a.g.hd + 2);
   if (a.n_split > 1) {
-    ULB_CHECK(per * a.n_split <= (long long)kTreeWsFloats && a.n_split <= 8192, ULB_EUNSUPPORTED,
-              "ulb_tree_attention: %d rows of %d heads over %d positions in pages of %d need %d splits, more than the workspace holds",
-              a.rows, a.H, a.max_len, a.g.page, a.n_split);
     a.po = c->tree_ws;
     a.pml = c->tree_ws + (long long)a.rows * a.H * a.g.hd * a.n_split;
   }
