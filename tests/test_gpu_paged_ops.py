@@ -587,6 +587,37 @@ def test_tree_attention_row_tiles_half_empty_over_long_pieces(tctx, D):
     tctx.sync()
 
 
+@pytest.mark.parametrize("where", ["past the end", "a slot"])
+@pytest.mark.parametrize("H,Hkv,rows", [(32, 8, 40), (16, 8, 40)])
+def test_tree_attention_values_that_nobody_sees_cost_nothing(tctx, where, H, Hkv, rows):
+    """NaN in V past the ends, or in a slot that no row sees, leaves the answer and the time as they are."""
+    a = Attention("bf16", H, Hkv, 128, 64, [(1000, rows)] * 24, seed=41)
+    for b in a.see:
+        b[:, 7] = False
+    a.mask = torch.as_tensor(np.concatenate([pack_bits(b, a.words) for b in a.see])).cuda()
+
+    def time():
+        out, _ = a.run(tctx)
+        ms = []
+        for _ in range(12):
+            t0, t1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            t0.record()
+            a.again()
+            t1.record()
+            t1.synchronize()
+            ms.append(t0.elapsed_time(t1))
+        return out, sorted(ms)[3]
+
+    want, clean = time()
+    for s in range(24):
+        for t in (range(a.len[s], 64 * len(a.table[s])) if where == "past the end" else [1007]):
+            a.v[int(a.table[s, t // 64]), :, t % 64] = math.nan
+    got, stale = time()
+    assert torch.equal(got, want)
+    # the same work; the bound is for the clock of a call of some 50 us
+    assert stale <= 1.5 * clean, (stale, clean)
+
+
 @pytest.mark.parametrize("kind,causal", [("f16", True), ("bf16", False)])
 def test_tree_attention_many_rows_over_many_small_pages(tctx, kind, causal):
     """Head dim 256, a thousand rows over 1537 pages of 16 positions, which one block walks: page ids

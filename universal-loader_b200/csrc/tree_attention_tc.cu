@@ -57,6 +57,7 @@ constexpr int kThreads = 384;  /* 4 role warps, 2 x 4 softmax warps */
 constexpr int kPairCost = 16;   /* what a pair costs besides its tiles, in tiles */
 constexpr int kMinTiles = 12;  /* places of the line a group takes at least */
 constexpr int kJoinRows = 8;   /* rows a block of the join kernel: a warp each */
+constexpr int kOddWords = 32;  /* bits for 1024 positions */
 
 __device__ __forceinline__ uint32_t sa(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mb_init(uint64_t* b, uint32_t n) {
@@ -292,6 +293,35 @@ __device__ __forceinline__ uint32_t sees32(const TreeArgs& a, const TreeSeq& q, 
   return v;
 }
 
+/*
+ * What infinities and NaN of V at the marked positions of [from, upto) add to columns [d0, d0 + 32) of row
+ * i's sum, if the row sees them.  Not inlined: with it in the kernel, 64 rows x 131072 keys took 342 us for 330.
+ */
+template <typename T>
+__device__ __noinline__ void add_odd(const TreeArgs& a, TreeSeq q, const uint32_t* marks, int s, int kvh, int i, const T* qr, int from,
+                                     int upto, int d0, float m, float* o) {
+  const int hd = a.g.hd;
+  for (int w = 0; w < kOddWords; ++w)
+    for (uint32_t bits = marks[w]; bits; bits &= bits - 1)
+      for (int pos = from + ((w * 32 + __ffs(bits) - 1 - from) & (32 * kOddWords - 1)); pos < upto; pos += 32 * kOddWords) {
+        const int j = pos >> a.g.page_shift;
+        const int pg = j < a.g.max_pages ? a.table[(long long)s * a.g.max_pages + j] : -1;
+        if (pg < 0 || pg >= a.g.n_pages || !tree_sees(a, q, i, pos)) continue;
+        const long long off = pg * a.g.pstride + (pos & (a.g.page - 1)) * a.g.pos + kvh * a.g.head;
+        const T *kr = (const T*)a.k + off, *vr = (const T*)a.v + off + d0;
+        bool hit = false;
+        for (int e = 0; e < min(32, hd - d0); ++e) hit |= !isfinite(to_f<T>(vr[e]));
+        if (!hit) continue;
+        float sc = 0.f;
+        for (int e = 0; e < hd; ++e) sc = __fmaf_rn(to_f<T>(qr[e]), to_f<T>(kr[e]), sc);
+        const float wt = ex2(__fmaf_rn(sc, a.scale2, -(m == -INFINITY ? 0.f : m)));
+        for (int e = 0; e < min(32, hd - d0); ++e) {
+          const float x = to_f<T>(vr[e]);
+          if (!isfinite(x)) o[e] += wt * x;
+        }
+      }
+}
+
 template <typename T, int HD, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ TreeArgs a,
@@ -310,7 +340,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint64_t k_full[C::NK], k_free[C::NK], v_full[C::NV], v_free[C::NV], s_full[2][2], p_full[2][2], o_done[2][2], v_seen[2],
       piece[2], q_full, mma_done;
   __shared__ uint32_t tmem_sh;
-  __shared__ int odd_v, sh_s, sh_base, sh_sum[kThreads / 32];
+  __shared__ int sh_s, sh_base, sh_sum[kThreads / 32];
+  __shared__ uint32_t odd[2][kOddWords + 1]; /* of a piece (its number modulo 2): which positions modulo 1024, before len, lost a V element; any */
   uint8_t* const sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* const q_sm = sm;
   uint8_t* const k_sm = sm + C::NQ * C::QTILE;
@@ -330,11 +361,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mb_init(&q_full, 8);
     mb_init(&mma_done, 2);
-    odd_v = 0;
     sh_s = 0;
     sh_base = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (tid < 2 * (kOddWords + 1)) odd[tid / (kOddWords + 1)][tid % (kOddWords + 1)] = 0;
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sa(&tmem_sh)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -684,7 +715,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (((w[e] >> 16) & E) == E) { w[e] &= 0x0000ffffu; hit = true; }
             }
             if (hit) {
-              odd_v = 1;
+              const int at = pos + (j >> 3) % TK; /* a key has 8 words in each half */
+              if (at < pc.q.len) {
+                atomicOr(&odd[pc.nth & 1][(at >> 5) % kOddWords], 1u << (at & 31));
+                odd[pc.nth & 1][kOddWords] = 1;
+              }
               v[j] = make_uint4(w[0], w[1], w[2], w[3]);
             }
           };
@@ -717,6 +752,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_before();
       sync_softmax(); /* both streams are through: Q may be replaced, O of either is whole */
       tc_after();
+      if (tid - 128 <= kOddWords) odd[(c.nth & 1) ^ 1][tid - 128] = 0; /* for the next piece */
       const bool whole = c.n == c.n_tile;
       const int slot = c.nth == 0 ? 0 : 1; /* only a CTA's first and last pieces can be parts */
       if (!whole && c.t0 == 0 && tid == 128) { /* the head of a pair that goes on in the next groups */
@@ -765,29 +801,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] += other ? __uint_as_float(u[e]) * g : 0.f;
           }
-          if (odd_v && live) { /* values taken out of masked tiles go to the rows that see them */
-            const T* qr = (const T*)a.q + at * hd;
+          if (odd[c.nth & 1][kOddWords] && live) { /* values taken out of masked tiles go to the rows that see them */
+            float more[32] = {};
             const int from = max(c.t0 * TK, min(open, c.q.len) / TK * TK), upto = min(c.q.len, (c.t0 + c.n) * TK);
-            for (int pos = from; pos < upto; ++pos) {
-              const int j = pos >> a.g.page_shift;
-              const int pg = j < a.g.max_pages ? a.table[(long long)c.s * a.g.max_pages + j] : -1;
-              if (pg < 0 || pg >= a.g.n_pages || !tree_sees(a, c.q, ri, pos)) continue;
-              const long long off = pg * a.g.pstride + (pos & (a.g.page - 1)) * a.g.pos + c.kvh * a.g.head;
-              const T *kr = (const T*)a.k + off, *vr = (const T*)a.v + off + d0;
-              bool hit = false;
-#pragma unroll 1
-              for (int e = 0; e < min(32, hd - d0); ++e) hit |= !isfinite(to_f<T>(vr[e]));
-              if (!hit) continue;
-              float s = 0.f;
-#pragma unroll 1
-              for (int e = 0; e < hd; ++e) s = __fmaf_rn(to_f<T>(qr[e]), to_f<T>(kr[e]), s);
-              const float w = ex2(__fmaf_rn(s, a.scale2, -(m == -INFINITY ? 0.f : m)));
+            add_odd<T>(a, c.q, odd[c.nth & 1], c.s, c.kvh, ri, (const T*)a.q + at * hd, from, upto, d0, m, more);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const float x = d0 + e < hd ? to_f<T>(vr[e]) : 0.f;
-                if (!isfinite(x)) o[e] += w * x;
-              }
-            }
+            for (int e = 0; e < 32; ++e) o[e] += more[e];
           }
           /* 32 rows x 32 columns change sides in shared memory, so that a row leaves in one piece (a lane
              writing its own row takes a transaction every 16 bytes): 16-byte word w of row y at w ^ y */
