@@ -328,11 +328,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                    const __grid_constant__ TcPlan p) {
   using C = TcCfg<HD, PAIR>;
   constexpr bool F16 = std::is_same<T, __half>::value;
-  /* Weights are at most 2^(RAISE + GROW): fp16, whose range ends at 2^16, holds 11 bits of one down to 2^-26
-     of the maximum (tree_attention.cu, kRaise); bf16 has the range without.  fp16, 64 rows x 64 heads x
-     131072 keys: 300 us with GROW 3 as with 8, 320 with 2; 346 against 318 where scores are four times
-     as wide. */
-  constexpr float RAISE = F16 ? 12.f : 0.f, GROW = F16 ? 3.f : 8.f;
+  /* Weights are at most 2^(RAISE + GROW): fp16, whose largest number is just under 2^16, holds 11 bits of one
+     down to 2^-26 of the maximum (tree_attention.cu, kRaise); bf16 has the range without.  fp16, 64 rows x 64
+     heads x 131072 keys: 290 us (331 with scores four times as wide), with GROW 3 300 (346), with 2 320 (356). */
+  constexpr float RAISE = F16 ? 12.f : 0.f, GROW = F16 ? 3.9f : 8.f;
   constexpr uint32_t FMT = F16 ? 0u : (1u << 7) | (1u << 10);
   constexpr uint32_t ID_S = (1u << 4) | FMT | ((TK >> 3) << 17) | ((128 >> 4) << 24);
   constexpr uint32_t ID_O = (1u << 4) | FMT | (1u << 16) | ((HD >> 3) << 17) | ((128 >> 4) << 24);
