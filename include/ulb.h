@@ -76,9 +76,10 @@ ULB_API int ulb_stream_sync(ulb_ctx* ctx);
  * around the calls.  NULL goes back to the stream ulb_init made; the legacy default stream is
  * named by its handle cudaStreamLegacy.  Work already enqueued by the context runs before work
  * enqueued after the switch (an event orders the two streams).  The stream must outlive its use
- * here; switching is refused during a capture (ulb_capture_begin), and the legacy stream
- * cannot be captured (speculative loops with use_graphs need another one).  ulb_stream returns
- * the stream in use.
+ * here.  Switching is refused while either stream is being captured, by ulb_capture_begin or by
+ * the caller (whose capture stays valid): switch to a stream before its capture begins.  The
+ * legacy stream cannot be captured (speculative loops with use_graphs need another one).
+ * ulb_stream returns the stream in use.
  */
 ULB_API int ulb_use_stream(ulb_ctx* ctx, void* stream);
 /*

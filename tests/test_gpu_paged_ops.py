@@ -540,6 +540,45 @@ def test_tree_attention_follows_the_stream(tctx):
         tctx.use_stream(torch.cuda.current_stream().cuda_stream)
 
 
+def test_use_stream_and_another_programs_capture():
+    """A stream under capture is refused and the capture goes on; a context switched to it before takes part."""
+    import ulb_capi as U
+    a = Attention("f16", 8, 2, 64, 64, [(300, 8)], seed=16)
+    st, x = torch.cuda.Stream(), torch.zeros(4, device="cuda")
+    with U.Context(0) as c:
+        want, _ = a.run(c)
+        c.sync()
+        with torch.cuda.stream(st):
+            g = torch.cuda.CUDAGraph()
+            x.add_(1)
+            st.synchronize()
+            g.capture_begin()
+            try:
+                refused(c.use_stream, st.cuda_stream, code=U.EINVAL)
+                x.add_(1)
+            finally:
+                g.capture_end()
+            g.replay()
+            st.synchronize()
+            assert x.tolist() == [2.0] * 4
+            c.use_stream(st.cuda_stream)
+            out, _ = a.run(c)
+            out.zero_()
+            st.synchronize()
+            h = torch.cuda.CUDAGraph()
+            h.capture_begin()
+            try:
+                a.again()
+                refused(c.use_stream, None, code=U.EINVAL)
+            finally:
+                h.capture_end()
+            assert not bool(out.any())
+            h.replay()
+            st.synchronize()
+            assert torch.equal(out, want)
+        c.use_stream(None)
+
+
 @pytest.mark.parametrize("D", [64, 80, 96, 128])
 @pytest.mark.parametrize("H,Hkv,rows", [(8, 1, 9), (16, 2, 16), (6, 2, 40), (8, 1, 33)])
 def test_tree_attention_tensor_core_form(tctx, D, H, Hkv, rows):

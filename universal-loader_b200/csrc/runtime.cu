@@ -252,9 +252,13 @@ int ulb_use_stream(ulb_ctx* ctx, void* stream) {
   const cudaStream_t to = stream ? (cudaStream_t)stream : c->own_stream;
   if (to == c->stream) return ULB_OK;
   ULB_CUDA(cudaSetDevice(c->device));
-  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-  ULB_CUDA(cudaStreamIsCapturing(c->stream, &st));
-  ULB_CHECK(st == cudaStreamCaptureStatusNone, ULB_EINVAL, "ulb_use_stream: the context's stream is being captured");
+  /* an event of one stream cannot be waited for in another's capture: that would break the capture */
+  for (cudaStream_t s : {to, c->stream}) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    ULB_CUDA(cudaStreamIsCapturing(s, &st));
+    ULB_CHECK(st == cudaStreamCaptureStatusNone, ULB_EINVAL, "ulb_use_stream: the %s stream is being captured",
+              s == to ? "given" : "context's");
+  }
   ULB_CUDA(cudaEventRecord(c->switch_ev, c->stream));
   ULB_CUDA(cudaStreamWaitEvent(to, c->switch_ev, 0));
   c->stream = to;
