@@ -540,6 +540,15 @@ def test_tree_attention_follows_the_stream(tctx):
         tctx.use_stream(torch.cuda.current_stream().cuda_stream)
 
 
+@pytest.mark.parametrize("rows", [299, 592, 600, 620])
+def test_tree_attention_row_tiles_for_every_sm_and_more(tctx, rows):
+    """64 heads a kv head: so many row tiles that one group of blocks walks all keys (299 rows: 75 tiles of
+    256 queries), exactly one an SM (592), and more than one pass over the rows."""
+    Attention("bf16", 128, 2, 64, 64, [(200, rows), (130, 3), (70, 0), (0, rows // 2)], causal=True, seed=rows).check(tctx)
+    Attention("f16", 64, 1, 128, 64, [(900, rows)], seed=rows + 1).check(tctx)
+    tctx.sync()
+
+
 def test_use_stream_and_another_programs_capture():
     """A stream under capture is refused and the capture goes on; a context switched to it before takes part."""
     import ulb_capi as U
