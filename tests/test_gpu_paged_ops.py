@@ -229,6 +229,19 @@ def test_rope_append(tctx, kin, kout, H, Hkv, D, page, nhd):
     r.close()
 
 
+def test_rope_arrays_at_odd_addresses(tctx):
+    import ulb_capi as U
+    r = U.Rope(tctx, 64)
+    x = torch.zeros(4096, device="cuda")
+    p = dev([0] * 8)
+    c = U.CacheDesc(dtype=U.T_F16, n_head_kv=1, head_dim=64, page=16, n_pages=1, n_seq=1, max_pages=1)
+    refused(r.apply, U.T_F32, ptr(x), 4, 1, ptr(p) + 2, ptr(x), code=U.EINVAL)
+    for i in range(4):
+        a = [ptr(p) + (2 if j == i else 0) for j in range(4)]
+        refused(r.append, c, U.T_F32, ptr(x), ptr(x), ptr(x), 1, *a, 4, ptr(x), ptr(x), ptr(x), code=U.EINVAL)
+    r.close()
+
+
 def test_rope_refusals(tctx):
     import ulb_capi as U
     for kw in (dict(head_dim=64, rot_dim=63), dict(head_dim=64, rot_dim=66), dict(head_dim=0), dict(head_dim=64, base=1.0),

@@ -66,3 +66,42 @@ def test_logits_arguments(bad):
         setattr(a, k, v)
     assert L.ulb_logits_process(C.c_void_p(16), C.byref(a)) in (U.EINVAL, U.EUNSUPPORTED)
     assert b"ulb_logits_process" in L.ulb_last_error()
+
+
+def _addresses(n, odd):
+    """n addresses, the one of number `odd` two bytes off."""
+    return [C.c_void_p(66 if i == odd else 64) for i in range(n)]
+
+
+@pytest.mark.parametrize("i", range(6))
+def test_tree_arrays_at_odd_addresses(i):
+    import ulb_capi as U
+    f, d = C.c_void_p(64), U.TreeDesc(4, 1, 1, 1, 1, 0.1)
+    table, start, prefix, length, mask, lse = _addresses(6, i)
+    assert U.lib().ulb_tree_attention(f, C.byref(_cache(U)), C.byref(d), f, f, f, table, start, prefix, length, mask, f, lse) == U.EINVAL
+    assert b"unaligned" in U.lib().ulb_last_error()
+
+
+@pytest.mark.parametrize("i", range(5))
+def test_page_move_arrays_at_odd_addresses(i):
+    import ulb_capi as U
+    f, c = C.c_void_p(64), C.byref(_cache(U))
+    a = _addresses(5, i)
+    if i == 0:
+        assert U.lib().ulb_pages_copy(f, c, f, f, a[0], 1) == U.EINVAL
+    else:
+        assert U.lib().ulb_pages_compact(f, c, f, f, *a[1:], 1) == U.EINVAL
+    assert b"unaligned" in U.lib().ulb_last_error()
+
+
+@pytest.mark.parametrize("name", ["row_start", "params", "history", "history_start", "prompt", "node_tokens", "mask", "bias_start",
+                                  "bias_tokens", "bias_values", "allow", "row_allow"])
+def test_logits_arrays_at_odd_addresses(name):
+    import ulb_capi as U
+    a = U.LogitsArgs(dtype=U.T_F32, V=100, n_seq=1, rows=1, max_rows=1, ld_in=100, ld_out=100, mask_words=1, n_allow=1)
+    for n, t in U.LogitsArgs._fields_:
+        if t is C.c_void_p:
+            setattr(a, n, 64)
+    setattr(a, name, 66)
+    assert U.lib().ulb_logits_process(C.c_void_p(64), C.byref(a)) == U.EINVAL
+    assert b"unaligned" in U.lib().ulb_last_error()

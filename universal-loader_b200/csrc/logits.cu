@@ -354,6 +354,9 @@ extern "C" int ulb_logits_process(ulb_ctx* ctx, const ulb_logits_args* a) {
   ULB_CHECK(!a->bias_start || (a->bias_tokens && a->bias_values), ULB_EINVAL, "ulb_logits_process: bias_start without biases");
   const int eb = dtype_bytes(a->dtype);
   ULB_CHECK((uintptr_t)a->in % eb == 0 && (uintptr_t)a->out % 4 == 0, ULB_EINVAL, "ulb_logits_process: unaligned pointer");
+  ULB_CHECK(words_aligned({a->row_start, a->params, a->history, a->history_start, a->prompt, a->node_tokens, a->mask, a->bias_start,
+                           a->bias_tokens, a->bias_values, a->allow, a->row_allow}),
+            ULB_EINVAL, "ulb_logits_process: unaligned array of 32-bit elements");
   ULB_CHECK((const void*)a->in != (const void*)a->out || (a->dtype == ULB_TYPE_F32 && a->ld_in == a->ld_out), ULB_EINVAL,
             "ulb_logits_process: in place needs F32 logits and equal leading dimensions");
   Ctx* c = &ctx->c;

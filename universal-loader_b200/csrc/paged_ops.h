@@ -6,6 +6,7 @@
 
 #include <cuda_bf16.h>
 
+#include <initializer_list>
 #include <type_traits>
 
 #include "ulb_internal.h"
@@ -52,6 +53,12 @@ inline int cache_geom(const char* who, const ulb_cache_desc* d, CacheGeom* g) {
   return ULB_OK;
 }
 
+/* arrays of 32-bit elements (NULL is aligned): a kernel that reads one at an odd address faults */
+inline bool words_aligned(std::initializer_list<const void*> arrays) {
+  for (const void* p : arrays)
+    if (reinterpret_cast<uintptr_t>(p) & 3) return false;
+  return true;
+}
 #define ULB_ALIGNED16(p) ((reinterpret_cast<uintptr_t>(p) & 15) == 0)
 #define ULB_LAUNCH(what, call)                                                 \
   do {                                                                         \

@@ -203,6 +203,7 @@ int ulb_pages_copy(ulb_ctx* ctx, const ulb_cache_desc* cache, void* k, void* v, 
   if (n == 0) return ULB_OK;
   ULB_CHECK(k && v && moves, ULB_EINVAL, "ulb_pages_copy: NULL argument");
   ULB_CHECK(ULB_ALIGNED16(k) && ULB_ALIGNED16(v), ULB_EINVAL, "ulb_pages_copy: the pools must be 16-byte aligned");
+  ULB_CHECK(words_aligned({moves}), ULB_EINVAL, "ulb_pages_copy: unaligned array of int32");
   ULB_CUDA(cudaSetDevice(ctx->c.device));
   return launch_copy(&ctx->c, g, k, v, moves, MoveList{}, n);
 }
@@ -216,6 +217,7 @@ int ulb_pages_compact(ulb_ctx* ctx, const ulb_cache_desc* cache, void* k, void* 
   if (max_src == 0) return ULB_OK;
   ULB_CHECK(k && v && table && base && count && src, ULB_EINVAL, "ulb_pages_compact: NULL argument");
   ULB_CHECK(ULB_ALIGNED16(k) && ULB_ALIGNED16(v), ULB_EINVAL, "ulb_pages_compact: the pools must be 16-byte aligned");
+  ULB_CHECK(words_aligned({table, base, count, src}), ULB_EINVAL, "ulb_pages_compact: unaligned array of int32");
   ULB_CHECK(g.n_seq <= 65535, ULB_EUNSUPPORTED, "ulb_pages_compact: %d sequences (at most 65535)", g.n_seq);
   Ctx* c = &ctx->c;
   ULB_CUDA(cudaSetDevice(c->device));

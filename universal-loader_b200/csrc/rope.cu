@@ -403,6 +403,7 @@ int ulb_rope_append(ulb_ctx* ctx, const ulb_rope* r, const ulb_cache_desc* cache
   const int eb = dtype_bytes(in_dtype);
   ULB_CHECK((uintptr_t)q % eb == 0 && (uintptr_t)k % eb == 0 && (uintptr_t)v % eb == 0 && (uintptr_t)q_out % 2 == 0, ULB_EINVAL,
             "ulb_rope_append: unaligned pointer");
+  ULB_CHECK(words_aligned({pos, row_seq, slot, table}), ULB_EINVAL, "ulb_rope_append: unaligned array of int32");
   ULB_CHECK(ULB_ALIGNED16(k_pool) && ULB_ALIGNED16(v_pool), ULB_EINVAL, "ulb_rope_append: the pools must be 16-byte aligned");
   a.turn = r->turn;
   a.mscale = r->mscale;

@@ -571,6 +571,7 @@ extern "C" int ulb_tree_attention(ulb_ctx* ctx, const ulb_cache_desc* cache, con
   ULB_CHECK(!mask == (d->mask_words == 0), ULB_EINVAL, "ulb_tree_attention: mask without mask_words, or the reverse");
   ULB_CHECK(ULB_ALIGNED16(q) && ULB_ALIGNED16(k) && ULB_ALIGNED16(v) && ULB_ALIGNED16(out), ULB_EINVAL,
             "ulb_tree_attention: q, the pools and out must be 16-byte aligned");
+  ULB_CHECK(words_aligned({table, row_start, prefix, len, mask, lse}), ULB_EINVAL, "ulb_tree_attention: unaligned array of 32-bit elements");
   a.H = d->n_head;
   a.G = d->n_head / a.g.n_head_kv;
   a.rows = d->rows;
