@@ -21,7 +21,7 @@
  * Used for head dim 256 and for calls too small for the tcgen05 form (tree_attention_tc.cu, which has
  * the rule).  Measured: 1 row x 500 keys, 32 heads over 4, hd 64: 8.6 us, a launch each for the splits
  * and their join; 64 rows x 300 keys, 32 kv heads of 64: 38 us; 1 row x 30000 keys, 64 heads over 8 of
- * 256 (246 MB): 62 us, 61 % of the copy rate, bound by the two stages that fit at hd 256.
+ * 256 (246 MB): 64 us, 60 % of the copy rate, bound by the two stages that fit at hd 256.
  *
  * Rows of shared memory are hd + 8 elements apart: 16-byte row pitch odd in units of 16 bytes,
  * so the eight rows of an ldmatrix phase fall in eight different bank groups.
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(WM* WK * 32, Cfg<HD, WM, WK>::MIN_BLOCKS) tree
   extern __shared__ __align__(16) uint8_t sm[];
   __shared__ int tbl[kTbl];
   __shared__ float sh_m[WK][C::RT], sh_l[WK][C::RT];
-  __shared__ int odd_v;
+  __shared__ int odd_v, n_ids; /* page ids seen so far, of a split of more than kTbl pages */
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int wm = warp / WK, wk = warp % WK;
 
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(WM* WK * 32, Cfg<HD, WM, WK>::MIN_BLOCKS) tree
 
   /* the split's pages */
   const int p0 = k0 >> a.g.page_shift, np = k1 > k0 ? ((k1 - 1) >> a.g.page_shift) - p0 + 1 : 0;
-  if (tid == 0) odd_v = 0;
+  if (tid == 0) { odd_v = 0; n_ids = kTbl; }
   auto page_ids = [&](int from, int to) { /* is one of them unmapped? */
     int bad = 0;
     for (int i = from + tid; i < to; i += C::NT) {
@@ -143,9 +143,9 @@ __global__ void __launch_bounds__(WM* WK * 32, Cfg<HD, WM, WK>::MIN_BLOCKS) tree
     return __syncthreads_or(bad);
   };
   auto page_of = [&](int pos) { return tbl[((pos >> a.g.page_shift) - p0) & (kTbl - 1)]; };
-  int have = min(np, kTbl), bad = page_ids(0, have);
-  auto ids_upto = [&]() { return have < np ? (p0 + have) << a.g.page_shift : 0x7fffffff; }; /* positions whose page ids are here */
-  int upto = ids_upto();
+  /* the first tile that the page ids in shared memory do not cover, less the stages ahead */
+  auto covered = [&](int have) { return have < np ? (((p0 + have) << a.g.page_shift) - k0) / BK - C::NST : 0x7fffffff; };
+  int bad = page_ids(0, min(np, kTbl)), reload = covered(kTbl);
 
   const T* const kb = (const T*)a.k + kvh * a.g.head;
   const T* const vb = (const T*)a.v + kvh * a.g.head;
@@ -200,10 +200,11 @@ __global__ void __launch_bounds__(WM* WK * 32, Cfg<HD, WM, WK>::MIN_BLOCKS) tree
     cp_wait<C::NST - 2>();
     __syncthreads();
     if (it + C::NST - 1 < n_it) {
-      if (k0 + (it + C::NST) * BK > upto) { /* every 256 pages of a longer split */
+      if (it > reload) { /* every 256 pages of a longer split */
+        const int have = n_ids;
         bad |= page_ids(have, min(np, have + kTbl / 2));
-        have = min(np, have + kTbl / 2);
-        upto = ids_upto();
+        reload = covered(have + kTbl / 2);
+        if (tid == 0) n_ids = have + kTbl / 2;
       }
       stage(it + C::NST - 1);
     }
