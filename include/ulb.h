@@ -294,11 +294,15 @@ ULB_API int ulb_spec_accept(ulb_ctx* ctx, const float* dev_p_logits, const float
  * sampling, and move what a step leaves in the cache.  None of them has a counterpart in the
  * reference, whose cache is one flat host array (src/inference/model.h:49-77).  All enqueue on
  * the context's stream and return without synchronising; all can be captured
- * (ulb_capture_begin) after a first call outside a capture.  Contents of device arrays (page
+ * (ulb_capture_begin) after a first call outside a capture.  A graph that holds them, the
+ * caller's own too, uses the context's workspace: its launches must not overlap other calls on
+ * the context.  A change of the page book under capture changes the book at once, and the table
+ * and the pages, as that change asks, at every launch of the graph.  Contents of device arrays (page
  * ids, positions, slots, row ranges, token ids, indexes) cannot be checked by the call: the kernels
  * check them against the sizes given here and skip what lies outside, so a wrong entry costs
  * results, never an access out of bounds.  Offsets into arrays whose size no argument gives
- * (history_start, bias_start) are taken as they are.
+ * (history_start, bias_start) are taken as they are.  Arrays of 32-bit elements at addresses that
+ * are no multiple of 4 are refused.
  *
  * A cache as the operators see it: one pool for K, one of the same layout for V.  Element d of
  * position t of page p for kv head h of layer l is at
@@ -393,9 +397,11 @@ ULB_API int ulb_rope_append(ulb_ctx* ctx, const ulb_rope* r, const ulb_cache_des
  * GQA: head h reads kv head h / (n_head / n_head_kv).  A row that sees nothing gives out = 0 and
  * lse = -inf; what it does not see (stale slots, positions past len[s], infinities and NaN there)
  * never touches its result.  head_dim 64, 80, 96, 128 or 256; n_head / n_head_kv <= 64.
- * max_rows >= every sequence's rows, max_len >= every len[s] (clamped otherwise).  Scores, statistics and sums are fp32; the probabilities of the
- * second product are rounded to the cache type (small bf16 calls keep two parts of them).  The first call on a context allocates 128 MiB of
- * device memory for partial results, kept until ulb_destroy.
+ * max_rows >= every sequence's rows, max_len >= every len[s] (clamped otherwise).  Scores, statistics
+ * and sums are fp32; the probabilities of the second product are rounded to the cache type (small
+ * bf16 calls keep two parts of them; fp16 ones use the type's whole range, for scores up to 1e7).
+ * The first call on a context allocates 128 MiB of device memory for partial results, kept until
+ * ulb_destroy.
  */
 typedef struct ulb_tree_desc {
   int n_head, rows, max_rows, max_len, mask_words;

@@ -22,8 +22,8 @@
  *
  * Measured: 504 tree rows x 128256 (fp16 in, 308 MB) 78 us, 64 rows x 128256 (fp32) 24.5 us, one row x
  * 32000 5 us: 62 %, 42 % and a launch.  Instructions bound the first (some 70 for four tokens a lane),
- * with occupancy: five blocks an SM and one unit in flight a warp, 96 us with two in flight and three
- * blocks; the second is mostly the counting's latency in each of its blocks.
+ * with occupancy: five blocks an SM (48 registers, 36 bytes of them spilled) and one unit in flight a warp,
+ * 96 us with two in flight and three blocks; the second is mostly the counting's latency in each of its blocks.
  */
 #include <algorithm>
 
@@ -297,8 +297,8 @@ __global__ void __launch_bounds__(kWarps * 32, 5) logits_kernel(const __grid_con
 
 template <typename T, int V>
 int launch_logits(Ctx* c, const ulb_logits_args& a) {
-  /* slices: trees (eight rows or more) about six waves of three blocks an SM, so that the last
-     one wastes little; fewer rows, which do not pay for many countings, larger ones: a unit a warp */
+  /* slices: trees (eight rows or more) about 18 blocks an SM, at most five of them at once, so that the last
+     wave wastes little; fewer rows, which do not pay for many countings, larger ones: a unit a warp */
   const long long want = (long long)c->n_sm * 18;
   long long slice = ((long long)a.V * a.n_seq + want - 1) / want;
   if (a.max_rows >= kWarps) slice = (slice + 511) / 512 * 512;

@@ -230,8 +230,9 @@ int pick_rope(Ctx* c, RopeArgs& a) {
   };
   /* 16 bytes a load (32 a thread, f32 in units of eight, measured 117 us where units of four took 111:
      16381 rows of 40 heads), and several heads a thread once that still fills the device: one pass
-     of sines for all of them and as many loads in flight.  1024 rows of 80 heads of 128: two heads a
-     thread 15.2 us, four 17.8, one 17.6. */
+     of sines for all of them and as many loads in flight.  1024 rows of 80 heads of 128 (fp32): two heads a
+     thread 15.2 us, four 17.8, one 17.6; 16381 rows of 40 take four.  The bounds lie between those sizes and
+     are not measured nearer; 16-bit rows follow the same rule. */
   constexpr int W = sizeof(TI) == 4 ? 4 : 8;
   if (fits(W)) {
     const long long full = (long long)c->n_sm * 2048, units = (long long)a.M * heads * (a.hd / W);

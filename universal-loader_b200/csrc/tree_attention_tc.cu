@@ -16,26 +16,34 @@
  * is rescaled only when a row's maximum has grown by more than 2^GROW since the last time (weights
  * stay below 2^(RAISE + GROW), sums are fp32, so the result is the same ratio).
  *
- * Warps: 0 TMA (pages -> 128-byte-swizzled tiles, one box a page, pages that are unmapped or past
- * the end read as zero through an out-of-range coordinate), 1 issues every MMA and the commits
- * that free tiles, 2 - 3 take V elements that are not finite out of masked tiles, 4 - 7 and 8 - 11
- * softmax.  Barriers carry it: K / V tiles full and free, S full, P full, O += P V done (looked at only to
- * rescale O).  A stream has two score buffers; one thread issues its MMAs and they complete in order,
+ * Warps: 0 and 3 copy K and V tiles by TMA (pages -> 128-byte-swizzled tiles, one box a page, pages
+ * that are unmapped or past the end read as zero through an out-of-range coordinate), 1 and 2 issue
+ * the MMAs of a stream each and the commits that free tiles, 4 - 7 and 8 - 11 softmax; they also take V
+ * elements that are not finite out of masked tiles.  Barriers carry it: K / V tiles full and free, S full,
+ * P full, O += P V done (looked at only to rescale O); the order in which the warps pass the rings is
+ * tree_plan.h's.  A stream has two score buffers; one thread issues its MMAs and they complete in order,
  * so a buffer is free for the tile after the next once the product that reads its weights has been
  * issued, and the scores of the next tile are there while weights are computed (128-key tiles with one
  * buffer, weights handed over in halves, took 339 us where this took 300).
  *
- * Work is cut evenly: the tiles of all (sequence, kv head) pairs form one line, every CTA (group
- * of CTAs, when more than 256 rows need several row tiles: its members walk the same keys side by
- * side, so K / V come from HBM once) takes an equal stretch of it, whatever the lengths, and
- * walks whole sequences and pieces of two.  A pair that falls into several stretches leaves one
- * partial a stretch, joined by a small kernel.
+ * Weights are rounded to 16 bits once: two parts, as the mma.sync form keeps of bf16, would double the
+ * second product, which here is half of the tensor cores' work.  Against 64 bits the outputs are off by
+ * 2.3e-3 relative in bf16 and 2.8e-4 in fp16, of which 1.7e-3 and 2.1e-4 are the output's own rounding.
  *
- * Measured: 64 rows x 64 heads (8 kv heads of 128) x 131072 keys 289 us, 950 TFLOP/s (57 % of the measured
+ * Work is cut evenly over the lengths: the tiles of all (sequence, kv head) pairs form one line, every CTA
+ * (group of CTAs, when more than 256 rows need several row tiles: its members walk the same keys side by
+ * side, so K / V come from HBM once) takes an equal stretch of it and walks whole sequences and pieces
+ * of two.  A pair that falls into several stretches leaves one partial a stretch, joined by a small
+ * kernel.  It is not cut over rows: a group has as many members as the longest of the sequences has row
+ * tiles, members without rows of a sequence pass it by, and causal rows walk the keys after their last.
+ *
+ * Measured: 64 rows x 64 heads (8 kv heads of 128) x 131072 keys 286 us, 961 TFLOP/s (58 % of the measured
  * burst): the round trip between products and softmax, with two streams of two score buffers, which is
- * what TMEM holds, bounds it (tensor pipe 54 %, exponentials 44 %).  64 sequences of 256 to 4096 keys with
- * 8 to 16 rows, 32 heads over 8: 123 us, 4.8 TB/s of K and V: HBM and some 6 us a (sequence, kv head).
- * 63 rows x 8191 keys, 32 kv heads: 39 us, of which 12 are a CTA's start and end and 5 the join.
+ * what TMEM holds, bounds it (tensor pipe 55 %, exponentials 45 %).  64 sequences of 256 to 4096 keys with
+ * 8 to 16 rows, 32 heads over 8: 128 us, 4.6 TB/s of K and V: HBM and some 6 us a (sequence, kv head).
+ * 63 rows x 8191 keys, 32 kv heads: 40 us, of which 12 are a CTA's start and end and 5 the join.
+ * 160 to 190 bytes a thread are spilled at the 168 registers of the launch, which are what the compiler
+ * allots to every role, whatever the split at run time gives.
  *
  * Every mbarrier wait has a limit: past it a role raises bit 3 of the device error word,
  * arrives nowhere and issues nothing any more, so that the others run into theirs; the CTA still
@@ -983,7 +991,11 @@ int pick_tc(Ctx* c, TreeArgs& a) {
  * what a (sequence, kv head) costs besides its tiles outweigh the tensor cores.  Measured here / mma.sync
  * form, us (rows x keys): 1 x 500, 8 queries 14.3 / 8.6; 1 x 4000, 8 queries 17.3 / 8.4; 64 x 1 x 1000 mha
  * 167 / 80; 16 x 1 x 2000, 4 queries 32.6 / 34.4; 64 x 1 x 4000, 4 queries 114 / 149; 1 x 8000 mha 34 / 47;
- * 8 x 16 x 1000, 64 queries 21.7 / 33.6; 1 x 63 x 2000 mha 22.6 / 27.7; 1 x 64 x 1000, 512 queries 35.3 / 35.6.
+ * 8 x 16 x 1000, 64 queries 21.7 / 33.6; 1 x 63 x 2000 mha 22.6 / 27.7.  From 65 queries on, with the join
+ * (sequences x rows x keys): 64 x 70 x 170, 32 kv heads of 128 154 / 290, of 64 115 / 162; 64 x 20 x 170, 80 queries
+ * 52 / 87; 16 x 20 x 500 30 / 72; 1 x 70 x 1000 mha 26 / 32; 4 x 33 x 300, 132 queries 30 / 36; 1 x 9 x 200, 72 queries
+ * 20 / 23; but 1 x 16 x 2000, 128 queries 27 / 26, 1 x 64 x 1000, 512 queries 40 / 36 and 1 x 128 x 600, 512
+ * queries 37 / 30: one sequence of few keys leaves most SMs without a stretch.
  * The line is counted in 32 bits.
  */
 bool tree_tc_fits(const Ctx* c, const TreeArgs& a) {

@@ -80,7 +80,7 @@ struct Ctx {
   bool pdl = true; /* programmatic dependent launch between consecutive kernels */
   std::map<void*, size_t> user_allocs; /* buffers handed out by ulb_malloc */
   uint64_t launches = 0;               /* kernels launched through launch_k (not graph replays) */
-  int* dev_err = nullptr;              /* device error word: bit 1 = a bounded wait gave up */
+  int* dev_err = nullptr;              /* device error word: bits 1, 8 and 16, what gave up */
   void* zero_row = nullptr;            /* kZeroRowHalves fp16 zeros: padding activation rows */
   void* nccl = nullptr;                /* ncclComm_t of ulb_tp_init (tensor parallelism) */
   float* tc_ws = nullptr;              /* split-K partial sums of the tensor-core GEMM */
@@ -88,7 +88,7 @@ struct Ctx {
   int* tc_cnt = nullptr;               /* kTcCounters arrival counters, zero between launches */
   int tp_rank = 0, tp_world = 1;
   int attn_form = 0; /* ULB_ATTN_AUTO / SPLIT / STREAM */
-  float* tree_ws = nullptr; /* split partials of ulb_tree_attention, made by its first split call */
+  float* tree_ws = nullptr; /* split partials of ulb_tree_attention, made by its first call */
   /* timing of the tensor-parallel all-reduces (on while a round is profiled): a CUDA event
      pair is recorded around each ncclAllReduce, events[2i] before and events[2i+1] after */
   /* host-side bound on waits for a stream holding tensor-parallel collectives (ms, 0 = none):
