@@ -494,6 +494,116 @@ typedef struct ulb_logits_args {
 } ulb_logits_args;
 ULB_API int ulb_logits_process(ulb_ctx* ctx, const ulb_logits_args* args);
 
+/*
+ * Norms of the q and k heads of M rows, and their rotary positions, in one pass.  Head x of a row
+ * (head_dim elements, a multiple of 8 up to 256) becomes
+ *   y = R(pos) (w x f),  f = 1 / sqrt(mean x^2 + eps)
+ * with R the rotation of the handle (its m on the elements that turn; rot_dim a multiple of 16 for
+ * ULB_ROPE_HALF) and one weight a head element, fp32 [head_dim], for all q heads and one for all k heads.
+ * q and k are F32, F16 or BF16 rows of n_head and n_head_kv heads, element d of head h of row m at
+ * m * row + h * head + d (0: dense); outputs are dense and of the same type, and may be the inputs where those
+ * are dense too.  Computed in fp32, rounded once.  n_head_kv = 0: no k (its pointers unused).  Rows may be
+ * at any element's address; 16-byte aligned pointers and strides of whole 16 bytes take wide loads.
+ */
+typedef struct ulb_norm_rope_args {
+  int dtype, M, n_head, n_head_kv;
+  float eps; /* > 0 */
+  int64_t q_row, q_head, k_row, k_head;
+  const void *q, *k;
+  const float *q_weight, *k_weight;
+  const int32_t* pos; /* [M] */
+} ulb_norm_rope_args;
+ULB_API int ulb_norm_rope_apply(ulb_ctx* ctx, const ulb_rope* r, const ulb_norm_rope_args* args, void* dev_q_out, void* dev_k_out);
+/*
+ * Its gradient: with g = R(pos)^T dy and n = x f,
+ *   dx = f (w g - n mean(w g n)),   dw = sum of g n over the rows and heads that share w
+ * dq_out, dk_out: the gradients of the outputs, dense, of the rows' type; dq, dk: of the rows, dense (may be
+ * dq_out, dk_out); dq_weight, dk_weight: fp32 [head_dim], overwritten (M = 0: zeros).  The sums of dw are fp32
+ * in a fixed order: the same call gives the same bits.
+ */
+ULB_API int ulb_norm_rope_grad(ulb_ctx* ctx, const ulb_rope* r, const ulb_norm_rope_args* args, const void* dev_dq_out,
+                       const void* dev_dk_out, void* dev_dq, void* dev_dk, float* dev_dq_weight, float* dev_dk_weight);
+
+/*
+ * A paged cache held in 8 or 4 bits.  Every (position, kv head) is a row of ulb_quant_row_bytes bytes:
+ * the codes, then the scales of its head_dim / 32 groups of 32 elements, then unused bytes up to a
+ * multiple of 16:
+ *   ULB_TYPE_Q8_0  int8 codes in order, fp16 scales:                      x = d c,  d = max |x| / 127
+ *   ULB_TYPE_Q4_1  4-bit codes, pairs of an fp16 scale and minimum:       x = d c + m, m = min x, d = (max x - m) / 15
+ * (the values of GGUF's blocks of those types).  32-bit word i (0 .. 7) of each 32 bytes of 4-bit codes holds
+ * elements 4 i .. 4 i + 3 of two neighbouring groups: the first group's at bits 0, 16, 4, 20, the second's
+ * at bits 8, 24, 12, 28.  A group that holds an infinity or a NaN reads as NaN; scales past 65504 saturate.
+ * Pools are dense and 16-byte aligned, [n_pages][n_head_kv][page] rows for one layer; layers may follow one
+ * another.  Block tables as for ulb_cache_desc.  ulb_quant_pages gives the same pools of n_layer layers as a
+ * ulb_cache_desc of 16-bit elements, for ulb_pages_copy / _compact and the page book.
+ */
+#define ULB_TYPE_Q4_1 3 /* quantised caches only */
+typedef struct ulb_quant_desc {
+  int format;                /* ULB_TYPE_Q8_0 or ULB_TYPE_Q4_1                     */
+  int dtype;                 /* F16 or BF16: q and outputs                          */
+  int n_head_kv, head_dim;   /* head_dim 64, 128 or 256                             */
+  int page;                  /* positions per page: 16, 32, 64, 128 or 256          */
+  int n_pages, n_seq, max_pages;
+} ulb_quant_desc;
+ULB_API int ulb_quant_row_bytes(const ulb_quant_desc* desc, int* out_bytes);
+ULB_API int ulb_quant_pages(const ulb_quant_desc* desc, int n_layer, ulb_cache_desc* out);
+/*
+ * ulb_rope_append into a quantised cache: q, k and v rows (in_dtype F32, F16 or BF16, heads dense inside rows of
+ * stride q_row / k_row / v_row, 0: dense), q and k normed (weights as in ulb_norm_rope_args, each NULL: not) and
+ * turned, q written to dev_q_out (desc's dtype, dense), k and v quantised into their slots.  Rows whose slot is
+ * unmapped, negative or past the table write q only.  Two rows must not share a slot.
+ */
+typedef struct ulb_quant_append_args {
+  int in_dtype, M, n_head;
+  float eps;
+  int64_t q_row, k_row, v_row;
+  const void *q, *k, *v;
+  const float *q_weight, *k_weight;
+  const int32_t *pos, *row_seq, *slot, *block_table;
+  void *q_out, *k_pool, *v_pool;
+} ulb_quant_append_args;
+ULB_API int ulb_quant_append(ulb_ctx* ctx, const ulb_rope* r, const ulb_quant_desc* desc, const ulb_quant_append_args* args);
+/*
+ * Rows read back: slot dev_slot[m] of sequence dev_row_seq[m] for m < M into dense [M][n_head_kv][head_dim] rows of
+ * out_dtype (F32, F16 or BF16; rounded once); zeros where the slot is unmapped, negative or past the table.  Read the positions
+ * before a chunk of a prompt this way and give them to ulb_prompt_attention with the chunk's own.
+ */
+ULB_API int ulb_quant_read(ulb_ctx* ctx, const ulb_quant_desc* desc, int out_dtype, const void* dev_k_pool, const void* dev_v_pool,
+                   const int32_t* dev_block_table, const int32_t* dev_row_seq, const int32_t* dev_slot, int M, void* dev_k_out,
+                   void* dev_v_out);
+/*
+ * ulb_tree_attention over a quantised cache, for the new tokens of a step: one row a sequence, a chain of drafts
+ * (mask_words = 0) or a tree.  Rows, lengths, masks, outputs and what is promised of them as there; q and out of
+ * desc's dtype; n_head / n_head_kv <= 64.  Codes are multiplied exactly, scores, statistics and sums are fp32, a
+ * weight times a group's scale is rounded once to 11 bits.  Made for few queries a kv head (rows x grouped heads):
+ * past 32 (16 for head_dim 256) the keys are walked once for each 32 (16).  The first call on a context allocates
+ * 32 MiB of device memory for partial results, kept until ulb_destroy.
+ */
+ULB_API int ulb_quant_attention(ulb_ctx* ctx, const ulb_quant_desc* cache, const ulb_tree_desc* desc, const void* dev_q,
+                        const void* dev_k_pool, const void* dev_v_pool, const int32_t* dev_block_table,
+                        const int32_t* dev_row_start, const int32_t* dev_prefix, const int32_t* dev_len,
+                        const uint32_t* dev_mask, void* dev_out, float* dev_lse);
+
+/*
+ * Causal attention of whole prompts packed one behind the other.  Rows [q_start[s], q_start[s + 1]) of q
+ * [q_rows][n_head][head_dim] and [k_start[s], k_start[s + 1]) of k, v [k_rows][n_head_kv][head_dim] belong to
+ * sequence s.  The rows are the last of the keys: row i of n sees keys 0 .. n_k - n + i (a prompt's later chunk has
+ * more keys than rows).  out and lse as ulb_tree_attention's; rows behind the last sequence are left as they were.  A row
+ * that sees nothing gives out = 0 and lse = -inf; what a row does not see never touches its result.  q_row, k_row,
+ * v_row: elements between rows (0: dense; heads are dense inside a row), multiples of 8.  dtype F16 or BF16,
+ * head_dim 64, 80, 96, 128 or 256, n_head / n_head_kv <= 64.  max_q, max_k >= every sequence's rows and keys (clamped
+ * otherwise: the first of them count).  Scores, statistics and sums are fp32, weights are rounded to the rows' type.
+ * The first call on a context allocates the 128 MiB of ulb_tree_attention's partial results.
+ */
+typedef struct ulb_prompt_desc {
+  int dtype, n_head, n_head_kv, head_dim;
+  int n_seq, q_rows, k_rows, max_q, max_k;
+  float scale;
+  int64_t q_row, k_row, v_row;
+} ulb_prompt_desc;
+ULB_API int ulb_prompt_attention(ulb_ctx* ctx, const ulb_prompt_desc* desc, const void* dev_q, const void* dev_k, const void* dev_v,
+                         const int32_t* dev_q_start, const int32_t* dev_k_start, void* dev_out, float* dev_lse);
+
 /* ------------------------------------------------------------------ models */
 /*
  * A LLaMA-family model resident in HBM.  Replaces Model / LayerWeights / KVCache

@@ -68,6 +68,14 @@ inline bool words_aligned(std::initializer_list<const void*> arrays) {
 
 }  // namespace ulb
 
+/* a rotary handle: the frequencies of its pairs as 64-bit fractions of a turn (rope.cu), the factor on what turns */
+struct ulb_rope {
+  ulb_ctx* owner = nullptr;
+  int hd = 0, rot = 0, half = 0;
+  float mscale = 1.f;
+  unsigned long long* turn = nullptr;
+};
+
 #ifdef __CUDACC__
 namespace ulb {
 

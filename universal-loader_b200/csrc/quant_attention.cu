@@ -1,0 +1,824 @@
+/*
+ * quant_attention.cu — attention of a step's new rows over a paged cache held in 8 or 4 bits
+ * (ulb_quant_attention).  Rows, masks and promises are those of ulb_tree_attention (tree_attention.cu);
+ * the reference has no quantised cache (src/inference/model.h:49-77).
+ *
+ * Mathematics.  A K or V row is d_g c (+ m_g) with integer codes c and a scale (and minimum) a group g of 32
+ * elements; 4-bit codes are taken less 8 and m_g as the middle m_g + 8 d_g, so that the weighted codes are no larger than
+ * what they add up to (with codes from 0 the rounding of their weights showed 2.4 times the output's own).  Nothing is
+ * expanded to 16-bit values:
+ *   s_t   = scale sum_g [ d_tg (q_g . c_tg) + m_tg sum(q_g) ]          fp32 sums of exact products
+ *   o_gi  = sum_t (p_t d_tg) c_tgi + sum_t p_t m_tg,   p_t = exp(s_t - M)
+ * The codes are exact fp16 integers, so the one rounding is that of the weight p_t d_tg to fp16.  M is the running
+ * maximum of s_t + log d_t (d_t the largest scale of the V row), so weights are at most 2^(RAISE + GROW) whatever the
+ * scales are, and fp16 keeps 11 bits of one down to 2^-26 of the heaviest; p_t itself and what it sums to
+ * are fp32 (a scale is at least 2^-24, so p_t stays in range).  q is scaled by a power of two a row, which makes
+ * bf16 rows fp16 ones without loss.  It drops out of the scores exactly.
+ *
+ * Work.  HBM bounds it: a K and a V row of 80 (4 bits) or 144 bytes at head_dim 128.  K^T Q and V P are
+ * mma.sync m16n8k16 with the codes as the 16-row operand (keys x dims, then dims x keys) and eight queries as
+ * columns, so a product wastes nothing on padding at eight queries and a code is unpacked once for all of them.
+ * Two nibbles or bytes become two fp16 integers by one LOP3 / PRMT and one HADD2 / HFMA2.  The dims a lane
+ * takes of a row are four in a row of each 16, for the first product, and four of each 32 for the second, so every
+ * shared-memory read is a conflict-free 32-bit word of the rows as they lie in HBM.
+ *
+ * A warp walks 32-key tiles of its own through its own ring of bulk copies; nothing is shared
+ * but the rows of q and the join of the warps' (M, l, o) at the end.  The tiles of all (sequence, row tile, kv head)
+ * units form one line that is cut evenly over the CTAs, so lengths may differ as they like; a unit in several
+ * CTAs leaves a partial in each and the last of them to arrive joins them in order.
+ */
+#include "quant_cache.h"
+#include "tcgen05.h"
+#include "tree_attention.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace ulb {
+namespace {
+
+constexpr int KT = 32;          /* keys a tile */
+constexpr int kUnitCost = 8;    /* what a unit costs besides its tiles, in tiles */
+constexpr int kMinTiles = 24;   /* places of the line a CTA takes at least */
+constexpr float kRaise = 12.f, kGrow = 3.9f; /* weights <= 2^15.9 < 65504 */
+constexpr int kRingBytes = 212 * 1024;
+constexpr unsigned kAll = 0xffffffffu;
+
+template <bool Q4, int HD, int NT>
+struct QCfg {
+  static constexpr int RB = quant_row_bytes(Q4, HD), CB = quant_code_bytes(Q4, HD);
+  static constexpr int STAGE = 2 * KT * RB;
+  static constexpr int W = HD == 256 ? 4 : 8; /* warps */
+  static constexpr int RT = 8 * NT;           /* queries a CTA */
+  static constexpr int JD = NT == 4 ? 32 : 64; /* dims the warps join at a time */
+  static constexpr int NG = HD / kGroup, KS = HD / 16;
+  static constexpr int QB = NT * KS * 256, JB = W * RT * JD * 4; /* bytes of q's fragments and of the join */
+  static constexpr int ROOM = (kRingBytes - QB - JB) / (W * STAGE);
+  static constexpr int NST = ROOM > 6 ? 6 : ROOM;
+  static constexpr int SMEM = W * NST * STAGE + QB + JB;
+  static_assert(NST >= 2 && SMEM <= 222 * 1024, "shared memory");
+};
+
+struct QuantPlan {
+  int groups, min_tiles;
+  int* tail; /* [groups][2]: arrivals at the unit that begins in this CTA and goes on, the slot of its first piece */
+};
+
+/* the line of work, in tiles: a unit takes kUnitCost places before its tiles.  CTA c's stretch. */
+struct QLine {
+  int total, groups, per, rem;
+  __device__ __forceinline__ void cut(int n) {
+    groups = n;
+    per = total / n;
+    rem = total - per * n;
+  }
+  __device__ __forceinline__ int begin(int c) const { return c * per + min(c, rem); }
+  __device__ __forceinline__ int group_of(int place) const {
+    const int big = rem * (per + 1);
+    return place < big ? place / (per + 1) : rem + (place - big) / per;
+  }
+};
+
+struct QPiece {
+  TreeSeq q;
+  int s, kvh, q0, nq;     /* sequence, kv head, first query (row x group + head) of the row tile, queries in it */
+  int t0, n, n_tile;      /* tiles [t0, t0 + n) of n_tile */
+  int first, last;        /* places of the unit's first and last tiles on the line */
+  int nth;                /* pieces of this CTA before it */
+};
+
+template <int RT>
+struct QWalk {
+  int at, end, base, cnt, s, n_tile, n_pass, nth;
+  TreeSeq q;
+  __device__ __forceinline__ void load(const TreeArgs& a) {
+    q = tree_seq(a, s);
+    n_tile = max(1, (q.len + KT - 1) / KT);
+    n_pass = (q.n * a.G + RT - 1) / RT;
+    cnt = (n_tile + kUnitCost) * n_pass * a.g.n_head_kv;
+  }
+  __device__ __forceinline__ bool next(const TreeArgs& a, QPiece* o) {
+    while (at < end) {
+      while (at >= base + cnt) { /* ends: at < end <= total */
+        base += cnt;
+        ++s;
+        load(a);
+      }
+      const int len = n_tile + kUnitCost, u = (at - base) / len, in = at - base - u * len, upto = min(len, in + end - at);
+      o->t0 = max(in - kUnitCost, 0);
+      o->n = max(upto - kUnitCost, 0) - o->t0;
+      o->first = base + u * len + kUnitCost;
+      o->last = base + u * len + len - 1;
+      at += upto - in;
+      if (o->n <= 0) continue; /* none of its tiles yet */
+      o->kvh = u / n_pass;
+      o->q0 = (u - o->kvh * n_pass) * RT;
+      o->nq = min(RT, q.n * a.G - o->q0);
+      o->q = q;
+      o->s = s;
+      o->n_tile = n_tile;
+      o->nth = nth++;
+      return true;
+    }
+    return false;
+  }
+};
+
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t h2(float a, float b) { return pack2<__half>(a, b); }
+__device__ __forceinline__ uint32_t lds32(const uint8_t* p) { return *reinterpret_cast<const uint32_t*>(p); }
+__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t magic) { /* a - magic, fp16 pairs */
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&magic));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+/* nibbles at bits 0 and 16 as two fp16 integers n - 8: 0x6400 | n is 1024 + n, 0x6408 is 1032 */
+__device__ __forceinline__ uint32_t nib_lo(uint32_t w) { return sub2((w & 0x000f000fu) | 0x64006400u, 0x64086408u); }
+/* nibbles at bits 4 and 20: 1024 + 16 n, then x / 16 - 72 */
+__device__ __forceinline__ uint32_t nib_hi(uint32_t w) {
+  const uint32_t x = (w & 0x00f000f0u) | 0x64006400u, s = 0x2c002c00u, o = 0xd480d480u; /* 1/16, -72 */
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&s), *reinterpret_cast<const __half2*>(&o));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+/* bytes lo and lo + 1 of w (offset binary, int8 + 128) as two fp16 integers: 0x64xx is 1024 + xx; 0x6480 is 1152 */
+template <int LO> __device__ __forceinline__ uint32_t byte2(uint32_t w) {
+  return sub2(__byte_perm(w, 0x64646464u, LO ? 0x4342 : 0x4140), 0x64806480u);
+}
+
+/* scales of a row (and the middles m + 8 d, which go with codes less 8) */
+template <bool Q4, int NG>
+__device__ __forceinline__ void row_scales(const uint8_t* p, float (&d)[NG], float (&m)[NG]) {
+  if constexpr (Q4) {
+#pragma unroll
+    for (int i = 0; i < NG; i += 2) {
+      const uint2 w = *reinterpret_cast<const uint2*>(p + 4 * i);
+      const float2 x = unpack2<__half>(w.x), y = unpack2<__half>(w.y);
+      d[i] = x.x;
+      m[i] = __fmaf_rn(8.f, x.x, x.y);
+      d[i + 1] = y.x;
+      m[i + 1] = __fmaf_rn(8.f, y.x, y.y);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NG; i += 2) {
+      const float2 x = unpack2<__half>(lds32(p + 2 * i));
+      d[i] = x.x;
+      d[i + 1] = x.y;
+    }
+  }
+}
+
+template <typename T, bool Q4, int HD, int NT>
+__global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
+    quant_attn_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ QuantPlan p) {
+  using C = QCfg<Q4, HD, NT>;
+  constexpr int W = C::W, NG = C::NG, NTH = W * 32, JD = C::JD;
+  extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ uint64_t full[W][C::NST];
+  __shared__ uint8_t sh_map[W][C::NST]; /* which 16-key halves of a tile are mapped */
+  __shared__ float2 sh_ml[W][C::RT];
+  __shared__ float sh_f[W][C::RT], sh_l[C::RT], sh_m[C::RT], sh_qs[C::RT], sh_qsum[NG][C::RT];
+  __shared__ int sh_s, sh_base, sh_sum[W], sh_last;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* const ring = sm + warp * C::NST * C::STAGE;
+  uint2* const qf = reinterpret_cast<uint2*>(sm + W * C::NST * C::STAGE);
+  float* const jb = reinterpret_cast<float*>(sm + W * C::NST * C::STAGE + C::QB);
+
+  if (lane == 0) {
+    for (int i = 0; i < C::NST; ++i) mb_init(&full[warp][i], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (tid == 0) { sh_s = 0; sh_base = 0; }
+  pdl_wait();
+  pdl_trigger();
+
+  /* the line's length, then this CTA's stretch and the sequence that holds its begin */
+  QWalk<C::RT> walk;
+  auto places_of = [&](int s) {
+    if (s >= a.g.n_seq) return 0;
+    QWalk<C::RT> w;
+    w.s = s;
+    w.load(a);
+    return w.cnt;
+  };
+  const int cnt0 = places_of(tid);
+  int mine = cnt0;
+  for (int s = tid + NTH; s < a.g.n_seq; s += NTH) mine += places_of(s);
+  mine = __reduce_add_sync(kAll, mine);
+  if (lane == 0) sh_sum[warp] = mine;
+  __syncthreads();
+  QLine line;
+  line.total = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) line.total += sh_sum[w];
+  line.cut(max(1, min(p.groups, (line.total + p.min_tiles - 1) / p.min_tiles)));
+  const int grp_id = blockIdx.x;
+  walk.at = grp_id < line.groups ? line.begin(grp_id) : line.total;
+  walk.end = grp_id < line.groups ? line.begin(grp_id + 1) : line.total;
+  {
+    int base = 0;
+    for (int s0 = 0; s0 < a.g.n_seq && walk.at < walk.end; s0 += NTH) {
+      const int c = s0 == 0 ? cnt0 : places_of(s0 + tid);
+      int x = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(kAll, x, o);
+        if (lane >= o) x += y;
+      }
+      __syncthreads();
+      if (lane == 31) sh_sum[warp] = x;
+      __syncthreads();
+      int all = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if (w < warp) x += sh_sum[w];
+        all += sh_sum[w];
+      }
+      const int b = base + x - c;
+      if (c > 0 && b <= walk.at && walk.at < b + c) {
+        sh_s = s0 + tid;
+        sh_base = b;
+      }
+      base += all;
+      if (base > walk.at) break; /* the same for every thread */
+    }
+    __syncthreads();
+  }
+  if (walk.at >= walk.end) return; /* the whole CTA */
+  walk.s = sh_s;
+  walk.base = sh_base;
+  walk.nth = 0;
+  walk.load(a);
+
+  /* ---- the warp's own tiles, copied ahead of their use and past the ends of pieces */
+  QWalk<C::RT> ahead = walk;
+  QPiece fp;
+  int f_i = 0, f_n = 0, f_id0 = 0, f_id1 = 0, f_slot = 0, f_base = 0;
+  bool f_more = true, ok = true;
+  const uint8_t* const kb = (const uint8_t*)a.k;
+  const uint8_t* const vb = (const uint8_t*)a.v;
+  auto page_at = [&](int s, int pos, int len) {
+    const int j = pos >> a.g.page_shift;
+    const int x = pos < len && j < a.g.max_pages ? a.table[(long long)s * a.g.max_pages + j] : -1;
+    return x >= 0 && x < a.g.n_pages ? x : -1;
+  };
+  auto feed = [&]() { /* the next tile into slot f_slot, which nobody reads any more */
+    while (f_more && f_i >= f_n) {
+      f_more = ahead.next(a, &fp);
+      f_i = 0;
+      f_n = f_more ? (fp.n + W - 1 - warp) / W : 0;
+      f_base = -32;
+    }
+    if (!f_more) return;
+    if (f_i >= f_base + 32) { /* the pages of the next 32 tiles, a tile a lane */
+      f_base = f_i;
+      const int pos = (fp.t0 + warp + (f_i + lane) * W) * KT;
+      const bool in = f_i + lane < f_n;
+      f_id0 = in ? page_at(fp.s, pos, fp.q.len) : -1;
+      f_id1 = in && a.g.page == 16 ? page_at(fp.s, pos + 16, fp.q.len) : f_id0;
+    }
+    const int id0 = __shfl_sync(kAll, f_id0, f_i - f_base), id1 = __shfl_sync(kAll, f_id1, f_i - f_base);
+    if (lane == 0) {
+      const int pos = (fp.t0 + warp + f_i * W) * KT, rows = min(KT, fp.q.len - pos), in = pos & (a.g.page - 1);
+      uint8_t* const d = ring + f_slot * C::STAGE;
+      const long long h = fp.kvh * a.g.head;
+      uint64_t* const bar = &full[warp][f_slot];
+      if (a.g.page == 16) {
+        const int r0 = id0 >= 0 ? min(rows, 16) : 0, r1 = id1 >= 0 ? rows - 16 : 0; /* rows <= 0: none */
+        sh_map[warp][f_slot] = (id0 >= 0 ? 1 : 0) | (id1 >= 0 ? 2 : 0);
+        mb_expect(bar, (uint32_t)(2 * (max(r0, 0) + max(r1, 0)) * C::RB));
+        if (r0 > 0) {
+          bulk_copy(d, kb + id0 * a.g.pstride + h, r0 * C::RB, bar);
+          bulk_copy(d + KT * C::RB, vb + id0 * a.g.pstride + h, r0 * C::RB, bar);
+        }
+        if (r1 > 0) {
+          bulk_copy(d + 16 * C::RB, kb + id1 * a.g.pstride + h, r1 * C::RB, bar);
+          bulk_copy(d + (KT + 16) * C::RB, vb + id1 * a.g.pstride + h, r1 * C::RB, bar);
+        }
+      } else {
+        const int r = id0 >= 0 ? max(rows, 0) : 0;
+        sh_map[warp][f_slot] = id0 >= 0 ? 3 : 0;
+        mb_expect(bar, (uint32_t)(2 * r * C::RB));
+        if (r > 0) {
+          const long long off = id0 * a.g.pstride + h + (long long)in * C::RB;
+          bulk_copy(d, kb + off, r * C::RB, bar);
+          bulk_copy(d + KT * C::RB, vb + off, r * C::RB, bar);
+        }
+      }
+    }
+    __syncwarp();
+    ++f_i;
+    if (++f_slot == C::NST) f_slot = 0;
+  };
+  for (int i = 0; i < C::NST; ++i) feed();
+
+  int slot = 0;
+  uint32_t phase = 0;
+  QPiece pc;
+  while (walk.next(a, &pc)) {
+    /* ---- rows of q: scaled by a power of two, as fragments; sums of the groups */
+    for (int qi = warp; qi < C::RT; qi += W) {
+      constexpr int N4 = HD / 128 > 0 ? HD / 128 : 1; /* runs of four elements a lane */
+      float x[N4][4];
+      float top = 0.f;
+      const int gq = pc.q0 + qi;
+      const T* src = (const T*)a.q + ((long long)(pc.q.r0 + gq / a.G) * a.H + pc.kvh * a.G + gq % a.G) * HD;
+#pragma unroll
+      for (int i = 0; i < N4; ++i) {
+        const int d = (i * 32 + lane) * 4;
+        uint2 w = make_uint2(0, 0);
+        if (qi < pc.nq && d < HD) w = *reinterpret_cast<const uint2*>(src + d);
+        const float2 u = unpack2<T>(w.x), v = unpack2<T>(w.y);
+        x[i][0] = u.x; x[i][1] = u.y; x[i][2] = v.x; x[i][3] = v.y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[i][e]));
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
+      const int ex = max(-126, min(127, top > 0.f ? ilogbf(top) : 0));
+#pragma unroll
+      for (int i = 0; i < N4; ++i) {
+        const int d = (i * 32 + lane) * 4;
+        const uint32_t lo = h2(ldexpf(x[i][0], -ex), ldexpf(x[i][1], -ex)), hi = h2(ldexpf(x[i][2], -ex), ldexpf(x[i][3], -ex));
+        const float2 u = unpack2<__half>(lo), v = unpack2<__half>(hi);
+        float sum = (u.x + u.y) + (v.x + v.y);
+#pragma unroll
+        for (int o = 4; o; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+        if (d < HD) {
+          qf[((qi >> 3) * C::KS + (d >> 4)) * 32 + (qi & 7) * 4 + ((d >> 2) & 3)] = make_uint2(lo, hi);
+          if ((lane & 7) == 0) sh_qsum[d >> 5][qi] = sum;
+        }
+      }
+      if (lane == 0) sh_qs[qi] = ldexpf(1.f, ex) * a.scale2;
+    }
+    __syncthreads();
+
+    float sc[NT][2], m[NT][2], l[NT][2];
+    float qs[Q4 ? NG : 1][NT][2], om[Q4 ? NG : 1][NT][2];
+    float o[HD / 16][NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        sc[n][e] = sh_qs[n * 8 + 2 * t + e];
+        m[n][e] = -INFINITY;
+        l[n][e] = 0.f;
+        if constexpr (Q4) {
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+            qs[i][n][e] = sh_qsum[i][n * 8 + 2 * t + e];
+            om[i][n][e] = 0.f;
+          }
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
+    const int open = min(tree_open(a, pc.q), pc.q.len);
+    uint2 qr[NT == 1 ? C::KS : 1];
+    if constexpr (NT == 1) {
+#pragma unroll
+      for (int i = 0; i < C::KS; ++i) qr[i] = qf[i * 32 + lane];
+    }
+
+    const int n_own = (pc.n + W - 1 - warp) / W;
+    for (int it = 0; it < n_own && ok; ++it) {
+      const int pos0 = (pc.t0 + warp + it * W) * KT;
+      if (!mb_wait_warp(&full[warp][slot], phase)) { ok = false; break; }
+      const uint8_t* const kt = ring + slot * C::STAGE;
+      const uint8_t* const vt = kt + KT * C::RB;
+      const int map = sh_map[warp][slot];
+      const bool masked = pos0 + KT > open || map != 3;
+      float s[2][NT][4];
+      /* ---- scores of 2 x 16 keys */
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint8_t *r0 = kt + (u * 16 + g) * C::RB, *r1 = r0 + 8 * C::RB;
+        float d0[NG], d1[NG], m0[NG], m1[NG];
+        row_scales<Q4, NG>(r0 + C::CB, d0, m0);
+        row_scales<Q4, NG>(r1 + C::CB, d1, m1);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[u][n][0] = s[u][n][1] = s[u][n][2] = s[u][n][3] = 0.f;
+        auto group = [&](int i, const uint32_t (&a0)[4], const uint32_t (&a1)[4]) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint2 b0 = NT == 1 ? qr[(2 * i) % (NT == 1 ? C::KS : 1)] : qf[(n * C::KS + 2 * i) * 32 + lane];
+            const uint2 b1 = NT == 1 ? qr[(2 * i + 1) % (NT == 1 ? C::KS : 1)] : qf[(n * C::KS + 2 * i + 1) * 32 + lane];
+            mma16(c, a0, b0.x, b0.y);
+            mma16(c, a1, b1.x, b1.y);
+            s[u][n][0] = __fmaf_rn(d0[i], c[0], s[u][n][0]);
+            s[u][n][1] = __fmaf_rn(d0[i], c[1], s[u][n][1]);
+            s[u][n][2] = __fmaf_rn(d1[i], c[2], s[u][n][2]);
+            s[u][n][3] = __fmaf_rn(d1[i], c[3], s[u][n][3]);
+            if constexpr (Q4) {
+              s[u][n][0] = __fmaf_rn(m0[i], qs[i][n][0], s[u][n][0]);
+              s[u][n][1] = __fmaf_rn(m0[i], qs[i][n][1], s[u][n][1]);
+              s[u][n][2] = __fmaf_rn(m1[i], qs[i][n][0], s[u][n][2]);
+              s[u][n][3] = __fmaf_rn(m1[i], qs[i][n][1], s[u][n][3]);
+            }
+          }
+        };
+        if constexpr (Q4) {
+#pragma unroll
+          for (int i = 0; i < NG; i += 2) {
+            const int at = i * 16 + 4 * t;
+            uint32_t x0 = lds32(r0 + at), x1 = lds32(r1 + at), y0 = lds32(r0 + at + 16), y1 = lds32(r1 + at + 16);
+            {
+              const uint32_t f0[4] = {nib_lo(x0), nib_lo(x1), nib_hi(x0), nib_hi(x1)}, f1[4] = {nib_lo(y0), nib_lo(y1), nib_hi(y0), nib_hi(y1)};
+              group(i, f0, f1);
+            }
+            x0 >>= 8; x1 >>= 8; y0 >>= 8; y1 >>= 8;
+            {
+              const uint32_t f0[4] = {nib_lo(x0), nib_lo(x1), nib_hi(x0), nib_hi(x1)}, f1[4] = {nib_lo(y0), nib_lo(y1), nib_hi(y0), nib_hi(y1)};
+              group(i + 1, f0, f1);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+            const int at = i * 32 + 4 * t;
+            const uint32_t x0 = lds32(r0 + at) ^ 0x80808080u, x1 = lds32(r1 + at) ^ 0x80808080u, y0 = lds32(r0 + at + 16) ^ 0x80808080u,
+                           y1 = lds32(r1 + at + 16) ^ 0x80808080u;
+            const uint32_t f0[4] = {byte2<0>(x0), byte2<0>(x1), byte2<1>(x0), byte2<1>(x1)},
+                           f1[4] = {byte2<0>(y0), byte2<0>(y1), byte2<1>(y0), byte2<1>(y1)};
+            group(i, f0, f1);
+          }
+        }
+      }
+      /* ---- V's scales of the lane's four keys, the logarithm of the largest */
+      float vd[2][2][NG], vm[2][2][NG], lg[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          row_scales<Q4, NG>(vt + (u * 16 + r * 8 + g) * C::RB + C::CB, vd[u][r], vm[u][r]);
+          float x = 5.9604645e-8f; /* 2^-24, the smallest scale there is: a row of zeros counts as that */
+#pragma unroll
+          for (int i = 0; i < NG; ++i) x = fmaxf(x, fabsf(vd[u][r][i]));
+          lg[u][r] = __log2f(x);
+        }
+      float top[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        top[n][0] = top[n][1] = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x = s[u][n][2 * r + e] * sc[n][e];
+              if (masked) {
+                const int pos = pos0 + u * 16 + r * 8 + g, qi = pc.q0 + n * 8 + 2 * t + e;
+                const bool see = (map >> u & 1) && pos < pc.q.len && qi < pc.q0 + pc.nq && (pos < open || tree_sees(a, pc.q, qi / a.G, pos));
+                if (!see) x = -INFINITY;
+              }
+              s[u][n][2 * r + e] = x;
+              top[n][e] = fmaxf(top[n][e], x + lg[u][r]);
+            }
+      }
+      bool grow = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(kAll, top[n][e], x));
+          grow |= top[n][e] - kRaise - kGrow > m[n][e];
+        }
+      if (__any_sync(kAll, grow)) { /* a row's first keys, seldom later */
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float to = top[n][e] - kRaise;
+            if (to - kGrow > m[n][e]) {
+              const float f = m[n][e] == -INFINITY ? 0.f : ex2(m[n][e] - to);
+              m[n][e] = to;
+              l[n][e] *= f;
+#pragma unroll
+              for (int i = 0; i < HD / 16; ++i) {
+                o[i][n][e] *= f;
+                o[i][n][2 + e] *= f;
+              }
+              if constexpr (Q4) {
+#pragma unroll
+                for (int i = 0; i < NG; ++i) om[i][n][e] *= f;
+              }
+            }
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float mm = m[n][e] == -INFINITY ? 0.f : m[n][e];
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float x = ex2(s[u][n][2 * r + e] - mm);
+              s[u][n][2 * r + e] = x;
+              l[n][e] += x;
+            }
+        }
+      /* ---- o += V^T (p d), minima apart */
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint8_t* const v0 = vt + (u * 16 + 2 * t) * C::RB;
+        /* weights of group i as the second operand; in a masked tile what is not seen is zero whatever its scale holds */
+        auto weights = [&](int i, int n, uint32_t* b) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = s[u][n][e];
+            w[e] = x * vd[u][e >> 1][i];
+            if (masked && x == 0.f) w[e] = 0.f;
+            if constexpr (Q4) om[i][n][e & 1] += masked && x == 0.f ? 0.f : x * vm[u][e >> 1][i];
+          }
+          b[0] = transpose8(h2(w[0], w[1]));
+          b[1] = transpose8(h2(w[2], w[3]));
+        };
+        auto product = [&](int i, const uint32_t (&f0)[4], const uint32_t (&f1)[4]) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            uint32_t b[2];
+            weights(i, n, b);
+            mma16(o[2 * i][n], f0, b[0], b[1]);
+            mma16(o[2 * i + 1][n], f1, b[0], b[1]);
+          }
+        };
+        if constexpr (Q4) {
+#pragma unroll
+          for (int i = 0; i < NG; i += 2) {
+            const uint8_t* const w = v0 + i * 16 + 4 * g;
+            const uint32_t w0 = lds32(w), w1 = lds32(w + C::RB), w2 = lds32(w + 8 * C::RB), w3 = lds32(w + 9 * C::RB);
+            uint32_t x0 = __byte_perm(w0, w1, 0x5410), x1 = __byte_perm(w0, w1, 0x7632), y0 = __byte_perm(w2, w3, 0x5410),
+                     y1 = __byte_perm(w2, w3, 0x7632); /* elements 0, 2 and 1, 3 of keys 2 t, 2 t + 1 and 2 t + 8, 2 t + 9 */
+            {
+              const uint32_t f0[4] = {nib_lo(x0), nib_lo(x1), nib_lo(y0), nib_lo(y1)}, f1[4] = {nib_hi(x0), nib_hi(x1), nib_hi(y0), nib_hi(y1)};
+              product(i, f0, f1);
+            }
+            x0 >>= 8; x1 >>= 8; y0 >>= 8; y1 >>= 8;
+            {
+              const uint32_t f0[4] = {nib_lo(x0), nib_lo(x1), nib_lo(y0), nib_lo(y1)}, f1[4] = {nib_hi(x0), nib_hi(x1), nib_hi(y0), nib_hi(y1)};
+              product(i + 1, f0, f1);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+            const uint8_t* const w = v0 + i * 32 + 4 * g;
+            const uint32_t w0 = lds32(w) ^ 0x80808080u, w1 = lds32(w + C::RB) ^ 0x80808080u, w2 = lds32(w + 8 * C::RB) ^ 0x80808080u,
+                           w3 = lds32(w + 9 * C::RB) ^ 0x80808080u;
+            const uint32_t x0 = __byte_perm(w0, w1, 0x5140), x1 = __byte_perm(w0, w1, 0x7362), y0 = __byte_perm(w2, w3, 0x5140),
+                           y1 = __byte_perm(w2, w3, 0x7362); /* elements 0, 1 and 2, 3, two keys each */
+            const uint32_t f0[4] = {byte2<0>(x0), byte2<1>(x0), byte2<0>(y0), byte2<1>(y0)},
+                           f1[4] = {byte2<0>(x1), byte2<1>(x1), byte2<0>(y1), byte2<1>(y1)};
+            product(i, f0, f1);
+          }
+        }
+      }
+      __syncwarp(); /* every lane has read the tile */
+      if (++slot == C::NST) { slot = 0; phase ^= 1; }
+      feed();
+    }
+
+    /* ---- the warps join */
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(kAll, l[n][e], x);
+        if constexpr (Q4) {
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) om[i][n][e] += __shfl_xor_sync(kAll, om[i][n][e], x);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              o[2 * i + x][n][e] += om[i][n][e];
+              o[2 * i + x][n][2 + e] += om[i][n][e];
+            }
+          }
+        }
+        if (g == 0) sh_ml[warp][n * 8 + 2 * t + e] = make_float2(m[n][e], l[n][e]);
+      }
+    __syncthreads();
+    if (tid < C::RT) {
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) M = fmaxf(M, sh_ml[w][tid].x);
+      const float U = M == -INFINITY ? 0.f : M;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float f = ex2(sh_ml[w][tid].x - U);
+        sh_f[w][tid] = f;
+        L += sh_ml[w][tid].y * f;
+      }
+      sh_m[tid] = M;
+      sh_l[tid] = L;
+    }
+    const bool whole = pc.n == pc.n_tile;
+    const int my_slot = pc.nth == 0 ? 0 : 1; /* only a CTA's first and last pieces can be parts */
+    const long long ps = ((long long)grp_id * 2 + my_slot) * C::RT;
+    auto out_row = [&](int qi) { return (long long)(pc.q.r0 + (pc.q0 + qi) / a.G) * a.H + pc.kvh * a.G + (pc.q0 + qi) % a.G; };
+#pragma unroll
+    for (int d0 = 0; d0 < HD; d0 += JD) {
+      if (d0) __syncthreads(); /* the words of the pass before are read */
+#pragma unroll
+      for (int i = 0; i < JD / 32; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int f = d0 / 16 + 2 * i;
+            *reinterpret_cast<float4*>(jb + (warp * C::RT + n * 8 + 2 * t + e) * JD + i * 32 + 4 * g) =
+                make_float4(o[f][n][e], o[f][n][2 + e], o[f + 1][n][e], o[f + 1][n][2 + e]);
+          }
+      __syncthreads();
+      for (int i = tid; i < pc.nq * (JD / 4); i += NTH) {
+        const int qi = i / (JD / 4), d = (i % (JD / 4)) * 4;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float f = sh_f[w][qi];
+          const float4 y = *reinterpret_cast<const float4*>(jb + (w * C::RT + qi) * JD + d);
+          x.x += y.x * f;
+          x.y += y.y * f;
+          x.z += y.z * f;
+          x.w += y.w * f;
+        }
+        if (whole) {
+          const float L = sh_l[qi], inv = L == 0.f ? 0.f : __fdividef(1.f, L); /* 0: the row sees nothing */
+          *reinterpret_cast<uint2*>((T*)a.out + out_row(qi) * HD + d0 + d) = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+        } else {
+          __stcg(reinterpret_cast<float4*>(a.po + (ps + qi) * HD + d0 + d), x);
+        }
+      }
+    }
+    if (tid < pc.nq) {
+      if (!whole) __stcg(reinterpret_cast<float2*>(a.pml + (ps + tid) * 2), make_float2(sh_m[tid], sh_l[tid]));
+      else if (a.lse) a.lse[out_row(tid)] = sh_l[tid] == 0.f ? -INFINITY : (sh_m[tid] + log2f(sh_l[tid])) * kLn2;
+    }
+    if (!whole) {
+      /* the last of the unit's CTAs to get here joins them, in the order of their keys */
+      const int c0 = line.group_of(pc.first), pieces = line.group_of(pc.last) - c0 + 1;
+      if (pc.t0 == 0 && tid == 0) p.tail[2 * c0 + 1] = my_slot;
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const int n = atomicAdd(&p.tail[2 * c0], 1);
+        sh_last = n == pieces - 1;
+        if (n == pieces - 1) p.tail[2 * c0] = 0; /* for the next launch */
+      }
+      __syncthreads();
+      if (sh_last) {
+        __threadfence();
+        const int slot0 = __ldcg(&p.tail[2 * c0 + 1]);
+        auto place = [&](int i, int qi) { return ((long long)(c0 + i) * 2 + (i == 0 ? slot0 : 0)) * C::RT + qi; };
+        for (int i = tid; i < pc.nq * (HD / 4); i += NTH) {
+          const int qi = i / (HD / 4), d = (i % (HD / 4)) * 4;
+          float M = -INFINITY, L = 0.f;
+          for (int k = 0; k < pieces; ++k) M = fmaxf(M, __ldcg(a.pml + place(k, qi) * 2));
+          const float U = M == -INFINITY ? 0.f : M;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+          for (int k = 0; k < pieces; ++k) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.pml + place(k, qi) * 2));
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(a.po + place(k, qi) * HD + d));
+            const float f = ex2(ml.x - U);
+            L += ml.y * f;
+            x.x += y.x * f;
+            x.y += y.y * f;
+            x.z += y.z * f;
+            x.w += y.w * f;
+          }
+          const float inv = L == 0.f ? 0.f : __fdividef(1.f, L);
+          *reinterpret_cast<uint2*>((T*)a.out + out_row(qi) * HD + d) = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+          if (d == 0 && a.lse) a.lse[out_row(qi)] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+        }
+      }
+    }
+    __syncthreads(); /* q's fragments and the statistics may be replaced */
+  }
+  if (!ok) { /* no copy is in flight when the CTA ends */
+    for (int i = 0; i < C::NST; ++i) mb_wait_warp(&full[warp][slot], phase), slot = slot + 1 == C::NST ? (phase ^= 1, 0) : slot + 1;
+    if (lane == 0) atomicOr(a.err, 8);
+  }
+}
+
+constexpr size_t kQuantWsFloats = (size_t)8 << 20; /* 32 MiB */
+constexpr size_t kQuantTail = 4096;                /* of them, ints of arrivals */
+
+template <typename T, bool Q4, int HD, int NT>
+int launch_quant(Ctx* c, TreeArgs& a) {
+  using C = QCfg<Q4, HD, NT>;
+  static uint64_t attr = 0; /* devices it is set on */
+  if (!(attr >> (c->device & 63) & 1)) {
+    ULB_CUDA(cudaFuncSetAttribute(quant_attn_kernel<T, Q4, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    attr |= 1ull << (c->device & 63);
+  }
+  const long long units = (long long)a.g.n_seq * a.g.n_head_kv * (((long long)a.max_rows * a.G + C::RT - 1) / C::RT);
+  ULB_CHECK(units * (std::max(1, (a.max_len + KT - 1) / KT) + kUnitCost) < (1ll << 31) - 65536, ULB_EUNSUPPORTED,
+            "ulb_quant_attention: %d sequences of %d positions and %d rows", a.g.n_seq, a.max_len, a.max_rows);
+  QuantPlan p;
+  p.groups = c->n_sm;
+  p.min_tiles = kMinTiles;
+  const size_t rows = (size_t)p.groups * 2 * C::RT;
+  ULB_CHECK(kQuantTail + rows * (HD + 2) <= kQuantWsFloats && 2 * (size_t)p.groups <= kQuantTail, ULB_EUNSUPPORTED,
+            "ulb_quant_attention: workspace for %d SMs", c->n_sm);
+  p.tail = reinterpret_cast<int*>(c->quant_ws);
+  a.po = c->quant_ws + kQuantTail;
+  a.pml = a.po + rows * HD;
+  ULB_LAUNCH("quant attention launch", launch_k(c, quant_attn_kernel<T, Q4, HD, NT>, dim3(p.groups), dim3(C::W * 32), C::SMEM, a, p));
+  return ULB_OK;
+}
+
+template <typename T, bool Q4, int HD>
+int pick_rows(Ctx* c, TreeArgs& a) {
+  const long long nq = (long long)a.max_rows * a.G;
+  if (nq <= 8) return launch_quant<T, Q4, HD, 1>(c, a);
+  if (nq <= 16 || HD == 256) return launch_quant<T, Q4, HD, 2>(c, a);
+  if constexpr (HD < 256) return launch_quant<T, Q4, HD, 4>(c, a);
+  return ULB_OK;
+}
+template <typename T, bool Q4>
+int pick_quant(Ctx* c, TreeArgs& a) {
+  if (a.g.hd == 64) return pick_rows<T, Q4, 64>(c, a);
+  if (a.g.hd == 128) return pick_rows<T, Q4, 128>(c, a);
+  return pick_rows<T, Q4, 256>(c, a);
+}
+
+}  // namespace
+}  // namespace ulb
+
+using namespace ulb;
+
+extern "C" int ulb_quant_attention(ulb_ctx* ctx, const ulb_quant_desc* cache, const ulb_tree_desc* d, const void* q, const void* k,
+                                   const void* v, const int32_t* table, const int32_t* row_start, const int32_t* prefix,
+                                   const int32_t* len, const uint32_t* mask, void* out, float* lse) {
+  ULB_CHECK(ctx && d, ULB_EINVAL, "ulb_quant_attention: NULL argument");
+  TreeArgs a = {};
+  ULB_TRY(quant_geom("ulb_quant_attention", cache, &a.g));
+  ULB_CHECK(d->n_head > 0 && d->n_head % a.g.n_head_kv == 0 && d->n_head / a.g.n_head_kv <= 64, ULB_EINVAL,
+            "ulb_quant_attention: %d heads over %d kv heads", d->n_head, a.g.n_head_kv);
+  ULB_CHECK(d->rows >= 0 && d->max_rows >= 0 && d->max_len >= 0 && d->mask_words >= 0, ULB_EINVAL,
+            "ulb_quant_attention: %d rows, at most %d a sequence over %d positions, %d mask words", d->rows, d->max_rows, d->max_len,
+            d->mask_words);
+  ULB_CHECK(std::isfinite(d->scale) && d->scale > 0.f, ULB_EINVAL, "ulb_quant_attention: scale %g", (double)d->scale);
+  if (d->rows == 0 || d->max_rows == 0) return ULB_OK;
+  ULB_CHECK(q && k && v && table && row_start && prefix && len && out, ULB_EINVAL, "ulb_quant_attention: NULL argument");
+  ULB_CHECK(!mask == (d->mask_words == 0), ULB_EINVAL, "ulb_quant_attention: mask without mask_words, or the reverse");
+  ULB_CHECK(ULB_ALIGNED16(q) && ULB_ALIGNED16(k) && ULB_ALIGNED16(v) && ULB_ALIGNED16(out), ULB_EINVAL,
+            "ulb_quant_attention: q, the pools and out must be 16-byte aligned");
+  ULB_CHECK(words_aligned({table, row_start, prefix, len, mask, lse}), ULB_EINVAL, "ulb_quant_attention: unaligned array of 32-bit elements");
+  a.H = d->n_head;
+  a.G = d->n_head / a.g.n_head_kv;
+  a.rows = d->rows;
+  a.max_rows = std::min(d->max_rows, d->rows);
+  a.max_len = std::min(d->max_len, a.g.max_pages * a.g.page);
+  ULB_CHECK((long long)a.max_rows * a.G < (1ll << 31) && (long long)d->rows * d->n_head < (1ll << 31), ULB_EUNSUPPORTED,
+            "ulb_quant_attention: %d rows of %d heads", d->rows, d->n_head);
+  ULB_CHECK(a.max_len <= 0x7fff0000, ULB_EUNSUPPORTED, "ulb_quant_attention: %d positions", a.max_len);
+  a.words = d->mask_words;
+  a.scale2 = d->scale * kLog2e;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.table = table;
+  a.row_start = row_start;
+  a.prefix = prefix;
+  a.len = len;
+  a.mask = mask;
+  a.out = out;
+  a.lse = lse;
+  a.err = ctx->c.dev_err;
+  Ctx* c = &ctx->c;
+  ULB_CUDA(cudaSetDevice(c->device));
+  if (!c->quant_ws) { /* at the first call, whatever its shape, so that any later one can be captured */
+    float* ws = nullptr;
+    ULB_CUDA(cudaMalloc((void**)&ws, kQuantWsFloats * sizeof(float)));
+    const cudaError_t e = cudaMemsetAsync(ws, 0, kQuantTail * sizeof(int), c->stream);
+    if (e != cudaSuccess) {
+      cudaFree(ws);
+      return cuda_error(e, "ulb_quant_attention", __FILE__, __LINE__);
+    }
+    c->quant_ws = ws;
+  }
+  if (cache->dtype == ULB_TYPE_F16) return cache->format == ULB_TYPE_Q4_1 ? pick_quant<__half, true>(c, a) : pick_quant<__half, false>(c, a);
+  return cache->format == ULB_TYPE_Q4_1 ? pick_quant<__nv_bfloat16, true>(c, a) : pick_quant<__nv_bfloat16, false>(c, a);
+}
+
+ULB_TRACE_UNIT(quant_attention)

@@ -255,13 +255,6 @@ static long double pair_with_turns(long double t, long double rot, long double L
   return rot * logl(L / (kTwoPi * t)) / (2.0L * logl(base));
 }
 
-struct ulb_rope {
-  ulb_ctx* owner = nullptr;
-  int hd = 0, rot = 0, half = 0;
-  float mscale = 1.f;
-  unsigned long long* turn = nullptr;
-};
-
 extern "C" {
 
 int ulb_rope_create(ulb_ctx* ctx, const ulb_rope_desc* d, const float* ff, ulb_rope** out) {

@@ -240,6 +240,8 @@ int ulb_destroy(ulb_ctx* ctx) {
   cudaFree(ctx->c.tc_ws);
   cudaFree(ctx->c.tc_cnt);
   cudaFree(ctx->c.tree_ws);
+  cudaFree(ctx->c.norm_ws);
+  cudaFree(ctx->c.quant_ws);
   cudaEventDestroy(ctx->c.switch_ev);
   cudaStreamDestroy(ctx->c.own_stream);
   delete ctx;

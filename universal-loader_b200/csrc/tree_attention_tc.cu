@@ -49,9 +49,8 @@
  * arrives nowhere and issues nothing any more, so that the others run into theirs; the CTA still
  * waits (bounded) for its MMAs before it frees TMEM.
  */
+#include "tcgen05.h"
 #include "tree_attention.h"
-
-#include <cuda.h>
 
 #include <algorithm>
 #include <mutex>
@@ -67,123 +66,8 @@ constexpr int kMinTiles = 12;  /* places of the line a group takes at least */
 constexpr int kJoinRows = 8;   /* rows a block of the join kernel: a warp each */
 constexpr int kOddWords = 32;  /* bits for 1024 positions */
 
-__device__ __forceinline__ uint32_t sa(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void mb_init(uint64_t* b, uint32_t n) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sa(b)), "r"(n) : "memory");
-}
-__device__ __forceinline__ void mb_expect(uint64_t* b, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(sa(b)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mb_arrive(uint64_t* b) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sa(b)) : "memory");
-}
-__device__ __forceinline__ bool mb_try(uint64_t* b, uint32_t parity) {
-  uint32_t ok;
-  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-               : "=r"(ok) : "r"(sa(b)), "r"(parity) : "memory");
-  return ok != 0;
-}
-/* wait for the phase with this parity; false after kTries looks, each of which the hardware may stretch
-   (seconds in all; reading a clock between looks costs more than the looks) */
-constexpr int kTries = 1 << 21;
-__device__ __forceinline__ bool mb_wait(uint64_t* b, uint32_t parity) {
-  for (int i = 0; i < kTries; ++i)
-    if (mb_try(b, parity)) return true;
-  return false;
-}
-/* the same for a converged warp, one answer for all lanes (a vote: a shuffle would queue behind the
-   softmax warps' exponentials, as every shared-memory operation does, for some 300 cycles) */
-__device__ __forceinline__ bool mb_wait_warp(uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, mb_wait(b, parity)); }
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void commit(uint64_t* b) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sa(b)) : "memory");
-}
-__device__ __forceinline__ void tma4(void* dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* bar) {
-  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-               ::"r"(sa(dst)), "l"(m), "r"(x), "r"(y), "r"(z), "r"(w), "r"(sa(bar)) : "memory");
-}
-/* one lane of a converged warp: the compiler knows that what the branch holds runs once, and keeps
-   the operands of tcgen05 instructions in uniform registers (under `lane == 0` each MMA took about
-   70 cycles to issue) */
-__device__ __forceinline__ bool elect() {
-  uint32_t p;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
-  return p != 0;
-}
-/* D (TMEM) (+)= A (shared) B (shared) and D (+)= A (TMEM) B (shared), K = 16 */
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n"
-               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u) : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n"
-               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u) : "memory");
-}
-/* 32 consecutive columns of the thread's TMEM lane */
-__device__ __forceinline__ void tm_ld(uint32_t t, uint32_t* r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-                 "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-                 "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-               : "r"(t));
-}
-__device__ __forceinline__ void tm_st(uint32_t t, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
-               ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-               "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-               "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-               "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(t) : "memory");
-}
-__device__ __forceinline__ void tm_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tm_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-/* two fp32 operations in one instruction */
-__device__ __forceinline__ uint64_t two(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 both(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 /* the 256 softmax threads */
 __device__ __forceinline__ void sync_softmax() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-
-/* shared-memory descriptors of 128-byte-swizzled tiles (rows of 64 elements, 8-row groups 1024 bytes
-   apart): K-major (Q, K: a row is an index of M or N, its 64 elements 64 of hd), and MN-major
-   (V: a row is a key = K index, its 64 elements 64 of N; the next 64 of N one half tile on) */
-__device__ __forceinline__ uint64_t desc_k(uint32_t s) {
-  return (uint64_t)((s >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t s) {
-  return (uint64_t)((s >> 4) & 0x3FFFu) | ((uint64_t)((TK * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-         ((uint64_t)2 << 61);
-}
-/* byte of 16-byte chunk c (of 8) of row r in a half tile */
-__device__ __forceinline__ uint32_t sw128(int r, int c) { return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4)); }
 
 template <int HD, bool PAIR>
 struct TcCfg {
@@ -500,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t qp = 0, pp = 0; /* phases of q_full, and of p_full[X][b] in bit b */
       int ks = 0, vs = 0;      /* next tile of the rings, and its phase */
       uint32_t kp = 0, vp = 0;
-      const uint64_t dq = desc_k(sa(q_sm)) + (PAIR ? X * (C::QTILE >> 4) : 0), dk = desc_k(sa(k_sm)), dv = desc_mn(sa(v_sm));
+      const uint64_t dq = desc_k(sa(q_sm)) + (PAIR ? X * (C::QTILE >> 4) : 0), dk = desc_k(sa(k_sm)), dv = desc_mn<TK>(sa(v_sm));
       const uint32_t ds = tmem + X * 128, dov = tmem + 256 + X * HD;
       while (ok && walk.next(a, p, &pc)) {
         ok = mb_wait_warp(&q_full, qp);

@@ -88,7 +88,9 @@ struct Ctx {
   int* tc_cnt = nullptr;               /* kTcCounters arrival counters, zero between launches */
   int tp_rank = 0, tp_world = 1;
   int attn_form = 0; /* ULB_ATTN_AUTO / SPLIT / STREAM */
-  float* tree_ws = nullptr; /* split partials of ulb_tree_attention, made by its first call */
+  float* tree_ws = nullptr; /* split partials of ulb_tree_attention and ulb_prompt_attention, made by the first call */
+  float* norm_ws = nullptr;  /* the blocks' shares of the weights' gradients, made by ulb_norm_rope_grad's first call */
+  float* quant_ws = nullptr; /* partials and arrival counters of ulb_quant_attention, made by its first call */
   /* timing of the tensor-parallel all-reduces (on while a round is profiled): a CUDA event
      pair is recorded around each ncclAllReduce, events[2i] before and events[2i+1] after */
   /* host-side bound on waits for a stream holding tensor-parallel collectives (ms, 0 = none):
@@ -101,6 +103,7 @@ struct Ctx {
 };
 /* fp32 sum over the communicator's ranks, in place, on the context stream */
 int tp_allreduce_sum(Ctx* c, float* buf, size_t n);
+constexpr int kNormBlocks = 4; /* blocks an SM of ulb_norm_rope_grad at most */
 constexpr int kZeroRowHalves = 65536 + 64;
 
 /* read and clear the device error word (synchronises the stream) */

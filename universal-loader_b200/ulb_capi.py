@@ -15,7 +15,7 @@ LIB_PATH = os.path.join(HERE, "libulb_cuda.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "ulb.h")
 
 OK, EINVAL, ENOMEM, ECUDA, ENCCL, ETIMEOUT, EFORMAT, EUNSUPPORTED = 0, -1, -2, -3, -4, -5, -6, -7
-T_F32, T_F16, T_Q4_0, T_Q4_K, T_BF16 = 0, 1, 2, 12, 30
+T_F32, T_F16, T_Q4_0, T_Q4_1, T_Q8_0, T_Q4_K, T_BF16 = 0, 1, 2, 3, 8, 12, 30
 RNG_DRAFT, RNG_ACCEPT, RNG_RESID, RNG_FIRST = 1, 2, 3, 4
 
 P = C.c_void_p
@@ -70,6 +70,41 @@ class LogitsArgs(C.Structure):
                                   "row_allow")])
 
 
+class NormRopeArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("M", C.c_int), ("n_head", C.c_int), ("n_head_kv", C.c_int), ("eps", C.c_float),
+                ("q_row", C.c_int64), ("q_head", C.c_int64), ("k_row", C.c_int64), ("k_head", C.c_int64), ("q", P), ("k", P),
+                ("q_weight", P), ("k_weight", P), ("pos", P)]
+
+
+class QuantDesc(C.Structure):
+    """A paged cache in 8 or 4 bits: format T_Q8_0 or T_Q4_1, dtype of q and outputs."""
+    _fields_ = [(n, C.c_int) for n in ("format", "dtype", "n_head_kv", "head_dim", "page", "n_pages", "n_seq", "max_pages")]
+
+    @property
+    def row_bytes(self):
+        n = C.c_int()
+        check(lib().ulb_quant_row_bytes(C.byref(self), C.byref(n)))
+        return n.value
+
+    def pages_view(self, n_layer=1):
+        """The pools as a CacheDesc of 16-bit elements, for page moves and the page book."""
+        d = CacheDesc()
+        check(lib().ulb_quant_pages(C.byref(self), n_layer, C.byref(d)))
+        return d
+
+
+class QuantAppendArgs(C.Structure):
+    _fields_ = [("in_dtype", C.c_int), ("M", C.c_int), ("n_head", C.c_int), ("eps", C.c_float), ("q_row", C.c_int64),
+                ("k_row", C.c_int64), ("v_row", C.c_int64)] + [
+                (n, P) for n in ("q", "k", "v", "q_weight", "k_weight", "pos", "row_seq", "slot", "block_table", "q_out", "k_pool",
+                                 "v_pool")]
+
+
+class PromptDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "n_head", "n_head_kv", "head_dim", "n_seq", "q_rows", "k_rows", "max_q", "max_k")] + [
+                ("scale", C.c_float), ("q_row", C.c_int64), ("k_row", C.c_int64), ("v_row", C.c_int64)]
+
+
 ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
 ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "wavelength": 4}
 _DTYPE_IDS = {"f32": T_F32, "f16": T_F16, "bf16": T_BF16}
@@ -95,6 +130,14 @@ _SIGS = {
     "ulb_rope_append": (C.c_int, [P, P, P, C.c_int, P, C.c_int64, P, C.c_int64, P, C.c_int64, C.c_int, P, P, P, P,
                                   C.c_int, P, P, P]),
     "ulb_tree_attention": (C.c_int, [P, P, P, P, P, P, P, P, P, P, P, P, P]),
+    "ulb_norm_rope_apply": (C.c_int, [P, P, P, P, P]),
+    "ulb_norm_rope_grad": (C.c_int, [P, P, P, P, P, P, P, P, P]),
+    "ulb_quant_row_bytes": (C.c_int, [P, C.POINTER(C.c_int)]),
+    "ulb_quant_pages": (C.c_int, [P, C.c_int, P]),
+    "ulb_quant_append": (C.c_int, [P, P, P, P]),
+    "ulb_quant_read": (C.c_int, [P, P, C.c_int, P, P, P, P, P, C.c_int, P, P]),
+    "ulb_quant_attention": (C.c_int, [P, P, P, P, P, P, P, P, P, P, P, P, P]),
+    "ulb_prompt_attention": (C.c_int, [P, P, P, P, P, P, P, P, P]),
     "ulb_pages_copy": (C.c_int, [P, P, P, P, P, C.c_int]),
     "ulb_pages_compact": (C.c_int, [P, P, P, P, P, P, P, P, C.c_int]),
     "ulb_pages_create": (C.c_int, [P, P, P, P, C.POINTER(P)]),
@@ -266,6 +309,20 @@ class Context:
         check(lib().ulb_tree_attention(self.h, C.byref(cache), C.byref(d), q, k_pool, v_pool, block_table, row_start, prefix,
                                        length, mask, out, lse))
 
+    def quant_read(self, cache, dtype, k_pool, v_pool, block_table, row_seq, slot, M, k_out, v_out):
+        check(lib().ulb_quant_read(self.h, C.byref(cache), dtype, k_pool, v_pool, block_table, row_seq, slot, M, k_out, v_out))
+
+    def quant_attention(self, cache, n_head, rows, max_rows, max_len, scale, q, k_pool, v_pool, block_table, row_start, prefix,
+                        length, mask, mask_words, out, lse=None):
+        d = TreeDesc(n_head, rows, max_rows, max_len, mask_words, scale)
+        check(lib().ulb_quant_attention(self.h, C.byref(cache), C.byref(d), q, k_pool, v_pool, block_table, row_start, prefix,
+                                        length, mask, out, lse))
+
+    def prompt_attention(self, dtype, n_head, n_head_kv, head_dim, n_seq, q_rows, k_rows, max_q, max_k, scale, q, k, v, q_start,
+                         k_start, out, lse=None, q_row=0, k_row=0, v_row=0):
+        d = PromptDesc(dtype, n_head, n_head_kv, head_dim, n_seq, q_rows, k_rows, max_q, max_k, scale, q_row, k_row, v_row)
+        check(lib().ulb_prompt_attention(self.h, C.byref(d), q, k, v, q_start, k_start, out, lse))
+
     def pages_copy(self, cache, k_pool, v_pool, moves, n):
         check(lib().ulb_pages_copy(self.h, C.byref(cache), k_pool, v_pool, moves, n))
 
@@ -380,6 +437,25 @@ class Rope:
                k_row=0, v_row=0):
         check(lib().ulb_rope_append(self.ctx.h, self.h, C.byref(cache), in_dtype, q, q_row, k, k_row, v, v_row, n_head, pos,
                                     row_seq, slot, block_table, M, q_out, k_pool, v_pool))
+
+    def norm_apply(self, dtype, q, k, M, n_head, n_head_kv, q_weight, k_weight, eps, pos, q_out, k_out, q_row=0, q_head=0, k_row=0,
+                   k_head=0):
+        """q and k heads normed, weighted and turned."""
+        a = NormRopeArgs(dtype, M, n_head, n_head_kv, eps, q_row, q_head, k_row, k_head, q, k, q_weight, k_weight, pos)
+        check(lib().ulb_norm_rope_apply(self.ctx.h, self.h, C.byref(a), q_out, k_out))
+
+    def norm_grad(self, dtype, q, k, dq_out, dk_out, M, n_head, n_head_kv, q_weight, k_weight, eps, pos, dq, dk, dq_weight,
+                  dk_weight, q_row=0, q_head=0, k_row=0, k_head=0):
+        """norm_apply's gradient with respect to q, k and the weights."""
+        a = NormRopeArgs(dtype, M, n_head, n_head_kv, eps, q_row, q_head, k_row, k_head, q, k, q_weight, k_weight, pos)
+        check(lib().ulb_norm_rope_grad(self.ctx.h, self.h, C.byref(a), dq_out, dk_out, dq, dk, dq_weight, dk_weight))
+
+    def quant_append(self, cache, in_dtype, q, k, v, n_head, pos, row_seq, slot, block_table, M, q_out, k_pool, v_pool, q_row=0,
+                     k_row=0, v_row=0, q_weight=None, k_weight=None, eps=1e-6):
+        """append into a quantised cache, q and k normed first where their weights are given."""
+        a = QuantAppendArgs(in_dtype, M, n_head, eps, q_row, k_row, v_row, q, k, v, q_weight, k_weight, pos, row_seq, slot,
+                            block_table, q_out, k_pool, v_pool)
+        check(lib().ulb_quant_append(self.ctx.h, self.h, C.byref(cache), C.byref(a)))
 
     def close(self):
         if self.h:
