@@ -22,7 +22,7 @@ CUDA_HOME = os.path.dirname(os.path.dirname(NVCC))
 
 CU_SOURCES = ["runtime.cu", "qgemv.cu", "qgemm_tc.cu", "attention.cu", "sampling.cu", "model.cu", "spec.cu",
               "rope.cu", "head_norm.cu", "tree_attention.cu", "tree_attention_tc.cu", "pages.cu", "logits.cu",
-              "quant_attention.cu", "prompt_attention.cu"]
+              "quant_attention.cu", "prompt_attention.cu", "prompt_attention_tc.cu"]
 CUDA_LIB = os.path.join(PKG, "libulb_cuda.so")
 BUILD_TRACE = os.path.join(PKG, "_build_trace")
 CUDA_LIB_TRACE = os.path.join(PKG, "libulb_cuda_trace.so")

@@ -53,7 +53,6 @@
 #include "tree_attention.h"
 
 #include <algorithm>
-#include <mutex>
 
 namespace ulb {
 namespace {
@@ -790,21 +789,6 @@ __global__ void __launch_bounds__(kJoinRows * 32) tree_tc_join_kernel(const __gr
   T* out = (T*)a.out + at * hd + lane * E;
   if constexpr (E == 4) *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(x[0] * inv, x[1] * inv), pack2<T>(x[2] * inv, x[3] * inv));
   else *reinterpret_cast<uint32_t*>(out) = pack2<T>(x[0] * inv, x[1] * inv);
-}
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_tiled() {
-  static std::once_flag once;
-  static EncodeTiledFn fn = nullptr;
-  std::call_once(once, [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-      fn = (EncodeTiledFn)f;
-  });
-  return fn;
 }
 
 /* K or V pool as [page][head][position][hd], a box = 64 of hd x the positions of a page in a tile */
