@@ -498,7 +498,7 @@ ULB_API int ulb_logits_process(ulb_ctx* ctx, const ulb_logits_args* args);
  * Norms of the q and k heads of M rows, and their rotary positions, in one pass.  Head x of a row
  * (head_dim elements, a multiple of 8 up to 256) becomes
  *   y = R(pos) (w x f),  f = 1 / sqrt(mean x^2 + eps)
- * with R the rotation of the handle (its m on the elements that turn; rot_dim a multiple of 16 for
+ * with R the rotation of the handle (its m on the elements that turn; rot_dim a multiple of 8 for
  * ULB_ROPE_HALF) and one weight a head element, fp32 [head_dim], for all q heads and one for all k heads.
  * q and k are F32, F16 or BF16 rows of n_head and n_head_kv heads, element d of head h of row m at
  * m * row + h * head + d (0: dense); outputs are dense and of the same type, and may be the inputs where those
@@ -551,7 +551,8 @@ ULB_API int ulb_quant_pages(const ulb_quant_desc* desc, int n_layer, ulb_cache_d
  * ulb_rope_append into a quantised cache: q, k and v rows (in_dtype F32, F16 or BF16, heads dense inside rows of
  * stride q_row / k_row / v_row, 0: dense), q and k normed (weights as in ulb_norm_rope_args, each NULL: not) and
  * turned, q written to dev_q_out (desc's dtype, dense), k and v quantised into their slots.  Rows whose slot is
- * unmapped, negative or past the table write q only.  Two rows must not share a slot.
+ * unmapped, negative or past the table write q only.  Two rows must not share a slot.  A handle of the half layout turns the
+ * whole head here (rot_dim = head_dim).
  */
 typedef struct ulb_quant_append_args {
   int in_dtype, M, n_head;

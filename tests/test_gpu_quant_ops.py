@@ -30,7 +30,7 @@ def norm_case(rng, kind, M, H, KV, D, wide):
     return qkv, row, q, k, w, pos
 
 
-SHAPES = [(1, 1, 1, 64, 64), (3, 5, 5, 80, 48), (7, 32, 8, 128, 128), (300, 9, 3, 96, 96), (2, 3, 1, 256, 64), (5, 2, 0, 8, 0x10 // 2),
+SHAPES = [(1, 1, 1, 64, 64), (3, 5, 5, 80, 48), (7, 32, 8, 128, 128), (300, 9, 3, 96, 96), (2, 3, 1, 256, 64), (5, 2, 0, 8, 8), (6, 3, 1, 80, 24), (9, 5, 3, 64, 56),
           (4, 3, 2, 72, 32), (1030, 40, 8, 128, 64), (17, 64, 8, 64, 64)]
 
 
@@ -39,10 +39,6 @@ SHAPES = [(1, 1, 1, 64, 64), (3, 5, 5, 80, 48), (7, 32, 8, 128, 128), (300, 9, 3
 @pytest.mark.parametrize("M,H,KV,D,rot", SHAPES)
 def test_norm_rope_matches_formula(tctx, kind, layout, M, H, KV, D, rot):
     import ulb_capi as U
-    if layout == "half" and rot % 16:
-        rot = 0
-    if rot == 0:
-        pytest.skip("no such rotation in this layout")
     rng = np.random.default_rng(M * D + rot)
     wide = 8 if M % 2 else 3  # rows that are, and are not, whole 16-byte steps apart
     qkv, row, q, k, (wq, wk), pos = norm_case(rng, kind, M, H, KV, D, wide)
@@ -206,7 +202,7 @@ def test_norm_rope_refusals(tctx):
              dk=p + 8192, dq_weight=p + 12000, dk_weight=p + 12800)
     for bad in (dict(dq_weight=None), dict(dk_weight=None), dict(dq_out=None), dict(dk=None), dict(dq_weight=p + 2), dict(dq=p + 2), dict(eps=-1.0)):
         refused(r.norm_grad, **{**g, **bad})
-    for bad in (dict(head_dim=66), dict(head_dim=264), dict(head_dim=64, rot_dim=40, layout="half")):
+    for bad in (dict(head_dim=66), dict(head_dim=264), dict(head_dim=64, rot_dim=36, layout="half")):
         h = U.Rope(tctx, **bad)
         refused(h.norm_apply, **good, code=U.EUNSUPPORTED)
         h.close()
@@ -323,6 +319,45 @@ def test_append_writes_ggufs_blocks_and_read_gives_their_values(tctx, fmt, M, H,
 
 
 @pytest.mark.parametrize("fmt", ["q8", "q4"])
+@pytest.mark.parametrize("layout,rot,D", [("interleaved", 64, 64), ("interleaved", 40, 128), ("half", 64, 64), ("half", 256, 256)])
+def test_append_layouts_and_rows_at_any_address(tctx, fmt, layout, rot, D):
+    """The same rows 16-byte aligned and one element further on give the same bytes, and K their rotation."""
+    import ulb_capi as U
+    rng = np.random.default_rng(D + rot)
+    M, H, KV, page = 19, 3, 2, 32
+    x = torch.as_tensor(rng.standard_normal((M, H + 2 * KV, D)), dtype=torch.float32).cuda()
+    d = U.QuantDesc(FORMATS[fmt], U.T_F16, KV, D, page, 1, 1, 1)
+    r = U.Rope(tctx, D, rot_dim=rot, layout=layout)
+    pos, seq, slot, table = dev(rng.integers(0, 9999, M)), dev([0] * M), dev(rng.permutation(page)[:M]), dev([[0]])
+    w = dev(rng.uniform(0.5, 1.5, D), torch.float32)
+    row, got = (H + 2 * KV) * D, []
+    for shift in (0, 1):
+        flat = torch.zeros(M * (row + 1) + 8, device="cuda")
+        rows = flat[shift:shift + M * (row + shift)].view(M, row + shift)
+        rows[:, :row] = x.reshape(M, row)
+        k, v = (torch.zeros(1, KV, page, d.row_bytes, dtype=torch.uint8, device="cuda") for _ in range(2))
+        q_out = torch.zeros(M * H * D + 1, dtype=torch.float16, device="cuda")
+        at, n = ptr(rows), (row + shift)
+        r.quant_append(d, U.T_F32, at, at + H * D * 4, at + (H + KV) * D * 4, H, ptr(pos), ptr(seq), ptr(slot), ptr(table), M,
+                       ptr(q_out) + 2 * shift, ptr(k), ptr(v), q_row=n, k_row=n, v_row=n, k_weight=ptr(w), eps=1e-6)
+        got.append((k, v, q_out[shift:shift + M * H * D]))
+        KEEP.extend([flat, rows])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    f, m = frequencies(rot, 10000.0)
+    x64, half = x.double().cpu().numpy(), layout == "half"
+    k64 = rotate(normed(x64[:, H:H + KV], w.double().cpu().numpy(), 1e-6), pos.cpu().numpy(), f, m, rot, half)
+    q64 = rotate(x64[:, :H], pos.cpu().numpy(), f, m, rot, half)
+    assert np.abs(got[0][2].double().cpu().numpy().reshape(q64.shape) - q64).max() <= (2.0 ** -11 + 2.0 ** -19) * np.abs(q64).max() * 1.5
+    val = values(fmt, got[0][0].cpu().numpy()[0].transpose(1, 0, 2)[slot.cpu().numpy()], D).reshape(M, KV, -1, 32)
+    g = k64.reshape(val.shape)
+    step = np.abs(g).max(-1) / 127 if fmt == "q8" else (g.max(-1) - g.min(-1)) / 15
+    most = 127 if fmt == "q8" else 15  # as in the test above
+    slack = step * (0.5 + most * 2.0 ** -11 + 0.001) + (np.abs(g.min(-1)) * 2.0 ** -11 if fmt == "q4" else 0) + 2.0 ** -18 * np.abs(k64).max() * 1.5
+    assert (np.abs(val - g) <= slack[..., None]).all()
+    r.close()
+
+
+@pytest.mark.parametrize("fmt", ["q8", "q4"])
 def test_groups_of_odd_values(tctx, fmt):
     """Zeros, one value throughout, tiny, huge and not finite values, each in a group of its own."""
     import ulb_capi as U
@@ -392,10 +427,11 @@ def test_rows_without_a_place(tctx, fmt):
     for bad in (dict(in_dtype=8), dict(n_head=0), dict(M=-1), dict(q=None), dict(q_out=None), dict(slot=None), dict(k_pool=ptr(k) + 8),
                 dict(q=ptr(qkv) + 2), dict(row_seq=ptr(seq) + 2), dict(q_row=-8), dict(q_weight=ptr(qkv), eps=0.0), dict(k_weight=ptr(qkv) + 2)):
         refused(r.quant_append, **{**good, **bad})
-    h = U.Rope(tctx, 128)
-    refused(h.quant_append, **good)
+    for other in (dict(head_dim=128), dict(head_dim=64, rot_dim=32, layout="half")):
+        h = U.Rope(tctx, **other)
+        refused(h.quant_append, **good)
+        h.close()
     r.quant_append(**{**good, "M": 0, "q": None})
-    h.close()
     r.close()
 
 

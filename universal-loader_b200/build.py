@@ -21,7 +21,7 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 CUDA_HOME = os.path.dirname(os.path.dirname(NVCC))
 
 CU_SOURCES = ["runtime.cu", "qgemv.cu", "qgemm_tc.cu", "attention.cu", "sampling.cu", "model.cu", "spec.cu",
-              "rope.cu", "head_norm.cu", "tree_attention.cu", "tree_attention_tc.cu", "pages.cu", "logits.cu",
+              "rope.cu", "head_norm.cu", "quant_rows.cu", "tree_attention.cu", "tree_attention_tc.cu", "pages.cu", "logits.cu",
               "quant_attention.cu", "prompt_attention.cu", "prompt_attention_tc.cu"]
 CUDA_LIB = os.path.join(PKG, "libulb_cuda.so")
 BUILD_TRACE = os.path.join(PKG, "_build_trace")
