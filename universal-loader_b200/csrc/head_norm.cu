@@ -17,100 +17,110 @@
 namespace ulb {
 namespace {
 
-template <typename T, int LPH, bool VEC, bool HALF>
-__global__ void __launch_bounds__(kWarps * 32) norm_rope_kernel(const __grid_constant__ HeadArgs a) {
+template <typename T, int LPH, bool HALF>
+__global__ void __launch_bounds__(kWarps * 32, 3) norm_rope_kernel(const __grid_constant__ HeadArgs a, int wide) {
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const Place at = place_of<LPH, HALF>(a, lane);
-  const int gw = blockIdx.x * kWarps + (threadIdx.x >> 5), part = gw % a.wpr, n_rows = gridDim.x * kWarps / a.wpr;
-  float wq[8], wk[8];
-  lane_weights(a.wq, at, wq);
-  lane_weights(a.wk, at, wk);
-  const int first_k = part_of(part, a.nq, a.wpr, 32 / LPH);
-  auto load = [&](const T* p, float* x) {
-    load4<T, VEC>(p + at.d0, x);
-    load4<T, VEC>(p + at.d1, x + 4);
-  };
-  for (int m = gw / a.wpr; m < a.M; m += n_rows) {
-    Turn t;
-    turn_at<HALF>(a, a.pos[m], at, &t);
-    auto rows = [&](T* o) {
-      return [&, o](int h, bool mine, const float (&y)[8]) {
+  __shared__ HeadWeights sw;
+  const Place at = place_of<LPH, HALF>(a, threadIdx.x & 31);
+  const Pairs pairs = pairs_of<HALF>(a, at);
+  const float inv_hd = 1.f / a.hd;
+  load_weights(a, &sw);
+  Turn t;
+  walk_rows<Eight<T>, LPH, sizeof(T) == 4 ? 2 : 4>(
+      a, a.nq + a.nk, at.on,
+      [&](int m, int h, bool mine) {
+        Eight<T> e = zero8<T>();
+        if (mine) {
+          const T* p = h < a.nq ? (const T*)a.q + m * a.q_row + h * a.q_head : (const T*)a.k + m * a.k_row + (h - a.nq) * a.k_head;
+          load_run(p + at.d0, wide, &e.r[0]);
+          load_run(p + at.d1, wide, &e.r[1]);
+        }
+        return e;
+      },
+      [&](int, int pos) { turn_at(pairs, pos, a.mscale, &t); },
+      [&](int m, int h, bool mine, const Eight<T>& e) {
+        float x[8], w[8];
+        unpack8(e, x);
+        const bool is_q = h < a.nq;
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = __fmaf_rn(x[j], x[j], ss);
+        const float f = rsqrtf(__fmaf_rn(head_sum<LPH>(ss), inv_hd, a.eps));
+        lane_weights(sw, is_q ? 0 : 1, at, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= f * w[j];
+        turn<HALF>(t, 1.f, x);
         if (!mine) return;
-        store4<T, VEC>(o + (long long)h * a.hd + at.d0, y);
-        store4<T, VEC>(o + (long long)h * a.hd + at.d1, y + 4);
-      };
-    };
-    walk_heads<T, LPH, HALF, 4>(a, (const T*)a.q + m * a.q_row, a.q_head, a.nq, part * (32 / LPH), at, t, true, wq, true, load,
-                                rows((T*)a.oq + (long long)m * a.nq * a.hd));
-    walk_heads<T, LPH, HALF, 4>(a, (const T*)a.k + m * a.k_row, a.k_head, a.nk, first_k, at, t, true, wk, true, load,
-                                rows((T*)a.ok + (long long)m * a.nk * a.hd));
-  }
+        T* o = is_q ? (T*)a.oq + ((long long)m * a.nq + h) * a.hd : (T*)a.ok + ((long long)m * a.nk + h - a.nq) * a.hd;
+        store4(o + at.d0, wide, x);
+        store4(o + at.d1, wide, x + 4);
+      });
 }
 
-template <typename T, int LPH, bool VEC, bool HALF>
-__global__ void __launch_bounds__(kWarps * 32) norm_rope_grad_kernel(const __grid_constant__ HeadArgs a) {
+/* x and the gradient of the output */
+template <typename T>
+struct Both {
+  Eight<T> x, y;
+};
+template <typename T, int LPH, bool HALF>
+__global__ void __launch_bounds__(kWarps * 32, 2) norm_rope_grad_kernel(const __grid_constant__ HeadArgs a, int wide) {
   pdl_wait();
   pdl_trigger();
-  constexpr int HPS = 32 / LPH, U = 2;
+  __shared__ HeadWeights sw;
   __shared__ float sh[kWarps][2][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = lane / LPH;
   const Place at = place_of<LPH, HALF>(a, lane);
-  const int gw = blockIdx.x * kWarps + warp, part = gw % a.wpr, n_rows = gridDim.x * kWarps / a.wpr;
-  float wq[8], wk[8], sq[8] = {}, sk[8] = {};
-  lane_weights(a.M ? a.wq : nullptr, at, wq); /* no rows: they may be NULL */
-  lane_weights(a.M && a.nk ? a.wk : nullptr, at, wk);
+  const Pairs pairs = pairs_of<HALF>(a, at);
   const float inv_hd = 1.f / a.hd;
-  for (int m = gw / a.wpr; m < a.M; m += n_rows) {
-    Turn t;
-    turn_at<HALF>(a, a.pos[m], at, &t);
-    auto heads = [&](const T* x0, long long stride, const T* y0, T* o0, int n, int h_row, const float (&w)[8], float (&sum)[8]) {
-      const int first = part_of(part, h_row, a.wpr, HPS);
-      for (int h0 = first; h0 < n; h0 += a.wpr * HPS * U) {
-        float x[U][8], y[U][8];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int h = h0 + u * a.wpr * HPS + grp;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[u][j] = y[u][j] = 0.f;
-          if (h >= n || !at.on) continue;
-          const T *p = x0 + h * stride, *g = y0 + (long long)h * a.hd;
-          load4<T, VEC>(p + at.d0, x[u]);
-          load4<T, VEC>(p + at.d1, x[u] + 4);
-          load4<T, VEC>(g + at.d0, y[u]);
-          load4<T, VEC>(g + at.d1, y[u] + 4);
+  load_weights(a, &sw);
+  float sq[8] = {}, sk[8] = {};
+  Turn t;
+  walk_rows<Both<T>, LPH, 2>(
+      a, a.nq + a.nk, at.on,
+      [&](int m, int h, bool mine) {
+        Both<T> e = {zero8<T>(), zero8<T>()};
+        if (mine) {
+          const bool is_q = h < a.nq;
+          const T* p = is_q ? (const T*)a.q + m * a.q_row + h * a.q_head : (const T*)a.k + m * a.k_row + (h - a.nq) * a.k_head;
+          const T* g = is_q ? (const T*)a.gq + ((long long)m * a.nq + h) * a.hd : (const T*)a.gk + ((long long)m * a.nk + h - a.nq) * a.hd;
+          load_run(p + at.d0, wide, &e.x.r[0]);
+          load_run(p + at.d1, wide, &e.x.r[1]);
+          load_run(g + at.d0, wide, &e.y.r[0]);
+          load_run(g + at.d1, wide, &e.y.r[1]);
         }
+        return e;
+      },
+      [&](int, int pos) { turn_at(pairs, pos, a.mscale, &t); },
+      [&](int m, int h, bool mine, const Both<T>& e) {
+        float x[8], y[8], w[8];
+        unpack8(e.x, x);
+        unpack8(e.y, y);
+        const bool is_q = h < a.nq;
+        turn<HALF>(t, -1.f, y); /* g */
+        lane_weights(sw, is_q ? 0 : 1, at, w);
+        float ss = 0.f, sg = 0.f;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (h0 + u * a.wpr * HPS >= n) break;
-          const int h = h0 + u * a.wpr * HPS + grp;
-          turn<HALF>(t, -1.f, y[u]); /* g */
-          float ss = 0.f, sg = 0.f;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            ss = __fmaf_rn(x[u][j], x[u][j], ss);
-            sg = __fmaf_rn(y[u][j] * w[j], x[u][j], sg);
-          }
-          ss = head_sum<LPH>(ss);
-          sg = head_sum<LPH>(sg);
-          const float f = rsqrtf(__fmaf_rn(ss, inv_hd, a.eps)), c = f * f * (sg * inv_hd);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            sum[j] = __fmaf_rn(y[u][j], x[u][j] * f, sum[j]); /* zero past the heads */
-            x[u][j] = f * (y[u][j] * w[j] - x[u][j] * c);
-          }
-          if (h >= n || !at.on) continue;
-          T* o = o0 + (long long)h * a.hd;
-          store4<T, VEC>(o + at.d0, x[u]);
-          store4<T, VEC>(o + at.d1, x[u] + 4);
+        for (int j = 0; j < 8; ++j) {
+          w[j] *= y[j];
+          ss = __fmaf_rn(x[j], x[j], ss);
+          sg = __fmaf_rn(w[j], x[j], sg);
         }
-      }
-    };
-    heads((const T*)a.q + m * a.q_row, a.q_head, (const T*)a.gq + (long long)m * a.nq * a.hd, (T*)a.oq + (long long)m * a.nq * a.hd, a.nq, 0, wq, sq);
-    heads((const T*)a.k + m * a.k_row, a.k_head, (const T*)a.gk + (long long)m * a.nk * a.hd, (T*)a.ok + (long long)m * a.nk * a.hd, a.nk, a.nq, wk,
-          sk);
-  }
+        ss = head_sum<LPH>(ss);
+        sg = head_sum<LPH>(sg);
+        const float f = rsqrtf(__fmaf_rn(ss, inv_hd, a.eps)), c = f * f * f * (sg * inv_hd), fq = is_q ? f : 0.f, fk = is_q ? 0.f : f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float gx = y[j] * x[j]; /* zero past the heads */
+          sq[j] = __fmaf_rn(gx, fq, sq[j]);
+          sk[j] = __fmaf_rn(gx, fk, sk[j]);
+          x[j] = f * w[j] - x[j] * c;
+        }
+        if (!mine) return;
+        T* o = is_q ? (T*)a.oq + ((long long)m * a.nq + h) * a.hd : (T*)a.ok + ((long long)m * a.nk + h - a.nq) * a.hd;
+        store4(o + at.d0, wide, x);
+        store4(o + at.d1, wide, x + 4);
+      });
   /* the block's share of dw: groups of a warp by shuffles, warps in order */
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -155,40 +165,36 @@ __global__ void __launch_bounds__(kSumCols* kSumWays) norm_rope_sum_kernel(const
   }
 }
 
-template <typename T, bool VEC, bool HALF>
-int launch_apply(Ctx* c, HeadArgs& a) {
-  const int lph = lanes_of(a.hd), blocks = plan_rows(c, a, head_steps(a), c->n_sm * 8);
+template <typename T, bool HALF>
+int launch_apply(Ctx* c, HeadArgs& a, int wide) {
+  const int lph = lanes_of(a.hd), blocks = plan_rows(c, a, head_steps(a), c->n_sm * 3);
   auto go = [&](auto kern) -> int {
-    ULB_LAUNCH("norm rope launch", launch_k(c, kern, dim3(blocks), dim3(kWarps * 32), 0, a));
+    ULB_LAUNCH("norm rope launch", launch_k(c, kern, dim3(blocks), dim3(kWarps * 32), 0, a, wide));
     return ULB_OK;
   };
-  if (lph == 8) return go(norm_rope_kernel<T, 8, VEC, HALF>);
-  if (lph == 16) return go(norm_rope_kernel<T, 16, VEC, HALF>);
-  return go(norm_rope_kernel<T, 32, VEC, HALF>);
+  if (lph == 8) return go(norm_rope_kernel<T, 8, HALF>);
+  if (lph == 16) return go(norm_rope_kernel<T, 16, HALF>);
+  return go(norm_rope_kernel<T, 32, HALF>);
 }
 template <typename T>
-int pick_apply(Ctx* c, HeadArgs& a, bool vec) {
-  if (a.half) return vec ? launch_apply<T, true, true>(c, a) : launch_apply<T, false, true>(c, a);
-  return vec ? launch_apply<T, true, false>(c, a) : launch_apply<T, false, false>(c, a);
-}
-template <typename T, bool VEC, bool HALF>
-int launch_grad(Ctx* c, HeadArgs& a, float* dwq, float* dwk) {
+int pick_apply(Ctx* c, HeadArgs& a, int wide) { return a.half ? launch_apply<T, true>(c, a, wide) : launch_apply<T, false>(c, a, wide); }
+template <typename T, bool HALF>
+int launch_grad(Ctx* c, HeadArgs& a, int wide, float* dwq, float* dwk) {
   const int lph = lanes_of(a.hd), blocks = plan_rows(c, a, head_steps(a), c->n_sm * kNormBlocks);
   auto go = [&](auto kern) -> int {
-    ULB_LAUNCH("norm rope gradient launch", launch_k(c, kern, dim3(blocks), dim3(kWarps * 32), 0, a));
+    ULB_LAUNCH("norm rope gradient launch", launch_k(c, kern, dim3(blocks), dim3(kWarps * 32), 0, a, wide));
     return ULB_OK;
   };
-  if (lph == 8) ULB_TRY(go(norm_rope_grad_kernel<T, 8, VEC, HALF>));
-  else if (lph == 16) ULB_TRY(go(norm_rope_grad_kernel<T, 16, VEC, HALF>));
-  else ULB_TRY(go(norm_rope_grad_kernel<T, 32, VEC, HALF>));
+  if (lph == 8) ULB_TRY(go(norm_rope_grad_kernel<T, 8, HALF>));
+  else if (lph == 16) ULB_TRY(go(norm_rope_grad_kernel<T, 16, HALF>));
+  else ULB_TRY(go(norm_rope_grad_kernel<T, 32, HALF>));
   ULB_LAUNCH("norm rope gradient sum launch", launch_k(c, norm_rope_sum_kernel, dim3((2 * a.hd + kSumCols - 1) / kSumCols),
                                                        dim3(kSumCols * kSumWays), 0, (const float*)a.part, blocks, a.hd, dwq, dwk));
   return ULB_OK;
 }
 template <typename T>
-int pick_grad(Ctx* c, HeadArgs& a, bool vec, float* dwq, float* dwk) {
-  if (a.half) return vec ? launch_grad<T, true, true>(c, a, dwq, dwk) : launch_grad<T, false, true>(c, a, dwq, dwk);
-  return vec ? launch_grad<T, true, false>(c, a, dwq, dwk) : launch_grad<T, false, false>(c, a, dwq, dwk);
+int pick_grad(Ctx* c, HeadArgs& a, int wide, float* dwq, float* dwk) {
+  return a.half ? launch_grad<T, true>(c, a, wide, dwq, dwk) : launch_grad<T, false>(c, a, wide, dwq, dwk);
 }
 
 int norm_args(const char* who, const ulb_rope* r, const ulb_norm_rope_args* p, HeadArgs* a) {
@@ -238,7 +244,7 @@ int ulb_norm_rope_apply(ulb_ctx* ctx, const ulb_rope* r, const ulb_norm_rope_arg
   a.ok = k_out;
   Ctx* c = &ctx->c;
   ULB_CUDA(cudaSetDevice(c->device));
-  const bool v = wide(eb, {a.q, a.k, q_out, k_out}, a.q_row | a.q_head | a.k_row | a.k_head);
+  const int v = wide(eb, {a.q, a.k, q_out, k_out}, a.q_row | a.q_head | a.k_row | a.k_head);
   switch (p->dtype) {
     case ULB_TYPE_F32: return pick_apply<float>(c, a, v);
     case ULB_TYPE_F16: return pick_apply<__half>(c, a, v);
@@ -258,6 +264,7 @@ int ulb_norm_rope_grad(ulb_ctx* ctx, const ulb_rope* r, const ulb_norm_rope_args
   const int eb = dtype_bytes(p->dtype);
   ULB_CHECK(element_aligned(eb, {a.q, a.k, dq_out, dk_out, dq, dk}) && words_aligned({a.wq, a.wk, a.pos, dwq, dwk}), ULB_EINVAL,
             "ulb_norm_rope_grad: unaligned pointer");
+  if (a.M == 0) a.wq = a.wk = nullptr; /* nothing is read */
   a.gq = dq_out;
   a.gk = dk_out;
   a.oq = dq;
@@ -267,7 +274,7 @@ int ulb_norm_rope_grad(ulb_ctx* ctx, const ulb_rope* r, const ulb_norm_rope_args
   /* at the first call, whatever its shape, so that any later one can be captured */
   if (!c->norm_ws) ULB_CUDA(cudaMalloc((void**)&c->norm_ws, (size_t)c->n_sm * kNormBlocks * 2 * 256 * sizeof(float)));
   a.part = c->norm_ws;
-  const bool v = wide(eb, {a.q, a.k, dq_out, dk_out, dq, dk}, a.q_row | a.q_head | a.k_row | a.k_head);
+  const int v = wide(eb, {a.q, a.k, dq_out, dk_out, dq, dk}, a.q_row | a.q_head | a.k_row | a.k_head);
   switch (p->dtype) {
     case ULB_TYPE_F32: return pick_grad<float>(c, a, v, dwq, dwk);
     case ULB_TYPE_F16: return pick_grad<__half>(c, a, v, dwq, dwk);

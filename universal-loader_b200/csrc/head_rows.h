@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "quant_cache.h"
 
@@ -36,24 +37,45 @@ struct HeadArgs {
   unsigned char *kp, *vp;
 };
 
-/* four consecutive elements between memory and fp32 registers */
-template <typename T, bool VEC>
-__device__ __forceinline__ void load4(const T* p, float* v) {
-  if constexpr (!VEC) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = to_f<T>(p[i]);
+/* a lane's two runs of four elements as they lie in memory */
+template <typename T>
+struct Eight {
+  using Run = std::conditional_t<sizeof(T) == 4, float4, uint2>;
+  Run r[2];
+};
+template <typename T>
+__device__ __forceinline__ void load_run(const T* p, bool wide, typename Eight<T>::Run* r) {
+  if (wide) {
+    *r = *reinterpret_cast<const typename Eight<T>::Run*>(p);
   } else if constexpr (sizeof(T) == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(p);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    *r = make_float4(p[0], p[1], p[2], p[3]);
   } else {
-    const uint2 a = *reinterpret_cast<const uint2*>(p);
-    const float2 x = unpack2<T>(a.x), y = unpack2<T>(a.y);
-    v[0] = x.x; v[1] = x.y; v[2] = y.x; v[3] = y.y;
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+    *r = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
   }
 }
-template <typename T, bool VEC>
-__device__ __forceinline__ void store4(T* p, const float* v) {
-  if constexpr (!VEC) {
+template <typename T>
+__device__ __forceinline__ void unpack8(const Eight<T>& e, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      v[4 * i] = e.r[i].x; v[4 * i + 1] = e.r[i].y; v[4 * i + 2] = e.r[i].z; v[4 * i + 3] = e.r[i].w;
+    } else {
+      const float2 x = unpack2<T>(e.r[i].x), y = unpack2<T>(e.r[i].y);
+      v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = y.x; v[4 * i + 3] = y.y;
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ Eight<T> zero8() {
+  Eight<T> e;
+  if constexpr (sizeof(T) == 4) e.r[0] = e.r[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+  else e.r[0] = e.r[1] = make_uint2(0, 0);
+  return e;
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, bool wide, const float* v) {
+  if (!wide) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) p[i] = from_f<T>(v[i]);
   } else if constexpr (sizeof(T) == 4) {
@@ -95,20 +117,30 @@ __device__ __forceinline__ Place place_of(const HeadArgs& a, int lane) {
 struct Turn {
   float co[4], si[4];
 };
+/* the frequencies of those pairs (zero: does not turn) and which of them do */
+struct Pairs {
+  unsigned long long f[4];
+  bool turns[4];
+};
 template <bool HALF>
-__device__ __forceinline__ void turn_at(const HeadArgs& a, long long pos, const Place& at, Turn* t) {
-  const int p0 = HALF ? at.d0 : at.d0 >> 1, n = a.rot >> 1;
+__device__ __forceinline__ Pairs pairs_of(const HeadArgs& a, const Place& at) {
+  const int p0 = HALF ? at.d0 : at.d0 >> 1;
+  Pairs p;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    t->co[j] = 1.f;
-    t->si[j] = 0.f;
-    if (at.on && p0 + j < n) {
-      const unsigned long long ph = (unsigned long long)pos * a.turn[p0 + j]; /* rope.cu: modulo one turn */
-      float s, c;
-      sincospif((float)(int)(ph >> 32) * 4.656612873077393e-10f, &s, &c);
-      t->co[j] = c * a.mscale;
-      t->si[j] = s * a.mscale;
-    }
+    p.turns[j] = at.on && p0 + j < (a.rot >> 1);
+    p.f[j] = p.turns[j] ? a.turn[p0 + j] : 0;
+  }
+  return p;
+}
+__device__ __forceinline__ void turn_at(const Pairs& p, long long pos, float mscale, Turn* t) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned long long ph = (unsigned long long)pos * p.f[j]; /* rope.cu: modulo one turn */
+    float s, c;
+    sincospif((float)(int)(ph >> 32) * 4.656612873077393e-10f, &s, &c);
+    t->co[j] = p.turns[j] ? c * mscale : 1.f;
+    t->si[j] = p.turns[j] ? s * mscale : 0.f;
   }
 }
 /* sign 1: R y, -1: R^T y */
@@ -123,53 +155,69 @@ __device__ __forceinline__ void turn(const Turn& t, float sign, float (&y)[8]) {
   }
 }
 
-/* the warp's weights of its lanes' elements (NULL: ones) */
-__device__ __forceinline__ void lane_weights(const float* w, const Place& at, float (&v)[8]) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = at.on && w ? __ldg(w + (j < 4 ? at.d0 + j : at.d1 + j - 4)) : 1.f;
+/* weights of a block's heads, q's, k's and ones, in shared memory */
+struct HeadWeights {
+  float w[3][256];
+};
+__device__ __forceinline__ void load_weights(const HeadArgs& a, HeadWeights* s) {
+  for (int i = threadIdx.x; i < 256; i += kWarps * 32) {
+    s->w[0][i] = a.wq && i < a.hd ? a.wq[i] : 1.f;
+    s->w[1][i] = a.wk && i < a.hd ? a.wk[i] : 1.f;
+    s->w[2][i] = 1.f;
+  }
+  __syncthreads();
 }
-
-/* the first of a segment's heads that part `part` of a row's warps takes; the segment begins at the row's head `before` */
-__device__ __forceinline__ int part_of(int part, int before, int wpr, int hps) {
-  const int steps = (before + hps - 1) / hps % wpr;
-  return (part >= steps ? part - steps : part - steps + wpr) * hps;
+__device__ __forceinline__ void lane_weights(const HeadWeights& s, int kind, const Place& at, float (&v)[8]) {
+  const float4 x = *reinterpret_cast<const float4*>(&s.w[kind][at.d0 & 255]), y = *reinterpret_cast<const float4*>(&s.w[kind][at.d1 & 255]);
+  v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
 }
 
 /*
- * n heads at x0, `stride` elements apart, of the row that the warp is at: loaded U steps at a time, normed by
- * 1 / sqrt(mean x^2 + eps) and w, turned, and handed to out(head, whether this lane has elements of it, values).
+ * The heads of the warp's rows in steps of 32 / LPH heads, U steps (a batch) at a time; while a batch is worked on, the
+ * next one's loads are under way, past the end of the row too.  load(m, h) gives what a lane keeps of head h of row m,
+ * row(m, position) is called before the row's first batch, work(m, h, mine, kept) for every step by the whole warp;
+ * lanes that are not `mine` keep zeros.
  */
-template <typename T, int LPH, bool HALF, int U, typename Load, typename Out>
-__device__ __forceinline__ void walk_heads(const HeadArgs& a, const T* x0, long long stride, int n, int first, const Place& at, const Turn& t,
-                                           bool normed, const float (&w)[8], bool turns, Load&& load, Out&& out) {
+template <typename Kept, int LPH, int U, typename Load, typename Row, typename Work>
+__device__ __forceinline__ void walk_rows(const HeadArgs& a, int heads, bool on, Load&& load, Row&& row, Work&& work) {
   constexpr int HPS = 32 / LPH;
-  const int grp = (threadIdx.x & 31) / LPH;
-  const float inv_hd = 1.f / a.hd;
-  for (int h0 = first; h0 < n; h0 += a.wpr * HPS * U) {
-    float x[U][8];
+  const int grp = (threadIdx.x & 31) / LPH, gw = blockIdx.x * kWarps + (threadIdx.x >> 5), part = gw % a.wpr;
+  const int n_rows = gridDim.x * kWarps / a.wpr, per = HPS * a.wpr, batches = (heads + per * U - 1) / (per * U);
+  int m = gw / a.wpr, b = 0, pos = 0;
+  if (m >= a.M) return;
+  Kept now[U], next[U];
+  auto fetch = [&](int m, int b, Kept (&k)[U]) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * a.wpr * HPS + grp;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[u][j] = 0.f;
-      if (h >= n || !at.on) continue;
-      load(x0 + h * stride, x[u]);
+      const int h = (b * U + u) * per + part * HPS + grp;
+      k[u] = load(m, h, on && h < heads);
+    }
+  };
+  fetch(m, 0, now);
+  pos = a.pos[m];
+  while (true) {
+    if (b == 0) row(m, pos);
+    int m2 = m, b2 = b + 1;
+    if (b2 == batches) {
+      b2 = 0;
+      m2 += n_rows;
+    }
+    if (m2 < a.M) {
+      fetch(m2, b2, next);
+      if (b2 == 0) pos = a.pos[m2];
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (h0 + u * a.wpr * HPS >= n) break; /* the whole warp */
-      const int h = h0 + u * a.wpr * HPS + grp;
-      if (normed) {
-        float ss = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ss = __fmaf_rn(x[u][j], x[u][j], ss);
-        const float f = rsqrtf(__fmaf_rn(head_sum<LPH>(ss), inv_hd, a.eps));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[u][j] *= f * w[j];
-      }
-      if (turns) turn<HALF>(t, 1.f, x[u]);
-      out(h, h < n && at.on, x[u]);
+      const int h0 = (b * U + u) * per + part * HPS;
+      if (h0 >= heads) break; /* the whole warp */
+      work(m, h0 + grp, on && h0 + grp < heads, now[u]);
     }
+    if (m2 >= a.M) return;
+#pragma unroll
+    for (int u = 0; u < U; ++u) now[u] = next[u];
+    m = m2;
+    b = b2;
   }
 }
 

@@ -37,7 +37,6 @@
 namespace ulb {
 namespace {
 
-constexpr int KT = 32;          /* keys a tile */
 constexpr int kUnitCost = 8;    /* what a unit costs besides its tiles, in tiles */
 constexpr int kMinTiles = 24;   /* places of the line a CTA takes at least */
 constexpr float kRaise = 12.f, kGrow = 3.9f; /* weights <= 2^15.9 < 65504 */
@@ -47,10 +46,11 @@ constexpr unsigned kAll = 0xffffffffu;
 template <bool Q4, int HD, int NT>
 struct QCfg {
   static constexpr int RB = quant_row_bytes(Q4, HD), CB = quant_code_bytes(Q4, HD);
+  static constexpr int KT = 32;               /* keys a tile */
   static constexpr int STAGE = 2 * KT * RB;
-  static constexpr int W = HD == 256 ? 4 : 8; /* warps */
+  static constexpr int W = NT == 1 && (HD < 256) && (Q4 || HD == 64) ? 16 : HD == 256 ? 4 : 8; /* warps */
   static constexpr int RT = 8 * NT;           /* queries a CTA */
-  static constexpr int JD = NT == 4 ? 32 : 64; /* dims the warps join at a time */
+  static constexpr int JD = NT >= 3 ? 32 : 64; /* dims the warps join at a time */
   static constexpr int NG = HD / kGroup, KS = HD / 16;
   static constexpr int QB = NT * KS * 256, JB = W * RT * JD * 4; /* bytes of q's fragments and of the join */
   static constexpr int ROOM = (kRingBytes - QB - JB) / (W * STAGE);
@@ -87,7 +87,7 @@ struct QPiece {
   int nth;                /* pieces of this CTA before it */
 };
 
-template <int RT>
+template <int RT, int KT>
 struct QWalk {
   int at, end, base, cnt, s, n_tile, n_pass, nth;
   TreeSeq q;
@@ -176,16 +176,35 @@ __device__ __forceinline__ void row_scales(const uint8_t* p, float (&d)[NG], flo
   }
 }
 
+/* the largest size of a row's scales, 2^-24 at least: the smallest there is, and a row of zeros counts as that */
+template <bool Q4, int NG>
+__device__ __forceinline__ float row_largest(const uint8_t* p) {
+  float x = 5.9604645e-8f;
+#pragma unroll
+  for (int i = 0; i < NG; i += 2) {
+    float2 y;
+    if constexpr (Q4) {
+      const uint2 w = *reinterpret_cast<const uint2*>(p + 4 * i);
+      y = unpack2<__half>(__byte_perm(w.x, w.y, 0x5410));
+    } else {
+      y = unpack2<__half>(lds32(p + 2 * i));
+    }
+    x = max3(x, fabsf(y.x), fabsf(y.y));
+  }
+  return x;
+}
+
 template <typename T, bool Q4, int HD, int NT>
 __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
     quant_attn_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ QuantPlan p) {
   using C = QCfg<Q4, HD, NT>;
-  constexpr int W = C::W, NG = C::NG, NTH = W * 32, JD = C::JD;
+  constexpr int W = C::W, NG = C::NG, NTH = W * 32, JD = C::JD, KT = C::KT, US = KT / 16;
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ uint64_t full[W][C::NST];
   __shared__ uint8_t sh_map[W][C::NST]; /* which 16-key halves of a tile are mapped */
   __shared__ float2 sh_ml[W][C::RT];
-  __shared__ float sh_f[W][C::RT], sh_l[C::RT], sh_m[C::RT], sh_qs[C::RT], sh_qsum[NG][C::RT];
+  __shared__ float sh_f[W][C::RT], sh_l[C::RT], sh_m[C::RT], sh_qs[C::RT];
+  __shared__ __align__(8) float sh_qsum[NG][C::RT];
   __shared__ int sh_s, sh_base, sh_sum[W], sh_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* const ring = sm + warp * C::NST * C::STAGE;
@@ -201,10 +220,10 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
   pdl_trigger();
 
   /* the line's length, then this CTA's stretch and the sequence that holds its begin */
-  QWalk<C::RT> walk;
+  QWalk<C::RT, C::KT> walk;
   auto places_of = [&](int s) {
     if (s >= a.g.n_seq) return 0;
-    QWalk<C::RT> w;
+    QWalk<C::RT, C::KT> w;
     w.s = s;
     w.load(a);
     return w.cnt;
@@ -259,7 +278,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
   walk.load(a);
 
   /* ---- the warp's own tiles, copied ahead of their use and past the ends of pieces */
-  QWalk<C::RT> ahead = walk;
+  QWalk<C::RT, C::KT> ahead = walk;
   QPiece fp;
   int f_i = 0, f_n = 0, f_id0 = 0, f_id1 = 0, f_slot = 0, f_base = 0;
   bool f_more = true, ok = true;
@@ -292,7 +311,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
       const long long h = fp.kvh * a.g.head;
       uint64_t* const bar = &full[warp][f_slot];
       if (a.g.page == 16) {
-        const int r0 = id0 >= 0 ? min(rows, 16) : 0, r1 = id1 >= 0 ? rows - 16 : 0; /* rows <= 0: none */
+        const int r0 = id0 >= 0 ? min(rows, 16) : 0, r1 = KT > 16 && id1 >= 0 ? rows - 16 : 0; /* rows <= 0: none */
         sh_map[warp][f_slot] = (id0 >= 0 ? 1 : 0) | (id1 >= 0 ? 2 : 0);
         mb_expect(bar, (uint32_t)(2 * (max(r0, 0) + max(r1, 0)) * C::RB));
         if (r0 > 0) {
@@ -362,7 +381,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
     __syncthreads();
 
     float sc[NT][2], m[NT][2], l[NT][2];
-    float qs[Q4 ? NG : 1][NT][2], om[Q4 ? NG : 1][NT][2];
+    float om[Q4 ? NG : 1][NT][2];
     float o[HD / 16][NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -373,10 +392,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
         l[n][e] = 0.f;
         if constexpr (Q4) {
 #pragma unroll
-          for (int i = 0; i < NG; ++i) {
-            qs[i][n][e] = sh_qsum[i][n * 8 + 2 * t + e];
-            om[i][n][e] = 0.f;
-          }
+          for (int i = 0; i < NG; ++i) om[i][n][e] = 0.f;
         }
       }
 #pragma unroll
@@ -398,10 +414,10 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
       const uint8_t* const vt = kt + KT * C::RB;
       const int map = sh_map[warp][slot];
       const bool masked = pos0 + KT > open || map != 3;
-      float s[2][NT][4];
-      /* ---- scores of 2 x 16 keys */
+      float s[US][NT][4];
+      /* ---- scores, 16 keys at a time */
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < US; ++u) {
         const uint8_t *r0 = kt + (u * 16 + g) * C::RB, *r1 = r0 + 8 * C::RB;
         float d0[NG], d1[NG], m0[NG], m1[NG];
         row_scales<Q4, NG>(r0 + C::CB, d0, m0);
@@ -421,10 +437,11 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
             s[u][n][2] = __fmaf_rn(d1[i], c[2], s[u][n][2]);
             s[u][n][3] = __fmaf_rn(d1[i], c[3], s[u][n][3]);
             if constexpr (Q4) {
-              s[u][n][0] = __fmaf_rn(m0[i], qs[i][n][0], s[u][n][0]);
-              s[u][n][1] = __fmaf_rn(m0[i], qs[i][n][1], s[u][n][1]);
-              s[u][n][2] = __fmaf_rn(m1[i], qs[i][n][0], s[u][n][2]);
-              s[u][n][3] = __fmaf_rn(m1[i], qs[i][n][1], s[u][n][3]);
+              const float2 qs = *reinterpret_cast<const float2*>(&sh_qsum[i][n * 8 + 2 * t]);
+              s[u][n][0] = __fmaf_rn(m0[i], qs.x, s[u][n][0]);
+              s[u][n][1] = __fmaf_rn(m0[i], qs.y, s[u][n][1]);
+              s[u][n][2] = __fmaf_rn(m1[i], qs.x, s[u][n][2]);
+              s[u][n][3] = __fmaf_rn(m1[i], qs.y, s[u][n][3]);
             }
           }
         };
@@ -455,24 +472,18 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
           }
         }
       }
-      /* ---- V's scales of the lane's four keys, the logarithm of the largest */
-      float vd[2][2][NG], vm[2][2][NG], lg[2][2];
+      /* ---- the logarithm of the largest scale of each V row */
+      float lg[US][2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < US; ++u)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          row_scales<Q4, NG>(vt + (u * 16 + r * 8 + g) * C::RB + C::CB, vd[u][r], vm[u][r]);
-          float x = 5.9604645e-8f; /* 2^-24, the smallest scale there is: a row of zeros counts as that */
-#pragma unroll
-          for (int i = 0; i < NG; ++i) x = fmaxf(x, fabsf(vd[u][r][i]));
-          lg[u][r] = __log2f(x);
-        }
+        for (int r = 0; r < 2; ++r) lg[u][r] = __log2f(row_largest<Q4, NG>(vt + (u * 16 + r * 8 + g) * C::RB + C::CB));
       float top[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         top[n][0] = top[n][1] = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < US; ++u)
 #pragma unroll
           for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -487,20 +498,16 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
               top[n][e] = fmaxf(top[n][e], x + lg[u][r]);
             }
       }
-      bool grow = false;
+      bool grow = false; /* the lane's own keys; m is the same in all lanes of a query */
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(kAll, top[n][e], x));
-          grow |= top[n][e] - kRaise - kGrow > m[n][e];
-        }
+      for (int n = 0; n < NT; ++n) grow |= top[n][0] - kRaise - kGrow > m[n][0] || top[n][1] - kRaise - kGrow > m[n][1];
       if (__any_sync(kAll, grow)) { /* a row's first keys, seldom later */
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(kAll, top[n][e], x));
             const float to = top[n][e] - kRaise;
             if (to - kGrow > m[n][e]) {
               const float f = m[n][e] == -INFINITY ? 0.f : ex2(m[n][e] - to);
@@ -524,7 +531,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
         for (int e = 0; e < 2; ++e) {
           const float mm = m[n][e] == -INFINITY ? 0.f : m[n][e];
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+          for (int u = 0; u < US; ++u)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               const float x = ex2(s[u][n][2 * r + e] - mm);
@@ -534,17 +541,20 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
         }
       /* ---- o += V^T (p d), minima apart */
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < US; ++u) {
         const uint8_t* const v0 = vt + (u * 16 + 2 * t) * C::RB;
+        float vd[2][NG], vm[2][NG];
+        row_scales<Q4, NG>(vt + (u * 16 + g) * C::RB + C::CB, vd[0], vm[0]);
+        row_scales<Q4, NG>(vt + (u * 16 + 8 + g) * C::RB + C::CB, vd[1], vm[1]);
         /* weights of group i as the second operand; in a masked tile what is not seen is zero whatever its scale holds */
         auto weights = [&](int i, int n, uint32_t* b) {
           float w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float x = s[u][n][e];
-            w[e] = x * vd[u][e >> 1][i];
+            w[e] = x * vd[e >> 1][i];
             if (masked && x == 0.f) w[e] = 0.f;
-            if constexpr (Q4) om[i][n][e & 1] += masked && x == 0.f ? 0.f : x * vm[u][e >> 1][i];
+            if constexpr (Q4) om[i][n][e & 1] += masked && x == 0.f ? 0.f : x * vm[e >> 1][i];
           }
           b[0] = transpose8(h2(w[0], w[1]));
           b[1] = transpose8(h2(w[2], w[3]));
@@ -731,7 +741,7 @@ int launch_quant(Ctx* c, TreeArgs& a) {
     attr |= 1ull << (c->device & 63);
   }
   const long long units = (long long)a.g.n_seq * a.g.n_head_kv * (((long long)a.max_rows * a.G + C::RT - 1) / C::RT);
-  ULB_CHECK(units * (std::max(1, (a.max_len + KT - 1) / KT) + kUnitCost) < (1ll << 31) - 65536, ULB_EUNSUPPORTED,
+  ULB_CHECK(units * (std::max(1, (a.max_len + C::KT - 1) / C::KT) + kUnitCost) < (1ll << 31) - 65536, ULB_EUNSUPPORTED,
             "ulb_quant_attention: %d sequences of %d positions and %d rows", a.g.n_seq, a.max_len, a.max_rows);
   QuantPlan p;
   p.groups = c->n_sm;
@@ -751,7 +761,11 @@ int pick_rows(Ctx* c, TreeArgs& a) {
   const long long nq = (long long)a.max_rows * a.G;
   if (nq <= 8) return launch_quant<T, Q4, HD, 1>(c, a);
   if (nq <= 16 || HD == 256) return launch_quant<T, Q4, HD, 2>(c, a);
-  if constexpr (HD < 256) return launch_quant<T, Q4, HD, 4>(c, a);
+  if constexpr (HD < 256) {
+    const long long passes = (nq + 31) / 32;
+    if ((nq + passes - 1) / passes <= 24) return launch_quant<T, Q4, HD, 3>(c, a);
+    return launch_quant<T, Q4, HD, 4>(c, a);
+  }
   return ULB_OK;
 }
 template <typename T, bool Q4>

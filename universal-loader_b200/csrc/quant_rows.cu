@@ -129,54 +129,69 @@ __device__ __forceinline__ long long slot_place(const HeadArgs& a, int m) {
 }
 
 template <typename TI, bool Q4, int LPH, bool HALF>
-__global__ void __launch_bounds__(kWarps * 32) quant_append_kernel(const __grid_constant__ HeadArgs a, int f16, int wide_in, int wide_out) {
+__global__ void __launch_bounds__(kWarps * 32, 3) quant_append_kernel(const __grid_constant__ HeadArgs a, int f16, int wide_in, int wide_out) {
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const Place at = place_of<LPH, HALF>(a, lane);
-  const int gw = blockIdx.x * kWarps + (threadIdx.x >> 5), part = gw % a.wpr, n_rows = gridDim.x * kWarps / a.wpr;
-  float wq[8], wk[8];
-  lane_weights(a.wq, at, wq);
-  lane_weights(a.wk, at, wk);
-  const int first_k = part_of(part, a.nq, a.wpr, 32 / LPH), first_v = part_of(part, a.nq + a.nk, a.wpr, 32 / LPH);
-  auto load = [&](const TI* p, float* x) { /* the same for all threads */
-    if (wide_in) {
-      load4<TI, true>(p + at.d0, x);
-      load4<TI, true>(p + at.d1, x + 4);
-    } else {
-      load4<TI, false>(p + at.d0, x);
-      load4<TI, false>(p + at.d1, x + 4);
-    }
-  };
-  auto put = [&](auto* o, const float* y) {
-    using T = std::remove_pointer_t<decltype(o)>;
-    if (wide_out) store4<T, true>(o, y);
-    else store4<T, false>(o, y);
-  };
-  for (int m = gw / a.wpr; m < a.M; m += n_rows) {
-    Turn t;
-    turn_at<HALF>(a, a.pos[m], at, &t);
-    const long long place = slot_place(a, m);
-    walk_heads<TI, LPH, HALF, 4>(a, (const TI*)a.q + m * a.q_row, a.q_head, a.nq, part * (32 / LPH), at, t, a.wq, wq, true, load,
-                                 [&](int h, bool mine, const float (&y)[8]) {
-                                   if (!mine) return;
-                                   const long long o = ((long long)m * a.nq + h) * a.hd;
-                                   if (f16) {
-                                     put((__half*)a.oq + o + at.d0, y);
-                                     put((__half*)a.oq + o + at.d1, y + 4);
-                                   } else {
-                                     put((__nv_bfloat16*)a.oq + o + at.d0, y);
-                                     put((__nv_bfloat16*)a.oq + o + at.d1, y + 4);
-                                   }
-                                 });
-    auto cache = [&](unsigned char* pool) {
-      return [&, pool](int h, bool mine, const float (&y)[8]) {
-        quantise8<Q4, HALF>(y, mine && place >= 0 ? pool + place + (long long)h * a.g.head : nullptr, a.hd, at);
-      };
-    };
-    walk_heads<TI, LPH, HALF, 4>(a, (const TI*)a.k + m * a.k_row, a.k_head, a.nk, first_k, at, t, a.wk, wk, true, load, cache(a.kp));
-    walk_heads<TI, LPH, HALF, 4>(a, (const TI*)a.v + m * a.v_row, a.v_head, a.nv, first_v, at, t, false, wk, false, load, cache(a.vp));
-  }
+  __shared__ HeadWeights sw;
+  const Place at = place_of<LPH, HALF>(a, threadIdx.x & 31);
+  const Pairs pairs = pairs_of<HALF>(a, at);
+  const float inv_hd = 1.f / a.hd;
+  load_weights(a, &sw);
+  Turn t;
+  long long place = -1;
+  walk_rows<Eight<TI>, LPH, sizeof(TI) == 4 ? 2 : 4>(
+      a, a.nq + a.nk + a.nv, at.on,
+      [&](int m, int h, bool mine) {
+        Eight<TI> e = zero8<TI>();
+        if (mine) {
+          const TI* p = h < a.nq          ? (const TI*)a.q + m * a.q_row + h * a.q_head
+                        : h < a.nq + a.nk ? (const TI*)a.k + m * a.k_row + (h - a.nq) * a.k_head
+                                          : (const TI*)a.v + m * a.v_row + (h - a.nq - a.nk) * a.v_head;
+          load_run(p + at.d0, wide_in, &e.r[0]);
+          load_run(p + at.d1, wide_in, &e.r[1]);
+        }
+        return e;
+      },
+      [&](int m, int pos) {
+        turn_at(pairs, pos, a.mscale, &t);
+        place = slot_place(a, m);
+      },
+      [&](int m, int h, bool mine, const Eight<TI>& e) {
+        float x[8], y[8], w[8];
+        unpack8(e, x);
+        const int kind = h < a.nq ? 0 : h < a.nq + a.nk ? 1 : 2;
+        float f = 1.f;
+        if (a.wq || a.wk) { /* the same for all threads */
+          float ss = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ss = __fmaf_rn(x[j], x[j], ss);
+          ss = head_sum<LPH>(ss);
+          if (kind == 0 ? a.wq != nullptr : kind == 1 && a.wk) f = rsqrtf(__fmaf_rn(ss, inv_hd, a.eps));
+        }
+        lane_weights(sw, kind, at, w); /* ones where there are none */
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = x[j] * (f * w[j]);
+        turn<HALF>(t, 1.f, y);
+        if (kind == 2) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = x[j];
+        }
+        if (__any_sync(kAll, kind != 0)) {
+          unsigned char* const r = !mine || kind == 0 || place < 0 ? nullptr
+                                   : kind == 1 ? a.kp + place + (long long)(h - a.nq) * a.g.head
+                                               : a.vp + place + (long long)(h - a.nq - a.nk) * a.g.head;
+          quantise8<Q4, HALF>(y, r, a.hd, at);
+        }
+        if (!mine || kind != 0) return;
+        const long long o = ((long long)m * a.nq + h) * a.hd;
+        if (f16) {
+          store4((__half*)a.oq + o + at.d0, wide_out, y);
+          store4((__half*)a.oq + o + at.d1, wide_out, y + 4);
+        } else {
+          store4((__nv_bfloat16*)a.oq + o + at.d0, wide_out, y);
+          store4((__nv_bfloat16*)a.oq + o + at.d1, wide_out, y + 4);
+        }
+      });
 }
 
 /* rows read back: a warp a row (or several), a lane eight elements of a head of K or of V at a time */
@@ -219,8 +234,8 @@ __global__ void __launch_bounds__(kWarps * 32) quant_read_kernel(const __grid_co
         if constexpr (sizeof(T) == 2) {
           *reinterpret_cast<uint4*>(o) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
         } else {
-          store4<T, true>(o, x);
-          store4<T, true>(o + 4, x + 4);
+          store4(o, true, x);
+          store4(o + 4, true, x + 4);
         }
       }
     }
@@ -229,7 +244,7 @@ __global__ void __launch_bounds__(kWarps * 32) quant_read_kernel(const __grid_co
 
 template <typename TI, bool Q4, bool HALF>
 int launch_append(Ctx* c, HeadArgs& a, int f16, int wide_in, int wide_out) {
-  const int lph = lanes_of(a.hd), blocks = plan_rows(c, a, head_steps(a), c->n_sm * 8);
+  const int lph = lanes_of(a.hd), blocks = plan_rows(c, a, head_steps(a), c->n_sm * 3);
   auto go = [&](auto kern) -> int {
     ULB_LAUNCH("quant append launch", launch_k(c, kern, dim3(blocks), dim3(kWarps * 32), 0, a, f16, wide_in, wide_out));
     return ULB_OK;

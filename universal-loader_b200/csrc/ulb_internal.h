@@ -103,7 +103,7 @@ struct Ctx {
 };
 /* fp32 sum over the communicator's ranks, in place, on the context stream */
 int tp_allreduce_sum(Ctx* c, float* buf, size_t n);
-constexpr int kNormBlocks = 4; /* blocks an SM of ulb_norm_rope_grad at most */
+constexpr int kNormBlocks = 2; /* blocks an SM of ulb_norm_rope_grad at most */
 constexpr int kZeroRowHalves = 65536 + 64;
 
 /* read and clear the device error word (synchronises the stream) */
