@@ -46,13 +46,19 @@ constexpr unsigned kAll = 0xffffffffu;
 template <bool Q4, int HD, int NT>
 struct QCfg {
   static constexpr int RB = quant_row_bytes(Q4, HD), CB = quant_code_bytes(Q4, HD);
-  static constexpr int KT = 32;               /* keys a tile */
+  static constexpr int KT = 32;
   static constexpr int STAGE = 2 * KT * RB;
-  static constexpr int W = NT == 1 && (HD < 256) && (Q4 || HD == 64) ? 16 : HD == 256 ? 4 : 8; /* warps */
+#ifndef QW4
+#define QW4 16
+#define QW8 8
+#define QKT 32
+#endif
+  static constexpr int W = HD == 256 ? 4 : NT == 1 ? (Q4 ? QW4 : QW8) : 8; /* warps */
   static constexpr int RT = 8 * NT;           /* queries a CTA */
   static constexpr int JD = NT >= 3 ? 32 : 64; /* dims the warps join at a time */
   static constexpr int NG = HD / kGroup, KS = HD / 16;
-  static constexpr int QB = NT * KS * 256, JB = W * RT * JD * 4; /* bytes of q's fragments and of the join */
+  static constexpr int NW = Q4 ? NG : NG / 2, NC = (NW + 3) / 4; /* 32-bit words of a row's scales, products that take them */
+  static constexpr int QB = NT * (KS + NC) * 256, JB = W * RT * JD * 4; /* bytes of q's fragments and of the join */
   static constexpr int ROOM = (kRingBytes - QB - JB) / (W * STAGE);
   static constexpr int NST = ROOM > 6 ? 6 : ROOM;
   static constexpr int SMEM = W * NST * STAGE + QB + JB;
@@ -152,6 +158,9 @@ __device__ __forceinline__ uint32_t nib_hi(uint32_t w) {
 template <int LO> __device__ __forceinline__ uint32_t byte2(uint32_t w) {
   return sub2(__byte_perm(w, 0x64646464u, LO ? 0x4342 : 0x4140), 0x64806480u);
 }
+/* K's codes need no more than their place: the bits of a small integer n are the subnormal n 2^-24.  (V's sums run over many
+   keys, in which an offset that is taken off at the end would cost bits, so its codes are centred.) */
+template <int LO> __device__ __forceinline__ uint32_t raw2(uint32_t w) { return __byte_perm(w, 0u, LO ? 0x4342 : 0x4140); }
 
 /* scales of a row (and the middles m + 8 d, which go with codes less 8) */
 template <bool Q4, int NG>
@@ -176,22 +185,21 @@ __device__ __forceinline__ void row_scales(const uint8_t* p, float (&d)[NG], flo
   }
 }
 
-/* the largest size of a row's scales, 2^-24 at least: the smallest there is, and a row of zeros counts as that */
+/* the scales alone */
 template <bool Q4, int NG>
-__device__ __forceinline__ float row_largest(const uint8_t* p) {
-  float x = 5.9604645e-8f;
+__device__ __forceinline__ void first_scales(const uint8_t* p, float (&d)[NG]) {
 #pragma unroll
   for (int i = 0; i < NG; i += 2) {
-    float2 y;
+    float2 x;
     if constexpr (Q4) {
       const uint2 w = *reinterpret_cast<const uint2*>(p + 4 * i);
-      y = unpack2<__half>(__byte_perm(w.x, w.y, 0x5410));
+      x = make_float2(unpack2<__half>(w.x).x, unpack2<__half>(w.y).x);
     } else {
-      y = unpack2<__half>(lds32(p + 2 * i));
+      x = unpack2<__half>(lds32(p + 2 * i));
     }
-    x = max3(x, fabsf(y.x), fabsf(y.y));
+    d[i] = x.x;
+    d[i + 1] = x.y;
   }
-  return x;
 }
 
 template <typename T, bool Q4, int HD, int NT>
@@ -204,11 +212,11 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
   __shared__ uint8_t sh_map[W][C::NST]; /* which 16-key halves of a tile are mapped */
   __shared__ float2 sh_ml[W][C::RT];
   __shared__ float sh_f[W][C::RT], sh_l[C::RT], sh_m[C::RT], sh_qs[C::RT];
-  __shared__ __align__(8) float sh_qsum[NG][C::RT];
   __shared__ int sh_s, sh_base, sh_sum[W], sh_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* const ring = sm + warp * C::NST * C::STAGE;
   uint2* const qf = reinterpret_cast<uint2*>(sm + W * C::NST * C::STAGE);
+  uint2* const qc = qf + NT * C::KS * 32; /* second operands of the products with K's scales */
   float* const jb = reinterpret_cast<float*>(sm + W * C::NST * C::STAGE + C::QB);
 
   if (lane == 0) {
@@ -216,6 +224,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (tid == 0) { sh_s = 0; sh_base = 0; }
+  for (int i = tid; i < NT * C::NC * 32; i += NTH) qc[i] = make_uint2(0, 0); /* words that a row does not have */
   pdl_wait();
   pdl_trigger();
 
@@ -366,14 +375,22 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
 #pragma unroll
       for (int i = 0; i < N4; ++i) {
         const int d = (i * 32 + lane) * 4;
-        const uint32_t lo = h2(ldexpf(x[i][0], -ex), ldexpf(x[i][1], -ex)), hi = h2(ldexpf(x[i][2], -ex), ldexpf(x[i][3], -ex));
+        /* 4 bits: elements 2 and 3 of a word come as 16 n */
+        const int eh = Q4 ? -ex - 4 : -ex;
+        const uint32_t lo = h2(ldexpf(x[i][0], -ex), ldexpf(x[i][1], -ex)), hi = h2(ldexpf(x[i][2], eh), ldexpf(x[i][3], eh));
         const float2 u = unpack2<__half>(lo), v = unpack2<__half>(hi);
-        float sum = (u.x + u.y) + (v.x + v.y);
+        float sum = (u.x + u.y) + (Q4 ? 16.f : 1.f) * (v.x + v.y);
 #pragma unroll
         for (int o = 4; o; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
-        if (d < HD) {
-          qf[((qi >> 3) * C::KS + (d >> 4)) * 32 + (qi & 7) * 4 + ((d >> 2) & 3)] = make_uint2(lo, hi);
-          if ((lane & 7) == 0) sh_qsum[d >> 5][qi] = sum;
+        if (d < HD) qf[((qi >> 3) * C::KS + (d >> 4)) * 32 + (qi & 7) * 4 + ((d >> 2) & 3)] = make_uint2(lo, hi);
+        /* s has sum(q) m (4 bits), or -128 sum(q) d (codes are offset by 128), of each group: the words of a row's scales
+           as operands (d, m) or (d, d of the next), these sums in two parts beside them */
+        if (!Q4) sum *= -128.f;
+        const float next = __shfl_down_sync(kAll, sum, 8), top16 = to_f<__half>(from_f<__half>(sum)), next16 = to_f<__half>(from_f<__half>(next));
+        const int word = Q4 ? d >> 5 : d >> 6;
+        if (d < HD && d % (Q4 ? 32 : 64) == 0) {
+          const int at = ((qi >> 3) * C::NC + (word >> 2)) * 32 + (qi & 7) * 4 + (word & 3);
+          qc[at] = Q4 ? make_uint2(h2(0.f, top16), h2(0.f, sum - top16)) : make_uint2(h2(top16, next16), h2(sum - top16, next - next16));
         }
       }
       if (lane == 0) sh_qs[qi] = ldexpf(1.f, ex) * a.scale2;
@@ -414,158 +431,171 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
       const uint8_t* const vt = kt + KT * C::RB;
       const int map = sh_map[warp][slot];
       const bool masked = pos0 + KT > open || map != 3;
-      float s[US][NT][4];
-      /* ---- scores, 16 keys at a time */
-#pragma unroll
-      for (int u = 0; u < US; ++u) {
-        const uint8_t *r0 = kt + (u * 16 + g) * C::RB, *r1 = r0 + 8 * C::RB;
-        float d0[NG], d1[NG], m0[NG], m1[NG];
-        row_scales<Q4, NG>(r0 + C::CB, d0, m0);
-        row_scales<Q4, NG>(r1 + C::CB, d1, m1);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) s[u][n][0] = s[u][n][1] = s[u][n][2] = s[u][n][3] = 0.f;
-        auto group = [&](int i, const uint32_t (&a0)[4], const uint32_t (&a1)[4]) {
+#pragma unroll 1
+      for (int u = 0; u < US; ++u) { /* 16 keys at a time: half the code, which would not fit the instruction cache */
+        const uint8_t *const k0 = kt + (u * 16 + g) * C::RB, *const k1 = k0 + 8 * C::RB, *const vr = vt + (u * 16 + g) * C::RB;
+        float s[NT][4];
+        /* ---- scores: sums of codes by group, in units of 2^-24, and the part that the scales alone give */
+        {
+          float d0[NG], d1[NG];
+          first_scales<Q4, NG>(k0 + C::CB, d0);
+          first_scales<Q4, NG>(k1 + C::CB, d1);
+          float c0[NT][4];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
-            const uint2 b0 = NT == 1 ? qr[(2 * i) % (NT == 1 ? C::KS : 1)] : qf[(n * C::KS + 2 * i) * 32 + lane];
-            const uint2 b1 = NT == 1 ? qr[(2 * i + 1) % (NT == 1 ? C::KS : 1)] : qf[(n * C::KS + 2 * i + 1) * 32 + lane];
-            mma16(c, a0, b0.x, b0.y);
-            mma16(c, a1, b1.x, b1.y);
-            s[u][n][0] = __fmaf_rn(d0[i], c[0], s[u][n][0]);
-            s[u][n][1] = __fmaf_rn(d0[i], c[1], s[u][n][1]);
-            s[u][n][2] = __fmaf_rn(d1[i], c[2], s[u][n][2]);
-            s[u][n][3] = __fmaf_rn(d1[i], c[3], s[u][n][3]);
-            if constexpr (Q4) {
-              const float2 qs = *reinterpret_cast<const float2*>(&sh_qsum[i][n * 8 + 2 * t]);
-              s[u][n][0] = __fmaf_rn(m0[i], qs.x, s[u][n][0]);
-              s[u][n][1] = __fmaf_rn(m0[i], qs.y, s[u][n][1]);
-              s[u][n][2] = __fmaf_rn(m1[i], qs.x, s[u][n][2]);
-              s[u][n][3] = __fmaf_rn(m1[i], qs.y, s[u][n][3]);
+            s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+            c0[n][0] = c0[n][1] = c0[n][2] = c0[n][3] = 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < C::NC; ++i) {
+            uint32_t f[4] = {0, 0, 0, 0};
+            if (C::NW % 4 == 0 || i * 4 + t < C::NW) {
+              f[0] = f[2] = lds32(k0 + C::CB + i * 16 + 4 * t);
+              f[1] = f[3] = lds32(k1 + C::CB + i * 16 + 4 * t);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint2 y = qc[(n * C::NC + i) * 32 + lane];
+              mma16(c0[n], f, y.x, y.y);
             }
           }
-        };
-        if constexpr (Q4) {
+          auto group = [&](int i, const uint32_t (&a0)[4], const uint32_t (&a1)[4]) {
 #pragma unroll
-          for (int i = 0; i < NG; i += 2) {
-            const int at = i * 16 + 4 * t;
-            uint32_t x0 = lds32(r0 + at), x1 = lds32(r1 + at), y0 = lds32(r0 + at + 16), y1 = lds32(r1 + at + 16);
-            {
-              const uint32_t f0[4] = {nib_lo(x0), nib_lo(x1), nib_hi(x0), nib_hi(x1)}, f1[4] = {nib_lo(y0), nib_lo(y1), nib_hi(y0), nib_hi(y1)};
+            for (int n = 0; n < NT; ++n) {
+              float c[4] = {0.f, 0.f, 0.f, 0.f};
+              const uint2 b0 = NT == 1 ? qr[(2 * i) % (NT == 1 ? C::KS : 1)] : qf[(n * C::KS + 2 * i) * 32 + lane];
+              const uint2 b1 = NT == 1 ? qr[(2 * i + 1) % (NT == 1 ? C::KS : 1)] : qf[(n * C::KS + 2 * i + 1) * 32 + lane];
+              mma16(c, a0, b0.x, b0.y);
+              mma16(c, a1, b1.x, b1.y);
+              s[n][0] = __fmaf_rn(d0[i], c[0], s[n][0]);
+              s[n][1] = __fmaf_rn(d0[i], c[1], s[n][1]);
+              s[n][2] = __fmaf_rn(d1[i], c[2], s[n][2]);
+              s[n][3] = __fmaf_rn(d1[i], c[3], s[n][3]);
+            }
+          };
+          if constexpr (Q4) {
+#pragma unroll
+            for (int i = 0; i < NG; i += 2) {
+              const int at = i * 16 + 4 * t;
+              uint32_t x0 = lds32(k0 + at), x1 = lds32(k1 + at), y0 = lds32(k0 + at + 16), y1 = lds32(k1 + at + 16);
+              constexpr uint32_t L = 0x000f000fu, H = 0x00f000f0u;
+              {
+                const uint32_t f0[4] = {x0 & L, x1 & L, x0 & H, x1 & H}, f1[4] = {y0 & L, y1 & L, y0 & H, y1 & H};
+                group(i, f0, f1);
+              }
+              x0 >>= 8; x1 >>= 8; y0 >>= 8; y1 >>= 8;
+              {
+                const uint32_t f0[4] = {x0 & L, x1 & L, x0 & H, x1 & H}, f1[4] = {y0 & L, y1 & L, y0 & H, y1 & H};
+                group(i + 1, f0, f1);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+              const int at = i * 32 + 4 * t;
+              const uint32_t x0 = lds32(k0 + at) ^ 0x80808080u, x1 = lds32(k1 + at) ^ 0x80808080u, y0 = lds32(k0 + at + 16) ^ 0x80808080u,
+                             y1 = lds32(k1 + at + 16) ^ 0x80808080u;
+              const uint32_t f0[4] = {raw2<0>(x0), raw2<0>(x1), raw2<1>(x0), raw2<1>(x1)}, f1[4] = {raw2<0>(y0), raw2<0>(y1), raw2<1>(y0), raw2<1>(y1)};
               group(i, f0, f1);
             }
-            x0 >>= 8; x1 >>= 8; y0 >>= 8; y1 >>= 8;
-            {
-              const uint32_t f0[4] = {nib_lo(x0), nib_lo(x1), nib_hi(x0), nib_hi(x1)}, f1[4] = {nib_lo(y0), nib_lo(y1), nib_hi(y0), nib_hi(y1)};
-              group(i + 1, f0, f1);
-            }
           }
-        } else {
 #pragma unroll
-          for (int i = 0; i < NG; ++i) {
-            const int at = i * 32 + 4 * t;
-            const uint32_t x0 = lds32(r0 + at) ^ 0x80808080u, x1 = lds32(r1 + at) ^ 0x80808080u, y0 = lds32(r0 + at + 16) ^ 0x80808080u,
-                           y1 = lds32(r1 + at + 16) ^ 0x80808080u;
-            const uint32_t f0[4] = {byte2<0>(x0), byte2<0>(x1), byte2<1>(x0), byte2<1>(x1)},
-                           f1[4] = {byte2<0>(y0), byte2<0>(y1), byte2<1>(y0), byte2<1>(y1)};
-            group(i, f0, f1);
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = __fmaf_rn(s[n][e], 16777216.f, c0[n][e]);
+        }
+        /* ---- V's scales and middles, the logarithm of each row's largest scale */
+        float vd[2][NG], vm[2][NG], lg[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          row_scales<Q4, NG>(vr + r * 8 * C::RB + C::CB, vd[r], vm[r]);
+          float x = 5.9604645e-8f; /* 2^-24, the smallest scale there is: a row of zeros counts as that */
+#pragma unroll
+          for (int i = 0; i < NG; i += 2) x = max3(x, vd[r][i], vd[r][i + 1]);
+          lg[r] = __log2f(x);
+        }
+        uint32_t seen[NT][2]; /* of both queries of key g and of key g + 8, as a mask on packed weights */
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          seen[n][0] = seen[n][1] = 0xffffffffu;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] *= sc[n][e & 1];
+        }
+        if (masked) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int pos = pos0 + u * 16 + (e >> 1) * 8 + g, qi = pc.q0 + n * 8 + 2 * t + (e & 1);
+              const bool see = (map >> u & 1) && pos < pc.q.len && qi < pc.q0 + pc.nq && (pos < open || tree_sees(a, pc.q, qi / a.G, pos));
+              if (!see) {
+                s[n][e] = -INFINITY;
+                seen[n][e >> 1] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+              }
+            }
+          if constexpr (Q4) { /* a group that is not finite is so in its scale */
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int i = 0; i < NG; ++i)
+                if (!isfinite(vm[r][i])) vm[r][i] = 0.f;
           }
         }
-      }
-      /* ---- the logarithm of the largest scale of each V row */
-      float lg[US][2];
-#pragma unroll
-      for (int u = 0; u < US; ++u)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) lg[u][r] = __log2f(row_largest<Q4, NG>(vt + (u * 16 + r * 8 + g) * C::RB + C::CB));
-      float top[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        top[n][0] = top[n][1] = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < US; ++u)
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float x = s[u][n][2 * r + e] * sc[n][e];
-              if (masked) {
-                const int pos = pos0 + u * 16 + r * 8 + g, qi = pc.q0 + n * 8 + 2 * t + e;
-                const bool see = (map >> u & 1) && pos < pc.q.len && qi < pc.q0 + pc.nq && (pos < open || tree_sees(a, pc.q, qi / a.G, pos));
-                if (!see) x = -INFINITY;
-              }
-              s[u][n][2 * r + e] = x;
-              top[n][e] = fmaxf(top[n][e], x + lg[u][r]);
-            }
-      }
-      bool grow = false; /* the lane's own keys; m is the same in all lanes of a query */
-#pragma unroll
-      for (int n = 0; n < NT; ++n) grow |= top[n][0] - kRaise - kGrow > m[n][0] || top[n][1] - kRaise - kGrow > m[n][1];
-      if (__any_sync(kAll, grow)) { /* a row's first keys, seldom later */
+        float top[NT][2];
+        bool grow = false; /* by the lane's own keys; m is the same in all lanes of a query */
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(kAll, top[n][e], x));
-            const float to = top[n][e] - kRaise;
-            if (to - kGrow > m[n][e]) {
-              const float f = m[n][e] == -INFINITY ? 0.f : ex2(m[n][e] - to);
-              m[n][e] = to;
-              l[n][e] *= f;
-#pragma unroll
-              for (int i = 0; i < HD / 16; ++i) {
-                o[i][n][e] *= f;
-                o[i][n][2 + e] *= f;
-              }
-              if constexpr (Q4) {
-#pragma unroll
-                for (int i = 0; i < NG; ++i) om[i][n][e] *= f;
-              }
-            }
+            top[n][e] = fmaxf(s[n][e] + lg[0], s[n][2 + e] + lg[1]);
+            grow |= top[n][e] - kRaise - kGrow > m[n][e];
           }
-      }
+        if (__any_sync(kAll, grow)) { /* a row's first keys, seldom later */
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float mm = m[n][e] == -INFINITY ? 0.f : m[n][e];
+            for (int e = 0; e < 2; ++e) {
 #pragma unroll
-          for (int u = 0; u < US; ++u)
+              for (int x = 4; x < 32; x <<= 1) top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(kAll, top[n][e], x));
+              const float to = top[n][e] - kRaise;
+              if (to - kGrow > m[n][e]) {
+                const float f = m[n][e] == -INFINITY ? 0.f : ex2(m[n][e] - to);
+                m[n][e] = to;
+                l[n][e] *= f;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const float x = ex2(s[u][n][2 * r + e] - mm);
-              s[u][n][2 * r + e] = x;
-              l[n][e] += x;
+                for (int i = 0; i < HD / 16; ++i) {
+                  o[i][n][e] *= f;
+                  o[i][n][2 + e] *= f;
+                }
+                if constexpr (Q4) {
+#pragma unroll
+                  for (int i = 0; i < NG; ++i) om[i][n][e] *= f;
+                }
+              }
             }
         }
-      /* ---- o += V^T (p d), minima apart */
 #pragma unroll
-      for (int u = 0; u < US; ++u) {
-        const uint8_t* const v0 = vt + (u * 16 + 2 * t) * C::RB;
-        float vd[2][NG], vm[2][NG];
-        row_scales<Q4, NG>(vt + (u * 16 + g) * C::RB + C::CB, vd[0], vm[0]);
-        row_scales<Q4, NG>(vt + (u * 16 + 8 + g) * C::RB + C::CB, vd[1], vm[1]);
-        /* weights of group i as the second operand; in a masked tile what is not seen is zero whatever its scale holds */
-        auto weights = [&](int i, int n, uint32_t* b) {
-          float w[4];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = s[u][n][e];
-            w[e] = x * vd[e >> 1][i];
-            if (masked && x == 0.f) w[e] = 0.f;
-            if constexpr (Q4) om[i][n][e & 1] += masked && x == 0.f ? 0.f : x * vm[e >> 1][i];
+          for (int e = 0; e < 2; ++e) {
+            const float mm = m[n][e] == -INFINITY ? 0.f : m[n][e];
+            s[n][e] = ex2(s[n][e] - mm);
+            s[n][2 + e] = ex2(s[n][2 + e] - mm);
+            l[n][e] += s[n][e] + s[n][2 + e];
           }
-          b[0] = transpose8(h2(w[0], w[1]));
-          b[1] = transpose8(h2(w[2], w[3]));
-        };
+        /* ---- o += V^T (p d), middles apart */
+        const uint8_t* const v0 = vt + (u * 16 + 2 * t) * C::RB;
         auto product = [&](int i, const uint32_t (&f0)[4], const uint32_t (&f1)[4]) {
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            uint32_t b[2];
-            weights(i, n, b);
-            mma16(o[2 * i][n], f0, b[0], b[1]);
-            mma16(o[2 * i + 1][n], f1, b[0], b[1]);
+            if constexpr (Q4) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) om[i][n][e] = __fmaf_rn(s[n][2 + e], vm[1][i], __fmaf_rn(s[n][e], vm[0][i], om[i][n][e]));
+            }
+            const uint32_t b0 = transpose8(h2(s[n][0] * vd[0][i], s[n][1] * vd[0][i]) & seen[n][0]),
+                           b1 = transpose8(h2(s[n][2] * vd[1][i], s[n][3] * vd[1][i]) & seen[n][1]);
+            mma16(o[2 * i][n], f0, b0, b1);
+            mma16(o[2 * i + 1][n], f1, b0, b1);
           }
         };
         if constexpr (Q4) {
