@@ -599,7 +599,14 @@ def test_what_is_not_seen_never_touches_a_result(tctx, fmt):
     bad = torch.zeros(6, H, D, dtype=torch.bool, device="cuda")
     bad[4:, :H // KV, :32] = True
     assert torch.isnan(got[bad]).all()
-    assert torch.equal(got[~bad], want[~bad])
+    # the other elements of the rows that see the key: its weights are taken against the largest scale that it has left, so the
+    # weights of both calls may round differently, each by 2^-11 of a term, and their outputs by half a step
+    rest = ~bad
+    rest[4:, :H // KV, 32:] = False
+    assert torch.equal(got[rest], want[rest])
+    mag = attend64(fmt, q.double().cpu().numpy(), kp, vp, table, page, D, [0, 6], [n - 6], [n], bits, 0.1)[2][4:, :H // KV, 32:]
+    a, b = (x[4:, :H // KV, 32:].double().cpu().numpy() for x in (got, want))
+    assert (np.abs(a - b) <= 2 * 2.0 ** -11 * (mag + np.abs(b))).all()
 
 
 @pytest.mark.parametrize("fmt", ["q8", "q4"])

@@ -37,8 +37,11 @@
 namespace ulb {
 namespace {
 
-constexpr int kUnitCost = 8;    /* what a unit costs besides its tiles, in tiles */
-constexpr int kMinTiles = 24;   /* places of the line a CTA takes at least */
+#ifndef QUC
+#define QUC 32
+#endif
+constexpr int kUnitCost = QUC;    /* what a unit costs besides its tiles, in tiles */
+constexpr int kMinTiles = 48;   /* places of the line a CTA takes at least */
 constexpr float kRaise = 12.f, kGrow = 3.9f; /* weights <= 2^15.9 < 65504 */
 constexpr int kRingBytes = 212 * 1024;
 constexpr unsigned kAll = 0xffffffffu;
@@ -49,20 +52,22 @@ struct QCfg {
   static constexpr int KT = 32;
   static constexpr int STAGE = 2 * KT * RB;
 #ifndef QW4
-#define QW4 16
-#define QW8 8
-#define QKT 32
+#define QW4 11
+#define QJD 128
+#define QREG 1
 #endif
-  static constexpr int W = HD == 256 ? 4 : NT == 1 ? (Q4 ? QW4 : QW8) : 8; /* warps */
+  /* warps that work, with the copying one a multiple of four: registers are given out so */
+  static constexpr int W = HD == 256 ? (Q4 ? 7 : 3) : NT == 1 ? (HD == 64 ? 15 : Q4 ? QW4 : 7) : HD == 64 && NT < 4 ? 11 : 7;
   static constexpr int RT = 8 * NT;           /* queries a CTA */
-  static constexpr int JD = NT >= 3 ? 32 : 64; /* dims the warps join at a time */
+  static constexpr int JD = NT >= 3 ? 32 : NT == 2 || HD == 64 ? 64 : QJD; /* dims the warps join at a time */
   static constexpr int NG = HD / kGroup, KS = HD / 16;
   static constexpr int NW = Q4 ? NG : NG / 2, NC = (NW + 3) / 4; /* 32-bit words of a row's scales, products that take them */
-  static constexpr int QB = NT * (KS + NC) * 256, JB = W * RT * JD * 4; /* bytes of q's fragments and of the join */
+  static constexpr int QB = 2 * NT * (KS + NC) * 256, JB = W * RT * JD * 4; /* bytes of two units' fragments of q and of the join */
+  static constexpr int QS = QB / 2 / 8;       /* 8-byte words of one unit's */
   static constexpr int ROOM = (kRingBytes - QB - JB) / (W * STAGE);
   static constexpr int NST = ROOM > 6 ? 6 : ROOM;
   static constexpr int SMEM = W * NST * STAGE + QB + JB;
-  static_assert(NST >= 2 && SMEM <= 222 * 1024, "shared memory");
+  static_assert(NST >= 2 && SMEM <= 222 * 1024 && W <= 31, "shared memory, a lane a ring");
 };
 
 struct QuantPlan {
@@ -203,28 +208,31 @@ __device__ __forceinline__ void first_scales(const uint8_t* p, float (&d)[NG]) {
 }
 
 template <typename T, bool Q4, int HD, int NT>
-__global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
+__global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32 + 32, 1)
     quant_attn_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ QuantPlan p) {
   using C = QCfg<Q4, HD, NT>;
-  constexpr int W = C::W, NG = C::NG, NTH = W * 32, JD = C::JD, KT = C::KT, US = KT / 16;
+  constexpr int W = C::W, NG = C::NG, NTH = W * 32 + 32, JD = C::JD, KT = C::KT, US = KT / 16;
   extern __shared__ __align__(128) uint8_t sm[];
-  __shared__ uint64_t full[W][C::NST];
+  __shared__ uint64_t full[W][C::NST], empty[W][C::NST];
   __shared__ uint8_t sh_map[W][C::NST]; /* which 16-key halves of a tile are mapped */
-  __shared__ float2 sh_ml[W][C::RT];
-  __shared__ float sh_f[W][C::RT], sh_l[C::RT], sh_m[C::RT], sh_qs[C::RT];
-  __shared__ int sh_s, sh_base, sh_sum[W], sh_last;
+  __shared__ float2 sh_ml[2][W][C::RT];
+  __shared__ float sh_qs[2][C::RT];
+  __shared__ QWalk<C::RT, C::KT> sh_walk;
+  __shared__ QPiece sh_pc[4];
+  __shared__ int sh_have[4], sh_s, sh_base, sh_sum[W + 1], sh_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* const ring = sm + warp * C::NST * C::STAGE;
-  uint2* const qf = reinterpret_cast<uint2*>(sm + W * C::NST * C::STAGE);
-  uint2* const qc = qf + NT * C::KS * 32; /* second operands of the products with K's scales */
+  uint2* const q_sm = reinterpret_cast<uint2*>(sm + W * C::NST * C::STAGE);
   float* const jb = reinterpret_cast<float*>(sm + W * C::NST * C::STAGE + C::QB);
 
-  if (lane == 0) {
-    for (int i = 0; i < C::NST; ++i) mb_init(&full[warp][i], 1);
+  if (lane == 0 && warp < W) {
+    for (int i = 0; i < C::NST; ++i) {
+      mb_init(&full[warp][i], 1);
+      mb_init(&empty[warp][i], 1);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (tid == 0) { sh_s = 0; sh_base = 0; }
-  for (int i = tid; i < NT * C::NC * 32; i += NTH) qc[i] = make_uint2(0, 0); /* words that a row does not have */
+  for (int i = tid; i < 2 * C::QS; i += NTH) q_sm[i] = make_uint2(0, 0); /* scales that a row does not have */
   pdl_wait();
   pdl_trigger();
 
@@ -246,7 +254,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
   QLine line;
   line.total = 0;
 #pragma unroll
-  for (int w = 0; w < W; ++w) line.total += sh_sum[w];
+  for (int w = 0; w <= W; ++w) line.total += sh_sum[w];
   line.cut(max(1, min(p.groups, (line.total + p.min_tiles - 1) / p.min_tiles)));
   const int grp_id = blockIdx.x;
   walk.at = grp_id < line.groups ? line.begin(grp_id) : line.total;
@@ -266,7 +274,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
       __syncthreads();
       int all = 0;
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
+      for (int w = 0; w <= W; ++w) {
         if (w < warp) x += sh_sum[w];
         all += sh_sum[w];
       }
@@ -286,84 +294,112 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
   walk.nth = 0;
   walk.load(a);
 
-  /* ---- the warp's own tiles, copied ahead of their use and past the ends of pieces */
-  QWalk<C::RT, C::KT> ahead = walk;
-  QPiece fp;
-  int f_i = 0, f_n = 0, f_id0 = 0, f_id1 = 0, f_slot = 0, f_base = 0;
-  bool f_more = true, ok = true;
-  const uint8_t* const kb = (const uint8_t*)a.k;
-  const uint8_t* const vb = (const uint8_t*)a.v;
-  auto page_at = [&](int s, int pos, int len) {
-    const int j = pos >> a.g.page_shift;
-    const int x = pos < len && j < a.g.max_pages ? a.table[(long long)s * a.g.max_pages + j] : -1;
-    return x >= 0 && x < a.g.n_pages ? x : -1;
-  };
-  auto feed = [&]() { /* the next tile into slot f_slot, which nobody reads any more */
-    while (f_more && f_i >= f_n) {
-      f_more = ahead.next(a, &fp);
-      f_i = 0;
-      f_n = f_more ? (fp.n + W - 1 - warp) / W : 0;
-      f_base = -32;
-    }
-    if (!f_more) return;
-    if (f_i >= f_base + 32) { /* the pages of the next 32 tiles, a tile a lane */
-      f_base = f_i;
-      const int pos = (fp.t0 + warp + (f_i + lane) * W) * KT;
-      const bool in = f_i + lane < f_n;
-      f_id0 = in ? page_at(fp.s, pos, fp.q.len) : -1;
-      f_id1 = in && a.g.page == 16 ? page_at(fp.s, pos + 16, fp.q.len) : f_id0;
-    }
-    const int id0 = __shfl_sync(kAll, f_id0, f_i - f_base), id1 = __shfl_sync(kAll, f_id1, f_i - f_base);
-    if (lane == 0) {
-      const int pos = (fp.t0 + warp + f_i * W) * KT, rows = min(KT, fp.q.len - pos), in = pos & (a.g.page - 1);
-      uint8_t* const d = ring + f_slot * C::STAGE;
-      const long long h = fp.kvh * a.g.head;
-      uint64_t* const bar = &full[warp][f_slot];
-      if (a.g.page == 16) {
-        const int r0 = id0 >= 0 ? min(rows, 16) : 0, r1 = KT > 16 && id1 >= 0 ? rows - 16 : 0; /* rows <= 0: none */
-        sh_map[warp][f_slot] = (id0 >= 0 ? 1 : 0) | (id1 >= 0 ? 2 : 0);
-        mb_expect(bar, (uint32_t)(2 * (max(r0, 0) + max(r1, 0)) * C::RB));
-        if (r0 > 0) {
-          bulk_copy(d, kb + id0 * a.g.pstride + h, r0 * C::RB, bar);
-          bulk_copy(d + KT * C::RB, vb + id0 * a.g.pstride + h, r0 * C::RB, bar);
-        }
-        if (r1 > 0) {
-          bulk_copy(d + 16 * C::RB, kb + id1 * a.g.pstride + h, r1 * C::RB, bar);
-          bulk_copy(d + (KT + 16) * C::RB, vb + id1 * a.g.pstride + h, r1 * C::RB, bar);
-        }
-      } else {
-        const int r = id0 >= 0 ? max(rows, 0) : 0;
-        sh_map[warp][f_slot] = id0 >= 0 ? 3 : 0;
-        mb_expect(bar, (uint32_t)(2 * r * C::RB));
-        if (r > 0) {
-          const long long off = id0 * a.g.pstride + h + (long long)in * C::RB;
-          bulk_copy(d, kb + off, r * C::RB, bar);
-          bulk_copy(d + KT * C::RB, vb + off, r * C::RB, bar);
+  if (warp == W) {
+    /* ------------------------------------------------ the copying warp: a lane feeds a working warp's ring, ahead of its
+       use and past the ends of pieces */
+    const uint8_t* const kb = (const uint8_t*)a.k;
+    const uint8_t* const vb = (const uint8_t*)a.v;
+    uint8_t* const ring = sm + min(lane, W - 1) * C::NST * C::STAGE;
+    uint64_t *const f_bar = full[min(lane, W - 1)], *const e_bar = empty[min(lane, W - 1)];
+    int slot = 0;
+    uint32_t phase = 1; /* the first round passes */
+    bool ok = true;
+    QPiece pc;
+    __syncthreads(); /* with the working warps' first */
+    while (ok && walk.next(a, &pc)) {
+      auto page_at = [&](int pos) {
+        const int j = pos >> a.g.page_shift;
+        const int x = pos < pc.q.len && j < a.g.max_pages ? a.table[(long long)pc.s * a.g.max_pages + j] : -1;
+        return x >= 0 && x < a.g.n_pages ? x : -1;
+      };
+      const long long h = pc.kvh * a.g.head;
+      const int in_page = a.g.page - 1;
+      int id0 = -1, id1 = -1;
+      auto ids = [&](int i) { /* the pages of tile i, read a round ahead */
+        const int pos = (pc.t0 + i) * KT;
+        const bool mine = lane < W && i < pc.n;
+        id0 = mine ? page_at(pos) : -1;
+        id1 = mine && a.g.page == 16 && KT > 16 ? page_at(pos + 16) : id0;
+      };
+      ids(lane);
+      for (int i0 = 0; i0 < pc.n && ok; i0 += W) {
+        const int i = i0 + lane, p0 = id0, p1 = id1;
+        const bool mine = lane < W && i < pc.n;
+        if (i0 + W < pc.n) ids(i + W);
+        if (mine) ok = mb_wait(&e_bar[slot], phase);
+        ok = __all_sync(kAll, ok);
+        if (mine && ok) {
+          const int pos = (pc.t0 + i) * KT, rows = min(KT, pc.q.len - pos);
+          uint8_t* const d = ring + slot * C::STAGE;
+          uint64_t* const bar = &f_bar[slot];
+          if (a.g.page == 16) {
+            const int r0 = p0 >= 0 ? min(rows, 16) : 0, r1 = KT > 16 && p1 >= 0 ? rows - 16 : 0; /* rows <= 0: none */
+            sh_map[lane][slot] = (p0 >= 0 ? 1 : 0) | (p1 >= 0 ? 2 : 0);
+            mb_expect(bar, (uint32_t)(2 * (max(r0, 0) + max(r1, 0)) * C::RB));
+            if (r0 > 0) {
+              bulk_copy(d, kb + p0 * a.g.pstride + h, r0 * C::RB, bar);
+              bulk_copy(d + KT * C::RB, vb + p0 * a.g.pstride + h, r0 * C::RB, bar);
+            }
+            if (r1 > 0) {
+              bulk_copy(d + 16 * C::RB, kb + p1 * a.g.pstride + h, r1 * C::RB, bar);
+              bulk_copy(d + (KT + 16) * C::RB, vb + p1 * a.g.pstride + h, r1 * C::RB, bar);
+            }
+          } else {
+            const int r = p0 >= 0 ? max(rows, 0) : 0;
+            sh_map[lane][slot] = p0 >= 0 ? 3 : 0;
+            mb_expect(bar, (uint32_t)(2 * r * C::RB));
+            if (r > 0) {
+              const long long off = p0 * a.g.pstride + h + (long long)(pos & in_page) * C::RB;
+              bulk_copy(d, kb + off, r * C::RB, bar);
+              bulk_copy(d + KT * C::RB, vb + off, r * C::RB, bar);
+            }
+          }
+          if (++slot == C::NST) { slot = 0; phase ^= 1; }
         }
       }
     }
+    /* no copy is in flight when the CTA ends: the working warps wait for all of them, and this one where they gave up */
+    if (!ok) {
+      for (int i = 0; i < C::NST; ++i) mb_wait(&f_bar[i], phase ^ (i < slot ? 0u : 1u));
+      if (lane == 0) atomicOr(a.err, 8);
+    }
+    return;
+  }
+  /* ------------------------------------------------ the working warps */
+  uint8_t* const ring = sm + warp * C::NST * C::STAGE;
+  bool ok = true;
+  /* piece k is in place k % 4; warp 0 looks for piece k + 2 at the end of piece k */
+  auto advance = [&](int k) {
+    QWalk<C::RT, C::KT> w = sh_walk;
+    QPiece x;
+    const bool more = w.next(a, &x);
     __syncwarp();
-    ++f_i;
-    if (++f_slot == C::NST) f_slot = 0;
+    if (lane == 0) {
+      sh_walk = w;
+      sh_pc[k & 3] = x;
+      sh_have[k & 3] = more;
+    }
+    __syncwarp();
   };
-  for (int i = 0; i < C::NST; ++i) feed();
-
   int slot = 0;
   uint32_t phase = 0;
-  QPiece pc;
-  while (walk.next(a, &pc)) {
-    /* ---- rows of q: scaled by a power of two, as fragments; sums of the groups */
+  auto sync_work = [] { asm volatile("bar.sync 1, %0;" ::"n"(W * 32) : "memory"); };
+  /* rows of q: scaled by a power of two, as fragments; sums of the groups.  Two buffers: a unit's rows are made while the
+     warps before it still work */
+  auto load_q = [&](const QPiece& c, int buf) {
+    uint2* const qb = q_sm + buf * C::QS;
+    uint2* const qc = qb + NT * C::KS * 32; /* second operands of the products with K's scales */
     for (int qi = warp; qi < C::RT; qi += W) {
       constexpr int N4 = HD / 128 > 0 ? HD / 128 : 1; /* runs of four elements a lane */
       float x[N4][4];
       float top = 0.f;
-      const int gq = pc.q0 + qi;
-      const T* src = (const T*)a.q + ((long long)(pc.q.r0 + gq / a.G) * a.H + pc.kvh * a.G + gq % a.G) * HD;
+      const int gq = c.q0 + qi;
+      const T* src = (const T*)a.q + ((long long)(c.q.r0 + gq / a.G) * a.H + c.kvh * a.G + gq % a.G) * HD;
 #pragma unroll
       for (int i = 0; i < N4; ++i) {
         const int d = (i * 32 + lane) * 4;
         uint2 w = make_uint2(0, 0);
-        if (qi < pc.nq && d < HD) w = *reinterpret_cast<const uint2*>(src + d);
+        if (qi < c.nq && d < HD) w = *reinterpret_cast<const uint2*>(src + d);
         const float2 u = unpack2<T>(w.x), v = unpack2<T>(w.y);
         x[i][0] = u.x; x[i][1] = u.y; x[i][2] = v.x; x[i][3] = v.y;
 #pragma unroll
@@ -382,7 +418,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
         float sum = (u.x + u.y) + (Q4 ? 16.f : 1.f) * (v.x + v.y);
 #pragma unroll
         for (int o = 4; o; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
-        if (d < HD) qf[((qi >> 3) * C::KS + (d >> 4)) * 32 + (qi & 7) * 4 + ((d >> 2) & 3)] = make_uint2(lo, hi);
+        if (d < HD) qb[((qi >> 3) * C::KS + (d >> 4)) * 32 + (qi & 7) * 4 + ((d >> 2) & 3)] = make_uint2(lo, hi);
         /* s has sum(q) m (4 bits), or -128 sum(q) d (codes are offset by 128), of each group: the words of a row's scales
            as operands (d, m) or (d, d of the next), these sums in two parts beside them */
         if (!Q4) sum *= -128.f;
@@ -393,10 +429,23 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
           qc[at] = Q4 ? make_uint2(h2(0.f, top16), h2(0.f, sum - top16)) : make_uint2(h2(top16, next16), h2(sum - top16, next - next16));
         }
       }
-      if (lane == 0) sh_qs[qi] = ldexpf(1.f, ex) * a.scale2;
+      if (lane == 0) sh_qs[buf][qi] = ldexpf(1.f, ex) * a.scale2;
     }
-    __syncthreads();
-
+  };
+  if (warp == 0) {
+    if (lane == 0) sh_walk = walk;
+    __syncwarp();
+    advance(0);
+    advance(1);
+  }
+  __syncthreads();
+  if (sh_have[0]) load_q(sh_pc[0], 0); /* the stretch may hold no tile */
+  sync_work();
+  for (int k = 0; sh_have[k & 3]; ++k) {
+    const int buf = k & 1;
+    const QPiece& pc = sh_pc[k & 3];
+    const uint2* const qf = q_sm + buf * C::QS;
+    const uint2* const qc = qf + NT * C::KS * 32;
     float sc[NT][2], m[NT][2], l[NT][2];
     float om[Q4 ? NG : 1][NT][2];
     float o[HD / 16][NT][4];
@@ -404,7 +453,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        sc[n][e] = sh_qs[n * 8 + 2 * t + e];
+        sc[n][e] = sh_qs[buf][n * 8 + 2 * t + e];
         m[n][e] = -INFINITY;
         l[n][e] = 0.f;
         if constexpr (Q4) {
@@ -417,15 +466,16 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
 #pragma unroll
       for (int n = 0; n < NT; ++n) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
     const int open = min(tree_open(a, pc.q), pc.q.len);
-    uint2 qr[NT == 1 ? C::KS : 1];
-    if constexpr (NT == 1) {
+    constexpr bool QR = NT == 1 && QREG; /* fragments of q in registers */
+    uint2 qr[QR ? C::KS : 1];
+    if constexpr (QR) {
 #pragma unroll
       for (int i = 0; i < C::KS; ++i) qr[i] = qf[i * 32 + lane];
     }
 
-    const int n_own = (pc.n + W - 1 - warp) / W;
+    const int n_own = (pc.n + W - 1 - warp) / W, first = (pc.t0 + warp) * KT;
     for (int it = 0; it < n_own && ok; ++it) {
-      const int pos0 = (pc.t0 + warp + it * W) * KT;
+      const int pos0 = first + it * W * KT;
       if (!mb_wait_warp(&full[warp][slot], phase)) { ok = false; break; }
       const uint8_t* const kt = ring + slot * C::STAGE;
       const uint8_t* const vt = kt + KT * C::RB;
@@ -463,8 +513,8 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               float c[4] = {0.f, 0.f, 0.f, 0.f};
-              const uint2 b0 = NT == 1 ? qr[(2 * i) % (NT == 1 ? C::KS : 1)] : qf[(n * C::KS + 2 * i) * 32 + lane];
-              const uint2 b1 = NT == 1 ? qr[(2 * i + 1) % (NT == 1 ? C::KS : 1)] : qf[(n * C::KS + 2 * i + 1) * 32 + lane];
+              const uint2 b0 = QR ? qr[(2 * i) % (QR ? C::KS : 1)] : qf[(n * C::KS + 2 * i) * 32 + lane];
+              const uint2 b1 = QR ? qr[(2 * i + 1) % (QR ? C::KS : 1)] : qf[(n * C::KS + 2 * i + 1) * 32 + lane];
               mma16(c, a0, b0.x, b0.y);
               mma16(c, a1, b1.x, b1.y);
               s[n][0] = __fmaf_rn(d0[i], c[0], s[n][0]);
@@ -630,17 +680,21 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
         }
       }
       __syncwarp(); /* every lane has read the tile */
+      if (lane == 0) mb_arrive(&empty[warp][slot]);
       if (++slot == C::NST) { slot = 0; phase ^= 1; }
-      feed();
     }
 
-    /* ---- the warps join */
+    /* ---- the next unit's rows, then the warps join: each scales its sums to the common maximum */
+    if (warp == 0) advance(k + 2);
+    if (sh_have[(k + 1) & 3]) load_q(sh_pc[(k + 1) & 3], buf ^ 1);
+    const QPiece& c = pc;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(kAll, l[n][e], x);
+        if (g == 0) sh_ml[buf][warp][n * 8 + 2 * t + e] = make_float2(m[n][e], l[n][e]);
         if constexpr (Q4) {
 #pragma unroll
           for (int i = 0; i < NG; ++i) {
@@ -653,30 +707,33 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
             }
           }
         }
-        if (g == 0) sh_ml[warp][n * 8 + 2 * t + e] = make_float2(m[n][e], l[n][e]);
       }
-    __syncthreads();
-    if (tid < C::RT) {
-      float M = -INFINITY, L = 0.f;
+    sync_work();
+    auto joined = [&](int qi, float* M, float* L) { /* of all warps */
+      *M = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < W; ++w) M = fmaxf(M, sh_ml[w][tid].x);
-      const float U = M == -INFINITY ? 0.f : M;
+      for (int w = 0; w < W; ++w) *M = fmaxf(*M, sh_ml[buf][w][qi].x);
+      const float U = *M == -INFINITY ? 0.f : *M;
+      *L = 0.f;
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float f = ex2(sh_ml[w][tid].x - U);
-        sh_f[w][tid] = f;
-        L += sh_ml[w][tid].y * f;
+      for (int w = 0; w < W; ++w) *L += sh_ml[buf][w][qi].y * ex2(sh_ml[buf][w][qi].x - U);
+    };
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < W; ++w) M = fmaxf(M, sh_ml[buf][w][n * 8 + 2 * t + e].x);
+        m[n][e] = ex2(m[n][e] - (M == -INFINITY ? 0.f : M)); /* from here on the factor */
       }
-      sh_m[tid] = M;
-      sh_l[tid] = L;
-    }
-    const bool whole = pc.n == pc.n_tile;
-    const int my_slot = pc.nth == 0 ? 0 : 1; /* only a CTA's first and last pieces can be parts */
+    const bool whole = c.n == c.n_tile;
+    const int my_slot = c.nth == 0 ? 0 : 1; /* only a CTA's first and last pieces can be parts */
     const long long ps = ((long long)grp_id * 2 + my_slot) * C::RT;
-    auto out_row = [&](int qi) { return (long long)(pc.q.r0 + (pc.q0 + qi) / a.G) * a.H + pc.kvh * a.G + (pc.q0 + qi) % a.G; };
+    auto out_row = [&](int qi) { return (long long)(c.q.r0 + (c.q0 + qi) / a.G) * a.H + c.kvh * a.G + (c.q0 + qi) % a.G; };
 #pragma unroll
     for (int d0 = 0; d0 < HD; d0 += JD) {
-      if (d0) __syncthreads(); /* the words of the pass before are read */
+      if (d0) sync_work(); /* the words of the pass before are read */
 #pragma unroll
       for (int i = 0; i < JD / 32; ++i)
 #pragma unroll
@@ -684,51 +741,51 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int f = d0 / 16 + 2 * i;
+            const float x = m[n][e];
             *reinterpret_cast<float4*>(jb + (warp * C::RT + n * 8 + 2 * t + e) * JD + i * 32 + 4 * g) =
-                make_float4(o[f][n][e], o[f][n][2 + e], o[f + 1][n][e], o[f + 1][n][2 + e]);
+                make_float4(o[f][n][e] * x, o[f][n][2 + e] * x, o[f + 1][n][e] * x, o[f + 1][n][2 + e] * x);
           }
-      __syncthreads();
-      for (int i = tid; i < pc.nq * (JD / 4); i += NTH) {
+      sync_work();
+      for (int i = tid; i < c.nq * (JD / 4); i += W * 32) {
         const int qi = i / (JD / 4), d = (i % (JD / 4)) * 4;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 x = *reinterpret_cast<const float4*>(jb + qi * JD + d);
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const float f = sh_f[w][qi];
+        for (int w = 1; w < W; ++w) {
           const float4 y = *reinterpret_cast<const float4*>(jb + (w * C::RT + qi) * JD + d);
-          x.x += y.x * f;
-          x.y += y.y * f;
-          x.z += y.z * f;
-          x.w += y.w * f;
+          x.x += y.x;
+          x.y += y.y;
+          x.z += y.z;
+          x.w += y.w;
         }
+        float M, L;
+        joined(qi, &M, &L);
         if (whole) {
-          const float L = sh_l[qi], inv = L == 0.f ? 0.f : __fdividef(1.f, L); /* 0: the row sees nothing */
+          const float inv = L == 0.f ? 0.f : __fdividef(1.f, L); /* 0: the row sees nothing */
           *reinterpret_cast<uint2*>((T*)a.out + out_row(qi) * HD + d0 + d) = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+          if (d0 + d == 0 && a.lse) a.lse[out_row(qi)] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
         } else {
           __stcg(reinterpret_cast<float4*>(a.po + (ps + qi) * HD + d0 + d), x);
+          if (d0 + d == 0) __stcg(reinterpret_cast<float2*>(a.pml + (ps + qi) * 2), make_float2(M, L));
         }
       }
     }
-    if (tid < pc.nq) {
-      if (!whole) __stcg(reinterpret_cast<float2*>(a.pml + (ps + tid) * 2), make_float2(sh_m[tid], sh_l[tid]));
-      else if (a.lse) a.lse[out_row(tid)] = sh_l[tid] == 0.f ? -INFINITY : (sh_m[tid] + log2f(sh_l[tid])) * kLn2;
-    }
     if (!whole) {
       /* the last of the unit's CTAs to get here joins them, in the order of their keys */
-      const int c0 = line.group_of(pc.first), pieces = line.group_of(pc.last) - c0 + 1;
-      if (pc.t0 == 0 && tid == 0) p.tail[2 * c0 + 1] = my_slot;
+      const int c0 = line.group_of(c.first), pieces = line.group_of(c.last) - c0 + 1;
+      if (c.t0 == 0 && tid == 0) p.tail[2 * c0 + 1] = my_slot;
       __threadfence();
-      __syncthreads();
+      sync_work();
       if (tid == 0) {
         const int n = atomicAdd(&p.tail[2 * c0], 1);
         sh_last = n == pieces - 1;
         if (n == pieces - 1) p.tail[2 * c0] = 0; /* for the next launch */
       }
-      __syncthreads();
+      sync_work();
       if (sh_last) {
         __threadfence();
         const int slot0 = __ldcg(&p.tail[2 * c0 + 1]);
         auto place = [&](int i, int qi) { return ((long long)(c0 + i) * 2 + (i == 0 ? slot0 : 0)) * C::RT + qi; };
-        for (int i = tid; i < pc.nq * (HD / 4); i += NTH) {
+        for (int i = tid; i < c.nq * (HD / 4); i += W * 32) {
           const int qi = i / (HD / 4), d = (i % (HD / 4)) * 4;
           float M = -INFINITY, L = 0.f;
           for (int k = 0; k < pieces; ++k) M = fmaxf(M, __ldcg(a.pml + place(k, qi) * 2));
@@ -751,7 +808,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32, 1)
         }
       }
     }
-    __syncthreads(); /* q's fragments and the statistics may be replaced */
+    /* what a warp writes next into the other halves of the buffers, others have read before the barriers above */
   }
   if (!ok) { /* no copy is in flight when the CTA ends */
     for (int i = 0; i < C::NST; ++i) mb_wait_warp(&full[warp][slot], phase), slot = slot + 1 == C::NST ? (phase ^= 1, 0) : slot + 1;
@@ -782,7 +839,7 @@ int launch_quant(Ctx* c, TreeArgs& a) {
   p.tail = reinterpret_cast<int*>(c->quant_ws);
   a.po = c->quant_ws + kQuantTail;
   a.pml = a.po + rows * HD;
-  ULB_LAUNCH("quant attention launch", launch_k(c, quant_attn_kernel<T, Q4, HD, NT>, dim3(p.groups), dim3(C::W * 32), C::SMEM, a, p));
+  ULB_LAUNCH("quant attention launch", launch_k(c, quant_attn_kernel<T, Q4, HD, NT>, dim3(p.groups), dim3(C::W * 32 + 32), C::SMEM, a, p));
   return ULB_OK;
 }
 
