@@ -507,7 +507,7 @@ ULB_API int ulb_logits_process(ulb_ctx* ctx, const ulb_logits_args* args);
  */
 typedef struct ulb_norm_rope_args {
   int dtype, M, n_head, n_head_kv;
-  float eps; /* > 0 */
+  float eps; /* positive, not subnormal */
   int64_t q_row, q_head, k_row, k_head;
   const void *q, *k;
   const float *q_weight, *k_weight;

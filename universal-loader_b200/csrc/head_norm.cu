@@ -18,7 +18,7 @@ namespace ulb {
 namespace {
 
 template <typename T, int LPH, bool HALF>
-__global__ void __launch_bounds__(kWarps * 32, 3) norm_rope_kernel(const __grid_constant__ HeadArgs a, int wide) {
+__global__ void __launch_bounds__(kWarps * 32, 2) norm_rope_kernel(const __grid_constant__ HeadArgs a, int wide) {
   pdl_wait();
   pdl_trigger();
   __shared__ HeadWeights sw;
@@ -26,35 +26,47 @@ __global__ void __launch_bounds__(kWarps * 32, 3) norm_rope_kernel(const __grid_
   const Pairs pairs = pairs_of<HALF>(a, at);
   const float inv_hd = 1.f / a.hd;
   load_weights(a, &sw);
+  const int qs = (int)a.q_head * (int)sizeof(T), ks = (int)a.k_head * (int)sizeof(T), os = a.hd * (int)sizeof(T);
+  const int run = (at.d1 - at.d0) * (int)sizeof(T); /* bytes between a lane's runs */
   Turn t;
+  char *oq = nullptr, *ok = nullptr;
   walk_rows<Eight<T>, LPH, sizeof(T) == 4 ? 2 : 4>(
       a, a.nq + a.nk, at.on,
-      [&](int m, int h, bool mine) {
+      [&](int m) {
+        return HeadBase{(const char*)((const T*)a.q + m * a.q_row + at.d0), (const char*)((const T*)a.k + m * a.k_row + at.d0) - (long long)a.nq * ks,
+                        nullptr};
+      },
+      [&](const HeadBase& from, int h, bool mine) {
         Eight<T> e = zero8<T>();
         if (mine) {
-          const T* p = h < a.nq ? (const T*)a.q + m * a.q_row + h * a.q_head : (const T*)a.k + m * a.k_row + (h - a.nq) * a.k_head;
-          load_run(p + at.d0, wide, &e.r[0]);
-          load_run(p + at.d1, wide, &e.r[1]);
+          const bool is_q = h < a.nq;
+          const char* p = (is_q ? from.q : from.k) + (long long)h * (is_q ? qs : ks);
+          load_run((const T*)p, wide, &e.r[0]);
+          load_run((const T*)(p + run), wide, &e.r[1]);
         }
         return e;
       },
-      [&](int, int pos) { turn_at(pairs, pos, a.mscale, &t); },
-      [&](int m, int h, bool mine, const Eight<T>& e) {
+      [&](int m, int pos) {
+        turn_at(pairs, pos, a.mscale, &t);
+        oq = (char*)((T*)a.oq + (long long)m * a.nq * a.hd + at.d0);
+        ok = (char*)((T*)a.ok + ((long long)m * a.nk - a.nq) * a.hd + at.d0);
+      },
+      [&](int h, bool mine, const Eight<T>& e) {
         float x[8], w[8];
         unpack8(e, x);
         const bool is_q = h < a.nq;
         float ss = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss = __fmaf_rn(x[j], x[j], ss);
-        const float f = rsqrtf(__fmaf_rn(head_sum<LPH>(ss), inv_hd, a.eps));
+        const float f = rsqrt_near(__fmaf_rn(head_sum<LPH>(ss), inv_hd, a.eps));
         lane_weights(sw, is_q ? 0 : 1, at, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] *= f * w[j];
         turn<HALF>(t, 1.f, x);
         if (!mine) return;
-        T* o = is_q ? (T*)a.oq + ((long long)m * a.nq + h) * a.hd : (T*)a.ok + ((long long)m * a.nk + h - a.nq) * a.hd;
-        store4(o + at.d0, wide, x);
-        store4(o + at.d1, wide, x + 4);
+        char* o = (is_q ? oq : ok) + (long long)h * os;
+        store4((T*)o, wide, x);
+        store4((T*)(o + run), wide, x + 4);
       });
 }
 
@@ -74,25 +86,40 @@ __global__ void __launch_bounds__(kWarps * 32, 2) norm_rope_grad_kernel(const __
   const Pairs pairs = pairs_of<HALF>(a, at);
   const float inv_hd = 1.f / a.hd;
   load_weights(a, &sw);
+  const int qs = (int)a.q_head * (int)sizeof(T), ks = (int)a.k_head * (int)sizeof(T), os = a.hd * (int)sizeof(T);
+  const int run = (at.d1 - at.d0) * (int)sizeof(T);
   float sq[8] = {}, sk[8] = {};
   Turn t;
-  walk_rows<Both<T>, LPH, 2>(
+  char *oq = nullptr, *ok = nullptr;
+  struct Source {
+    const char *q, *k, *gq, *gk;
+  };
+  walk_rows<Both<T>, LPH, sizeof(T) == 4 ? 1 : 2>(
       a, a.nq + a.nk, at.on,
-      [&](int m, int h, bool mine) {
+      [&](int m) {
+        const long long oq = (long long)m * a.nq * a.hd + at.d0, ok = ((long long)m * a.nk - a.nq) * a.hd + at.d0;
+        return Source{(const char*)((const T*)a.q + m * a.q_row + at.d0), (const char*)((const T*)a.k + m * a.k_row + at.d0) - (long long)a.nq * ks,
+                      (const char*)((const T*)a.gq + oq), (const char*)((const T*)a.gk + ok)};
+      },
+      [&](const Source& from, int h, bool mine) {
         Both<T> e = {zero8<T>(), zero8<T>()};
         if (mine) {
           const bool is_q = h < a.nq;
-          const T* p = is_q ? (const T*)a.q + m * a.q_row + h * a.q_head : (const T*)a.k + m * a.k_row + (h - a.nq) * a.k_head;
-          const T* g = is_q ? (const T*)a.gq + ((long long)m * a.nq + h) * a.hd : (const T*)a.gk + ((long long)m * a.nk + h - a.nq) * a.hd;
-          load_run(p + at.d0, wide, &e.x.r[0]);
-          load_run(p + at.d1, wide, &e.x.r[1]);
-          load_run(g + at.d0, wide, &e.y.r[0]);
-          load_run(g + at.d1, wide, &e.y.r[1]);
+          const char* p = (is_q ? from.q : from.k) + (long long)h * (is_q ? qs : ks);
+          const char* g = (is_q ? from.gq : from.gk) + (long long)h * os;
+          load_run((const T*)p, wide, &e.x.r[0]);
+          load_run((const T*)(p + run), wide, &e.x.r[1]);
+          load_run((const T*)g, wide, &e.y.r[0]);
+          load_run((const T*)(g + run), wide, &e.y.r[1]);
         }
         return e;
       },
-      [&](int, int pos) { turn_at(pairs, pos, a.mscale, &t); },
-      [&](int m, int h, bool mine, const Both<T>& e) {
+      [&](int m, int pos) {
+        turn_at(pairs, pos, a.mscale, &t);
+        oq = (char*)((T*)a.oq + (long long)m * a.nq * a.hd + at.d0);
+        ok = (char*)((T*)a.ok + ((long long)m * a.nk - a.nq) * a.hd + at.d0);
+      },
+      [&](int h, bool mine, const Both<T>& e) {
         float x[8], y[8], w[8];
         unpack8(e.x, x);
         unpack8(e.y, y);
@@ -108,18 +135,25 @@ __global__ void __launch_bounds__(kWarps * 32, 2) norm_rope_grad_kernel(const __
         }
         ss = head_sum<LPH>(ss);
         sg = head_sum<LPH>(sg);
-        const float f = rsqrtf(__fmaf_rn(ss, inv_hd, a.eps)), c = f * f * f * (sg * inv_hd), fq = is_q ? f : 0.f, fk = is_q ? 0.f : f;
+        const float f = rsqrt_near(__fmaf_rn(ss, inv_hd, a.eps)), c = f * f * f * (sg * inv_hd);
+        /* y x f, of the kind whose sum it belongs to (zero past the heads); both in one warp where heads are not whole steps */
+        if (__all_sync(kAll, is_q)) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float gx = y[j] * x[j]; /* zero past the heads */
-          sq[j] = __fmaf_rn(gx, fq, sq[j]);
-          sk[j] = __fmaf_rn(gx, fk, sk[j]);
-          x[j] = f * w[j] - x[j] * c;
+          for (int j = 0; j < 8; ++j) sq[j] = __fmaf_rn(y[j] * x[j], f, sq[j]);
+        } else {
+          const float fq = is_q ? f : 0.f, fk = is_q ? 0.f : f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            sq[j] = __fmaf_rn(y[j] * x[j], fq, sq[j]);
+            sk[j] = __fmaf_rn(y[j] * x[j], fk, sk[j]);
+          }
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = f * w[j] - x[j] * c;
         if (!mine) return;
-        T* o = is_q ? (T*)a.oq + ((long long)m * a.nq + h) * a.hd : (T*)a.ok + ((long long)m * a.nk + h - a.nq) * a.hd;
-        store4(o + at.d0, wide, x);
-        store4(o + at.d1, wide, x + 4);
+        char* o = (is_q ? oq : ok) + (long long)h * os;
+        store4((T*)o, wide, x);
+        store4((T*)(o + run), wide, x + 4);
       });
   /* the block's share of dw: groups of a warp by shuffles, warps in order */
 #pragma unroll
@@ -167,7 +201,7 @@ __global__ void __launch_bounds__(kSumCols* kSumWays) norm_rope_sum_kernel(const
 
 template <typename T, bool HALF>
 int launch_apply(Ctx* c, HeadArgs& a, int wide) {
-  const int lph = lanes_of(a.hd), blocks = plan_rows(c, a, head_steps(a), c->n_sm * 3);
+  const int lph = lanes_of(a.hd), blocks = plan_rows(c, a, head_steps(a), c->n_sm * 2);
   auto go = [&](auto kern) -> int {
     ULB_LAUNCH("norm rope launch", launch_k(c, kern, dim3(blocks), dim3(kWarps * 32), 0, a, wide));
     return ULB_OK;
@@ -202,8 +236,10 @@ int norm_args(const char* who, const ulb_rope* r, const ulb_norm_rope_args* p, H
   ULB_CHECK(dtype_bytes(p->dtype), ULB_EUNSUPPORTED, "%s: type %d (F32, F16 or BF16)", who, p->dtype);
   ULB_CHECK(p->M >= 0 && p->n_head > 0 && p->n_head_kv >= 0, ULB_EINVAL, "%s: %d rows of %d and %d heads", who, p->M, p->n_head, p->n_head_kv);
   ULB_CHECK((long long)p->n_head + p->n_head_kv <= (1 << 20), ULB_EUNSUPPORTED, "%s: %d and %d heads", who, p->n_head, p->n_head_kv);
-  ULB_CHECK(std::isfinite(p->eps) && p->eps > 0.f, ULB_EINVAL, "%s: eps %g", who, (double)p->eps);
+  ULB_CHECK(std::isfinite(p->eps) && p->eps >= kMinEps, ULB_EINVAL, "%s: eps %g", who, (double)p->eps);
   ULB_CHECK(p->q_row >= 0 && p->q_head >= 0 && p->k_row >= 0 && p->k_head >= 0, ULB_EINVAL, "%s: negative stride", who);
+  ULB_CHECK(p->q_head < (1 << 28) && p->k_head < (1 << 28), ULB_EUNSUPPORTED, "%s: heads %lld and %lld elements apart (under 2^28)", who,
+            (long long)p->q_head, (long long)p->k_head);
   a->eps = p->eps;
   a->M = p->M;
   a->nq = p->n_head;

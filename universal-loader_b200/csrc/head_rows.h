@@ -16,6 +16,7 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr unsigned kAll = 0xffffffffu;
+constexpr float kMinEps = 1.1754943508222875e-38f; /* the smallest normal number: what a norm divides by is one, too */
 
 struct HeadArgs {
   const unsigned long long* turn;
@@ -83,6 +84,12 @@ __device__ __forceinline__ void store4(T* p, bool wide, const float* v) {
   } else {
     *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
   }
+}
+/* 1 / sqrt(x) of a normal positive x, to 2^-22 */
+__device__ __forceinline__ float rsqrt_near(float x) {
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 /* sum over the LPH lanes of a head; every lane has it */
 template <int LPH>
@@ -175,51 +182,58 @@ __device__ __forceinline__ void lane_weights(const HeadWeights& s, int kind, con
 
 /*
  * The heads of the warp's rows in steps of 32 / LPH heads, U steps (a batch) at a time; while a batch is worked on, the
- * next one's loads are under way, past the end of the row too.  load(m, h) gives what a lane keeps of head h of row m,
- * row(m, position) is called before the row's first batch, work(m, h, mine, kept) for every step by the whole warp;
- * lanes that are not `mine` keep zeros.
+ * next one's loads are under way, past the end of the row too.  from(m) gives what load(from, h, mine) needs to find head h
+ * of row m and return what a lane keeps of it (zeros where it is not `mine`), row(m, position) is called before the row's
+ * first batch, work(h, mine, kept) for every step by the whole warp.
  */
-template <typename Kept, int LPH, int U, typename Load, typename Row, typename Work>
-__device__ __forceinline__ void walk_rows(const HeadArgs& a, int heads, bool on, Load&& load, Row&& row, Work&& work) {
+template <typename Kept, int LPH, int U, typename From, typename Load, typename Row, typename Work>
+__device__ __forceinline__ void walk_rows(const HeadArgs& a, int heads, bool on, From&& from, Load&& load, Row&& row, Work&& work) {
   constexpr int HPS = 32 / LPH;
-  const int grp = (threadIdx.x & 31) / LPH, gw = blockIdx.x * kWarps + (threadIdx.x >> 5), part = gw % a.wpr;
-  const int n_rows = gridDim.x * kWarps / a.wpr, per = HPS * a.wpr, batches = (heads + per * U - 1) / (per * U);
-  int m = gw / a.wpr, b = 0, pos = 0;
+  const int gw = blockIdx.x * kWarps + (threadIdx.x >> 5), part = gw % a.wpr, lead = part * HPS + (threadIdx.x & 31) / LPH;
+  const int n_rows = gridDim.x * kWarps / a.wpr, per = HPS * a.wpr;
+  int m = gw / a.wpr, pos = 0, h = lead; /* h: the lane's head in the first step of the batch */
   if (m >= a.M) return;
   Kept now[U], next[U];
-  auto fetch = [&](int m, int b, Kept (&k)[U]) {
+  auto src = from(m);
+  auto fetch = [&](int h, Kept (&k)[U]) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = (b * U + u) * per + part * HPS + grp;
-      k[u] = load(m, h, on && h < heads);
-    }
+    for (int u = 0; u < U; ++u) k[u] = load(src, h + u * per, on && h + u * per < heads);
   };
-  fetch(m, 0, now);
+  fetch(h, now);
   pos = a.pos[m];
   while (true) {
-    if (b == 0) row(m, pos);
-    int m2 = m, b2 = b + 1;
-    if (b2 == batches) {
-      b2 = 0;
+    if (h == lead) row(m, pos);
+    int m2 = m, h2 = h + per * U;
+    if (h2 - lead + part * HPS >= heads) { /* the same for the whole warp */
+      h2 = lead;
       m2 += n_rows;
+      if (m2 < a.M) {
+        src = from(m2);
+        pos = a.pos[m2];
+      }
     }
-    if (m2 < a.M) {
-      fetch(m2, b2, next);
-      if (b2 == 0) pos = a.pos[m2];
-    }
+    if (m2 < a.M) fetch(h2, next);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int h0 = (b * U + u) * per + part * HPS;
-      if (h0 >= heads) break; /* the whole warp */
-      work(m, h0 + grp, on && h0 + grp < heads, now[u]);
+      const int x = h + u * per;
+      if (x - lead + part * HPS >= heads) break; /* the whole warp */
+      work(x, on && x < heads, now[u]);
     }
     if (m2 >= a.M) return;
 #pragma unroll
     for (int u = 0; u < U; ++u) now[u] = next[u];
     m = m2;
-    b = b2;
+    h = h2;
   }
 }
+
+/* where the q and k (and v) heads of a row are, as addresses of a lane's first run less what comes before the kind's first
+   head, so that head h is at base + h stride; strides in bytes */
+struct HeadBase {
+  const char *q, *k, *v;
+};
+/* 0: q, 1: k, 2: v */
+__device__ __forceinline__ int kind_of(const HeadArgs& a, int h) { return h < a.nq ? 0 : h < a.nq + a.nk ? 1 : 2; }
 
 /* a grid of whole rows: as many warps a row as it takes to give every SM some, at most one a step of its `steps`; and at
    most `most` blocks, which then walk the rows */

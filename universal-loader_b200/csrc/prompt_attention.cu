@@ -405,7 +405,7 @@ extern "C" int ulb_prompt_attention(ulb_ctx* ctx, const ulb_prompt_desc* d, cons
   /* at the first call, whatever its shape, so that any later one can be captured */
   if (!c->tree_ws) ULB_CUDA(cudaMalloc((void**)&c->tree_ws, kTreeWsFloats * sizeof(float)));
   a.ws = c->tree_ws;
-  if (prompt_tc_fits(c, a)) return launch_prompt_tc(c, a, d->dtype == ULB_TYPE_F16);
+  if (prompt_tc_fits(a)) return launch_prompt_tc(c, a, d->dtype == ULB_TYPE_F16);
   return d->dtype == ULB_TYPE_F16 ? pick_dim<__half>(c, a) : pick_dim<__nv_bfloat16>(c, a);
 }
 

@@ -37,8 +37,8 @@ __device__ __forceinline__ PromptSeq prompt_seq(const PromptArgs& a, int s) {
 __device__ __forceinline__ int prompt_seen(const PromptSeq& q, int i) { return min(max(q.len - q.n + i + 1, 0), q.len); }
 #endif
 
-/* the tcgen05 form (prompt_attention_tc.cu): head dims up to 128 */
-bool prompt_tc_fits(const Ctx* c, const PromptArgs& a);
+/* the tcgen05 form (prompt_attention_tc.cu) */
+bool prompt_tc_fits(const PromptArgs& a);
 int launch_prompt_tc(Ctx* c, const PromptArgs& a, bool f16);
 
 }  // namespace ulb

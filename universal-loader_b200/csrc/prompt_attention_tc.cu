@@ -209,6 +209,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       int slot = 0, issued = 0;
       uint32_t phase = 1; /* of the free barrier: the first round passes */
       while (ok && walk.next(a, p, &pc)) {
+        if (warp == 3) /* its rows of q are wanted soon: a line a lane */
+          for (int i = lane; i * 64 < pc.nq * hd; i += 32) {
+            const int qi = pc.q0 + i * 64 / hd;
+            asm volatile("prefetch.global.L2 [%0];" ::"l"((const T*)a.q + (pc.q.r0 + qi / a.G) * a.q_row + (pc.kvh * a.G + qi % a.G) * hd + i * 64 % hd));
+          }
         ok = ring_copy(pc.n, [](int) {}, [&]() { return mb_wait_warp(&free[slot], phase); }, [&](int t) {
           if (elect()) {
             const int at = pc.q.k0 + (pc.t0 + t) * TK; /* rows past the sequence's, too: masked; past the array: zeros */
@@ -394,6 +399,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             sum = y.x + y.y;
             top = fmaxf(x0, x1);
           };
+          if (i == 0) { /* nothing to go by: the maximum first */
+            float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < TK; c += 4) {
+              x0 = max3(x0, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+              x1 = max3(x1, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
+            }
+            m = __fmaf_rn(fmaxf(x0, x1), a.scale2, -RAISE);
+          }
           weights(m == -INFINITY ? 0.f : m);
           const bool grow = __fmaf_rn(top, a.scale2, -m) > RAISE + GROW; /* m -inf: a first key */
           if (__any_sync(0xffffffffu, grow)) {
@@ -430,6 +444,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int lo = max(0, open - pos); /* first key of the tile that some row does not see */
           auto clear = [&](int j) {
             const uint4 x = v[j];
+            /* an exponent of all ones carries into the sign's place */
+            constexpr uint32_t N = 0x7fff7fffu, C1 = F16 ? 0x04000400u : 0x00800080u;
+            if (!((((x.x & N) + C1) | ((x.y & N) + C1) | ((x.z & N) + C1) | ((x.w & N) + C1)) & 0x80008000u)) return;
             uint32_t w[4] = {x.x, x.y, x.z, x.w};
             bool hit = false;
 #pragma unroll
@@ -458,17 +475,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0 && ok) mb_arrive(&p_full[X][b]);
         sp ^= 1u << b;
       }
-      /* ---- the piece's end; the next one's rows are brought into L2 meanwhile */
+      /* ---- the piece's end */
       const Piece c = pc;
       have = walk.next(a, p, &pc);
-      if (have) {
-#pragma unroll 1
-        for (int j = 0; j < QW; ++j) {
-          int r1, ch1;
-          const T* src = q_at(pc, j, &r1, &ch1);
-          if (src && (ch1 & 7) == 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(src));
-        }
-      }
       if (ok) ok = mb_wait_warp(&piece[X], op);
       op ^= 1;
       used += c.n;
@@ -681,16 +690,16 @@ int rows_map(const PromptArgs& a, bool f16, const void* rows, long long stride, 
   return ULB_OK;
 }
 
+constexpr int kShareTiles = 16; /* tiles a share has at least */
 /*
  * Into how many shares the keys of a row tile are cut: as many as fill the SMs best.  Units that are as many as the SMs
- * four times over stay whole (sorted by length they even out); a share costs a twentieth more for what it leaves to join,
- * and has at least 16 tiles.
+ * four times over stay whole (sorted by length they even out); a share costs a twentieth more for what it leaves to join.
  */
 int pick_shares(long long units, int tiles, int n_sm, long long most) {
   if (units >= 4ll * n_sm) return 1;
   int best = 1;
   double time = 1e30;
-  for (int s = 1; s <= 64 && (s == 1 || (tiles / s >= 16 && units * s <= most)); ++s) {
+  for (int s = 1; s <= 64 && (s == 1 || (tiles / s >= kShareTiles && units * s <= most)); ++s) {
     const double waves = (double)((units * s + n_sm - 1) / n_sm), t = waves / s * (s > 1 ? 1.05 : 1.0);
     if (t < time - 1e-9) {
       time = t;
@@ -746,14 +755,23 @@ int launch_tc(Ctx* c, const PromptArgs& a) {
 
 template <typename T>
 int pick_tc(Ctx* c, const PromptArgs& a) {
-  const bool pair = (long long)a.max_q * a.G > 128;
+  /* 256 queries a CTA share each K / V tile; where that leaves half of the SMs without a unit, and the keys are too few to be
+     cut into shares, 128 a CTA: 500 rows of 32 heads over 4 12.2 us against 17.0, but 513 rows after 30000 keys (shares) 303
+     against 278 */
+  const long long units = (long long)a.n_seq * (((long long)a.max_q * a.G + 255) / 256) * a.KV;
+  const bool pair = (long long)a.max_q * a.G > 128 && (units * 2 > c->n_sm || a.max_k >= 2 * kShareTiles * TK);
   if (a.hd == 64) return pair ? launch_tc<T, 64, true>(c, a) : launch_tc<T, 64, false>(c, a);
   return pair ? launch_tc<T, 128, true>(c, a) : launch_tc<T, 128, false>(c, a);
 }
 
 }  // namespace
 
-bool prompt_tc_fits(const Ctx* c, const PromptArgs& a) { return a.hd <= 128 && a.max_k > 0; }
+/*
+ * When this form runs: head dims up to 128 and more than 128 keys.  Below, encoding the tensor maps on the host and starting up
+ * cost more than the tensor cores give: 1 to 128 rows of as many keys 9.4 us here, 8.8 as mma.sync; 8 x 50-100 rows 12.9 /
+ * 13.5; 1 x 16 rows x 1016 keys, 32 kv heads 16.8 / 32; 1 row x 5001 keys 23 / 140.
+ */
+bool prompt_tc_fits(const PromptArgs& a) { return a.hd <= 128 && a.max_k > 128; }
 
 int launch_prompt_tc(Ctx* c, const PromptArgs& a, bool f16) { return f16 ? pick_tc<__half>(c, a) : pick_tc<__nv_bfloat16>(c, a); }
 

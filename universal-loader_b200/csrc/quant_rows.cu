@@ -129,7 +129,7 @@ __device__ __forceinline__ long long slot_place(const HeadArgs& a, int m) {
 }
 
 template <typename TI, bool Q4, int LPH, bool HALF>
-__global__ void __launch_bounds__(kWarps * 32, 3) quant_append_kernel(const __grid_constant__ HeadArgs a, int f16, int wide_in, int wide_out) {
+__global__ void __launch_bounds__(kWarps * 32, 2) quant_append_kernel(const __grid_constant__ HeadArgs a, int f16, int wide_in, int wide_out) {
   pdl_wait();
   pdl_trigger();
   __shared__ HeadWeights sw;
@@ -137,59 +137,68 @@ __global__ void __launch_bounds__(kWarps * 32, 3) quant_append_kernel(const __gr
   const Pairs pairs = pairs_of<HALF>(a, at);
   const float inv_hd = 1.f / a.hd;
   load_weights(a, &sw);
+  const int hs = a.hd * (int)sizeof(TI), run = (at.d1 - at.d0) * (int)sizeof(TI);
   Turn t;
-  long long place = -1;
+  long long place = -1, o_row = 0;
   walk_rows<Eight<TI>, LPH, sizeof(TI) == 4 ? 2 : 4>(
       a, a.nq + a.nk + a.nv, at.on,
-      [&](int m, int h, bool mine) {
+      [&](int m) {
+        return HeadBase{(const char*)((const TI*)a.q + m * a.q_row + at.d0), (const char*)((const TI*)a.k + m * a.k_row + at.d0) - (long long)a.nq * hs,
+                        (const char*)((const TI*)a.v + m * a.v_row + at.d0) - (long long)(a.nq + a.nk) * hs};
+      },
+      [&](const HeadBase& from, int h, bool mine) {
         Eight<TI> e = zero8<TI>();
         if (mine) {
-          const TI* p = h < a.nq          ? (const TI*)a.q + m * a.q_row + h * a.q_head
-                        : h < a.nq + a.nk ? (const TI*)a.k + m * a.k_row + (h - a.nq) * a.k_head
-                                          : (const TI*)a.v + m * a.v_row + (h - a.nq - a.nk) * a.v_head;
-          load_run(p + at.d0, wide_in, &e.r[0]);
-          load_run(p + at.d1, wide_in, &e.r[1]);
+          const int kind = kind_of(a, h);
+          const char* p = (kind == 0 ? from.q : kind == 1 ? from.k : from.v) + (long long)h * hs;
+          load_run((const TI*)p, wide_in, &e.r[0]);
+          load_run((const TI*)(p + run), wide_in, &e.r[1]);
         }
         return e;
       },
       [&](int m, int pos) {
         turn_at(pairs, pos, a.mscale, &t);
         place = slot_place(a, m);
+        o_row = (long long)m * a.nq;
       },
-      [&](int m, int h, bool mine, const Eight<TI>& e) {
-        float x[8], y[8], w[8];
+      [&](int h, bool mine, const Eight<TI>& e) {
+        float x[8];
         unpack8(e, x);
-        const int kind = h < a.nq ? 0 : h < a.nq + a.nk ? 1 : 2;
-        float f = 1.f;
-        if (a.wq || a.wk) { /* the same for all threads */
-          float ss = 0.f;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) ss = __fmaf_rn(x[j], x[j], ss);
-          ss = head_sum<LPH>(ss);
-          if (kind == 0 ? a.wq != nullptr : kind == 1 && a.wk) f = rsqrtf(__fmaf_rn(ss, inv_hd, a.eps));
-        }
-        lane_weights(sw, kind, at, w); /* ones where there are none */
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = x[j] * (f * w[j]);
-        turn<HALF>(t, 1.f, y);
-        if (kind == 2) {
+        const int kind = kind_of(a, h);
+        if (__any_sync(kAll, kind != 2)) { /* some of q or k */
+          float y[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) y[j] = x[j];
+          if (a.wq || a.wk) { /* the same for all threads */
+            float ss = 0.f, w[8], f = 1.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ss = __fmaf_rn(x[j], x[j], ss);
+            ss = head_sum<LPH>(ss);
+            if (kind == 0 ? a.wq != nullptr : a.wk != nullptr) f = rsqrt_near(__fmaf_rn(ss, inv_hd, a.eps));
+            lane_weights(sw, kind, at, w); /* ones where there are none */
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] *= f * w[j];
+          }
+          turn<HALF>(t, 1.f, y);
+          if (kind != 2) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = y[j];
+          }
         }
         if (__any_sync(kAll, kind != 0)) {
           unsigned char* const r = !mine || kind == 0 || place < 0 ? nullptr
                                    : kind == 1 ? a.kp + place + (long long)(h - a.nq) * a.g.head
                                                : a.vp + place + (long long)(h - a.nq - a.nk) * a.g.head;
-          quantise8<Q4, HALF>(y, r, a.hd, at);
+          quantise8<Q4, HALF>(x, r, a.hd, at);
         }
         if (!mine || kind != 0) return;
-        const long long o = ((long long)m * a.nq + h) * a.hd;
+        const long long o = (o_row + h) * a.hd;
         if (f16) {
-          store4((__half*)a.oq + o + at.d0, wide_out, y);
-          store4((__half*)a.oq + o + at.d1, wide_out, y + 4);
+          store4((__half*)a.oq + o + at.d0, wide_out, x);
+          store4((__half*)a.oq + o + at.d1, wide_out, x + 4);
         } else {
-          store4((__nv_bfloat16*)a.oq + o + at.d0, wide_out, y);
-          store4((__nv_bfloat16*)a.oq + o + at.d1, wide_out, y + 4);
+          store4((__nv_bfloat16*)a.oq + o + at.d0, wide_out, x);
+          store4((__nv_bfloat16*)a.oq + o + at.d1, wide_out, x + 4);
         }
       });
 }
@@ -201,7 +210,7 @@ __global__ void __launch_bounds__(kWarps * 32) quant_read_kernel(const __grid_co
   pdl_trigger();
   constexpr int U = 4;
   const int lane = threadIdx.x & 31, gw = blockIdx.x * kWarps + (threadIdx.x >> 5), part = gw % a.wpr, n_rows = gridDim.x * kWarps / a.wpr;
-  const int hd = a.g.hd, per = hd >> 3, units = a.g.n_head_kv * per; /* of K, and as many of V */
+  const int hd = a.g.hd, per2 = 31 - __clz(hd >> 3), units = a.g.n_head_kv << per2; /* of K, and as many of V; head dims are powers of two */
   for (int m = gw / a.wpr; m < a.M; m += n_rows) {
     const long long place = slot_place(a, m);
     for (int i0 = part * 32 + lane; i0 < 2 * units; i0 += a.wpr * 32 * U) {
@@ -209,7 +218,7 @@ __global__ void __launch_bounds__(kWarps * 32) quant_read_kernel(const __grid_co
       uint32_t sc[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * a.wpr * 32, v = i >= units, r = i - v * units, h = r / per, d0 = (r - h * per) * 8, grp = d0 >> 5;
+        const int i = i0 + u * a.wpr * 32, v = i >= units, r = i - v * units, h = r >> per2, d0 = (r & ((1 << per2) - 1)) * 8, grp = d0 >> 5;
         w[u] = make_uint2(0, 0);
         sc[u] = 0;
         if (place < 0 || i >= 2 * units) continue;
@@ -220,15 +229,25 @@ __global__ void __launch_bounds__(kWarps * 32) quant_read_kernel(const __grid_co
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * a.wpr * 32, v = i >= units, r = i - v * units, h = r / per, d0 = (r - h * per) * 8, grp = d0 >> 5;
+        const int i = i0 + u * a.wpr * 32, v = i >= units, r = i - v * units, h = r >> per2, d0 = (r & ((1 << per2) - 1)) * 8, grp = d0 >> 5;
         if (i >= 2 * units) break;
         const float2 dm = unpack2<__half>(sc[u]);
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const uint32_t y = j < 4 ? w[u].x : w[u].y;
-          if (Q4) x[j] = __fmaf_rn((float)((y >> (8 * (grp & 1) + 16 * (j & 1) + 4 * ((j >> 1) & 1))) & 15u), dm.x, dm.y);
-          else x[j] = (float)(int8_t)(y >> (8 * (j & 3))) * dm.x;
+          if (!Q4) x[j] = (float)(int8_t)(y >> (8 * (j & 3))) * dm.x;
+        }
+        if constexpr (Q4) { /* two codes at a time as fp16 integers: 0x6400 | n is 1024 + n, 0x6400 | 16 n is 1024 + 16 n */
+#pragma unroll
+          for (int j = 0; j < 8; j += 4) {
+            const uint32_t y = (j < 4 ? w[u].x : w[u].y) >> (8 * (grp & 1));
+            const float2 lo = unpack2<__half>((y & 0x000f000fu) | 0x64006400u), hi = unpack2<__half>((y & 0x00f000f0u) | 0x64006400u);
+            x[j] = __fmaf_rn(lo.x - 1024.f, dm.x, dm.y);
+            x[j + 1] = __fmaf_rn(lo.y - 1024.f, dm.x, dm.y);
+            x[j + 2] = __fmaf_rn(__fmaf_rn(hi.x, 0.0625f, -64.f), dm.x, dm.y);
+            x[j + 3] = __fmaf_rn(__fmaf_rn(hi.y, 0.0625f, -64.f), dm.x, dm.y);
+          }
         }
         T* o = (T*)(v ? a.ok : a.oq) + ((long long)m * a.g.n_head_kv + h) * hd + d0;
         if constexpr (sizeof(T) == 2) {
@@ -244,7 +263,7 @@ __global__ void __launch_bounds__(kWarps * 32) quant_read_kernel(const __grid_co
 
 template <typename TI, bool Q4, bool HALF>
 int launch_append(Ctx* c, HeadArgs& a, int f16, int wide_in, int wide_out) {
-  const int lph = lanes_of(a.hd), blocks = plan_rows(c, a, head_steps(a), c->n_sm * 3);
+  const int lph = lanes_of(a.hd), blocks = plan_rows(c, a, head_steps(a), c->n_sm * 2);
   auto go = [&](auto kern) -> int {
     ULB_LAUNCH("quant append launch", launch_k(c, kern, dim3(blocks), dim3(kWarps * 32), 0, a, f16, wide_in, wide_out));
     return ULB_OK;
@@ -304,7 +323,7 @@ int ulb_quant_append(ulb_ctx* ctx, const ulb_rope* r, const ulb_quant_desc* d, c
             "ulb_quant_append: %d rows of %d and %d heads", p->M, p->n_head, a.g.n_head_kv);
   ULB_CHECK(p->q_row >= 0 && p->k_row >= 0 && p->v_row >= 0, ULB_EINVAL, "ulb_quant_append: negative stride");
   const bool normed = p->q_weight || p->k_weight;
-  ULB_CHECK(!normed || (std::isfinite(p->eps) && p->eps > 0.f), ULB_EINVAL, "ulb_quant_append: eps %g", (double)p->eps);
+  ULB_CHECK(!normed || (std::isfinite(p->eps) && p->eps >= kMinEps), ULB_EINVAL, "ulb_quant_append: eps %g", (double)p->eps);
   if (p->M == 0) return ULB_OK;
   ULB_CHECK(p->q && p->k && p->v && p->pos && p->row_seq && p->slot && p->block_table && p->q_out && p->k_pool && p->v_pool, ULB_EINVAL,
             "ulb_quant_append: NULL argument");
