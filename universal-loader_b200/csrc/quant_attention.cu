@@ -37,37 +37,38 @@
 namespace ulb {
 namespace {
 
-#ifndef QUC
-#define QUC 32
-#endif
-constexpr int kUnitCost = QUC;    /* what a unit costs besides its tiles, in tiles */
-constexpr int kMinTiles = 48;   /* places of the line a CTA takes at least */
 constexpr float kRaise = 12.f, kGrow = 3.9f; /* weights <= 2^15.9 < 65504 */
-constexpr int kRingBytes = 212 * 1024;
 constexpr unsigned kAll = 0xffffffffu;
 
 template <bool Q4, int HD, int NT>
 struct QCfg {
   static constexpr int RB = quant_row_bytes(Q4, HD), CB = quant_code_bytes(Q4, HD);
-  static constexpr int KT = 32;
+  static constexpr int KT = HD == 256 && !Q4 ? 16 : 32; /* keys a tile */
   static constexpr int STAGE = 2 * KT * RB;
-#ifndef QW4
-#define QW4 11
-#define QJD 128
-#define QREG 1
-#endif
-  /* warps that work, with the copying one a multiple of four: registers are given out so */
-  static constexpr int W = HD == 256 ? (Q4 ? 7 : 3) : NT == 1 ? (HD == 64 ? 15 : Q4 ? QW4 : 7) : HD == 64 && NT < 4 ? 11 : 7;
-  static constexpr int RT = 8 * NT;           /* queries a CTA */
-  static constexpr int JD = NT >= 3 ? 32 : NT == 2 || HD == 64 ? 64 : QJD; /* dims the warps join at a time */
+  /*
+   * Working warps (one more copies), and blocks on an SM; with the copying warp a block's are a multiple of four wherever the
+   * registers do not say otherwise, since they are given out so.  Eight queries: two blocks of 5 hide what a unit costs
+   * besides its tiles behind each other's work: 64 sequences of 100 to 1000 keys, 32 kv heads of 64 71 us (one block of 11
+   * warps 94, three of 3 64), 64 x 256-8192 keys in 4 bits 113 (105, 121), 64 x 20-100 keys 16 (25, 19).  More queries: the
+   * registers of 7 warps.
+   */
+  static constexpr int W = HD == 256 ? 3 : NT == 1 ? 5 : HD == 64 && NT < 4 ? 11 : 7;
+  static constexpr int CTAS = HD == 256 || NT == 1 ? 2 : 1;
+  /* what a unit costs besides its tiles, in tiles, and the places of the line a block takes at least: fitted */
+  static constexpr int UNIT = NT == 1 && HD < 256 ? 16 : 32, MIN = UNIT / 2;
+  static constexpr int RT = 8 * NT; /* queries a CTA */
   static constexpr int NG = HD / kGroup, KS = HD / 16;
   static constexpr int NW = Q4 ? NG : NG / 2, NC = (NW + 3) / 4; /* 32-bit words of a row's scales, products that take them */
-  static constexpr int QB = 2 * NT * (KS + NC) * 256, JB = W * RT * JD * 4; /* bytes of two units' fragments of q and of the join */
-  static constexpr int QS = QB / 2 / 8;       /* 8-byte words of one unit's */
-  static constexpr int ROOM = (kRingBytes - QB - JB) / (W * STAGE);
+  static constexpr int QB = 2 * NT * (KS + NC) * 256; /* bytes of two units' fragments of q */
+  static constexpr int QS = QB / 2 / 8;               /* 8-byte words of one unit's */
+  static constexpr int ALL = 227 * 1024 / CTAS - 1024 - 2560; /* the SM's, less what a CTA has besides */
+  static constexpr int JD0 = HD == 64 || NT > 1 ? 64 : 128; /* dims the warps join at a time, 32 where the ring wants the room */
+  static constexpr int JD = (ALL - QB - W * RT * JD0 * 4) / (W * STAGE) >= 2 ? JD0 : 32;
+  static constexpr int JB = W * RT * JD * 4;
+  static constexpr int ROOM = (ALL - QB - JB) / (W * STAGE);
   static constexpr int NST = ROOM > 6 ? 6 : ROOM;
   static constexpr int SMEM = W * NST * STAGE + QB + JB;
-  static_assert(NST >= 2 && SMEM <= 222 * 1024 && W <= 31, "shared memory, a lane a ring");
+  static_assert(NST >= 2 && W <= 31, "shared memory, a lane a ring");
 };
 
 struct QuantPlan {
@@ -75,7 +76,7 @@ struct QuantPlan {
   int* tail; /* [groups][2]: arrivals at the unit that begins in this CTA and goes on, the slot of its first piece */
 };
 
-/* the line of work, in tiles: a unit takes kUnitCost places before its tiles.  CTA c's stretch. */
+/* the line of work, in tiles: a unit takes UNIT places before its tiles.  CTA c's stretch. */
 struct QLine {
   int total, groups, per, rem;
   __device__ __forceinline__ void cut(int n) {
@@ -98,7 +99,7 @@ struct QPiece {
   int nth;                /* pieces of this CTA before it */
 };
 
-template <int RT, int KT>
+template <int RT, int KT, int UNIT>
 struct QWalk {
   int at, end, base, cnt, s, n_tile, n_pass, nth;
   TreeSeq q;
@@ -106,7 +107,7 @@ struct QWalk {
     q = tree_seq(a, s);
     n_tile = max(1, (q.len + KT - 1) / KT);
     n_pass = (q.n * a.G + RT - 1) / RT;
-    cnt = (n_tile + kUnitCost) * n_pass * a.g.n_head_kv;
+    cnt = (n_tile + UNIT) * n_pass * a.g.n_head_kv;
   }
   __device__ __forceinline__ bool next(const TreeArgs& a, QPiece* o) {
     while (at < end) {
@@ -115,10 +116,10 @@ struct QWalk {
         ++s;
         load(a);
       }
-      const int len = n_tile + kUnitCost, u = (at - base) / len, in = at - base - u * len, upto = min(len, in + end - at);
-      o->t0 = max(in - kUnitCost, 0);
-      o->n = max(upto - kUnitCost, 0) - o->t0;
-      o->first = base + u * len + kUnitCost;
+      const int len = n_tile + UNIT, u = (at - base) / len, in = at - base - u * len, upto = min(len, in + end - at);
+      o->t0 = max(in - UNIT, 0);
+      o->n = max(upto - UNIT, 0) - o->t0;
+      o->first = base + u * len + UNIT;
       o->last = base + u * len + len - 1;
       at += upto - in;
       if (o->n <= 0) continue; /* none of its tiles yet */
@@ -208,7 +209,7 @@ __device__ __forceinline__ void first_scales(const uint8_t* p, float (&d)[NG]) {
 }
 
 template <typename T, bool Q4, int HD, int NT>
-__global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32 + 32, 1)
+__global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32 + 32, QCfg<Q4, HD, NT>::CTAS)
     quant_attn_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ QuantPlan p) {
   using C = QCfg<Q4, HD, NT>;
   constexpr int W = C::W, NG = C::NG, NTH = W * 32 + 32, JD = C::JD, KT = C::KT, US = KT / 16;
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32 + 32, 1)
   __shared__ uint8_t sh_map[W][C::NST]; /* which 16-key halves of a tile are mapped */
   __shared__ float2 sh_ml[2][W][C::RT];
   __shared__ float sh_qs[2][C::RT];
-  __shared__ QWalk<C::RT, C::KT> sh_walk;
+  __shared__ QWalk<C::RT, C::KT, C::UNIT> sh_walk;
   __shared__ QPiece sh_pc[4];
   __shared__ int sh_have[4], sh_s, sh_base, sh_sum[W + 1], sh_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -237,10 +238,10 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32 + 32, 1)
   pdl_trigger();
 
   /* the line's length, then this CTA's stretch and the sequence that holds its begin */
-  QWalk<C::RT, C::KT> walk;
+  QWalk<C::RT, C::KT, C::UNIT> walk;
   auto places_of = [&](int s) {
     if (s >= a.g.n_seq) return 0;
-    QWalk<C::RT, C::KT> w;
+    QWalk<C::RT, C::KT, C::UNIT> w;
     w.s = s;
     w.load(a);
     return w.cnt;
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32 + 32, 1)
   bool ok = true;
   /* piece k is in place k % 4; warp 0 looks for piece k + 2 at the end of piece k */
   auto advance = [&](int k) {
-    QWalk<C::RT, C::KT> w = sh_walk;
+    QWalk<C::RT, C::KT, C::UNIT> w = sh_walk;
     QPiece x;
     const bool more = w.next(a, &x);
     __syncwarp();
@@ -466,7 +467,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32 + 32, 1)
 #pragma unroll
       for (int n = 0; n < NT; ++n) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
     const int open = min(tree_open(a, pc.q), pc.q.len);
-    constexpr bool QR = NT == 1 && QREG; /* fragments of q in registers */
+    constexpr bool QR = NT == 1; /* fragments of q in registers */
     uint2 qr[QR ? C::KS : 1];
     if constexpr (QR) {
 #pragma unroll
@@ -785,18 +786,32 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32 + 32, 1)
         __threadfence();
         const int slot0 = __ldcg(&p.tail[2 * c0 + 1]);
         auto place = [&](int i, int qi) { return ((long long)(c0 + i) * 2 + (i == 0 ? slot0 : 0)) * C::RT + qi; };
+        /* the maximum and the sum of each query first: a warp a query, a lane every 32nd piece */
+        for (int qi = warp; qi < c.nq; qi += W) {
+          float M = -INFINITY, L = 0.f;
+          for (int k = lane; k < pieces; k += 32) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.pml + place(k, qi) * 2));
+            const float top = fmaxf(M, ml.x), u = top == -INFINITY ? 0.f : top;
+            L = L * ex2(M - u) + ml.y * ex2(ml.x - u);
+            M = top;
+          }
+#pragma unroll
+          for (int x = 16; x; x >>= 1) {
+            const float m2 = __shfl_xor_sync(kAll, M, x), l2 = __shfl_xor_sync(kAll, L, x), top = fmaxf(M, m2), u = top == -INFINITY ? 0.f : top;
+            L = L * ex2(M - u) + l2 * ex2(m2 - u);
+            M = top;
+          }
+          if (lane == 0) sh_ml[buf][0][qi] = make_float2(M, L);
+        }
+        sync_work();
         for (int i = tid; i < c.nq * (HD / 4); i += W * 32) {
           const int qi = i / (HD / 4), d = (i % (HD / 4)) * 4;
-          float M = -INFINITY, L = 0.f;
-          for (int k = 0; k < pieces; ++k) M = fmaxf(M, __ldcg(a.pml + place(k, qi) * 2));
-          const float U = M == -INFINITY ? 0.f : M;
+          const float M = sh_ml[buf][0][qi].x, L = sh_ml[buf][0][qi].y, U = M == -INFINITY ? 0.f : M;
           float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
           for (int k = 0; k < pieces; ++k) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.pml + place(k, qi) * 2));
+            const float f = ex2(__ldcg(a.pml + place(k, qi) * 2) - U);
             const float4 y = __ldcg(reinterpret_cast<const float4*>(a.po + place(k, qi) * HD + d));
-            const float f = ex2(ml.x - U);
-            L += ml.y * f;
             x.x += y.x * f;
             x.y += y.y * f;
             x.z += y.z * f;
@@ -825,14 +840,16 @@ int launch_quant(Ctx* c, TreeArgs& a) {
   static uint64_t attr = 0; /* devices it is set on */
   if (!(attr >> (c->device & 63) & 1)) {
     ULB_CUDA(cudaFuncSetAttribute(quant_attn_kernel<T, Q4, HD, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    prefer_max_shared((const void*)quant_attn_kernel<T, Q4, HD, NT>); /* before the launch does it: all of it, for CTAS blocks an SM */
+    ULB_CUDA(cudaFuncSetAttribute(quant_attn_kernel<T, Q4, HD, NT>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
     attr |= 1ull << (c->device & 63);
   }
   const long long units = (long long)a.g.n_seq * a.g.n_head_kv * (((long long)a.max_rows * a.G + C::RT - 1) / C::RT);
-  ULB_CHECK(units * (std::max(1, (a.max_len + C::KT - 1) / C::KT) + kUnitCost) < (1ll << 31) - 65536, ULB_EUNSUPPORTED,
+  ULB_CHECK(units * (std::max(1, (a.max_len + C::KT - 1) / C::KT) + C::UNIT) < (1ll << 31) - 65536, ULB_EUNSUPPORTED,
             "ulb_quant_attention: %d sequences of %d positions and %d rows", a.g.n_seq, a.max_len, a.max_rows);
   QuantPlan p;
-  p.groups = c->n_sm;
-  p.min_tiles = kMinTiles;
+  p.groups = c->n_sm * C::CTAS;
+  p.min_tiles = C::MIN;
   const size_t rows = (size_t)p.groups * 2 * C::RT;
   ULB_CHECK(kQuantTail + rows * (HD + 2) <= kQuantWsFloats && 2 * (size_t)p.groups <= kQuantTail, ULB_EUNSUPPORTED,
             "ulb_quant_attention: workspace for %d SMs", c->n_sm);
