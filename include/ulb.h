@@ -46,9 +46,9 @@ extern "C" {
 #define ULB_TYPE_F16 1
 #define ULB_TYPE_Q4_0 2
 #define ULB_TYPE_Q4_K 12
-#define ULB_TYPE_Q8_0 8  /* token_embd and output.weight only (as llama.cpp's Q4_0 files store them) */
+#define ULB_TYPE_Q8_0 8  /* token_embd and output.weight (as llama.cpp's Q4_0 files store them), quantised caches */
 #define ULB_TYPE_Q6_K 14 /* token_embd and output.weight only */
-#define ULB_TYPE_BF16 30 /* rotary, tree attention, cache page and logits operators only */
+#define ULB_TYPE_BF16 30 /* operators of the paged cache section only */
 
 typedef struct ulb_ctx ulb_ctx;
 typedef struct ulb_tensor ulb_tensor;
@@ -576,7 +576,7 @@ ULB_API int ulb_quant_read(ulb_ctx* ctx, const ulb_quant_desc* desc, int out_dty
  * ulb_tree_attention over a quantised cache, for the new tokens of a step: one row a sequence, a chain of drafts
  * (mask_words = 0) or a tree.  Rows, lengths, masks, outputs and what is promised of them as there; q and out of
  * desc's dtype; n_head / n_head_kv <= 64.  Codes are multiplied exactly, scores, statistics and sums are fp32, a
- * weight times a group's scale is rounded once to 11 bits.  Made for few queries a kv head (rows x grouped heads):
+ * weight times a group's scale is rounded once to 11 bits (fp16 outputs: 22).  Made for few queries a kv head (rows x grouped heads):
  * past 32 (16 for head_dim 256) the keys are walked once for each 32 (16).  The first call on a context allocates
  * 32 MiB of device memory for partial results, kept until ulb_destroy.
  */

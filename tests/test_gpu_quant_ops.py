@@ -528,7 +528,7 @@ def run_attention(tctx, fmt, kind, q, kp, vp, table, n_pages, most, page, D, KV,
 
 
 def check_attention(kind, got, lse, want, want_lse, mag, reach):
-    # weights are rounded once to 2^-11, exponentials and fp32 sums are good to 2^-18; a score's products are exact and
+    # weights are rounded once to 2^-11 (a bound for two parts, too), exponentials and fp32 sums are good to 2^-18; a score's products are exact and
     # its sum is off by at most 2^-18 of the sum of their sizes (`reach`); the output is rounded once
     part = 2.0 ** -11 + 2.0 ** -17 + 2 * reach * 2.0 ** -18
     tol = UNIT[kind] * np.abs(want) + part[..., None] * mag + 1e-6

@@ -9,8 +9,14 @@
  *
  * Work.  Memory bounds it: every element is read once and written once (gradient: two reads).  A lane owns eight
  * elements of a head, both sides of four pairs, and 8, 16 or 32 lanes a head, so the sums are shuffles and pairs turn in
- * registers.  A warp keeps to one row, whose sines it computes once for all its heads; the weights stay in registers
- * over the rows.  When there are few rows, several warps share the heads of one.
+ * registers.  A warp keeps to one row, whose sines it computes once for all its heads, and has the next batch of heads
+ * under way while it works on one; the weights are in shared memory.  When there are few rows, several warps share the heads
+ * of one.  The sums of dw stay in registers over all rows of a warp, and a second small kernel adds the blocks in order.
+ *
+ * Measured: 16381 bf16 rows of 32 and 8 heads of 128 68 us, 4.9 TB/s (75 % of the copy rate); their gradient 103 us
+ * (75 %); 1000 fp32 rows' gradient 19 us, of which the second kernel is 4; 8 rows 5 us, a launch.  About 160 instructions a
+ * warp for two heads of 128 bound the forward pass beside HBM.  One block of 256 threads less an SM, and half the heads in
+ * flight: 69 and 76 us.
  */
 #include "head_rows.h"
 
@@ -235,7 +241,8 @@ int norm_args(const char* who, const ulb_rope* r, const ulb_norm_rope_args* p, H
   ULB_TRY(rotary(who, r, a));
   ULB_CHECK(dtype_bytes(p->dtype), ULB_EUNSUPPORTED, "%s: type %d (F32, F16 or BF16)", who, p->dtype);
   ULB_CHECK(p->M >= 0 && p->n_head > 0 && p->n_head_kv >= 0, ULB_EINVAL, "%s: %d rows of %d and %d heads", who, p->M, p->n_head, p->n_head_kv);
-  ULB_CHECK((long long)p->n_head + p->n_head_kv <= (1 << 20), ULB_EUNSUPPORTED, "%s: %d and %d heads", who, p->n_head, p->n_head_kv);
+  ULB_CHECK((long long)p->n_head + p->n_head_kv <= (1 << 20) && p->M <= kMaxRows, ULB_EUNSUPPORTED, "%s: %d rows of %d and %d heads", who, p->M,
+            p->n_head, p->n_head_kv);
   ULB_CHECK(std::isfinite(p->eps) && p->eps >= kMinEps, ULB_EINVAL, "%s: eps %g", who, (double)p->eps);
   ULB_CHECK(p->q_row >= 0 && p->q_head >= 0 && p->k_row >= 0 && p->k_head >= 0, ULB_EINVAL, "%s: negative stride", who);
   ULB_CHECK(p->q_head < (1 << 28) && p->k_head < (1 << 28), ULB_EUNSUPPORTED, "%s: heads %lld and %lld elements apart (under 2^28)", who,

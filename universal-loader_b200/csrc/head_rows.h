@@ -16,6 +16,7 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr unsigned kAll = 0xffffffffu;
+constexpr int kMaxRows = 1 << 30; /* rows of a call: a row and the grid's step stay in 32 bits */
 constexpr float kMinEps = 1.1754943508222875e-38f; /* the smallest normal number: what a norm divides by is one, too */
 
 struct HeadArgs {

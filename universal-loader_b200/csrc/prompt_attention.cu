@@ -11,6 +11,9 @@
  * groups x WK key groups; a key group has its own (m, l, o), joined in shared memory.  Weights stay in
  * registers, rounded to the rows' type.
  *
+ * Used for head_dim 256 and for calls of at most 128 keys (prompt_attention_tc.cu, which has the rule): 64 rows of 32 heads over
+ * 8 of 64 9 us, the host's call; as the only form four prompts of 2 to 6 thousand rows took 2960 us.
+ *
  * What a row does not see never reaches its result: scores past its last key are replaced, keys past the tile's last
  * are zero-filled (the rows there belong to the next sequence), and an element of V in a tile on the diagonal that is
  * not finite is taken out and added to the rows that see it.

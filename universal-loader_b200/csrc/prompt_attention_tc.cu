@@ -1,6 +1,34 @@
 /*
  * prompt_attention_tc.cu — ulb_prompt_attention on the 5th-generation tensor cores, for head dims up to
- * 128.  (Comment of the design follows the measurements.)
+ * 128 (80 and 96 run in tiles of 128 whose other columns the copies fill with zeros).  Same mathematics and masking as
+ * prompt_attention.cu; the roles, rings and barriers are those of tree_attention_tc.cu, over rows of packed sequences in place
+ * of pages.
+ *
+ * A CTA works on 64-key tiles with M = 128 queries (row x head of the group) a stream, two streams, each with its running
+ * (m, l, o), its softmax warpgroup (one thread a query) and a warp that issues its MMAs:
+ *   PAIR = true   256 queries: the streams hold neighbouring tiles of 128 and share every K / V tile
+ *   PAIR = false  128 queries: both hold the same and take the even and the odd tiles; they join in shared memory
+ * S = Q K^T (both operands in shared memory, fp32 in TMEM); the query's thread reads S, updates m and l, writes P in the rows' type
+ * over S; O += P V with P from TMEM and V as the tile TMA wrote it.  O is rescaled only when a maximum has grown by more than
+ * 2^GROW.  Weights are rounded to 16 bits once: bf16 outputs are off by 2.2e-3 relative against 64 bits, fp16 ones by
+ * 2.4e-4, of which 1.7e-3 and 2.1e-4 are the output's own rounding.  K and V rows come by TMA from wherever a sequence begins; what a
+ * tile holds of the next sequence is masked, its infinities and NaN taken out of V with those past the diagonal.
+ *
+ * Work.  A unit is a (sequence, row tile, share of its keys, kv head) and walks the keys up to its last row's only.  The row
+ * tiles of all sequences are sorted by their keys in a small kernel, and a CTA takes every G-th of that list in
+ * turns that run back and forth, so all end together whatever the lengths; what fits the SMs once needs no list.  Few units
+ * with many keys are cut into shares, joined by a third kernel.
+ *
+ * Measured: four prompts of 2 to 6 thousand rows, 32 heads over 8 of 128 (682 GFLOP): 695 to 745 us, 0.92 to 0.98 PFLOP/s (56 to
+ * 60 % of the burst rate, 66 to 70 % of the sustained one: the clock falls to 1.4 GHz under the power cap); 513 rows after
+ * 30000 keys 280 to 310 us; 500 rows of 32 heads over 4 of 64 12 us; 16 prompts of 200 to 400 rows 70 us.  A pair of 64-key
+ * tiles takes 1980 cycles: 1240 of them on the tensor pipe (products with 64 columns read Q from shared memory every time),
+ * 1024 of exponentials, which overlap in part.  Tried and slower: scores and weights in separate columns, so that the next
+ * tile's scores start as soon as these are read (827 us for 770).  Short prompts pay about 15 us a unit: its rows in, its outputs out and
+ * the fill of both pipelines are not overlapped with the next unit's.
+ *
+ * Every mbarrier wait has a limit: past it a role raises bit 3 of the device error word, arrives nowhere and issues nothing any
+ * more, so that the others run into theirs; the CTA still waits (bounded) for its MMAs before it frees TMEM.
  */
 #include "tcgen05.h"
 #include "prompt_attention.h"
@@ -143,9 +171,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                    const __grid_constant__ PromptPlan p) {
   using C = TcCfg<HD, PAIR>;
   constexpr bool F16 = std::is_same<T, __half>::value;
-  /* Weights are at most 2^(RAISE + GROW): fp16, whose largest number is just under 2^16, holds 11 bits of one
-     down to 2^-26 of the maximum (tree_attention.cu, kRaise); bf16 has the range without.  fp16, 64 rows x 64
-     heads x 131072 keys: 290 us (331 with scores four times as wide), with GROW 3 300 (346), with 2 320 (356). */
+  /* weights are at most 2^(RAISE + GROW): fp16, whose largest number is just under 2^16, holds 11 bits of one down to 2^-26 of
+     the maximum (tree_attention.cu, kRaise); bf16 has the range without */
   constexpr float RAISE = F16 ? 12.f : 0.f, GROW = F16 ? 3.9f : 8.f;
   constexpr uint32_t FMT = F16 ? 0u : (1u << 7) | (1u << 10);
   constexpr uint32_t ID_S = (1u << 4) | FMT | ((TK >> 3) << 17) | ((128 >> 4) << 24);

@@ -9,23 +9,36 @@
  * expanded to 16-bit values:
  *   s_t   = scale sum_g [ d_tg (q_g . c_tg) + m_tg sum(q_g) ]          fp32 sums of exact products
  *   o_gi  = sum_t (p_t d_tg) c_tgi + sum_t p_t m_tg,   p_t = exp(s_t - M)
- * The codes are exact fp16 integers, so the one rounding is that of the weight p_t d_tg to fp16.  M is the running
+ * The codes are exact fp16 integers, so the one rounding is that of the weight p_t d_tg to fp16: 2^-11, an eighth of a bf16
+ * output's own; fp16 outputs take a second part of each weight, since one part adds as much as the output's rounding (500
+ * keys: 3.0e-4 against 64 bits, the rounding alone 2.1e-4).  M is the running
  * maximum of s_t + log d_t (d_t the largest scale of the V row), so weights are at most 2^(RAISE + GROW) whatever the
  * scales are, and fp16 keeps 11 bits of one down to 2^-26 of the heaviest; p_t itself and what it sums to
  * are fp32 (a scale is at least 2^-24, so p_t stays in range).  q is scaled by a power of two a row, which makes
  * bf16 rows fp16 ones without loss.  It drops out of the scores exactly.
  *
- * Work.  HBM bounds it: a K and a V row of 80 (4 bits) or 144 bytes at head_dim 128.  K^T Q and V P are
- * mma.sync m16n8k16 with the codes as the 16-row operand (keys x dims, then dims x keys) and eight queries as
- * columns, so a product wastes nothing on padding at eight queries and a code is unpacked once for all of them.
- * Two nibbles or bytes become two fp16 integers by one LOP3 / PRMT and one HADD2 / HFMA2.  The dims a lane
- * takes of a row are four in a row of each 16, for the first product, and four of each 32 for the second, so every
- * shared-memory read is a conflict-free 32-bit word of the rows as they lie in HBM.
+ * Work.  A K and a V row take 80 (4 bits) or 144 bytes at head_dim 128.  K^T Q and V P are mma.sync m16n8k16 with
+ * the codes as the 16-row operand (keys x dims, then dims x keys) and eight queries as columns, so a product wastes
+ * nothing on padding at eight queries and a code is unpacked once for all of them.  K's codes are masked out of their word and
+ * used as they are: the bits of a small integer n are the fp16 subnormal n 2^-24.  The parts of a score that only the scales
+ * give (m_g sum q, or -128 d_g sum q for offset bytes) are one more product, of the scales' own words with those sums in two
+ * fp16 parts.  V's codes are centred (one LOP3 or PRMT and one HADD2 or HFMA2 for two), because the sums run over
+ * many keys.  The dims a lane takes of a row are four in a row of each 16 for the first product and four of each 32 for the
+ * second, so every shared-memory read is a conflict-free 32-bit word of the rows as they lie in HBM (head_dim 256 in 4 bits:
+ * two ways).
  *
- * A warp walks 32-key tiles of its own through its own ring of bulk copies; nothing is shared
- * but the rows of q and the join of the warps' (M, l, o) at the end.  The tiles of all (sequence, row tile, kv head)
- * units form one line that is cut evenly over the CTAs, so lengths may differ as they like; a unit in several
- * CTAs leaves a partial in each and the last of them to arrive joins them in order.
+ * A warp walks 32-key tiles of its own, 16 keys at a time, through its own ring of bulk copies, which one more warp
+ * issues for all, a lane a ring.  The tiles of all (sequence, row tile, kv head) units form one line that is cut evenly
+ * over the blocks, so lengths may differ as they like; a unit in several blocks leaves a partial in each and the last
+ * of them to arrive joins them in order.  While a unit's tiles are worked on, the next unit's rows of q are made.
+ *
+ * Measured (bf16): 64 sequences of 256 to 8192 keys, 32 heads over 8 of 128, 4 bits: 113 us, 3.1 TB/s (48 % of the copy
+ * rate); 5 rows over 100001 keys, 64 heads over 8, 8 bits: 136 us; 1 x 20000 keys 20 (4 bits) and 22 us; 64 x 1000 keys in 8
+ * bits 44 us, half of the copy rate.  What bounds it is instructions: about 450 a warp for 16 keys of eight queries in 4
+ * bits, of which unpacking V, the weights of its groups and their transposition are half, at two to three a cycle; with
+ * more queries the weights of each 8 more, and past 32 the keys are walked again.  Tried and slower: 16 warps of 128
+ * registers (170 us for the 113), a warp that feeds itself (135), all 32 keys in one body (the code leaves the
+ * instruction cache; 157).
  */
 #include "quant_cache.h"
 #include "tcgen05.h"
@@ -361,7 +374,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32 + 32, QCfg<Q4, HD, NT
     }
     /* no copy is in flight when the CTA ends: the working warps wait for all of them, and this one where they gave up */
     if (!ok) {
-      for (int i = 0; i < C::NST; ++i) mb_wait(&f_bar[i], phase ^ (i < slot ? 0u : 1u));
+      for (int i = 0; i < C::NST; ++i) mb_wait(&f_bar[i], phase ^ (i < slot ? 1u : 0u)); /* this round's, the last one's */
       if (lane == 0) atomicOr(a.err, 8);
     }
     return;
@@ -437,10 +450,10 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32 + 32, QCfg<Q4, HD, NT
     if (lane == 0) sh_walk = walk;
     __syncwarp();
     advance(0);
-    advance(1);
   }
   __syncthreads();
   if (sh_have[0]) load_q(sh_pc[0], 0); /* the stretch may hold no tile */
+  if (warp == 0) advance(1);
   sync_work();
   for (int k = 0; sh_have[k & 3]; ++k) {
     const int buf = k & 1;
@@ -643,10 +656,17 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32 + 32, QCfg<Q4, HD, NT
 #pragma unroll
               for (int e = 0; e < 2; ++e) om[i][n][e] = __fmaf_rn(s[n][2 + e], vm[1][i], __fmaf_rn(s[n][e], vm[0][i], om[i][n][e]));
             }
-            const uint32_t b0 = transpose8(h2(s[n][0] * vd[0][i], s[n][1] * vd[0][i]) & seen[n][0]),
-                           b1 = transpose8(h2(s[n][2] * vd[1][i], s[n][3] * vd[1][i]) & seen[n][1]);
+            const float w0 = s[n][0] * vd[0][i], w1 = s[n][1] * vd[0][i], w2 = s[n][2] * vd[1][i], w3 = s[n][3] * vd[1][i];
+            const uint32_t y0 = h2(w0, w1) & seen[n][0], y1 = h2(w2, w3) & seen[n][1];
+            const uint32_t b0 = transpose8(y0), b1 = transpose8(y1);
             mma16(o[2 * i][n], f0, b0, b1);
             mma16(o[2 * i + 1][n], f1, b0, b1);
+            if constexpr (std::is_same<T, __half>::value) { /* what fp16 leaves of a weight is a second operand */
+              const float2 z0 = unpack2<__half>(y0), z1 = unpack2<__half>(y1);
+              const uint32_t c0 = transpose8(h2(w0 - z0.x, w1 - z0.y) & seen[n][0]), c1 = transpose8(h2(w2 - z1.x, w3 - z1.y) & seen[n][1]);
+              mma16(o[2 * i][n], f0, c0, c1);
+              mma16(o[2 * i + 1][n], f1, c0, c1);
+            }
           }
         };
         if constexpr (Q4) {
