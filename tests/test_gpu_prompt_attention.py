@@ -136,6 +136,22 @@ def test_many_values_that_are_not_finite(tctx):
     assert torch.equal(got[:, :, keep], want[:, :, keep]) and (got[:, :, 77] == math.inf).all()
 
 
+@pytest.mark.parametrize("D,H,KV", [(64, 4, 2), (128, 6, 1)])
+def test_many_prompts_of_every_length(tctx, D, H, KV):
+    """More sequences than the ordering block has warps, many without rows or keys, some long: a list of units and CTAs that
+    take several."""
+    rng = np.random.default_rng(D)
+    n = 700
+    rows = [int(x) for x in rng.integers(0, 40, n) * (rng.random(n) < 0.5)]
+    rows[333], rows[5] = 1200, 700
+    keys = [r + int(x) if rng.random() < 0.9 else int(x) for r, x in zip(rows, rng.integers(0, 30, n))]
+    qs, ks = starts(rows), starts(keys)
+    g = torch.Generator(device="cuda").manual_seed(D)
+    q, k, v = (torch.randn(m, h, D, device="cuda", generator=g).half() for m, h in ((qs[-1], H), (ks[-1], KV), (ks[-1], KV)))
+    got, lse = run(tctx, "f16", q, k, v, qs, ks, 0.1)
+    check("f16", got, lse, *attend64(q, k, v, qs, ks, 0.1))
+
+
 def test_packed_projections_bounds_and_clamps(tctx):
     """q, k and v as slices of one projection's rows; max_q and max_k below the sequences' own."""
     g = torch.Generator(device="cuda").manual_seed(8)

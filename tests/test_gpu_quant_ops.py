@@ -545,7 +545,7 @@ CASES = [  # sequences' lengths, rows each, H, KV, D, page
     ([1], [1], 1, 1, 64, 16), ([500], [1], 32, 4, 64, 256), ([33, 1, 0, 700], [1, 1, 1, 1], 8, 2, 128, 32),
     ([5000], [5], 64, 8, 128, 256), ([40, 17, 300], [3, 0, 9], 12, 4, 128, 16), ([2049] * 5, [1] * 5, 5, 5, 128, 128),
     ([1000, 129], [7, 12], 4, 4, 256, 64), ([64], [64], 8, 2, 64, 64), ([3, 2], [8, 4], 4, 1, 128, 16), ([12000], [1], 8, 1, 256, 256),
-    ([260] * 70, [1] * 70, 8, 2, 64, 16), ([257, 31], [33, 20], 6, 2, 128, 32)]
+    ([260] * 70, [1] * 70, 8, 2, 64, 16), ([257, 31], [33, 20], 6, 2, 128, 32), ([130, 40], [3, 1], 64, 1, 64, 32)]
 
 
 @pytest.mark.parametrize("fmt", ["q8", "q4"])
@@ -645,6 +645,49 @@ def test_quant_attention_bad_contents_of_arrays(tctx):
         assert torch.equal(got[i], want[i]) and torch.equal(lse[i], want_lse[i])
     got, lse = run_attention(tctx, fmt, "f16", q, kp, vp, table, *base, [-9, 1, 2, 1 << 30], [0] * 3, [50, -4, 70], None, 0.1, max_rows=1)
     assert torch.equal(got[0], want[0]) and not got[1].any() and torch.equal(got[2], want[2])
+
+
+def test_quant_attention_of_many_sequences(tctx):
+    """More sequences than a block has threads, most without rows or keys: those that have some keep their own."""
+    rng = np.random.default_rng(13)
+    fmt, D, KV, H, page, n_seq = "q4", 64, 2, 4, 16, 1500
+    lens = [int(x) if i % 7 == 0 else 0 for i, x in enumerate(rng.integers(0, 90, n_seq))]
+    rows = [int(x) for x in rng.integers(0, 3, n_seq) * (rng.random(n_seq) < 0.3)]
+    kp, vp, table, n_pages, most = pools_of(rng, fmt, lens, KV, page, D)
+    starts = np.concatenate([[0], np.cumsum(rows)]).tolist()
+    q = torch.as_tensor(rng.standard_normal((starts[-1], H, D))).half().cuda()
+    got, lse = run_attention(tctx, fmt, "f16", q, kp, vp, table, n_pages, most, page, D, KV, starts, [0] * n_seq, lens, None, 0.1)
+    check_attention("f16", got, lse, *attend64(fmt, q.double().cpu().numpy(), kp, vp, table, page, D, starts, None, lens, None, 0.1))
+
+
+@pytest.mark.parametrize("fmt", ["q8", "q4"])
+def test_pools_past_two_gigabytes(tctx, fmt):
+    """Rows written, read and attended on pages whose bytes begin past 2^31."""
+    import ulb_capi as U
+    rng = np.random.default_rng(14)
+    D, KV, H, page, n = 128, 8, 16, 256, 300
+    d = U.QuantDesc(FORMATS[fmt], U.T_F16, KV, D, page, 1, 1, 2)
+    d.n_pages = n_pages = 2 ** 31 // (KV * page * d.row_bytes) + 3
+    table = dev([[n_pages - 1, n_pages - 2]])
+    k, v = (torch.empty(n_pages, KV, page, d.row_bytes, dtype=torch.uint8, device="cuda") for _ in range(2))
+    row = (H + 2 * KV) * D
+    x = torch.as_tensor(rng.standard_normal((n, row))).half().cuda()
+    seq, slot, z = dev([0] * n), dev(np.arange(n)), dev([0])
+    q = torch.empty(n, H, D, dtype=torch.float16, device="cuda")
+    r = U.Rope(tctx, D)
+    r.quant_append(d, U.T_F16, ptr(x), ptr(x) + H * D * 2, ptr(x) + (H + KV) * D * 2, H, ptr(slot), ptr(seq), ptr(slot), ptr(table), n, ptr(q), ptr(k),
+                   ptr(v), q_row=row, k_row=row, v_row=row)
+    tail = [t[-2:].cpu().numpy() for t in (k, v)]
+    o = [torch.empty(n, KV, D, dtype=torch.float16, device="cuda") for _ in range(2)]
+    tctx.quant_read(d, U.T_F16, ptr(k), ptr(v), ptr(table), ptr(seq), ptr(slot), n, ptr(o[0]), ptr(o[1]))
+    at = np.arange(n)
+    for got, t in zip(o, tail):
+        assert torch.equal(got.cpu(), torch.as_tensor(values(fmt, t[1 - at // page, :, at % page], D, np.float32)).half())
+    out, lse = torch.empty(1, H, D, dtype=torch.float16, device="cuda"), torch.empty(1, H, device="cuda")
+    tctx.quant_attention(d, H, 1, 1, n, 0.1, ptr(q) + (n - 1) * H * D * 2, ptr(k), ptr(v), ptr(table), ptr(dev([0, 1])), ptr(z), ptr(dev([n])), None, 0,
+                         ptr(out), ptr(lse))
+    check_attention("f16", out, lse, *attend64(fmt, q[n - 1:].double().cpu().numpy(), *tail, np.array([[1, 0]]), page, D, [0, 1], None, [n], None, 0.1))
+    r.close()
 
 
 def test_quant_attention_captured_in_two_graphs_on_another_stream(tctx):
