@@ -65,7 +65,8 @@ struct PromptPlan {
   int shares;          /* the keys of a row tile are cut into so many */
   int row_tiles;       /* of the longest sequence */
   int direct;          /* every CTA takes the unit of its index, without a list */
-  const int2* list;    /* (sequence, row tile), the most keys first; a unit for each share and kv head */
+  const int2* list;    /* (sequence, row tile), the most keys first; a unit for each share and kv head.  Null: one sequence, from
+                          its last row tile on */
   const int* n_list;   /* entries there */
   float *po, *pml;     /* partials of (sequence, row tile, kv head, share): outputs, (max, sum) */
 };
@@ -103,7 +104,10 @@ struct Walk {
   int turn, nth;
   __device__ __forceinline__ bool next(const PromptArgs& a, const PromptPlan& p, Piece* o) {
     const int G = gridDim.x, c = blockIdx.x;
-    const int per = a.KV * p.shares, total = p.direct ? 0 : (int)min((long long)*p.n_list * per, 0x7ffe0000ll);
+    const int per = a.KV * p.shares;
+    int n_entry = 0;
+    if (!p.direct) n_entry = p.list ? *p.n_list : (prompt_seq(a, 0).n * a.G + RT - 1) / RT;
+    const int total = (int)min((long long)n_entry * per, 0x7ffe0000ll);
     for (;; ) {
       const int at = turn * G + (turn & 1 ? G - 1 - c : c);
       int s, rt, u;
@@ -119,7 +123,7 @@ struct Walk {
         if (at >= total) continue;
         const int e = at / per;
         u = at - e * per;
-        const int2 x = p.list[e];
+        const int2 x = p.list ? p.list[e] : make_int2(0, n_entry - 1 - e);
         s = x.x;
         rt = x.y;
       }
@@ -767,11 +771,13 @@ int launch_tc(Ctx* c, const PromptArgs& a) {
     ULB_CHECK(entries <= room && entries * a.KV * p.shares < 0x7ffe0000ll, ULB_EUNSUPPORTED, "ulb_prompt_attention: %d sequences of %d rows",
               a.n_seq, a.max_q);
     const int cap = (int)std::min<long long>(std::min(all, room), 0x7ffe0000ll);
-    int* const n_list = reinterpret_cast<int*>(ws);
-    int2* const list = reinterpret_cast<int2*>(ws + 4);
-    p.n_list = n_list;
-    p.list = list;
-    ULB_LAUNCH("prompt order launch", launch_k(c, prompt_order_kernel<C::RT>, dim3(1), dim3(1024), 0, a, list, n_list, cap));
+    if (a.n_seq > 1) {
+      int* const n_list = reinterpret_cast<int*>(ws);
+      int2* const list = reinterpret_cast<int2*>(ws + 4);
+      p.n_list = n_list;
+      p.list = list;
+      ULB_LAUNCH("prompt order launch", launch_k(c, prompt_order_kernel<C::RT>, dim3(1), dim3(1024), 0, a, list, n_list, cap));
+    }
   }
   const int grid = p.direct ? (int)(units * p.shares) : c->n_sm;
   ULB_LAUNCH("prompt attention launch", launch_k(c, prompt_tc_kernel<T, HD, PAIR>, dim3(grid), dim3(kThreads), C::SMEM, mk, mv, a, p));
