@@ -375,6 +375,10 @@ extern "C" int ulb_prompt_attention(ulb_ctx* ctx, const ulb_prompt_desc* d, cons
   a.KV = d->n_head_kv;
   a.G = a.H / a.KV;
   a.hd = d->head_dim;
+  unsigned log = 0;
+  while ((1 << log) < a.G) ++log;
+  a.g_mul = log ? (unsigned)(((1ull << (31 + log)) + a.G - 1) / a.G) : 0;
+  a.g_shift = log ? log - 1 : 0;
   a.q_row = d->q_row ? d->q_row : (long long)a.H * a.hd;
   a.k_row = d->k_row ? d->k_row : (long long)a.KV * a.hd;
   a.v_row = d->v_row ? d->v_row : (long long)a.KV * a.hd;

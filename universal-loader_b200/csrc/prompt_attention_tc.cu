@@ -19,13 +19,14 @@
  * turns that run back and forth, so all end together whatever the lengths; what fits the SMs once needs no list.  Few units
  * with many keys are cut into shares, joined by a third kernel.
  *
- * Measured: four prompts of 2 to 6 thousand rows, 32 heads over 8 of 128 (682 GFLOP): 695 to 745 us, 0.92 to 0.98 PFLOP/s (56 to
- * 60 % of the burst rate, 66 to 70 % of the sustained one: the clock falls to 1.4 GHz under the power cap); 513 rows after
- * 30000 keys 280 to 310 us; 500 rows of 32 heads over 4 of 64 12 us; 16 prompts of 200 to 400 rows 70 us.  A pair of 64-key
- * tiles takes 1980 cycles: 1240 of them on the tensor pipe (products with 64 columns read Q from shared memory every time),
- * 1024 of exponentials, which overlap in part.  Tried and slower: scores and weights in separate columns, so that the next
- * tile's scores start as soon as these are read (827 us for 770).  Short prompts pay about 15 us a unit: its rows in, its outputs out and
- * the fill of both pipelines are not overlapped with the next unit's.
+ * Measured: four prompts of 2 to 6 thousand rows, 32 heads over 8 of 128 (682 GFLOP): 670 to 720 us, 0.95 to 1.02 PFLOP/s (58
+ * to 62 % of the burst rate, 68 to 73 % of the sustained one: the clock falls to 1.4 GHz under the power cap); 513 rows after
+ * 30000 keys 276 to 300 us; 2000 rows 48 us; 500 rows of 32 heads over 4 of 64 12 us; 16 prompts of 200 to 400 rows 63 us.  A
+ * pair of 64-key tiles takes 1700 to 1980 cycles: 1240 of them on the tensor pipe (products with 64 columns read Q from shared
+ * memory every time), 1024 of exponentials, which overlap in part.  What a unit costs besides is not overlapped with the
+ * next one: its rows in (4000 to 6000 cycles) and its outputs out (5000), most of a short prompt's time.  Tried and slower:
+ * scores and weights in separate columns, so that the next tile's scores start as soon as these are read (827 us for 770 at
+ * the time); the next unit's rows held in registers while the outputs leave (spills; 16 short prompts 88 us for 70).
  *
  * Every mbarrier wait has a limit: past it a role raises bit 3 of the device error word, arrives nowhere and issues nothing any
  * more, so that the others run into theirs; the CTA still waits (bounded) for its MMAs before it frees TMEM.
@@ -88,8 +89,8 @@ __device__ __forceinline__ bool row_tile(const PromptArgs& a, int s, int rt, int
   o->q0 = rt * RT;
   o->nq = min(RT, o->q.n * a.G - o->q0);
   if (o->nq <= 0) return false;
-  o->open = prompt_seen(o->q, o->q0 / a.G);
-  o->n_tile = max(1, (prompt_seen(o->q, (o->q0 + o->nq - 1) / a.G) + TK - 1) / TK);
+  o->open = prompt_seen(o->q, div_group(a, o->q0));
+  o->n_tile = max(1, (prompt_seen(o->q, div_group(a, o->q0 + o->nq - 1)) + TK - 1) / TK);
   return true;
 }
 __device__ __forceinline__ void share_of(int n_tile, int share, int shares, int* t0, int* n) {
@@ -242,8 +243,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       while (ok && walk.next(a, p, &pc)) {
         if (warp == 3) /* its rows of q are wanted soon: a line a lane */
           for (int i = lane; i * 64 < pc.nq * hd; i += 32) {
-            const int qi = pc.q0 + i * 64 / hd;
-            asm volatile("prefetch.global.L2 [%0];" ::"l"((const T*)a.q + (pc.q.r0 + qi / a.G) * a.q_row + (pc.kvh * a.G + qi % a.G) * hd + i * 64 % hd));
+            const int qi = pc.q0 + i * 64 / hd, row = div_group(a, qi);
+            asm volatile("prefetch.global.L2 [%0];" ::"l"((const T*)a.q + (pc.q.r0 + row) * a.q_row + (pc.kvh * a.G + qi - row * a.G) * hd + i * 64 % hd));
           }
         ok = ring_copy(pc.n, [](int) {}, [&]() { return mb_wait_warp(&free[slot], phase); }, [&](int t) {
           if (elect()) {
@@ -353,26 +354,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t used = 0;       /* V tiles of earlier pieces */
     uint32_t sp = 0, op = 0, vsp = 0; /* phases of s_full[X][b] and o_done[X][b] in bit b, of piece and v_seen */
     constexpr int QW = C::NQ * TQ * (HD / 8) / 256; /* 16-byte words of Q a thread */
-    auto q_at = [&](const Piece& c, int j, int* r, int* ch) { /* word j of this thread; null past the tile's queries and past hd */
-      const int i = tid - 128 + j * 256;
-      *r = i / (HD / 8);
-      *ch = i % (HD / 8);
-      const int qi = c.q0 + *r;
-      return *r < c.nq && *ch * 8 < hd ? (const T*)a.q + (c.q.r0 + qi / a.G) * a.q_row + (c.kvh * a.G + qi % a.G) * hd + *ch * 8 : nullptr;
-    };
     bool have = walk.next(a, p, &pc);
     while (have) {
-      {
+      { /* the rows of Q: word j of this thread; zeros past the tile's queries and past hd */
         uint4 qx[QW];
-        int r, ch;
 #pragma unroll
         for (int j = 0; j < QW; ++j) {
-          const T* src = q_at(pc, j, &r, &ch);
-          qx[j] = src ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+          const int i = tid - 128 + j * 256, r = i / (HD / 8), ch = i % (HD / 8), qi = pc.q0 + r, row = div_group(a, qi);
+          const T* src = (const T*)a.q + (pc.q.r0 + row) * a.q_row + (pc.kvh * a.G + qi - row * a.G) * hd + ch * 8;
+          qx[j] = r < pc.nq && ch * 8 < hd ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int j = 0; j < QW; ++j) {
-          q_at(pc, j, &r, &ch);
+          const int i = tid - 128 + j * 256, r = i / (HD / 8), ch = i % (HD / 8);
           *reinterpret_cast<uint4*>(q_sm + (r >> 7) * C::QTILE + (ch >> 3) * (TQ * 128) + sw128(r & 127, ch & 7)) = qx[j];
         }
       }
@@ -382,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
       const int r = (PAIR ? X * 128 : 0) + row, qi = pc.q0 + r;
       const bool live = r < pc.nq, warp_live = r - lane < pc.nq;
-      const int ri = live ? qi / a.G : 0;
+      const int ri = live ? div_group(a, qi) : 0, head = qi - ri * a.G;
       const int n = n_of(X), open = pc.open, seen = prompt_seen(pc.q, ri);
       float m = -INFINITY, l = 0.f; /* m: the maximum that weights are taken against, less RAISE */
       for (int i = 0; i < n && ok; ++i) {
@@ -533,12 +527,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         m = top;
       }
       const bool own = n > 0, other = !PAIR && (X == 0 ? c.n > 1 : true);
-      const long long at = live ? (long long)(c.q.r0 + ri) * a.H + c.kvh * a.G + qi % a.G : 0;
+      const long long at = live ? (long long)(c.q.r0 + ri) * a.H + c.kvh * a.G + head : 0;
       const long long ps = ((((long long)c.s * p.row_tiles + c.rt) * a.KV + c.kvh) * p.shares + c.share) * C::RT + r;
       const float inv = l == 0.f ? 0.f : __fdividef(1.f, l); /* 0: the row sees nothing */
       if (warp_live && ok) {
         constexpr int COLS = PAIR ? HD : HD / 2;
         uint4* const stage = reinterpret_cast<uint4*>(stage_sm) + (warp - 4) * 256;
+        long long row_at[4]; /* of the rows whose words this lane writes */
+#pragma unroll
+        for (int k = 0; k < 4; ++k) row_at[k] = __shfl_sync(0xffffffffu, at, k * 8 + (lane >> 2));
 #pragma unroll 1
         for (int d0 = PAIR ? 0 : X * COLS; d0 < (PAIR ? HD : (X + 1) * COLS); d0 += 32) {
           if (d0 >= hd) break;
@@ -557,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (odd[c.nth & 1][kOddWords] && live) { /* values taken out of masked tiles go to the rows that see them */
             float more[32] = {};
             const int from = max(c.t0 * TK, open / TK * TK), upto = min(seen, (c.t0 + c.n) * TK);
-            add_odd<T>(a, c.q, odd[c.nth & 1], c.kvh, (const T*)a.q + (c.q.r0 + ri) * a.q_row + (c.kvh * a.G + qi % a.G) * hd, from, upto, d0, m, more);
+            add_odd<T>(a, c.q, odd[c.nth & 1], c.kvh, (const T*)a.q + (c.q.r0 + ri) * a.q_row + (c.kvh * a.G + head) * hd, from, upto, d0, m, more);
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] += more[e];
           }
@@ -573,9 +570,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const int y = k * 8 + (lane >> 2), w = lane & 3;
-              const long long row_at = __shfl_sync(0xffffffffu, at, y);
               const uint4 x = stage[y * 4 + (w ^ ((y >> 1) & 3))];
-              if (r - lane + y < c.nq && d0 + w * 8 < hd) *reinterpret_cast<uint4*>((T*)a.out + row_at * hd + d0 + w * 8) = x;
+              if (r - lane + y < c.nq && d0 + w * 8 < hd) *reinterpret_cast<uint4*>((T*)a.out + row_at[k] * hd + d0 + w * 8) = x;
             }
           } else {
 #pragma unroll
