@@ -141,21 +141,23 @@ __global__ void __launch_bounds__(kWarps * 32, 2) norm_rope_grad_kernel(const __
         }
         ss = head_sum<LPH>(ss);
         sg = head_sum<LPH>(sg);
-        const float f = rsqrt_near(__fmaf_rn(ss, inv_hd, a.eps)), c = f * f * f * (sg * inv_hd);
-        /* y x f, of the kind whose sum it belongs to (zero past the heads); both in one warp where heads are not whole steps */
+        /* dx as f (w g - n mean(w g n)) with n = x f: f alone may be 2^63 or 2^-63, f^3 is no fp32 number then */
+        const float f = rsqrt_near(__fmaf_rn(ss, inv_hd, a.eps)), c = f * (sg * inv_hd);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= f;
+        /* y n, of the kind whose sum it belongs to (zero past the heads); both in one warp where heads are not whole steps */
         if (__all_sync(kAll, is_q)) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) sq[j] = __fmaf_rn(y[j] * x[j], f, sq[j]);
+          for (int j = 0; j < 8; ++j) sq[j] = __fmaf_rn(y[j], x[j], sq[j]);
         } else {
-          const float fq = is_q ? f : 0.f, fk = is_q ? 0.f : f;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            sq[j] = __fmaf_rn(y[j] * x[j], fq, sq[j]);
-            sk[j] = __fmaf_rn(y[j] * x[j], fk, sk[j]);
+            sq[j] = __fmaf_rn(is_q ? y[j] : 0.f, x[j], sq[j]);
+            sk[j] = __fmaf_rn(is_q ? 0.f : y[j], x[j], sk[j]);
           }
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = f * w[j] - x[j] * c;
+        for (int j = 0; j < 8; ++j) x[j] = f * __fmaf_rn(-x[j], c, w[j]);
         if (!mine) return;
         char* o = (is_q ? oq : ok) + (long long)h * os;
         store4((T*)o, wide, x);
