@@ -64,3 +64,40 @@ def test_heads_of_any_size(tctx, kind, layout, eps, H, KV, D):
         chain = max(1.0, M * a.shape[1] / 64)
         assert (np.abs(dw[i].double().cpu().numpy() - (g * n).sum((0, 1))) <= (2.0 ** -18 + chain * 2.0 ** -24) * terms + 1e-30).all()
     r.close()
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("H,KV,D", [(5, 3, 64), (3, 3, 128), (3, 1, 80), (1, 2, 8)])
+def test_what_is_not_finite_stays_with_its_kind(tctx, kind, layout, H, KV, D):
+    """An infinity in the last q head, or in the first k head: the other kind's rows and weight keep their gradients to the bit,
+    although one warp works on both (heads are no whole steps of 4 or 2)."""
+    import ulb_capi as U
+    rng = np.random.default_rng(D)
+    M = 9
+    x, dy = (torch.as_tensor(rng.standard_normal((M, H + KV, D))).to(DT[kind]).cuda() for _ in range(2))
+    w = dev(rng.uniform(0.5, 1.5, D), torch.float32)
+    pos = dev(rng.integers(0, 999, M))
+    r = U.Rope(tctx, D, layout=layout)
+
+    def gradients(x, dy):
+        q, k, gq, gk = (t.contiguous() for t in (x[:, :H], x[:, H:], dy[:, :H], dy[:, H:]))
+        KEEP.extend([q, k, gq, gk])
+        out = [torch.empty_like(q), torch.empty_like(k), *(torch.empty(D, device="cuda") for _ in range(2))]
+        r.norm_grad(U.dtype_id(kind), ptr(q), ptr(k), ptr(gq), ptr(gk), M, H, KV, ptr(w), ptr(w), 1e-6, ptr(pos), *map(ptr, out))
+        return out
+
+    want = gradients(x, dy)
+    assert all(torch.isfinite(t).all() for t in want)
+    for which in (0, 1):
+        for value in (math.inf, math.nan):
+            bad = dy.clone()
+            bad[4, H - 1 + which, 5] = value
+            got = gradients(x, bad)
+            assert torch.equal(got[1 - which], want[1 - which]) and torch.equal(got[3 - which], want[3 - which])
+            assert not torch.isfinite(got[2 + which]).all()
+            head = H - 1 if which == 0 else 0
+            assert not torch.isfinite(got[which][4, head]).any()
+            got[which][4, head] = want[which][4, head]
+            assert torch.equal(got[which], want[which])
+    r.close()

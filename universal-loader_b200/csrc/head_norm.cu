@@ -145,15 +145,17 @@ __global__ void __launch_bounds__(kWarps * 32, 2) norm_rope_grad_kernel(const __
         const float f = rsqrt_near(__fmaf_rn(ss, inv_hd, a.eps)), c = f * (sg * inv_hd);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] *= f;
-        /* y n, of the kind whose sum it belongs to (zero past the heads); both in one warp where heads are not whole steps */
+        /* y n, of the kind whose sum it belongs to (zero past the heads); both in one warp where heads are not whole steps: the
+           other kind's sum keeps its value, whatever y n is */
         if (__all_sync(kAll, is_q)) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) sq[j] = __fmaf_rn(y[j], x[j], sq[j]);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            sq[j] = __fmaf_rn(is_q ? y[j] : 0.f, x[j], sq[j]);
-            sk[j] = __fmaf_rn(is_q ? 0.f : y[j], x[j], sk[j]);
+            const float to = __fmaf_rn(y[j], x[j], is_q ? sq[j] : sk[j]);
+            sq[j] = is_q ? to : sq[j];
+            sk[j] = is_q ? sk[j] : to;
           }
         }
 #pragma unroll
