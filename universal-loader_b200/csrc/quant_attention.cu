@@ -14,8 +14,11 @@
  * keys: 3.0e-4 against 64 bits, the rounding alone 2.1e-4).  M is the running
  * maximum of s_t + log d_t (d_t the largest scale of the V row), so weights are at most 2^(RAISE + GROW) whatever the
  * scales are, and fp16 keeps 11 bits of one down to 2^-26 of the heaviest; p_t itself and what it sums to
- * are fp32 (a scale is at least 2^-24, so p_t stays in range).  q is scaled by a power of two a row, which makes
- * bf16 rows fp16 ones without loss.  It drops out of the scores exactly.
+ * are fp32 (a scale is at least 2^-24, so p_t stays in range).  q is scaled by a power of two a row, which drops out of the
+ * scores exactly: the row's largest element comes to [2^15, 2^16), the top of fp16's range, so that the others keep their
+ * bits (11 of fp16, 8 of bf16) down to 2^-29 of that power of two and are off by 2^-40 of it below; the elements that
+ * 4 bits want as q / 16 (below) down to 2^-25, and 2^-36.  With the largest at 1, as the scores' range alone would have it, an
+ * element 2^-17 of it had 7 bits left, or 3.
  *
  * Work.  A K and a V row take 80 (4 bits) or 144 bytes at head_dim 128.  K^T Q and V P are mma.sync m16n8k16 with
  * the codes as the 16-row operand (keys x dims, then dims x keys) and eight queries as columns, so a product wastes
@@ -51,6 +54,8 @@ namespace ulb {
 namespace {
 
 constexpr float kRaise = 12.f, kGrow = 3.9f; /* weights <= 2^15.9 < 65504 */
+/* powers of two of a row's largest element and, against elements in [1, 2), of the sums of 32 (<= 64, so < 2^15) as fp16 */
+constexpr int kTopQ = 15, kTopSum = 9;
 constexpr unsigned kAll = 0xffffffffu;
 
 template <bool Q4, int HD, int NT>
@@ -421,21 +426,21 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32 + 32, QCfg<Q4, HD, NT
       }
 #pragma unroll
       for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
-      const int ex = max(-126, min(127, top > 0.f ? ilogbf(top) : 0));
+      const int ex = max(-126, min(127, top > 0.f ? ilogbf(top) : 0)), el = kTopQ - ex;
 #pragma unroll
       for (int i = 0; i < N4; ++i) {
         const int d = (i * 32 + lane) * 4;
         /* 4 bits: elements 2 and 3 of a word come as 16 n */
-        const int eh = Q4 ? -ex - 4 : -ex;
-        const uint32_t lo = h2(ldexpf(x[i][0], -ex), ldexpf(x[i][1], -ex)), hi = h2(ldexpf(x[i][2], eh), ldexpf(x[i][3], eh));
+        const int eh = Q4 ? el - 4 : el;
+        const uint32_t lo = h2(ldexpf(x[i][0], el), ldexpf(x[i][1], el)), hi = h2(ldexpf(x[i][2], eh), ldexpf(x[i][3], eh));
         const float2 u = unpack2<__half>(lo), v = unpack2<__half>(hi);
         float sum = (u.x + u.y) + (Q4 ? 16.f : 1.f) * (v.x + v.y);
 #pragma unroll
         for (int o = 4; o; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
         if (d < HD) qb[((qi >> 3) * C::KS + (d >> 4)) * 32 + (qi & 7) * 4 + ((d >> 2) & 3)] = make_uint2(lo, hi);
-        /* s has sum(q) m (4 bits), or -128 sum(q) d (codes are offset by 128), of each group: the words of a row's scales
-           as operands (d, m) or (d, d of the next), these sums in two parts beside them */
-        if (!Q4) sum *= -128.f;
+        /* s has sum(q) m (4 bits), or -128 sum(q) d (codes are offset by 128; the 2^7 comes with the score's factor), of each
+           group: the words of a row's scales as operands (d, m) or (d, d of the next), these sums in two parts beside them */
+        sum *= (Q4 ? 1.f : -1.f) / (float)(1 << (kTopQ - kTopSum));
         const float next = __shfl_down_sync(kAll, sum, 8), top16 = to_f<__half>(from_f<__half>(sum)), next16 = to_f<__half>(from_f<__half>(next));
         const int word = Q4 ? d >> 5 : d >> 6;
         if (d < HD && d % (Q4 ? 32 : 64) == 0) {
@@ -443,7 +448,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32 + 32, QCfg<Q4, HD, NT
           qc[at] = Q4 ? make_uint2(h2(0.f, top16), h2(0.f, sum - top16)) : make_uint2(h2(top16, next16), h2(sum - top16, next - next16));
         }
       }
-      if (lane == 0) sh_qs[buf][qi] = ldexpf(1.f, ex) * a.scale2;
+      if (lane == 0) sh_qs[buf][qi] = ldexpf(a.scale2, ex - kTopSum + (Q4 ? 0 : 7));
     }
   };
   if (warp == 0) {
@@ -499,7 +504,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32 + 32, QCfg<Q4, HD, NT
       for (int u = 0; u < US; ++u) { /* 16 keys at a time: half the code, which would not fit the instruction cache */
         const uint8_t *const k0 = kt + (u * 16 + g) * C::RB, *const k1 = k0 + 8 * C::RB, *const vr = vt + (u * 16 + g) * C::RB;
         float s[NT][4];
-        /* ---- scores: sums of codes by group, in units of 2^-24, and the part that the scales alone give */
+        /* ---- scores: sums of codes by group, in units of 2^-24 2^kTopQ, and the part that the scales alone give, of 2^kTopSum */
         {
           float d0[NG], d1[NG];
           first_scales<Q4, NG>(k0 + C::CB, d0);
@@ -566,7 +571,7 @@ __global__ void __launch_bounds__(QCfg<Q4, HD, NT>::W * 32 + 32, QCfg<Q4, HD, NT
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = __fmaf_rn(s[n][e], 16777216.f, c0[n][e]);
+            for (int e = 0; e < 4; ++e) s[n][e] = __fmaf_rn(s[n][e], (float)(1 << (24 - kTopQ + kTopSum - (Q4 ? 0 : 7))), c0[n][e]);
         }
         /* ---- V's scales and middles, the logarithm of each row's largest scale */
         float vd[2][NG], vm[2][NG], lg[2];
