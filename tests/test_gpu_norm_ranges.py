@@ -101,3 +101,59 @@ def test_what_is_not_finite_stays_with_its_kind(tctx, kind, layout, H, KV, D):
             got[which][4, head] = want[which][4, head]
             assert torch.equal(got[which], want[which])
     r.close()
+
+
+HANDLES = [(dict(scaling="yarn", factor=4.0, orig_len=4096), None), (dict(attn_scale=0.3), 0.3),
+           (dict(scaling="yarn", factor=40.0, orig_len=2048, attn_scale=2.5), 2.5), (dict(scaling="linear", factor=8.0), None)]
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("more,factor", HANDLES)
+@pytest.mark.parametrize("M,H,KV,D,rot", [(7, 5, 3, 64, 64), (33, 4, 2, 128, 64), (5, 3, 1, 80, 48), (4, 2, 0, 256, 256)])
+def test_handles_that_scale(tctx, kind, layout, more, factor, M, H, KV, D, rot):
+    """m multiplies what turns, and nothing past rot_dim, in the outputs, in their gradients and in those of the weights."""
+    import ulb_capi as U
+    rng = np.random.default_rng(M + rot)
+    eps, half = 1e-5, layout == "half"
+    f, m = frequencies(rot, 10000.0, scaling=more.get("scaling", "none"), factor=more.get("factor", 1.0), orig=more.get("orig_len", 4096))
+    m = m if factor is None else factor
+
+    def turn(x, pos, sign=1.0):
+        y = rotate(x, pos, f, m, rot, half, sign)
+        y[..., rot:] = x[..., rot:]
+        return y
+
+    x, dy = (torch.as_tensor(rng.standard_normal((M, H + KV, D))).to(DT[kind]).cuda() for _ in range(2))
+    w = [dev(rng.uniform(0.5, 1.5, D), torch.float32) for _ in range(2)]
+    pos = rng.integers(0, 131072, M)
+    r = U.Rope(tctx, D, rot_dim=rot, layout=layout, **more)
+    q, k, gq, gk = (t.contiguous() for t in (x[:, :H], x[:, H:], dy[:, :H], dy[:, H:]))
+    y, dx = ([torch.empty_like(q), torch.empty_like(k)] for _ in range(2))
+    dw = [torch.empty(D, device="cuda") for _ in range(2)]
+    p = ptr(dev(pos))
+    r.norm_apply(U.dtype_id(kind), ptr(q), ptr(k), M, H, KV, ptr(w[0]), ptr(w[1]), eps, p, ptr(y[0]), ptr(y[1]))
+    r.norm_grad(U.dtype_id(kind), ptr(q), ptr(k), ptr(gq), ptr(gk), M, H, KV, ptr(w[0]), ptr(w[1]), eps, p, ptr(dx[0]), ptr(dx[1]), ptr(dw[0]),
+                ptr(dw[1]))
+    top = max(m, 1.0)
+    for i, (a, b) in enumerate(((q, gq), (k, gk))):
+        if a.shape[1] == 0:
+            continue
+        x64, y64, w64 = (t.double().cpu().numpy() for t in (a, b, w[i]))
+        s = 1 / np.sqrt((x64 * x64).mean(-1, keepdims=True) + eps)
+        n, g = x64 * s, turn(y64, pos, -1.0)
+        out = turn(n * w64, pos)
+        # the roundings of the plain handle, times the factor
+        big = np.abs(n * w64).max(-1, keepdims=True) * 1.5 * top
+        assert (np.abs(y[i].double().cpu().numpy() - out) <= (UNIT[kind] + 2.0 ** -19) * big).all()
+        want = s * (w64 * g - n * (w64 * g * n).mean(-1, keepdims=True))
+        size = pair_sizes(y64, rot, half) * top  # what an element of g is made of: its error is below 2^-20 of this
+        big = s * ((np.abs(w64) * size).max(-1, keepdims=True) * (1 + np.abs(n).max(-1, keepdims=True) ** 2))
+        assert (np.abs(dx[i].double().cpu().numpy() - want) <= UNIT[kind] * np.abs(want) + 2.0 ** -18 * big).all()
+        assert (np.abs(dw[i].double().cpu().numpy() - (g * n).sum((0, 1))) <= 2.0 ** -17 * (size * np.abs(n)).sum((0, 1)) + 1e-30).all()
+        # differences of the 64-bit function along a random direction: the formula itself
+        u, v, h = rng.standard_normal(x64.shape), rng.standard_normal(D), 1e-5
+        loss = lambda z: (turn(normed(x64 + z * u, w64 + z * v, eps), pos) * y64).sum()  # noqa: E731
+        slope, along = (loss(h) - loss(-h)) / (2 * h), (want * u).sum() + ((g * n).sum((0, 1)) * v).sum()
+        assert abs(slope - along) <= 1e-5 * (np.abs(want * u).sum() + np.abs((g * n).sum((0, 1)) * v).sum())
+    r.close()
