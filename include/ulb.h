@@ -502,8 +502,9 @@ ULB_API int ulb_logits_process(ulb_ctx* ctx, const ulb_logits_args* args);
  * ULB_ROPE_HALF) and one weight a head element, fp32 [head_dim], for all q heads and one for all k heads.
  * q and k are F32, F16 or BF16 rows of n_head and n_head_kv heads, element d of head h of row m at
  * m * row + h * head + d (0: dense); outputs are dense and of the same type, and may be the inputs where those
- * are dense too.  Computed in fp32, rounded once.  n_head_kv = 0: no k (its pointers unused).  Rows may be
- * at any element's address; 16-byte aligned pointers and strides of whole 16 bytes take wide loads.
+ * are dense too.  Computed in fp32, rounded once; a head whose sum of squares passes fp32's range (elements of about
+ * 1e18) has no norm here.  n_head_kv = 0: no k (its pointers unused).  Rows may be at any element's address; 16-byte
+ * aligned pointers and strides of whole 16 bytes take wide loads.
  */
 typedef struct ulb_norm_rope_args {
   int dtype, M, n_head, n_head_kv;
@@ -532,7 +533,8 @@ ULB_API int ulb_norm_rope_grad(ulb_ctx* ctx, const ulb_rope* r, const ulb_norm_r
  *   ULB_TYPE_Q4_1  4-bit codes, pairs of an fp16 scale and minimum:       x = d c + m, m = min x, d = (max x - m) / 15
  * (the values of GGUF's blocks of those types).  32-bit word i (0 .. 7) of each 32 bytes of 4-bit codes holds
  * elements 4 i .. 4 i + 3 of two neighbouring groups: the first group's at bits 0, 16, 4, 20, the second's
- * at bits 8, 24, 12, 28.  A group that holds an infinity or a NaN reads as NaN; scales past 65504 saturate.
+ * at bits 8, 24, 12, 28.  A group that holds an infinity or a NaN reads as NaN; scales and minima past 65504 in size saturate; no
+ * scale is negative.
  * Pools are dense and 16-byte aligned, [n_pages][n_head_kv][page] rows for one layer; layers may follow one
  * another.  Block tables as for ulb_cache_desc.  ulb_quant_pages gives the same pools of n_layer layers as a
  * ulb_cache_desc of 16-bit elements, for ulb_pages_copy / _compact and the page book.
@@ -593,7 +595,9 @@ ULB_API int ulb_quant_attention(ulb_ctx* ctx, const ulb_quant_desc* cache, const
  * that sees nothing gives out = 0 and lse = -inf; what a row does not see never touches its result.  q_row, k_row,
  * v_row: elements between rows (0: dense; heads are dense inside a row), multiples of 8.  dtype F16 or BF16,
  * head_dim 64, 80, 96, 128 or 256, n_head / n_head_kv <= 64.  max_q, max_k >= every sequence's rows and keys (clamped
- * otherwise: the first of them count).  Scores, statistics and sums are fp32, weights are rounded to the rows' type.
+ * otherwise: the first of them count).  Scores, statistics and sums are fp32, weights are rounded to the rows' type.  How a call fills
+ * the GPU goes by n_seq, max_q and max_k as if all sequences were the longest: a chunk of few rows after many thousand keys is
+ * quicker in a call of its own than packed with short sequences, and close bounds are quicker than loose ones.
  * The first call on a context allocates the 128 MiB of ulb_tree_attention's partial results.
  */
 typedef struct ulb_prompt_desc {

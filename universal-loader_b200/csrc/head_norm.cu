@@ -5,7 +5,9 @@
  *
  * Mathematics.  With f = 1 / sqrt(mean x^2 + eps), n = x f and g = R^T dy (R^T turns by the negative angle):
  *   y = R (w n),   dx = f (w g - n mean(w g n)),   dw = sum over rows and heads of g n.
- * mean(w g n) = f mean(w g x), so both sums of a head, x^2 and w g x, are taken in one pass.
+ * mean(w g n) = f mean(w g x), so both sums of a head, x^2 and w g x, are taken in one pass.  f comes from the hardware's
+ * reciprocal square root (2^-22) and every sum is fp32: fp32 gradients are off by 1.6e-7 against 64 bits, where sums in 64
+ * bits would leave 7e-8; 16-bit rows by their own rounding.
  *
  * Work.  Memory bounds it: every element is read once and written once (gradient: two reads).  A lane owns eight
  * elements of a head, both sides of four pairs, and 8, 16 or 32 lanes a head, so the sums are shuffles and pairs turn in
@@ -13,10 +15,10 @@
  * under way while it works on one; the weights are in shared memory.  When there are few rows, several warps share the heads
  * of one.  The sums of dw stay in registers over all rows of a warp, and a second small kernel adds the blocks in order.
  *
- * Measured: 16381 bf16 rows of 32 and 8 heads of 128 68 us, 4.9 TB/s (75 % of the copy rate); their gradient 103 us
- * (75 %); 1000 fp32 rows' gradient 19 us, of which the second kernel is 4; 8 rows 5 us, a launch.  About 160 instructions a
- * warp for two heads of 128 bound the forward pass beside HBM.  Two blocks an SM with four steps of heads in flight; three
- * blocks 76 us, three with two steps 69, four 88 to 93.
+ * Measured: 16381 bf16 rows of 32 and 8 heads of 128 68 to 70 us, 4.8 TB/s (73 to 75 % of the copy rate); their gradient 102
+ * to 108 us (71 to 75 %); in fp32 117 and 170 us (87 and 90 %); 1000 fp32 rows' gradient 19 us, of which the second kernel is 4;
+ * 8 rows 5 us, a launch.  About 160 instructions a warp for two heads of 128 bound the forward pass beside HBM.  Two blocks
+ * an SM with four steps of heads in flight; three blocks 76 us, three with two steps 69, four 88 to 93.
  */
 #include "head_rows.h"
 

@@ -9,10 +9,13 @@
  * Work of a CTA: RT = 16 WM queries (row x head of the group, so a K / V tile serves all heads that share it) against
  * the keys up to the last row's, in tiles of 64 keys through a ring of cp.async stages.  The warps are WM row
  * groups x WK key groups; a key group has its own (m, l, o), joined in shared memory.  Weights stay in
- * registers, rounded to the rows' type.
+ * registers, rounded to the rows' type once: V has that type, and a second part of each weight would be half as many products
+ * again.  Outputs are off by 1.9e-3 (bf16) and 2.4e-4 (fp16) against 64 bits, of which 1.6e-3 and 2.0e-4 are their own rounding.
  *
  * Used for head_dim 256 and for calls of at most 128 keys (prompt_attention_tc.cu, which has the rule): 64 rows of 32 heads over
- * 8 of 64 9 us, the host's call; as the only form four prompts of 2 to 6 thousand rows took 2960 us.
+ * 8 of 64 9 us, the host's call; as the only form four prompts of 2 to 6 thousand rows of head_dim 128 took 2960 us.  At
+ * head_dim 256, 4096 rows of 32 heads over 8 take 1155 us (0.24 PFLOP/s), 500 rows 35 us: one CTA of 8 warps an SM (registers and
+ * shared memory), whose products, loads and softmax wait for each other (26 % of the issue slots, mma.sync's pipe 40 % of the time).
  *
  * What a row does not see never reaches its result: scores past its last key are replaced, keys past the tile's last
  * are zero-filled (the rows there belong to the next sequence), and an element of V in a tile on the diagonal that is

@@ -10,8 +10,9 @@
  *   PAIR = false  128 queries: both hold the same and take the even and the odd tiles; they join in shared memory
  * S = Q K^T (both operands in shared memory, fp32 in TMEM); the query's thread reads S, updates m and l, writes P in the rows' type
  * over S; O += P V with P from TMEM and V as the tile TMA wrote it.  O is rescaled only when a maximum has grown by more than
- * 2^GROW.  Weights are rounded to 16 bits once: bf16 outputs are off by 2.2e-3 relative against 64 bits, fp16 ones by
- * 2.4e-4, of which 1.7e-3 and 2.1e-4 are the output's own rounding.  K and V rows come by TMA from wherever a sequence begins; what a
+ * 2^GROW.  Weights are rounded to 16 bits once, since both operands of the product are of the rows' type and a second part
+ * would double it: bf16 outputs are off by 2.1e-3 to 2.3e-3 relative against 64 bits, fp16 ones by 2.4e-4 to 2.7e-4, of which
+ * 1.65e-3 and 2.0e-4 are the output's own rounding.  K and V rows come by TMA from wherever a sequence begins; what a
  * tile holds of the next sequence is masked, its infinities and NaN taken out of V with those past the diagonal.
  *
  * Work.  A unit is a (sequence, row tile, share of its keys, kv head) and walks the keys up to its last row's only.  The row
@@ -19,10 +20,11 @@
  * turns that run back and forth, so all end together whatever the lengths; what fits the SMs once needs no list.  Few units
  * with many keys are cut into shares, joined by a third kernel.
  *
- * Measured: four prompts of 2 to 6 thousand rows, 32 heads over 8 of 128 (682 GFLOP): 670 to 720 us, 0.95 to 1.02 PFLOP/s (58
- * to 62 % of the burst rate, 68 to 73 % of the sustained one: the clock falls to 1.4 GHz under the power cap); 513 rows after
- * 30000 keys 276 to 300 us; 2000 rows 48 us; 500 rows of 32 heads over 4 of 64 12 us; 16 prompts of 200 to 400 rows 63 us.  A
- * pair of 64-key tiles takes 1700 to 1980 cycles: 1240 of them on the tensor pipe (products with 64 columns read Q from shared
+ * Measured: four prompts of 2157 to 6001 rows, 32 heads over 8 of 128 (618 GFLOP): 647 to 732 us, 0.84 to 0.96 PFLOP/s (52 to
+ * 58 % of the burst rate, 61 to 69 % of the sustained one: the clock falls to 1.4 GHz under the power cap, by how much differs
+ * between runs and GPUs); 513 rows after 30000 keys 276 to 309 us; 4096 rows 150 us at head dim 128 (0.92 PFLOP/s), 148
+ * at 96 and at 80, whose tiles hold as many columns, 135 at 64; 2000 rows 48 us; 500 rows of 32 heads over 4 of 64 11 us; 16
+ * prompts of 200 to 400 rows 60 to 63 us.  A pair of 64-key tiles takes 1700 to 1980 cycles: 1240 of them on the tensor pipe (products with 64 columns read Q from shared
  * memory every time), 1024 of exponentials, which overlap in part.  What a unit costs besides is not overlapped with the
  * next one: its rows in (4000 to 6000 cycles) and its outputs out (5000), most of a short prompt's time.  Tried and slower:
  * scores and weights in separate columns, so that the next tile's scores start as soon as these are read (827 us for 770 at
@@ -721,6 +723,12 @@ constexpr int kShareTiles = 16; /* tiles a share has at least */
 /*
  * Into how many shares the keys of a row tile are cut: as many as fill the SMs best.  Units that are as many as the SMs
  * four times over stay whole (sorted by length they even out); a share costs a twentieth more for what it leaves to join.
+ * The lengths are on the device, so every sequence counts as the longest, which is wrong for a long chunk with short
+ * sequences beside it: 513 rows after 30000 keys take 276 us alone and 512 with one sequence of 10 rows beside them, 1 row
+ * after 20000 keys 27 alone and 184 with 15 (such a chunk is quicker in a call of its own; the header says so).  Counts that
+ * the host could make instead were no better: row tiles that q_rows can hold gave 297 to 520 us for these by chance of the
+ * waves, and 195 for 151 on three chunks of 300 rows after 8000 keys with five of 40 rows; k_rows / max_k sequences cut far too
+ * finely where max_k is a loose bound.
  */
 int pick_shares(long long units, int tiles, int n_sm, long long most) {
   if (units >= 4ll * n_sm) return 1;

@@ -35,13 +35,15 @@
  * over the blocks, so lengths may differ as they like; a unit in several blocks leaves a partial in each and the last
  * of them to arrive joins them in order.  While a unit's tiles are worked on, the next unit's rows of q are made.
  *
- * Measured (bf16): 64 sequences of 256 to 8192 keys, 32 heads over 8 of 128, 4 bits: 113 us, 3.1 TB/s (48 % of the copy
- * rate); 5 rows over 100001 keys, 64 heads over 8, 8 bits: 136 us; 1 x 20000 keys 20 (4 bits) and 22 us; 64 x 1000 keys in 8
- * bits 44 us, half of the copy rate.  What bounds it is instructions: about 450 a warp for 16 keys of eight queries in 4
- * bits, of which unpacking V, the weights of its groups and their transposition are half, at two to three a cycle; with
- * more queries the weights of each 8 more, and past 32 the keys are walked again.  Tried and slower: 16 warps of 128
- * registers (170 us for the 113), a warp that feeds itself (135), all 32 keys in one body (the code leaves the
- * instruction cache; 157).
+ * Measured (bf16): 64 sequences of 256 to 8192 keys, 32 heads over 8 of 128, 4 bits: 112 to 118 us, 3.0 to 3.1 TB/s (46 to
+ * 47 % of the copy rate); 5 rows over 100001 keys, 64 heads over 8, 8 bits: 137 to 141 us; 1 x 20000 keys 20 (4 bits) and 22
+ * us; 64 x 1000 keys in 8 bits 43 us, half of the copy rate; 16 x 4000 keys, 16 heads over 4 of 256, 45 (4 bits) and 41 us; 16
+ * rows of a tree over 4000 keys, 8 sequences, 108 and 97 us, as many in a chain 106 and 96.  No pipe is full (54 % of the
+ * issue slots): what bounds it is the order of dependent instructions in few warps, about 450 a warp for 16 keys of eight
+ * queries in 4 bits, of which unpacking V, the weights of its groups and their transposition are half; with more queries
+ * the weights of each 8 more, and past 32 the keys are walked again.  Tried and slower: 16 warps of 128 registers (170 us
+ * for the 113 of the time), a warp that feeds itself (135), all 32 keys in one body (the code leaves the instruction
+ * cache; 157).
  */
 #include "quant_cache.h"
 #include "tcgen05.h"
