@@ -24,9 +24,9 @@
  * 58 % of the burst rate, 61 to 69 % of the sustained one: the clock falls to 1.4 GHz under the power cap, by how much differs
  * between runs and GPUs); 513 rows after 30000 keys 276 to 309 us; 4096 rows 150 us at head dim 128 (0.92 PFLOP/s), 148
  * at 96 and at 80, whose tiles hold as many columns, 135 at 64; 2000 rows 48 us; 500 rows of 32 heads over 4 of 64 11 us; 16
- * prompts of 200 to 400 rows 60 to 63 us.  A pair of 64-key tiles takes 1700 to 1980 cycles: 1240 of them on the tensor pipe (products with 64 columns read Q from shared
- * memory every time), 1024 of exponentials, which overlap in part.  What a unit costs besides is not overlapped with the
- * next one: its rows in (4000 to 6000 cycles) and its outputs out (5000), most of a short prompt's time.  Tried and slower:
+ * prompts of 200 to 400 rows 60 to 63 us.  A pair of 64-key tiles takes 1700 to 1980 cycles: 1240 of them on the tensor pipe
+ * (products with 64 columns read Q from shared memory every time), 1024 of exponentials, which overlap in part.  What a unit
+ * costs besides is not overlapped with the next one: its rows in (4000 to 6000 cycles) and its outputs out (5000), most of a short prompt's time.  Tried and slower:
  * scores and weights in separate columns, so that the next tile's scores start as soon as these are read (827 us for 770 at
  * the time); the next unit's rows held in registers while the outputs leave (spills; 16 short prompts 88 us for 70).
  *
